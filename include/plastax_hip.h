@@ -1181,6 +1181,71 @@ PLX_EXPORT int plx_remap_merged(int64_t n, const int32_t* idx, int64_t off, int6
 PLX_EXPORT int plx_count_ids(int64_t n, const int32_t* ids, const uint8_t* skip, int32_t nbins, int32_t* counts,
                              void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Level pairs as whole matrices in few bits (no counterpart in the reference).
+ * 32 consecutive values of a line share one scale 2^(s - 127), s a byte: the
+ * least power of two under which the block's largest value is at most 6 (4
+ * bits) or 448 (8 bits), and at least 2^-125 or 2^-117. Values are rounded to
+ * the nearest, ties to the even code.
+ *   4 bits: e2m1 codes, two to a byte, the earlier value low; a line holds
+ *     ceil(n / 128) * 4 blocks of 16 bytes, zero codes past its end. A block
+ *     with an infinity or a NaN has s = 255 and stands for NaN.
+ *   8 bits: e4m3 codes without infinities, one to a byte; a line holds
+ *     ceil(n / 32) blocks of 32 bytes. An infinity or a NaN is kept as NaN in
+ *     its own place.
+ * codes start on 16 bytes. Sizes are at most 2^30. Strides are in elements. */
+#define PLX_LB_F32 0
+#define PLX_LB_BF16 1
+#define PLX_LB_F16 2
+
+#define PLX_LB_RELU 0
+#define PLX_LB_TANH 1
+#define PLX_LB_SIGMOID 2
+#define PLX_LB_SILU 3
+
+/* x (lines of n values) as 4-bit blocks along its lines. */
+PLX_EXPORT int plx_mx4_quantise(int64_t lines, int64_t n, int32_t dtype, const void* x, int64_t line_stride,
+                                int64_t stride, uint8_t* codes, uint8_t* scales, void* stream);
+
+/* out [lines][n] = the values that codes of `bits` 4 or 8 stand for. */
+PLX_EXPORT int plx_mx_values(int32_t bits, int64_t lines, int64_t n, const uint8_t* codes, const uint8_t* scales,
+                             int32_t dtype, void* out, void* stream);
+
+/* y = fn(h), and h in 8-bit blocks along its lines. */
+PLX_EXPORT int plx_mx8_activate(int64_t lines, int64_t n, int32_t dtype, int32_t fn, const void* h, int64_t h_line,
+                                int64_t h_elem, void* y, int64_t y_line, int64_t y_elem, uint8_t* codes,
+                                uint8_t* scales, void* stream);
+
+/* dh = dy fn'(q), q the values of plx_mx8_activate's blocks. */
+PLX_EXPORT int plx_mx8_activate_grad(int64_t lines, int64_t n, int32_t dtype, int32_t fn, const void* dy,
+                                     int64_t y_line, int64_t y_elem, const uint8_t* codes, const uint8_t* scales,
+                                     void* dh, int64_t h_line, int64_t h_elem, void* stream);
+
+/* Products of a level pair; w is [outputs][inputs] in 4-bit blocks along its
+ * lines, x [tokens][inputs] in 8-bit blocks:
+ *   PRODUCT              out [tokens][outputs] = a w^T, a [tokens][inputs]
+ *   PRODUCT_GRAD         out [tokens][inputs]  = a w,   a [tokens][outputs]
+ *   WEIGHT_GRAD          out [outputs][inputs] = a^T x, a [tokens][outputs],
+ *                        x's lines the tokens
+ *   WEIGHT_GRAD_COLUMNS  the same, x's lines the inputs (blocks along tokens)
+ * a(t, u) = a[t * token_stride + u * unit_stride] of `dtype`; out has the same
+ * type for the first two and float32 for the others. Sums are float32;
+ * products are exact. workspace: plx_mx_workspace() bytes, on 16 bytes. */
+#define PLX_LB_PRODUCT 0
+#define PLX_LB_PRODUCT_GRAD 1
+#define PLX_LB_WEIGHT_GRAD 2
+#define PLX_LB_WEIGHT_GRAD_COLUMNS 3
+PLX_EXPORT int64_t plx_mx_workspace(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs);
+PLX_EXPORT int plx_mx_product(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs, int32_t dtype,
+                              const void* a, int64_t token_stride, int64_t unit_stride, const uint8_t* codes,
+                              const uint8_t* scales, void* out, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+
+/* out [tokens][outputs] = x w^T with both in 4-bit blocks along the inputs. */
+PLX_EXPORT int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8_t* x_codes,
+                               const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales, int32_t dtype,
+                               void* out, void* stream);
+
 PLX_EXPORT int32_t plx_abi_version(void);
 
 #ifdef __cplusplus

@@ -18,7 +18,7 @@ LIB_PATH = pathlib.Path(
     or pathlib.Path(__file__).resolve().parent / "libplastax_hip.so"
 )
 
-ABI_VERSION = 29  # plx_abi_version() of the library these mirrors describe
+ABI_VERSION = 30  # plx_abi_version() of the library these mirrors describe
 
 PLX_MAX_INSTR = 48
 PLX_MAX_CONST = 32
@@ -562,6 +562,15 @@ _SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "plx_kill_incident": (c_i32, [c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, ctypes.c_float, c_vp]),
     "plx_unit_place": (c_i32, [c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp,
                                c_vp]),
+    "plx_mx4_quantise": (c_i32, [c_i64, c_i64, c_i32, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "plx_mx_values": (c_i32, [c_i32, c_i64, c_i64, c_vp, c_vp, c_i32, c_vp, c_vp]),
+    "plx_mx8_activate": (c_i32, [c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "plx_mx8_activate_grad": (c_i32, [c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64,
+                                      c_vp]),
+    "plx_mx_workspace": (c_i64, [c_i32, c_i64, c_i64, c_i64]),
+    "plx_mx_product": (c_i32, [c_i32, c_i64, c_i64, c_i64, c_i32, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64,
+                               c_vp]),
+    "plx_mx4_product": (c_i32, [c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp]),
 }
 
 # Entry points the header declares (checked by the CPU test suite).

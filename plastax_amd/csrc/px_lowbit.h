@@ -1,0 +1,199 @@
+// px_lowbit.h -- pieces shared by the kernels of level pairs in few bits: the
+// two block formats, the element types and the fragments of the matrix
+// instructions.
+//
+// A block is 32 consecutive values of a line under one scale 2^(s - 127), s
+// one byte. In 4 bits (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6, sign in bit 3) two
+// values share a byte, the earlier one low; in 8 bits (e4m3: 4 exponent bits
+// of bias 7, 3 behind the point, no infinities, 0x7f / 0xff NaN) each has one.
+// The scale is the least power of two under which the block's largest value
+// is not above 6 or 448.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/plastax_hip.h"
+
+namespace px {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ bf16x8 as_bf16x8(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
+
+// Element types of activations and gradients: float, __bf16, _Float16.
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+  return static_cast<float>(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {
+  return static_cast<T>(v);  // to the nearest, ties to even
+}
+
+// v[0..8) = p[0..8), p on 16 bytes.
+__device__ __forceinline__ void load8v(const float* p, float v[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+template <typename T>
+__device__ __forceinline__ void load8v(const T* p, float v[8]) {
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  const t8 a = *reinterpret_cast<const t8*>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_f32(a[i]);
+}
+
+// v[i] = p[i * stride] for i < n, zero from there on.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int64_t stride, int n, bool wide, float v[8]) {
+  if (wide && n >= 8) {
+    load8v(p, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i * stride]) : 0.0f;
+}
+
+__device__ __forceinline__ void store8v(float* p, const float v[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <typename T>
+__device__ __forceinline__ void store8v(T* p, const float v[8]) {
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  t8 a;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = from_f32<T>(v[i]);
+  *reinterpret_cast<t8*>(p) = a;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int64_t stride, int n, bool wide, const float v[8]) {
+  if (wide && n >= 8) {
+    store8v(p, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) p[i * stride] = from_f32<T>(v[i]);
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// The exponent e of a block whose largest |value| has these bits (finite):
+// amax <= (1 + mantissa / 2^23) 2^top 2^e, e >= least. Subnormal amax: the
+// exponent field is 0, and least stands above what it gives.
+__device__ __forceinline__ int block_exponent(uint32_t amax, uint32_t mantissa, int top, int least) {
+  const int e = static_cast<int>(amax >> 23) - 127 - top + ((amax & 0x7FFFFFu) > mantissa ? 1 : 0);
+  return e > least ? e : least;
+}
+__device__ __forceinline__ int exponent4(uint32_t amax) { return block_exponent(amax, 0x400000u, 2, -125); }
+__device__ __forceinline__ int exponent8(uint32_t amax) { return block_exponent(amax, 0x600000u, 8, -117); }
+
+// 2^e, e in [-126, 127].
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+// What a scale byte stands for; 255 is a block of NaN.
+__device__ __forceinline__ float scale_value(uint32_t s) {
+  return __uint_as_float(s == 255u ? 0x7FC00000u : s << 23);
+}
+
+// 8 values under the scale 2^e as 4-bit codes, to the nearest, ties to the
+// even code (the conversion instruction divides by its scale operand).
+__device__ __forceinline__ uint32_t codes4(const float v[8], float scale) {
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], scale, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], scale, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], scale, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], scale, 3);
+  return c;
+}
+
+// 8 values times inv = 2^-e as e4m3 codes; a value that is not finite is NaN.
+__device__ __forceinline__ uint2 codes8(const float v[8], float inv) {
+  float m[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m[i] = abs_bits(v[i]) >= kInfBits ? __builtin_nanf("") : v[i] * inv;
+  int a = 0, b = 0;
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(m[0], m[1], a, false);
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(m[2], m[3], a, true);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(m[4], m[5], b, false);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(m[6], m[7], b, true);
+  return make_uint2(static_cast<uint32_t>(a), static_cast<uint32_t>(b));
+}
+
+// The float32 values of 8 codes under a scale (exact: 2 or 4 significant
+// bits times a power of two, normal by the formats' least exponents).
+__device__ __forceinline__ void values4(uint32_t c, float scale, float v[8]) {
+  f32x2 p;
+  p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 0), v[0] = p[0], v[1] = p[1];
+  p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 1), v[2] = p[0], v[3] = p[1];
+  p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 2), v[4] = p[0], v[5] = p[1];
+  p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 3), v[6] = p[0], v[7] = p[1];
+}
+__device__ __forceinline__ void values8(uint2 c, float scale, float v[8]) {
+  f32x2 p;
+  p = __builtin_amdgcn_cvt_pk_f32_fp8(c.x, false), v[0] = p[0] * scale, v[1] = p[1] * scale;
+  p = __builtin_amdgcn_cvt_pk_f32_fp8(c.x, true), v[2] = p[0] * scale, v[3] = p[1] * scale;
+  p = __builtin_amdgcn_cvt_pk_f32_fp8(c.y, false), v[4] = p[0] * scale, v[5] = p[1] * scale;
+  p = __builtin_amdgcn_cvt_pk_f32_fp8(c.y, true), v[6] = p[0] * scale, v[7] = p[1] * scale;
+}
+
+// The same as bf16, exact for the same reason (bf16 has float32's exponents).
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  return (__float_as_uint(lo) >> 16) | (__float_as_uint(hi) & 0xFFFF0000u);
+}
+__device__ __forceinline__ uint4 bf16_of4(uint32_t c, float scale) {
+  uint4 r;
+  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0));
+  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1));
+  r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2));
+  r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3));
+  return r;
+}
+__device__ __forceinline__ uint4 bf16_of8(uint2 c, float scale) {
+  float v[8];
+  values8(c, scale, v);
+  return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+// 8 values as a sum of P bf16 pieces each, by cutting off 8 significant bits
+// at a time: exact for P = 1 (bf16), 2 (float16, 11 bits) and 3 (float32, 24
+// bits) down to bf16's least subnormal. An infinity or a NaN is its own first
+// piece and its others are zero.
+template <int P>
+__device__ __forceinline__ void pieces8(const float in[8], uint4 out[P]) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = in[i];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t u = __float_as_uint(v[i]);
+      if ((u & 0x7FFFFFFFu) > kInfBits) u |= 0x00400000u;  // a NaN stays one when its low bits go
+      h[i] = u & 0xFFFF0000u;
+      if (p + 1 < P) v[i] = (u & kInfBits) == kInfBits ? 0.0f : v[i] - __uint_as_float(h[i]);
+    }
+    out[p] = make_uint4((h[0] >> 16) | h[1], (h[2] >> 16) | h[3], (h[4] >> 16) | h[5], (h[6] >> 16) | h[7]);
+  }
+}
+template <typename T>
+struct Pieces {
+  static constexpr int n = 3;
+};
+template <>
+struct Pieces<__bf16> {
+  static constexpr int n = 1;
+};
+template <>
+struct Pieces<_Float16> {
+  static constexpr int n = 2;
+};
+
+}  // namespace px
