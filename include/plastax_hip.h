@@ -1230,21 +1230,25 @@ PLX_EXPORT int plx_mx8_activate_grad(int64_t lines, int64_t n, int32_t dtype, in
  *   WEIGHT_GRAD_COLUMNS  the same, x's lines the inputs (blocks along tokens)
  * a(t, u) = a[t * token_stride + u * unit_stride] of `dtype`; out has the same
  * type for the first two and float32 for the others. Sums are float32;
- * products are exact. workspace: plx_mx_workspace() bytes, on 16 bytes. */
+ * products are exact. workspace: plx_mx_workspace() bytes (of the same a: its
+ * alignment counts), on 16 bytes; -1 from it is a bad argument. */
 #define PLX_LB_PRODUCT 0
 #define PLX_LB_PRODUCT_GRAD 1
 #define PLX_LB_WEIGHT_GRAD 2
 #define PLX_LB_WEIGHT_GRAD_COLUMNS 3
-PLX_EXPORT int64_t plx_mx_workspace(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs);
+PLX_EXPORT int64_t plx_mx_workspace(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs, int32_t dtype,
+                                    const void* a, int64_t token_stride, int64_t unit_stride);
 PLX_EXPORT int plx_mx_product(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs, int32_t dtype,
                               const void* a, int64_t token_stride, int64_t unit_stride, const uint8_t* codes,
                               const uint8_t* scales, void* out, void* workspace, int64_t workspace_bytes,
                               void* stream);
 
-/* out [tokens][outputs] = x w^T with both in 4-bit blocks along the inputs. */
+/* out [tokens][outputs] = x w^T with both in 4-bit blocks along the inputs;
+ * workspace: plx_mx4_workspace() bytes, on 16 bytes. */
+PLX_EXPORT int64_t plx_mx4_workspace(int64_t tokens, int64_t inputs, int64_t outputs);
 PLX_EXPORT int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8_t* x_codes,
                                const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales, int32_t dtype,
-                               void* out, void* stream);
+                               void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
 PLX_EXPORT int32_t plx_abi_version(void);
 

@@ -567,10 +567,11 @@ _SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "plx_mx8_activate": (c_i32, [c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "plx_mx8_activate_grad": (c_i32, [c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64,
                                       c_vp]),
-    "plx_mx_workspace": (c_i64, [c_i32, c_i64, c_i64, c_i64]),
+    "plx_mx_workspace": (c_i64, [c_i32, c_i64, c_i64, c_i64, c_i32, c_vp, c_i64, c_i64]),
+    "plx_mx4_workspace": (c_i64, [c_i64, c_i64, c_i64]),
     "plx_mx_product": (c_i32, [c_i32, c_i64, c_i64, c_i64, c_i32, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64,
                                c_vp]),
-    "plx_mx4_product": (c_i32, [c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp]),
+    "plx_mx4_product": (c_i32, [c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp]),
 }
 
 # Entry points the header declares (checked by the CPU test suite).

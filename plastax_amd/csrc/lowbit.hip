@@ -11,6 +11,7 @@
 #include "../../include/plastax_hip.h"
 #include "px_common.h"
 #include "px_lowbit.h"
+#include "px_lowbit_gemm.h"
 #include "px_math.h"
 
 using plx_detail::check_launch;
@@ -500,9 +501,55 @@ __global__ __launch_bounds__(256) void k_mx4_gemm(int M, int N, int64_t blocks, 
 }
 
 // ---------------------------------------------------------------------------
+// Operands of the large products: bf16 lines padded with zeros.
+// ---------------------------------------------------------------------------
+// Piece p of line l at out + p * piece + l * out_line.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void k_big_pieces(int64_t lines, int64_t n, const T* x, int64_t sl, int64_t se,
+                                                       bool wide, uint16_t* out, int64_t out_lines, int64_t out_n,
+                                                       int64_t out_line, int64_t piece, int lx) {
+  constexpr int P = Pieces<T>::n;
+  const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
+  for (int64_t line = static_cast<int64_t>(blockIdx.x) * ly + ty; line < out_lines;
+       line += static_cast<int64_t>(gridDim.x) * ly) {
+    for (int64_t c = tx; c < out_n / 8; c += lx) {
+      const int64_t left = line < lines ? n - c * 8 : 0;
+      float v[8];
+      load8(x + line * sl + c * 8 * se, se, left > 8 ? 8 : left < 0 ? 0 : static_cast<int>(left), wide, v);
+      uint4 p[P];
+      pieces8<P>(v, p);
+#pragma unroll
+      for (int i = 0; i < P; ++i) *reinterpret_cast<uint4*>(out + i * piece + line * out_line + c * 8) = p[i];
+    }
+  }
+}
+
+template <int BITS>
+__global__ __launch_bounds__(kBlock) void k_big_values(int64_t lines, int64_t n, const uint8_t* codes,
+                                                       const uint8_t* scales, uint16_t* out, int64_t out_lines,
+                                                       int64_t out_n, int lx) {
+  const int64_t kept = BITS == 4 ? div_up(n, 128) * 16 : div_up(n, 32) * 4;
+  const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
+  for (int64_t line = static_cast<int64_t>(blockIdx.x) * ly + ty; line < out_lines;
+       line += static_cast<int64_t>(gridDim.x) * ly) {
+    for (int64_t c = tx; c < out_n / 8; c += lx) {
+      uint4 r = make_uint4(0, 0, 0, 0);
+      if (line < lines && c < kept) {
+        const float scale = scale_value(scales[line * (kept / 4) + c / 4]);
+        r = BITS == 4 ? bf16_of4(reinterpret_cast<const uint32_t*>(codes)[line * kept + c], scale)
+                      : bf16_of8(reinterpret_cast<const uint2*>(codes)[line * kept + c], scale);
+      }
+      *reinterpret_cast<uint4*>(out + line * out_n + c * 8) = r;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 constexpr int64_t kMaxDim = int64_t{1} << 30;
+constexpr int64_t kBigLeast = 256;              // m, n and k of a large product
+constexpr int64_t kBigLine = int64_t{1} << 22;  // elements of its lines: 256 of them stay below 2^32 bytes
 
 inline bool dims_fit(int64_t a, int64_t b) { return a >= 0 && b >= 0 && a <= kMaxDim && b <= kMaxDim; }
 inline int size_of(int dtype) { return dtype == PLX_LB_F32 ? 4 : 2; }
@@ -558,9 +605,117 @@ inline Shape shape_of(int kind, int64_t tokens, int64_t inputs, int64_t outputs)
   return {outputs, inputs, tokens};
 }
 
-int64_t workspace_of(const Shape& s) {
-  const int splits = splits_of(s.m, s.n, s.k);
-  return splits > 1 ? int64_t{4} * splits * s.m * s.n : 0;
+constexpr int64_t round_up(int64_t a, int64_t b) { return div_up(a, b) * b; }
+
+// How a product runs. `big`: through bf16 operands in memory (k_big_gemm); a
+// itself where it is one already.
+struct Plan {
+  bool big;
+  int splits;
+  bool across_a, across_b, direct;
+  int64_t kp;       // k padded to whole steps
+  int64_t mp, np;   // padded rows' lengths of "across" operands
+  int64_t bytes_a, bytes_b, bytes;
+};
+
+// Workgroups that a large product should fill: one per CU.
+int big_splits(int64_t m, int64_t n, int64_t steps) {
+  const int64_t tiles = div_up(m, kBig) * div_up(n, kBig);
+  int64_t s = cu_count() / (tiles > 0 ? tiles : 1);
+  s = s < steps / 8 ? s : steps / 8;
+  if (s < 2) return 1;
+  return static_cast<int>(div_up(steps, div_up(steps, s)));  // (no range is empty)
+}
+
+Plan plan_of(int kind, const Shape& s, int dtype, const void* a, int64_t sm, int64_t sk) {
+  Plan p{};
+  const int pieces = dtype == PLX_LB_F32 ? 3 : dtype == PLX_LB_F16 ? 2 : 1;
+  p.big = s.m >= kBigLeast && s.n >= kBigLeast && s.k >= kBigLeast;
+  if (!p.big) {
+    p.splits = splits_of(s.m, s.n, s.k);
+    p.bytes = p.splits > 1 ? int64_t{4} * p.splits * s.m * s.n : 0;
+    return p;
+  }
+  p.across_a = sm == 1 && sk != 1;
+  p.across_b = kind == PLX_LB_PRODUCT_GRAD || kind == PLX_LB_WEIGHT_GRAD;
+  p.kp = round_up(s.k, 64), p.mp = round_up(s.m, 8), p.np = round_up(s.n, 8);
+  const int64_t line = p.across_a ? sk : sm;
+  p.direct = dtype == PLX_LB_BF16 && s.k % 64 == 0 && on16(a) && line % 8 == 0 && line <= kBigLine &&
+             (p.across_a ? s.m % 8 == 0 : sk == 1);
+  p.bytes_a = p.direct ? 0 : round_up(2 * pieces * p.kp * (p.across_a ? p.mp : s.m), 256);
+  p.bytes_b = round_up(2 * p.kp * (p.across_b ? p.np : s.n), 256);
+  p.splits = big_splits(s.m, s.n, pieces * p.kp / 64);
+  p.bytes = p.bytes_a + p.bytes_b + (p.splits > 1 ? int64_t{4} * p.splits * s.m * s.n : 0);
+  return p;
+}
+
+// out [n] = the joined sums of `splits` ranges.
+template <typename OT>
+void launch_join(int64_t n, int splits, const float* part, OT* out, hipStream_t s) {
+  const int64_t groups = div_up(n, kBlock);
+  k_mx_join<OT><<<static_cast<unsigned>(groups < kMaxGroups ? groups : kMaxGroups), kBlock, 0, s>>>(n, splits, part, out);
+}
+
+template <typename T, int KIND, typename OT>
+void launch_big(const GemmArgs& g, const Plan& p, char* work, hipStream_t s) {
+  constexpr int P = Pieces<T>::n;
+  constexpr bool BA = KIND == kWT || KIND == kX;
+  BigArgs b{};
+  if (p.direct) {
+    b.a = static_cast<const char*>(g.a);
+    b.lda = 2 * (p.across_a ? g.sk : g.sm);
+    b.rows_a = g.M;
+  } else {
+    uint16_t* out = reinterpret_cast<uint16_t*>(work);
+    const int64_t lines = p.across_a ? g.K : g.M, n = p.across_a ? g.M : g.K;
+    const int64_t sl = p.across_a ? g.sk : g.sm, se = p.across_a ? g.sm : g.sk;
+    const int64_t out_lines = p.across_a ? p.kp : g.M, out_n = p.across_a ? p.mp : p.kp;
+    const int64_t out_line = p.across_a ? p.mp : P * p.kp, piece = p.across_a ? p.kp * p.mp : p.kp;
+    const int lx = lanes_along(out_n / 8);
+    const bool wide = se == 1 && on16(g.a) && (sl * sizeof(T)) % 16 == 0;
+    k_big_pieces<T><<<groups_along(out_lines, lx), kBlock, 0, s>>>(lines, n, static_cast<const T*>(g.a), sl, se, wide,
+                                                                   out, out_lines, out_n, out_line, piece, lx);
+    b.a = work;
+    b.lda = 2 * out_line;
+    b.rows_a = static_cast<int>(p.across_a ? p.mp : g.M);
+  }
+  uint16_t* vb = reinterpret_cast<uint16_t*>(work + p.bytes_a);
+  const int64_t lines = BA ? g.K : g.N, out_lines = BA ? p.kp : g.N, out_n = BA ? p.np : p.kp;
+  const int lx = lanes_along(out_n / 8);
+  k_big_values<KIND == kW || KIND == kWT ? 4 : 8><<<groups_along(out_lines, lx), kBlock, 0, s>>>(
+      lines, BA ? g.N : g.K, g.codes, g.scales, vb, out_lines, out_n, lx);
+  b.b = reinterpret_cast<const char*>(vb);
+  b.ldb = 2 * out_n;
+  b.rows_b = static_cast<int>(BA ? p.np : g.N);
+  b.out = g.out;
+  b.part = reinterpret_cast<float*>(work + p.bytes_a + p.bytes_b);
+  b.M = g.M, b.N = g.N;
+  b.wrap = static_cast<int>(p.kp / 64), b.steps = P * b.wrap;
+  b.split = static_cast<int>(div_up(b.steps, p.splits));
+  b.tiles_m = static_cast<int>(div_up(g.M, kBig)), b.tiles_n = static_cast<int>(div_up(g.N, kBig));
+  const dim3 grid(static_cast<unsigned>(b.tiles_m) * b.tiles_n, static_cast<unsigned>(p.splits));
+  if (p.across_a)
+    k_big_gemm<true, BA, OT><<<grid, kBigThreads, 0, s>>>(b);
+  else
+    k_big_gemm<false, BA, OT><<<grid, kBigThreads, 0, s>>>(b);
+  if (p.splits > 1) launch_join(static_cast<int64_t>(g.M) * g.N, p.splits, b.part, static_cast<OT*>(g.out), s);
+}
+
+// How a product of two in 4 bits runs; `big` takes the scales in its order.
+struct Plan4 {
+  bool big;
+  int steps, splits;
+  int64_t bytes_a, bytes_b, bytes;
+};
+Plan4 plan4_of(int64_t m, int64_t n, int64_t k) {
+  Plan4 p{};
+  p.big = m >= kBigLeast && n >= kBigLeast && k >= kBigLeast && k <= 8 * kBigLine;
+  if (!p.big) return p;
+  p.steps = static_cast<int>(div_up(k, 256));
+  p.splits = big_splits(m, n, p.steps);
+  p.bytes_a = div_up(m, 128) * p.steps * 64 * 16, p.bytes_b = div_up(n, 64) * p.steps * 64 * 8;
+  p.bytes = p.bytes_a + p.bytes_b + (p.splits > 1 ? 4 * p.splits * m * n : 0);
+  return p;
 }
 
 template <typename T, int KIND, typename OT>
@@ -580,12 +735,15 @@ void launch_gemm(GemmArgs g, void* workspace, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(div_up(g.M, kTile) * g.tiles_n), static_cast<unsigned>(splits));
     k_mx_gemm<T, KIND, OT><<<grid, 256, 0, s>>>(g);
   }
-  if (splits > 1) {  // (then there are few tiles: one launch)
-    const int64_t n = all * g.N;
-    const int64_t groups = div_up(n, kBlock);
-    k_mx_join<OT><<<static_cast<unsigned>(groups < kMaxGroups ? groups : kMaxGroups), kBlock, 0, s>>>(n, splits, g.part,
-                                                                                                    out);
-  }
+  if (splits > 1) launch_join(all * g.N, splits, g.part, out, s);  // (then there are few tiles: one launch)
+}
+
+template <typename T, int KIND, typename OT>
+void launch_product(const GemmArgs& g, const Plan& p, void* workspace, hipStream_t s) {
+  if (p.big)
+    launch_big<T, KIND, OT>(g, p, static_cast<char*>(workspace), s);
+  else
+    launch_gemm<T, KIND, OT>(g, workspace, s);
 }
 
 }  // namespace
@@ -696,11 +854,15 @@ int plx_mx8_activate_grad(int64_t lines, int64_t n, int32_t dtype, int32_t fn, c
   return check_launch("plx_mx8_activate_grad");
 }
 
-int64_t plx_mx_workspace(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs) {
-  if (kind < PLX_LB_PRODUCT || kind > PLX_LB_WEIGHT_GRAD_COLUMNS || !dims_fit(tokens, inputs) ||
+int64_t plx_mx_workspace(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs, int32_t dtype, const void* a,
+                         int64_t token_stride, int64_t unit_stride) {
+  if (kind < PLX_LB_PRODUCT || kind > PLX_LB_WEIGHT_GRAD_COLUMNS || !known(dtype) || !dims_fit(tokens, inputs) ||
       !dims_fit(outputs, outputs))
     return -1;
-  return workspace_of(shape_of(kind, tokens, inputs, outputs));
+  const bool grad = kind >= PLX_LB_WEIGHT_GRAD;
+  return plan_of(kind, shape_of(kind, tokens, inputs, outputs), dtype, a, grad ? unit_stride : token_stride,
+                 grad ? token_stride : unit_stride)
+      .bytes;
 }
 
 int plx_mx_product(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs, int32_t dtype, const void* a,
@@ -714,31 +876,37 @@ int plx_mx_product(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs
   if (sh.m == 0 || sh.n == 0) return PLX_OK;
   if (!out || (sh.k > 0 && (!a || !codes || !scales))) return fail(PLX_ERR_INVALID, "plx_mx_product: null pointer");
   if (!on16(codes)) return fail(PLX_ERR_INVALID, "plx_mx_product: codes not on 16 bytes");
-  const int64_t need = workspace_of(sh);
-  if (need > 0 && (!workspace || workspace_bytes < need))
-    return fail(PLX_ERR_INVALID, "plx_mx_product: workspace smaller than plx_mx_workspace() says");
   GemmArgs g{};
   g.a = a, g.codes = codes, g.scales = scales, g.out = out;
   g.M = static_cast<int>(sh.m), g.N = static_cast<int>(sh.n), g.K = static_cast<int>(sh.k);
-  const bool grad = kind == PLX_LB_WEIGHT_GRAD || kind == PLX_LB_WEIGHT_GRAD_COLUMNS;
+  const bool grad = kind >= PLX_LB_WEIGHT_GRAD;
   g.sm = grad ? unit_stride : token_stride, g.sk = grad ? token_stride : unit_stride;
   g.wide = g.sk == 1 && rows_on16(a, g.sm, dtype);
   g.blocks = grad ? div_up(kind == PLX_LB_WEIGHT_GRAD ? inputs : tokens, 32) : div_up(inputs, 128) * 4;
+  const Plan p = plan_of(kind, sh, dtype, a, g.sm, g.sk);
+  if (p.bytes > 0 && (!workspace || !on16(workspace) || workspace_bytes < p.bytes))
+    return fail(PLX_ERR_INVALID, "plx_mx_product: plx_mx_workspace() bytes on 16 bytes needed");
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_type(dtype, [&](auto* t) {
     using T = PLX_TYPE(t);
     switch (kind) {
-      case PLX_LB_PRODUCT: launch_gemm<T, kW, T>(g, workspace, s); break;
-      case PLX_LB_PRODUCT_GRAD: launch_gemm<T, kWT, T>(g, workspace, s); break;
-      case PLX_LB_WEIGHT_GRAD: launch_gemm<T, kX, float>(g, workspace, s); break;
-      default: launch_gemm<T, kXT, float>(g, workspace, s); break;
+      case PLX_LB_PRODUCT: launch_product<T, kW, T>(g, p, workspace, s); break;
+      case PLX_LB_PRODUCT_GRAD: launch_product<T, kWT, T>(g, p, workspace, s); break;
+      case PLX_LB_WEIGHT_GRAD: launch_product<T, kX, float>(g, p, workspace, s); break;
+      default: launch_product<T, kXT, float>(g, p, workspace, s); break;
     }
   });
   return check_launch("plx_mx_product");
 }
 
+int64_t plx_mx4_workspace(int64_t tokens, int64_t inputs, int64_t outputs) {
+  if (!dims_fit(tokens, inputs) || !dims_fit(outputs, outputs)) return -1;
+  return plan4_of(tokens, outputs, inputs).bytes;
+}
+
 int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8_t* x_codes, const uint8_t* x_scales,
-                    const uint8_t* w_codes, const uint8_t* w_scales, int32_t dtype, void* out, void* stream) {
+                    const uint8_t* w_codes, const uint8_t* w_scales, int32_t dtype, void* out, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
   if (!dims_fit(tokens, inputs) || !dims_fit(outputs, outputs))
     return fail(PLX_ERR_INVALID, "plx_mx4_product: bad size");
   if (!known(dtype)) return fail(PLX_ERR_UNSUPPORTED, "plx_mx4_product: unknown element type");
@@ -746,7 +914,32 @@ int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8
   if (!out || (inputs > 0 && (!x_codes || !x_scales || !w_codes || !w_scales)))
     return fail(PLX_ERR_INVALID, "plx_mx4_product: null pointer");
   if (!on16(x_codes) || !on16(w_codes)) return fail(PLX_ERR_INVALID, "plx_mx4_product: codes not on 16 bytes");
+  const Plan4 p = plan4_of(tokens, outputs, inputs);
+  if (p.bytes > 0 && (!workspace || !on16(workspace) || workspace_bytes < p.bytes))
+    return fail(PLX_ERR_INVALID, "plx_mx4_product: plx_mx4_workspace() bytes on 16 bytes needed");
   const int64_t blocks = div_up(inputs, 128) * 4;
+  if (p.big) {
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    char* work = static_cast<char*>(workspace);
+    Big4Args g{};
+    g.a = reinterpret_cast<const char*>(x_codes), g.b = reinterpret_cast<const char*>(w_codes);
+    g.sa = reinterpret_cast<const uint4*>(work), g.sb = reinterpret_cast<const uint2*>(work + p.bytes_a);
+    g.out = out, g.part = reinterpret_cast<float*>(work + p.bytes_a + p.bytes_b);
+    g.M = static_cast<int>(tokens), g.N = static_cast<int>(outputs), g.line = blocks * 16;
+    g.steps = p.steps, g.split = static_cast<int>(div_up(p.steps, p.splits));
+    g.tiles_m = static_cast<int>(div_up(tokens, kBig)), g.tiles_n = static_cast<int>(div_up(outputs, kBig));
+    const int64_t groups = div_up(p.bytes_a / 16 + p.bytes_b / 8, 256);
+    k_big_scales<<<static_cast<unsigned>(groups < kMaxGroups ? groups : kMaxGroups), 256, 0, s>>>(
+        g.M, g.N, blocks, p.steps, x_scales, w_scales, reinterpret_cast<uint8_t*>(work),
+        reinterpret_cast<uint8_t*>(work + p.bytes_a));
+    with_type(dtype, [&](auto* t) {
+      using T = PLX_TYPE(t);
+      const dim3 grid(static_cast<unsigned>(g.tiles_m) * g.tiles_n, static_cast<unsigned>(p.splits));
+      k_big4_gemm<T><<<grid, kBigThreads, 0, s>>>(g);
+      if (p.splits > 1) launch_join(tokens * outputs, p.splits, g.part, static_cast<T*>(out), s);
+    });
+    return check_launch("plx_mx4_product");
+  }
   const int tiles_n = static_cast<int>(div_up(outputs, kTile));
   const int64_t rows = (kMaxGroups / tiles_n > 0 ? kMaxGroups / tiles_n : 1) * kTile;  // of one launch
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -25,6 +25,12 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ bf16x8 as_bf16x8(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
 
+__device__ __forceinline__ i32x8 as_i32x8(bf16x8 v) {  // (4-bit operands take the first half)
+  typedef int i32x4 __attribute__((ext_vector_type(4)));
+  const i32x4 w = __builtin_bit_cast(i32x4, v);
+  return i32x8{w[0], w[1], w[2], w[3], 0, 0, 0, 0};
+}
+
 // Element types of activations and gradients: float, __bf16, _Float16.
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
@@ -80,6 +86,22 @@ __device__ __forceinline__ void store8(T* p, int64_t stride, int n, bool wide, c
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (i < n) p[i * stride] = from_f32<T>(v[i]);
+}
+
+// Four consecutive results of a row of n, `left` of them inside it.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int n, int left, f32x4 v) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  if (left >= 4 && (n & 3) == 0) {  // (rows start on a multiple of 4)
+    t4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<t4*>(p) = r;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < left) p[i] = from_f32<T>(v[i]);
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }

@@ -194,12 +194,21 @@ def activate_grad(dy: torch.Tensor, kept: Mx8, fn: str) -> torch.Tensor:
     return dh
 
 
+def _workspace(device: torch.device, name: str, *args: object) -> tuple[torch.Tensor | None, int | None, int]:
+    """(the workspace that keeps the memory, its address, its bytes)."""
+    need = getattr(_lib.load(), name)(*args)
+    if need <= 0:
+        _lib.check(int(need < 0), name)
+        return None, None, 0
+    work = torch.empty(need, dtype=torch.uint8, device=device)
+    return work, work.data_ptr(), need
+
+
 def _product(kind: int, a: torch.Tensor, m: Mx4 | Mx8, inputs: int, outputs: int, out: torch.Tensor) -> torch.Tensor:
-    tokens, need = a.shape[0], _lib.load().plx_mx_workspace(kind, a.shape[0], inputs, outputs)
-    work = torch.empty(need, dtype=torch.uint8, device=a.device) if need > 0 else None
-    _launch(a.device, "plx_mx_product", kind, tokens, inputs, outputs, DTYPES[a.dtype], a.data_ptr(), a.stride(0),
-            a.stride(1), m.codes.data_ptr(), m.scales.data_ptr(), out.data_ptr(),
-            work.data_ptr() if work is not None else None, need)
+    of_a = DTYPES[a.dtype], a.data_ptr(), a.stride(0), a.stride(1)
+    _work, at, need = _workspace(a.device, "plx_mx_workspace", kind, a.shape[0], inputs, outputs, *of_a)
+    _launch(a.device, "plx_mx_product", kind, a.shape[0], inputs, outputs, *of_a, m.codes.data_ptr(),
+            m.scales.data_ptr(), out.data_ptr(), at, need)
     return out
 
 
@@ -218,8 +227,9 @@ def product(x: torch.Tensor | Mx4, w: Mx4, dtype: torch.dtype | None = None) -> 
             raise TypeError(f"product: float32, bfloat16 or float16 expected, got {dtype}")
         _on_gpu("product", x.device, w.device)
         out = torch.empty((x.shape[0], outputs), dtype=dtype, device=x.device)
+        _work, at, need = _workspace(x.device, "plx_mx4_workspace", x.shape[0], inputs, outputs)
         _launch(x.device, "plx_mx4_product", x.shape[0], inputs, outputs, x.codes.data_ptr(), x.scales.data_ptr(),
-                w.codes.data_ptr(), w.scales.data_ptr(), DTYPES[dtype], out.data_ptr())
+                w.codes.data_ptr(), w.scales.data_ptr(), DTYPES[dtype], out.data_ptr(), at, need)
         return out
     _check("product", x)
     if dtype is not None and dtype != x.dtype:

@@ -19,6 +19,7 @@ LINES = [(1, 1), (3, 31), (5, 32), (2, 33), (7, 127), (4, 128), (3, 129), (65, 1
 # tokens, inputs, outputs
 SHAPES = [(1, 1, 1), (1, 33, 17), (2, 128, 64), (3, 129, 65), (15, 31, 128), (16, 256, 777), (17, 1003, 33),
           (63, 64, 96), (64, 512, 130), (65, 1100, 63), (130, 1, 70), (300, 130, 1100), (513, 770, 520),
+          (256, 256, 256), (257, 1344, 300), (600, 576, 904), (264, 2049, 1030), (1100, 520, 512),
           (1, 4096, 1024), (33, 2048, 2049)]
 
 
