@@ -12,7 +12,6 @@
 #include "px_common.h"
 #include "px_lowbit.h"
 #include "px_lowbit_gemm.h"
-#include "px_math.h"
 
 using plx_detail::check_launch;
 using plx_detail::cu_count;
@@ -57,7 +56,7 @@ __device__ __forceinline__ uint32_t max4(uint32_t m) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(kBlock) void k_mx4_along(int64_t lines, int64_t n, const T* x, int64_t stride, bool wide,
+__global__ __launch_bounds__(kBlock) void k_mx4_along(int64_t lines, int64_t n, const T* x, int64_t stride,
                                                       uint8_t* codes, uint8_t* scales, int lx) {
   const int64_t chunks = div_up(n, 128) * 16;  // a multiple of lx's quads
   const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
@@ -68,7 +67,7 @@ __global__ __launch_bounds__(kBlock) void k_mx4_along(int64_t lines, int64_t n, 
     for (int64_t c = tx; c < chunks; c += lx) {
       const int64_t left = n - c * 8;
       float v[8];
-      load8(row + c * 8, 1, left > 8 ? 8 : left < 0 ? 0 : static_cast<int>(left), wide, v);
+      load8(row + c * 8, 1, left > 8 ? 8 : left < 0 ? 0 : static_cast<int>(left), v);
       uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = m > abs_bits(v[i]) ? m : abs_bits(v[i]);
@@ -113,7 +112,7 @@ __global__ __launch_bounds__(kBlock) void k_mx4_across(int64_t lines, int64_t n,
 // BITS 4 or 8: the values that codes stand for, lines of n next to each other.
 template <int BITS, typename T>
 __global__ __launch_bounds__(kBlock) void k_mx_values(int64_t lines, int64_t n, const uint8_t* codes,
-                                                      const uint8_t* scales, T* out, bool wide, int lx) {
+                                                      const uint8_t* scales, T* out, int lx) {
   const int64_t kept = BITS == 4 ? div_up(n, 128) * 16 : div_up(n, 32) * 4, chunks = div_up(n, 8);
   const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
   for (int64_t line = static_cast<int64_t>(blockIdx.x) * ly + ty; line < lines;
@@ -126,7 +125,7 @@ __global__ __launch_bounds__(kBlock) void k_mx_values(int64_t lines, int64_t n, 
         values4(reinterpret_cast<const uint32_t*>(codes)[line * kept + c], scale, v);
       else
         values8(reinterpret_cast<const uint2*>(codes)[line * kept + c], scale, v);
-      store8(out + line * n + c * 8, 1, left > 8 ? 8 : static_cast<int>(left), wide, v);
+      store8(out + line * n + c * 8, left > 8 ? 8 : static_cast<int>(left), v);
     }
   }
 }
@@ -134,23 +133,52 @@ __global__ __launch_bounds__(kBlock) void k_mx_values(int64_t lines, int64_t n, 
 // ---------------------------------------------------------------------------
 // Activations. y = fn(h) from h itself; fn'(q) from what was kept.
 // ---------------------------------------------------------------------------
+// exp(-a), a >= 0, to 2 steps: the hardware's 2^f (1 step) of the fraction of
+// -a log2(e), whose rounding error goes on as a factor 1 + r ln 2, and ldexp,
+// which rounds once below the normal numbers.
+__device__ __forceinline__ float exp_neg(float a) {
+  a = a > 150.0f ? 150.0f : a;  // (a NaN stays)
+  const float hi = a * -1.44269502162933349609375f;
+  float lo = __builtin_fmaf(a, -1.44269502162933349609375f, -hi);
+  lo = __builtin_fmaf(a, -1.925963033500011e-8f, lo);
+  const float n = __builtin_rintf(hi);
+  const float p = __builtin_amdgcn_exp2f(hi - n);
+  return __builtin_ldexpf(__builtin_fmaf(p * lo, 0.693147182464599609375f, p), static_cast<int>(n));
+}
+// 1 / d, 1 <= d <= 2: the hardware's (1 step) and one Newton step.
+__device__ __forceinline__ float inverse(float d) {
+  const float r = __builtin_amdgcn_rcpf(d);
+  return __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+}
+
+// By exp(-|h|), so that nothing overflows and the tails keep their values:
+// sigmoid = 1 / (1 + t) or t / (1 + t), tanh = (1 - u) / (1 + u) with
+// u = exp(-2|h|), and below 0.625 Cephes' polynomial, which has no
+// cancellation.
 template <int FN>
 __device__ __forceinline__ float act(float h) {
   if (FN == PLX_LB_RELU) return h <= 0.0f ? 0.0f : h;  // (a NaN passes)
-  if (FN == PLX_LB_TANH) return tanhf_(h);
-  const float t = expf_(-fabsf(h)), d = 1.0f + t;  // (nothing overflows, so the tails keep their values)
-  const float s = (h < 0.0f ? t : 1.0f) / d;
+  const float a = fabsf(h);
+  const float t = exp_neg(FN == PLX_LB_TANH ? 2.0f * a : a), r = inverse(1.0f + t);
+  if (FN == PLX_LB_TANH) {
+    const float y = h * h;
+    float p = -5.70498872745e-3f;
+    p = __builtin_fmaf(p, y, 2.06390887954e-2f);
+    p = __builtin_fmaf(p, y, -5.37397155531e-2f);
+    p = __builtin_fmaf(p, y, 1.33314422036e-1f);
+    p = __builtin_fmaf(p, y, -3.33332819422e-1f);
+    return a < 0.625f ? __builtin_fmaf(p * y, h, h) : __builtin_copysignf((1.0f - t) * r, h);
+  }
+  const float s = h < 0.0f ? t * r : r;
   return FN == PLX_LB_SIGMOID ? s : h * s;
 }
-// By exp(-|q|), so that nothing overflows: tanh' = 4u / (1 + u)^2 with
-// u = exp(-2|q|), sigmoid' = t / (1 + t)^2 with t = exp(-|q|), and
+// tanh' = 4u / (1 + u)^2, sigmoid' = t / (1 + t)^2 and
 // silu' = sigmoid(q) + q sigmoid'(q).
 template <int FN>
 __device__ __forceinline__ float act_grad(float q) {
   if (FN == PLX_LB_RELU) return q > 0.0f ? 1.0f : 0.0f;
   const float a = fabsf(q);
-  const float t = expf_(FN == PLX_LB_TANH ? -2.0f * a : -a);
-  const float r = 1.0f / (1.0f + t), d = t * r * r;
+  const float t = exp_neg(FN == PLX_LB_TANH ? 2.0f * a : a), r = inverse(1.0f + t), d = t * r * r;
   if (FN == PLX_LB_TANH) return 4.0f * d;
   if (FN == PLX_LB_SIGMOID) return d;
   return (q >= 0.0f ? r : t * r) + (t == 0.0f ? 0.0f : q * d);  // (an infinite q has the slope 0 or 1)
@@ -158,7 +186,7 @@ __device__ __forceinline__ float act_grad(float q) {
 
 template <int FN, typename T>
 __global__ __launch_bounds__(kBlock) void k_act_along(int64_t lines, int64_t n, const T* h, int64_t sh, T* y,
-                                                      int64_t sy, bool wide, uint8_t* codes, uint8_t* scales, int lx) {
+                                                      int64_t sy, uint8_t* codes, uint8_t* scales, int lx) {
   const int64_t chunks = div_up(n, 32) * 4;
   const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
   for (int64_t line = static_cast<int64_t>(blockIdx.x) * ly + ty; line < lines;
@@ -167,7 +195,7 @@ __global__ __launch_bounds__(kBlock) void k_act_along(int64_t lines, int64_t n, 
       const int64_t left64 = n - c * 8;
       const int left = left64 > 8 ? 8 : left64 < 0 ? 0 : static_cast<int>(left64);
       float v[8], f[8];
-      load8(h + line * sh + c * 8, 1, left, wide, v);
+      load8(h + line * sh + c * 8, 1, left, v);
       uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -175,7 +203,7 @@ __global__ __launch_bounds__(kBlock) void k_act_along(int64_t lines, int64_t n, 
         m = a < kInfBits && a > m ? a : m;
         f[i] = act<FN>(v[i]);
       }
-      store8(y + line * sy + c * 8, 1, left, wide, f);
+      store8(y + line * sy + c * 8, left, f);
       const int e = exponent8(max4(m));
       reinterpret_cast<uint2*>(codes)[line * chunks + c] = codes8(v, pow2(-e));
       if ((tx & 3) == 0) scales[line * (chunks / 4) + c / 4] = static_cast<uint8_t>(e + 127);
@@ -217,7 +245,7 @@ __global__ __launch_bounds__(kBlock) void k_act_across(int64_t lines, int64_t n,
 template <int FN, typename T>
 __global__ __launch_bounds__(kBlock) void k_grad_along(int64_t lines, int64_t n, const T* dy, int64_t sy,
                                                        const uint8_t* codes, const uint8_t* scales, T* dh, int64_t sh,
-                                                       bool wide, int lx) {
+                                                       int lx) {
   const int64_t kept = div_up(n, 32) * 4, chunks = div_up(n, 8);
   const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
   for (int64_t line = static_cast<int64_t>(blockIdx.x) * ly + ty; line < lines;
@@ -226,12 +254,12 @@ __global__ __launch_bounds__(kBlock) void k_grad_along(int64_t lines, int64_t n,
       const int64_t left64 = n - c * 8;
       const int left = left64 > 8 ? 8 : static_cast<int>(left64);
       float v[8], q[8];
-      load8(dy + line * sy + c * 8, 1, left, wide, v);
+      load8(dy + line * sy + c * 8, 1, left, v);
       values8(reinterpret_cast<const uint2*>(codes)[line * kept + c], scale_value(scales[line * (kept / 4) + c / 4]),
               q);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= act_grad<FN>(q[i]);
-      store8(dh + line * sh + c * 8, 1, left, wide, v);
+      store8(dh + line * sh + c * 8, left, v);
     }
   }
 }
@@ -278,7 +306,6 @@ enum { kW = 0, kWT = 1, kX = 2, kXT = 3 };
 struct GemmArgs {
   const void* a;
   int64_t sm, sk;
-  bool wide;
   const uint8_t* codes;
   const uint8_t* scales;
   int64_t blocks;  // blocks of a line of codes
@@ -287,163 +314,199 @@ struct GemmArgs {
   int M, N, K, kper, tiles_n;
 };
 
-constexpr int kTile = 64;
+__device__ __forceinline__ void unit_pieces(Unit<__bf16>::type v, uint4 out[1]) {
+  out[0] = __builtin_bit_cast(uint4, v);
+}
+template <typename T8, int P>
+__device__ __forceinline__ void unit_pieces(T8 v, uint4 (&out)[P]) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = to_f32(v[i]);
+  pieces8<P>(f, out);
+}
 
-// 64 x 64 of the output by four waves of 32 x 32, k in steps of 64: both
-// operands go through registers (converted to bf16 on the way) into LDS, the
-// next step's loads in flight during this step's matrix instructions. In LDS
-// a row is 64 k (8 chunks of 16 bytes), chunk c of row r at c ^ (r & 7): the
-// 16 rows of a fragment's read then fall on different banks.
-template <typename T, int KIND, typename OT>
-__global__ __launch_bounds__(256) void k_mx_gemm(GemmArgs g) {
+// The sums of a tile of TS x TS, a wave's quarter of its group's in acc (with b's
+// rows as the matrix instruction's first operand a lane holds four consecutive
+// n of one m): the groups' sums are added in order through LDS.
+template <int TS, int KS, typename OT>
+__device__ __forceinline__ void tile_store(const f32x4 (&acc)[TS / 32][TS / 32], void* lds, int group, int wm, int wn, int m0,
+                                           int n0, int M, int N, OT* out, float* parts) {
+  const int tid = threadIdx.x, l15 = tid & 15, q = (tid & 63) >> 4;
+  float* part = gridDim.y > 1 ? parts + static_cast<int64_t>(blockIdx.y) * M * N : nullptr;
+  auto store = [&](int m, int n, f32x4 v) {
+    if (m >= M || n >= N) return;
+    const int64_t at = static_cast<int64_t>(m) * N + n;
+    if (part)
+      store4(part + at, N - n, v);
+    else
+      store4(out + at, N - n, v);
+  };
+  constexpr int F = TS / 32, kRow = TS / 4, kTileSums = TS * kRow;
+  if (KS == 1) {
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+      for (int j = 0; j < F; ++j) store(m0 + wm + j * 16 + l15, n0 + wn + i * 16 + q * 4, acc[i][j]);
+    return;
+  }
+  __syncthreads();
+  f32x4* sums = static_cast<f32x4*>(lds);  // [group][m][TS / 4 of n], four n at c ^ (m & (TS / 4 - 1))
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+      const int m = wm + j * 16 + l15, c = (wn >> 2) + i * 4 + q;
+      sums[group * kTileSums + m * kRow + (c ^ (m & (kRow - 1)))] = acc[i][j];
+    }
+  __syncthreads();
+  for (int t = tid; t < kTileSums; t += 256 * KS) {
+    const int m = t / kRow, c = t % kRow;
+    f32x4 v = sums[m * kRow + (c ^ (m & (kRow - 1)))];
+#pragma unroll
+    for (int k = 1; k < KS; ++k) v += sums[k * kTileSums + m * kRow + (c ^ (m & (kRow - 1)))];
+    store(m0 + m, n0 + c * 4, v);
+  }
+}
+
+// TS x TS (64 or 32) of the output by KS groups of four waves, k in steps
+// of 64 KS, a group's share 64 of them: both operands go through registers
+// (as bf16 pieces) into LDS, the next step's loads in flight during this
+// step's matrix instructions, and the groups' sums are added in order at the
+// end. Threads load 8 consecutive values of a line. A line of k ("along") is
+// a row of LDS, 8 chunks of 16 bytes with chunk c of row r at c ^ (r & 7), so
+// that the rows of a fragment's read fall on different banks; lines of m or n
+// ("across") are rows too, pairs of chunks at p ^ (k & 3) (k & 1 of 32), and their
+// fragments are read transposed.
+template <typename T, int KIND, typename OT, int TS, int KS, bool AA>
+__global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
   constexpr int P = Pieces<T>::n;
-  __shared__ uint4 la[P][kTile * 8];
-  __shared__ uint4 lb[kTile * 8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int m0 = (blockIdx.x / g.tiles_n) * kTile, n0 = (blockIdx.x % g.tiles_n) * kTile;
+  constexpr bool BA = KIND == kWT || KIND == kX;
+  constexpr int BITS = KIND == kW || KIND == kWT ? 4 : 8;
+  constexpr int F = TS / 32, kLine = TS / 8;                // (fragments a wave and side; chunks of a line across)
+  constexpr int kStep = 64 * KS, kSub = TS * 8, kU = TS / 32;  // (16-byte chunks of TS x 64 values; units a thread)
+  constexpr int kUints = (P + 1) * KS * kSub, kSums = KS * TS * TS / 4;
+  __shared__ uint4 lds[KS > 1 && kUints < kSums ? kSums : kUints];
+  uint4* la = lds;
+  uint4* lb = lds + P * KS * kSub;
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2;
+  const int m0 = (blockIdx.x / g.tiles_n) * TS, n0 = (blockIdx.x % g.tiles_n) * TS;
   const int kbeg = blockIdx.y * g.kper, kend = kbeg + g.kper < g.K ? kbeg + g.kper : g.K;
   const T* a = static_cast<const T*>(g.a);
-  const bool along = g.sk == 1;
+  typedef typename Unit<T>::type unit;
 
-  float ra[2][8];
-  uint4 rb = make_uint4(0, 0, 0, 0);
-  uint2 rs = make_uint2(0, 0);
-
-  auto load = [&](int k0) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int u = tid + 256 * i;
-      const int row = along ? u >> 3 : u & 63, c = along ? u & 7 : u >> 6;
-      const int m = m0 + row, k = k0 + c * 8;
-      const int left = m < g.M ? (kend - k > 8 ? 8 : kend - k) : 0;
-      load8(a + m * g.sm + k * g.sk, g.sk, left, g.wide, ra[i]);
+  struct Regs {
+    unit a[kU];
+    uint2 b[kU];
+    uint32_t s[kU];
+  } r0, r1;
+  // The line and the chunk of this thread's i-th unit, and its place in LDS.
+  auto place = [&](bool across, int i, int* line, int* chunk) {
+    const int u = tid + 256 * KS * i;
+    if (across) {
+      *line = u / kLine, *chunk = u % kLine;
+      const int c = *chunk, k = *line;
+      return (k >> 6) * kSub + (k & 63) * kLine + ((((c >> 1) ^ (k & (kLine / 2 - 1))) << 1) | (c & 1));
     }
-    rb = make_uint4(0, 0, 0, 0), rs = make_uint2(0, 0);
-    if (KIND == kW || KIND == kXT) {
-      const int n = n0 + (tid >> 2), k = k0 + (tid & 3) * 16;
-      if (n < g.N && k < kend) {  // (a started block is whole in memory)
-        const int64_t b = n * g.blocks + k / 32;
-        if (KIND == kW) {
-          const uint2 c = *reinterpret_cast<const uint2*>(g.codes + b * 16 + (k & 16) / 2);
-          rb.x = c.x, rb.y = c.y;
-        } else {
-          rb = *reinterpret_cast<const uint4*>(g.codes + b * 32 + (k & 16));
-        }
-        rs.x = g.scales[b];
-      }
-    } else {
-      const int n = n0 + (tid & 31) * 2, k = k0 + (tid >> 5) * 8;
-      uint32_t c[8], s[8];
+    *line = u / (8 * KS), *chunk = u % (8 * KS);
+    return (*chunk >> 3) * kSub + *line * 8 + ((*chunk & 7) ^ (*line & 7));
+  };
+  auto load = [&](Regs& r, int k0) {
+    if (k0 >= kend) return;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        c[i] = s[i] = 0;
-        if (k + i < kend && n < g.N) {
-          const int64_t b = (k + i) * g.blocks + n / 32;
-          c[i] = KIND == kWT ? g.codes[b * 16 + (n & 31) / 2]
-                             : *reinterpret_cast<const uint16_t*>(g.codes + b * 32 + (n & 31));
-          s[i] = g.scales[b];
-        }
+    for (int i = 0; i < kU; ++i) {
+      int line, chunk;
+      place(AA, i, &line, &chunk);
+      const int m = m0 + (AA ? chunk * 8 : line), k = k0 + (AA ? line : chunk * 8);
+      const int room = AA ? g.M - m : kend - k;
+      const bool in = AA ? k < kend : m < g.M;
+      r.a[i] = load_unit(a + m * g.sm + k * g.sk, AA ? g.sm : g.sk, in ? room : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+      int line, chunk;
+      place(BA, i, &line, &chunk);
+      const int64_t l = BA ? k0 + line : n0 + line;
+      const int pos = (BA ? n0 : k0) + chunk * 8;
+      r.b[i] = make_uint2(0, 0), r.s[i] = 127;
+      if (l < (BA ? kend : g.N) && pos < g.blocks * 32) {
+        const int64_t at = l * g.blocks * 4 + pos / 8;
+        if (BITS == 4)
+          r.b[i].x = reinterpret_cast<const uint32_t*>(g.codes)[at];
+        else
+          r.b[i] = reinterpret_cast<const uint2*>(g.codes)[at];
+        r.s[i] = g.scales[l * g.blocks + pos / 32];
       }
-      if (KIND == kWT) {
-        rb.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-        rb.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
-      } else {
-        rb = make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
-      }
-      rs.x = s[0] | s[1] << 8 | s[2] << 16 | s[3] << 24;
-      rs.y = s[4] | s[5] << 8 | s[6] << 16 | s[7] << 24;
     }
   };
-  auto put = [&]() {
+  auto put = [&](const Regs& r) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int u = tid + 256 * i;
-      const int row = along ? u >> 3 : u & 63, c = along ? u & 7 : u >> 6;
+    for (int i = 0; i < kU; ++i) {
+      int line, chunk;
+      const int at = place(AA, i, &line, &chunk);
       uint4 p[P];
-      pieces8<P>(ra[i], p);
+      unit_pieces(r.a[i], p);
 #pragma unroll
-      for (int j = 0; j < P; ++j) la[j][row * 8 + (c ^ (row & 7))] = p[j];
+      for (int j = 0; j < P; ++j) la[j * KS * kSub + at] = p[j];
     }
-    if (KIND == kW || KIND == kXT) {
-      const int row = tid >> 2, c = (tid & 3) * 2;
-      const float scale = scale_value(rs.x);
-      uint4 lo, hi;
-      if (KIND == kW) {
-        lo = bf16_of4(rb.x, scale), hi = bf16_of4(rb.y, scale);
-      } else {
-        lo = bf16_of8(make_uint2(rb.x, rb.y), scale), hi = bf16_of8(make_uint2(rb.z, rb.w), scale);
-      }
-      lb[row * 8 + (c ^ (row & 7))] = lo;
-      lb[row * 8 + ((c + 1) ^ (row & 7))] = hi;
-    } else {
-      const int row = (tid & 31) * 2, c = tid >> 5;
-      const uint32_t r[4] = {rb.x, rb.y, rb.z, rb.w}, s[2] = {rs.x, rs.y};
-      float even[8], odd[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float scale = scale_value(s[i / 4] >> (8 * (i % 4)) & 255u);
-        f32x2 v;
-        if (KIND == kWT) {
-          v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r[i / 4] >> (8 * (i % 4)), scale, 0);
-        } else {
-          v = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(r[i / 2] >> (16 * (i % 2))), false);
-          v[0] *= scale, v[1] *= scale;
-        }
-        even[i] = v[0], odd[i] = v[1];
-      }
-      uint4 p[1];
-      pieces8<1>(even, p);
-      lb[row * 8 + (c ^ (row & 7))] = p[0];
-      pieces8<1>(odd, p);
-      lb[(row + 1) * 8 + (c ^ ((row + 1) & 7))] = p[0];
+    for (int i = 0; i < kU; ++i) {
+      int line, chunk;
+      const int at = place(BA, i, &line, &chunk);
+      const float scale = scale_value(r.s[i]);
+      lb[at] = BITS == 4 ? bf16_of4(r.b[i].x, scale) : bf16_of8(r.b[i], scale);
     }
   };
+  auto frag = [&](const uint4* t, bool across, int row, int s) {
+    if (across) {
+      typedef __attribute__((address_space(3))) s16x4* p4;
+      const int k = s * 32 + q * 8 + (l15 >> 2);
+      const char* p = reinterpret_cast<const char*>(t) + k * kLine * 16 +
+                      (((row >> 4) ^ ((l15 >> 2) & (kLine / 2 - 1))) << 5) + (l15 & 3) * 8;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(p + 4 * kLine * 16));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    const int r = row + l15;
+    return as_bf16x8(t[r * 8 + ((s * 4 + q) ^ (r & 7))]);
+  };
 
-  f32x4 acc[2][2] = {};
-  const int wn = (wave & 1) * 32, wm = (wave >> 1) * 32, l15 = lane & 15, q = lane >> 4;
-  if (kbeg < kend) load(kbeg);
-  for (int k0 = kbeg; k0 < kend; k0 += 64) {
-    __syncthreads();
-    put();
-    __syncthreads();
-    if (k0 + 64 < kend) load(k0 + 64);
+  f32x4 acc[F][F] = {};
+  const int wn = (wave & 1) * (TS / 2), wm = ((wave >> 1) & 1) * (TS / 2);
+  auto compute = [&]() {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      bf16x8 fb[2], fa[2][P];
+      bf16x8 fb[F], fa[F][P];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int rn = wn + i * 16 + l15, rm = wm + i * 16 + l15, c = s * 4 + q;
-        fb[i] = as_bf16x8(lb[rn * 8 + (c ^ (rn & 7))]);
+      for (int i = 0; i < F; ++i) {
+        fb[i] = frag(lb + group * kSub, BA, wn + i * 16, s);
 #pragma unroll
-        for (int p = 0; p < P; ++p) fa[i][p] = as_bf16x8(la[p][rm * 8 + (c ^ (rm & 7))]);
+        for (int p = 0; p < P; ++p) fa[i][p] = frag(la + (p * KS + group) * kSub, AA, wm + i * 16, s);
       }
 #pragma unroll
       for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < F; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < F; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa[j][p], acc[i][j], 0, 0, 0);
     }
+  };
+  // Two steps' loads in flight: a step is shorter than a load's way.
+  auto step = [&](Regs& r, int k0) {
+    __syncthreads();
+    put(r);
+    __syncthreads();
+    load(r, k0 + 2 * kStep);
+    compute();
+  };
+  load(r0, kbeg);
+  load(r1, kbeg + kStep);
+  for (int k0 = kbeg; k0 < kend; k0 += 2 * kStep) {
+    step(r0, k0);
+    if (k0 + kStep < kend) step(r1, k0 + kStep);
   }
-  // With b's rows as the instruction's first operand a lane holds four
-  // consecutive n of one m.
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int m = m0 + wm + j * 16 + l15, n = n0 + wn + i * 16 + q * 4;
-      if (m >= g.M) continue;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (n + r >= g.N) break;
-        const int64_t at = static_cast<int64_t>(m) * g.N + n + r;
-        if (gridDim.y > 1)
-          g.part[static_cast<int64_t>(blockIdx.y) * g.M * g.N + at] = acc[i][j][r];
-        else
-          static_cast<OT*>(g.out)[at] = from_f32<OT>(acc[i][j][r]);
-      }
-    }
+  tile_store<TS, KS, OT>(acc, lds, group, wm, wn, m0, n0, g.M, g.N, static_cast<OT*>(g.out), g.part);
 }
 
 // out = the partial sums of the k ranges, in their order.
@@ -457,47 +520,164 @@ __global__ __launch_bounds__(kBlock) void k_mx_join(int64_t n, int splits, const
   }
 }
 
-// 4-bit times 4-bit blocks: the scaled matrix instruction takes 128 k of both
-// operands as they are kept, one block and its scale byte per lane.
-template <typename OT>
-__global__ __launch_bounds__(256) void k_mx4_gemm(int M, int N, int64_t blocks, const uint8_t* xc, const uint8_t* xs,
-                                                  const uint8_t* wc, const uint8_t* ws, OT* out, int tiles_n) {
+// y = x w^T of up to 16 tokens: 16 rows of w by the waves of a workgroup, each
+// with every kFewWaves-th group of 4 blocks; a lane takes a block and its 32
+// inputs of one token, straight into the matrix instruction, and the waves'
+// sums are added in order. Weights are read once, so what counts is how many
+// loads are in flight.
+constexpr int kFew = 16;
+template <bool ALONG>
+constexpr int kFewWaves = ALONG ? 16 : 8;
+// The unit of p[0..left), left < 8, of a row of 8 or more: the row's last
+// eight values moved down.
+template <typename T>
+__device__ __forceinline__ typename Unit<T>::type load_tail(const T* p, int left) {
+  typename Unit<T>::type r = load_unit(p - (8 - left), 1, 8), z = {};
+  const int by = 8 - left;
+  if (by & 4) r = __builtin_shufflevector(r, z, 4, 5, 6, 7, 8, 8, 8, 8);
+  if (by & 2) r = __builtin_shufflevector(r, z, 2, 3, 4, 5, 6, 7, 8, 8);
+  if (by & 1) r = __builtin_shufflevector(r, z, 1, 2, 3, 4, 5, 6, 7, 8);
+  return r;
+}
+// ALONG: inputs next to each other, 8 of them or more.
+template <typename T, bool ALONG>
+__global__ __launch_bounds__(64 * kFewWaves<ALONG>) void k_mx_few(GemmArgs g) {
+  constexpr int W = kFewWaves<ALONG>, P = Pieces<T>::n, kAhead = ALONG ? 2 : 1;
+  __shared__ f32x4 sums[W][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, q = lane >> 4;
-  const int m0 = (blockIdx.x / tiles_n) * kTile + (wave >> 1) * 32;
-  const int n0 = (blockIdx.x % tiles_n) * kTile + (wave & 1) * 32;
-  f32x4 acc[2][2] = {};
-  int64_t rm[2], rn[2];
+  const int n = blockIdx.x * 16 + l15;
+  const T* x = static_cast<const T*>(g.a) + l15 * g.sm;
+  const uint4* codes = reinterpret_cast<const uint4*>(g.codes) + n * g.blocks;
+  const uint8_t* scales = g.scales + n * g.blocks;
+  const int blocks = static_cast<int>(g.blocks);
+  f32x4 acc = {};
+  for (int b0 = wave * 4 + q; b0 - q < blocks; b0 += kAhead * W * 4) {
+    uint4 c[kAhead];
+    uint32_t s[kAhead];
+    typename Unit<T>::type v[kAhead][4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {  // (rows past the end read the last one; their results are not written)
-    const int m = m0 + i * 16 + l15, n = n0 + i * 16 + l15;
-    rm[i] = (m < M ? m : M - 1) * blocks, rn[i] = (n < N ? n : N - 1) * blocks;
-  }
-  for (int64_t b = q; b < blocks; b += 4) {
-    i32x8 fx[2], fw[2];
-    int sx[2], sw[2];
+    for (int i = 0; i < kAhead; ++i) {
+      const int b = b0 + i * W * 4;
+      c[i] = make_uint4(0, 0, 0, 0), s[i] = 127;
+      if (b < blocks && n < g.N) c[i] = codes[b], s[i] = scales[b];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 cx = reinterpret_cast<const uint4*>(xc)[rm[i] + b], cw = reinterpret_cast<const uint4*>(wc)[rn[i] + b];
-      fx[i] = i32x8{static_cast<int>(cx.x), static_cast<int>(cx.y), static_cast<int>(cx.z), static_cast<int>(cx.w)};
-      fw[i] = i32x8{static_cast<int>(cw.x), static_cast<int>(cw.y), static_cast<int>(cw.z), static_cast<int>(cw.w)};
-      sx[i] = xs[rm[i] + b], sw[i] = ws[rn[i] + b];
+      for (int j = 0; j < 4; ++j) {
+        const int64_t k = int64_t{b} * 32 + j * 8;
+        const int64_t left = l15 < g.M ? g.K - k : 0;
+        if (ALONG) {
+          v[i][j] = typename Unit<T>::type{};
+          if (left >= 8)
+            v[i][j] = load_unit(x + k, 1, 8);
+          else if (left > 0)
+            v[i][j] = load_tail(x + k, static_cast<int>(left));
+        } else {
+          v[i][j] = load_unit(x + k * g.sk, g.sk, left > 8 ? 8 : static_cast<int>(left));
+        }
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kAhead; ++i) {
+      const float scale = scale_value(s[i]);
+      const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[i], fx[j], acc[i][j], 4, 4, 0, sw[i], 0, sx[j]);
-  }
+      for (int j = 0; j < 4; ++j) {
+        uint4 p[P];
+        unit_pieces(v[i][j], p);
+        const bf16x8 fw = as_bf16x8(bf16_of4(w[j], scale));
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int m = m0 + j * 16 + l15, n = n0 + i * 16 + q * 4;
-      if (m >= M) continue;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (n + r < N) out[static_cast<int64_t>(m) * N + n + r] = from_f32<OT>(acc[i][j][r]);
+        for (int h = P - 1; h >= 0; --h) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, as_bf16x8(p[h]), acc, 0, 0, 0);
+      }
     }
+  }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0 || l15 >= g.M) return;
+#pragma unroll
+  for (int w = 1; w < W; ++w) acc += sums[w][lane];
+  const int at = blockIdx.x * 16 + q * 4;
+  if (at < g.N) store4(static_cast<T*>(g.out) + static_cast<int64_t>(l15) * g.N + at, g.N - at, acc);
+}
+
+// 4-bit times 4-bit blocks: the scaled matrix instruction takes 128 k of both
+// operands as they are kept, a block and its scale byte per lane. Tiles, groups
+// and LDS as in k_mx_gemm, a chunk of 16 bytes being one block here: a step is
+// 256 k a group.
+template <typename OT, int TS, int KS>
+__global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks, const uint8_t* xc, const uint8_t* xs,
+                                                       const uint8_t* wc, const uint8_t* ws, OT* out, float* parts,
+                                                       int tiles_n, int per) {
+  constexpr int F = TS / 32, kSub = TS * 8, kStep = 8 * KS;  // blocks of a step
+  constexpr int kUints = 2 * KS * kSub, kSums = KS * TS * TS / 4;
+  __shared__ uint4 lds[KS > 1 && kUints < kSums ? kSums : kUints];
+  __shared__ uint8_t lss[2 * KS * kSub];
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2;
+  const int m0 = (blockIdx.x / tiles_n) * TS, n0 = (blockIdx.x % tiles_n) * TS;
+  const int beg = blockIdx.y * per, end = beg + per < blocks ? beg + per : blocks;
+  struct Regs {
+    uint4 c[2 * F];
+    uint32_t s[2 * F];
+  } r0, r1;
+  auto load = [&](Regs& r, int b0) {
+    if (b0 >= end) return;
+#pragma unroll
+    for (int i = 0; i < 2 * F; ++i) {  // x's, then w's
+      const int u = tid + 256 * KS * (i % F), line = u / kStep, b = b0 + u % kStep;
+      const int row = (i < F ? m0 : n0) + line;
+      r.c[i] = make_uint4(0, 0, 0, 0), r.s[i] = 127;
+      if (row < (i < F ? M : N) && b < end) {
+        const int64_t at = static_cast<int64_t>(row) * blocks + b;
+        r.c[i] = reinterpret_cast<const uint4*>(i < F ? xc : wc)[at];
+        r.s[i] = (i < F ? xs : ws)[at];
+      }
+    }
+  };
+  auto put = [&](const Regs& r) {
+#pragma unroll
+    for (int i = 0; i < 2 * F; ++i) {
+      const int u = tid + 256 * KS * (i % F), line = u / kStep, b = u % kStep;
+      const int at = ((i < F ? 0 : KS) + (b >> 3)) * kSub + line * 8 + ((b & 7) ^ (line & 7));
+      lds[at] = r.c[i];
+      lss[at] = static_cast<uint8_t>(r.s[i]);
+    }
+  };
+  f32x4 acc[F][F] = {};
+  const int wn = (wave & 1) * (TS / 2), wm = ((wave >> 1) & 1) * (TS / 2);
+  auto compute = [&]() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      i32x8 fx[F], fw[F];
+      int sx[F], sw[F];
+#pragma unroll
+      for (int i = 0; i < F; ++i) {
+        const int rm = wm + i * 16 + l15, rn = wn + i * 16 + l15;
+        const int am = group * kSub + rm * 8 + ((h * 4 + q) ^ (rm & 7));
+        const int an = (KS + group) * kSub + rn * 8 + ((h * 4 + q) ^ (rn & 7));
+        fx[i] = as_i32x8(as_bf16x8(lds[am])), sx[i] = lss[am];
+        fw[i] = as_i32x8(as_bf16x8(lds[an])), sw[i] = lss[an];
+      }
+#pragma unroll
+      for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j)
+          acc[i][j] =
+              __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[i], fx[j], acc[i][j], 4, 4, 0, sw[i], 0, sx[j]);
+    }
+  };
+  auto step = [&](Regs& r, int b0) {
+    __syncthreads();
+    put(r);
+    __syncthreads();
+    load(r, b0 + 2 * kStep);
+    compute();
+  };
+  load(r0, beg);
+  load(r1, beg + kStep);
+  for (int b0 = beg; b0 < end; b0 += 2 * kStep) {
+    step(r0, b0);
+    if (b0 + kStep < end) step(r1, b0 + kStep);
+  }
+  tile_store<TS, KS, OT>(acc, lds, group, wm, wn, m0, n0, M, N, out, parts);
 }
 
 // ---------------------------------------------------------------------------
@@ -506,7 +686,7 @@ __global__ __launch_bounds__(256) void k_mx4_gemm(int M, int N, int64_t blocks, 
 // Piece p of line l at out + p * piece + l * out_line.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_big_pieces(int64_t lines, int64_t n, const T* x, int64_t sl, int64_t se,
-                                                       bool wide, uint16_t* out, int64_t out_lines, int64_t out_n,
+                                                       uint16_t* out, int64_t out_lines, int64_t out_n,
                                                        int64_t out_line, int64_t piece, int lx) {
   constexpr int P = Pieces<T>::n;
   const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
@@ -515,7 +695,7 @@ __global__ __launch_bounds__(kBlock) void k_big_pieces(int64_t lines, int64_t n,
     for (int64_t c = tx; c < out_n / 8; c += lx) {
       const int64_t left = line < lines ? n - c * 8 : 0;
       float v[8];
-      load8(x + line * sl + c * 8 * se, se, left > 8 ? 8 : left < 0 ? 0 : static_cast<int>(left), wide, v);
+      load8(x + line * sl + c * 8 * se, se, left > 8 ? 8 : left < 0 ? 0 : static_cast<int>(left), v);
       uint4 p[P];
       pieces8<P>(v, p);
 #pragma unroll
@@ -548,15 +728,10 @@ __global__ __launch_bounds__(kBlock) void k_big_values(int64_t lines, int64_t n,
 // Host side
 // ---------------------------------------------------------------------------
 constexpr int64_t kMaxDim = int64_t{1} << 30;
-constexpr int64_t kBigLeast = 256;              // m, n and k of a large product
 constexpr int64_t kBigLine = int64_t{1} << 22;  // elements of its lines: 256 of them stay below 2^32 bytes
 
 inline bool dims_fit(int64_t a, int64_t b) { return a >= 0 && b >= 0 && a <= kMaxDim && b <= kMaxDim; }
-inline int size_of(int dtype) { return dtype == PLX_LB_F32 ? 4 : 2; }
 inline bool known(int dtype) { return dtype == PLX_LB_F32 || dtype == PLX_LB_BF16 || dtype == PLX_LB_F16; }
-
-// Rows of this stride can be read 16 bytes at a time.
-inline bool rows_on16(const void* p, int64_t stride, int dtype) { return on16(p) && (stride * size_of(dtype)) % 16 == 0; }
 
 template <typename F>
 void with_type(int dtype, F f) {
@@ -585,14 +760,43 @@ inline unsigned groups_across(int64_t lines, int64_t blocks) {
   return static_cast<unsigned>(g < kMaxGroups ? g : kMaxGroups);
 }
 
-// The k ranges of a product: enough workgroups for two per CU, each range
-// four steps of 64 at least.
-int splits_of(int64_t m, int64_t n, int64_t k) {
-  const int64_t tiles = div_up(m, kTile) * div_up(n, kTile);
-  int64_t s = 2 * cu_count() / (tiles > 0 ? tiles : 1);
-  const int64_t most = div_up(k, 256);
-  s = s < most ? s : most;
-  return static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
+// A large product: 256 x 256 tiles have enough rows, columns and k, and the
+// operands' way through memory pays.
+constexpr double kBigLeast = 10e9;
+inline bool large(int64_t m, int64_t n, int64_t k) {
+  return m >= 256 && n >= 256 && k >= 256 && static_cast<double>(m) * n * k >= kBigLeast;
+}
+
+// How a product in small tiles runs: tiles of ts x ts, ks groups of waves in a
+// workgroup, each with `share` of k in a step, and ranges of k over workgroups.
+struct Tiles {
+  int ts, ks, splits, kper;
+};
+Tiles tiles_of(int64_t m, int64_t n, int64_t k, int64_t share) {
+  Tiles t{};
+  t.ts = 2 * div_up(m, 64) * div_up(n, 64) <= cu_count() && k <= 16 * share ? 32 : 64;
+  const int64_t tiles = div_up(m, t.ts) * div_up(n, t.ts);
+  t.ks = tiles >= 4 * cu_count() || k <= share ? 1 : 4;
+  const int64_t steps = div_up(k, share * t.ks);
+  int64_t s = cu_count() / (tiles > 0 ? tiles : 1);
+  s = s < steps / 4 ? s : steps / 4;
+  s = s < 1 ? 1 : s;
+  t.kper = static_cast<int>(div_up(steps, s) * share * t.ks);
+  t.splits = steps > 0 ? static_cast<int>(div_up(k, t.kper)) : 1;
+  return t;
+}
+
+template <typename F>
+void with_tiles(const Tiles& t, F f) {
+  using std::integral_constant;
+  if (t.ts == 64 && t.ks == 4)
+    f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  else if (t.ts == 64)
+    f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (t.ks == 4)
+    f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+  else
+    f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
 }
 
 // m, n, k and the kind of b of PLX_LB_* products.
@@ -630,9 +834,10 @@ int big_splits(int64_t m, int64_t n, int64_t steps) {
 Plan plan_of(int kind, const Shape& s, int dtype, const void* a, int64_t sm, int64_t sk) {
   Plan p{};
   const int pieces = dtype == PLX_LB_F32 ? 3 : dtype == PLX_LB_F16 ? 2 : 1;
-  p.big = s.m >= kBigLeast && s.n >= kBigLeast && s.k >= kBigLeast;
+  p.big = large(s.m, s.n, s.k * pieces);
   if (!p.big) {
-    p.splits = splits_of(s.m, s.n, s.k);
+    if (kind == PLX_LB_PRODUCT && s.m <= kFew) return p;
+    p.splits = tiles_of(s.m, s.n, s.k, 64).splits;
     p.bytes = p.splits > 1 ? int64_t{4} * p.splits * s.m * s.n : 0;
     return p;
   }
@@ -672,8 +877,7 @@ void launch_big(const GemmArgs& g, const Plan& p, char* work, hipStream_t s) {
     const int64_t out_lines = p.across_a ? p.kp : g.M, out_n = p.across_a ? p.mp : p.kp;
     const int64_t out_line = p.across_a ? p.mp : P * p.kp, piece = p.across_a ? p.kp * p.mp : p.kp;
     const int lx = lanes_along(out_n / 8);
-    const bool wide = se == 1 && on16(g.a) && (sl * sizeof(T)) % 16 == 0;
-    k_big_pieces<T><<<groups_along(out_lines, lx), kBlock, 0, s>>>(lines, n, static_cast<const T*>(g.a), sl, se, wide,
+    k_big_pieces<T><<<groups_along(out_lines, lx), kBlock, 0, s>>>(lines, n, static_cast<const T*>(g.a), sl, se,
                                                                    out, out_lines, out_n, out_line, piece, lx);
     b.a = work;
     b.lda = 2 * out_line;
@@ -709,8 +913,12 @@ struct Plan4 {
 };
 Plan4 plan4_of(int64_t m, int64_t n, int64_t k) {
   Plan4 p{};
-  p.big = m >= kBigLeast && n >= kBigLeast && k >= kBigLeast && k <= 8 * kBigLine;
-  if (!p.big) return p;
+  p.big = large(m, n, k) && k <= 8 * kBigLine;
+  if (!p.big) {
+    p.splits = tiles_of(m, n, k, 256).splits;
+    p.bytes = p.splits > 1 ? 4 * p.splits * m * n : 0;
+    return p;
+  }
   p.steps = static_cast<int>(div_up(k, 256));
   p.splits = big_splits(m, n, p.steps);
   p.bytes_a = div_up(m, 128) * p.steps * 64 * 16, p.bytes_b = div_up(n, 64) * p.steps * 64 * 8;
@@ -720,28 +928,40 @@ Plan4 plan4_of(int64_t m, int64_t n, int64_t k) {
 
 template <typename T, int KIND, typename OT>
 void launch_gemm(GemmArgs g, void* workspace, hipStream_t s) {
-  const int splits = splits_of(g.M, g.N, g.K);
-  g.kper = static_cast<int>(div_up(div_up(g.K, splits), 64) * 64);
-  g.tiles_n = static_cast<int>(div_up(g.N, kTile));
+  const Tiles t = tiles_of(g.M, g.N, g.K, 64);
+  const bool across = g.sm == 1 && g.sk != 1;
+  g.kper = t.kper;
+  g.tiles_n = static_cast<int>(div_up(g.N, t.ts));
   g.part = static_cast<float*>(workspace);
-  const int64_t rows = (kMaxGroups / g.tiles_n > 0 ? kMaxGroups / g.tiles_n : 1) * kTile;  // of one launch
+  const int64_t groups = kMaxGroups / (4 * t.splits);
+  const int64_t rows = (groups / g.tiles_n > 0 ? groups / g.tiles_n : 1) * t.ts;  // of one launch
   const T* a = static_cast<const T*>(g.a);
   OT* out = static_cast<OT*>(g.out);
   const int64_t all = g.M;
-  for (int64_t m = 0; m < all; m += rows) {
+  for (int64_t m = 0; m < all; m += rows) {  // (more than one launch only without splits)
     g.M = static_cast<int>(all - m < rows ? all - m : rows);
     g.a = a + m * g.sm;
     g.out = out + m * g.N;
-    const dim3 grid(static_cast<unsigned>(div_up(g.M, kTile) * g.tiles_n), static_cast<unsigned>(splits));
-    k_mx_gemm<T, KIND, OT><<<grid, 256, 0, s>>>(g);
+    const dim3 grid(static_cast<unsigned>(div_up(g.M, t.ts) * g.tiles_n), static_cast<unsigned>(t.splits));
+    with_tiles(t, [&](auto ts, auto ks) {
+      constexpr int TS = decltype(ts)::value, KS = decltype(ks)::value;
+      if (across)
+        k_mx_gemm<T, KIND, OT, TS, KS, true><<<grid, 256 * KS, 0, s>>>(g);
+      else
+        k_mx_gemm<T, KIND, OT, TS, KS, false><<<grid, 256 * KS, 0, s>>>(g);
+    });
   }
-  if (splits > 1) launch_join(all * g.N, splits, g.part, out, s);  // (then there are few tiles: one launch)
+  if (t.splits > 1) launch_join(all * g.N, t.splits, g.part, out, s);
 }
 
 template <typename T, int KIND, typename OT>
 void launch_product(const GemmArgs& g, const Plan& p, void* workspace, hipStream_t s) {
   if (p.big)
     launch_big<T, KIND, OT>(g, p, static_cast<char*>(workspace), s);
+  else if (KIND == kW && g.M <= kFew && g.sk == 1 && g.K >= 8)
+    k_mx_few<T, true><<<static_cast<unsigned>(div_up(g.N, 16)), 64 * kFewWaves<true>, 0, s>>>(g);
+  else if (KIND == kW && g.M <= kFew)
+    k_mx_few<T, false><<<static_cast<unsigned>(div_up(g.N, 16)), 64 * kFewWaves<false>, 0, s>>>(g);
   else
     launch_gemm<T, KIND, OT>(g, workspace, s);
 }
@@ -763,8 +983,7 @@ int plx_mx4_quantise(int64_t lines, int64_t n, int32_t dtype, const void* x, int
     const T* p = static_cast<const T*>(x);
     if (stride == 1) {
       const int lx = lanes_along(div_up(n, 128) * 16);
-      k_mx4_along<T><<<groups_along(lines, lx), kBlock, 0, s>>>(lines, n, p, line_stride,
-                                                                rows_on16(x, line_stride, dtype), codes, scales, lx);
+      k_mx4_along<T><<<groups_along(lines, lx), kBlock, 0, s>>>(lines, n, p, line_stride, codes, scales, lx);
     } else {
       k_mx4_across<T><<<groups_across(lines, div_up(n, 128) * 4), kBlock, 0, s>>>(lines, n, p, line_stride, stride,
                                                                                  codes, scales);
@@ -785,12 +1004,11 @@ int plx_mx_values(int32_t bits, int64_t lines, int64_t n, const uint8_t* codes, 
   const int lx = lanes_along(div_up(n, 8));
   with_type(dtype, [&](auto* t) {
     using T = PLX_TYPE(t);
-    const bool wide = rows_on16(out, n, dtype);
     if (bits == 4)
-      k_mx_values<4, T><<<groups_along(lines, lx), kBlock, 0, s>>>(lines, n, codes, scales, static_cast<T*>(out), wide,
+      k_mx_values<4, T><<<groups_along(lines, lx), kBlock, 0, s>>>(lines, n, codes, scales, static_cast<T*>(out),
                                                                    lx);
     else
-      k_mx_values<8, T><<<groups_along(lines, lx), kBlock, 0, s>>>(lines, n, codes, scales, static_cast<T*>(out), wide,
+      k_mx_values<8, T><<<groups_along(lines, lx), kBlock, 0, s>>>(lines, n, codes, scales, static_cast<T*>(out),
                                                                    lx);
   });
   return check_launch("plx_mx_values");
@@ -811,9 +1029,8 @@ int plx_mx8_activate(int64_t lines, int64_t n, int32_t dtype, int32_t fn, const 
       constexpr int FN = decltype(f)::value;
       if (h_elem == 1 && y_elem == 1) {
         const int lx = lanes_along(div_up(n, 32) * 4);
-        const bool wide = rows_on16(h, h_line, dtype) && rows_on16(y, y_line, dtype);
         k_act_along<FN, T><<<groups_along(lines, lx), kBlock, 0, s>>>(lines, n, static_cast<const T*>(h), h_line,
-                                                                      static_cast<T*>(y), y_line, wide, codes, scales,
+                                                                      static_cast<T*>(y), y_line, codes, scales,
                                                                       lx);
       } else {
         k_act_across<FN, T><<<groups_across(lines, div_up(n, 32)), kBlock, 0, s>>>(
@@ -841,9 +1058,8 @@ int plx_mx8_activate_grad(int64_t lines, int64_t n, int32_t dtype, int32_t fn, c
       constexpr int FN = decltype(f)::value;
       if (y_elem == 1 && h_elem == 1) {
         const int lx = lanes_along(div_up(n, 8));
-        const bool wide = rows_on16(dy, y_line, dtype) && rows_on16(dh, h_line, dtype);
         k_grad_along<FN, T><<<groups_along(lines, lx), kBlock, 0, s>>>(lines, n, static_cast<const T*>(dy), y_line,
-                                                                       codes, scales, static_cast<T*>(dh), h_line, wide,
+                                                                       codes, scales, static_cast<T*>(dh), h_line,
                                                                        lx);
       } else {
         k_grad_across<FN, T><<<groups_across(lines, div_up(n, 32)), kBlock, 0, s>>>(
@@ -881,7 +1097,6 @@ int plx_mx_product(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs
   g.M = static_cast<int>(sh.m), g.N = static_cast<int>(sh.n), g.K = static_cast<int>(sh.k);
   const bool grad = kind >= PLX_LB_WEIGHT_GRAD;
   g.sm = grad ? unit_stride : token_stride, g.sk = grad ? token_stride : unit_stride;
-  g.wide = g.sk == 1 && rows_on16(a, g.sm, dtype);
   g.blocks = grad ? div_up(kind == PLX_LB_WEIGHT_GRAD ? inputs : tokens, 32) : div_up(inputs, 128) * 4;
   const Plan p = plan_of(kind, sh, dtype, a, g.sm, g.sk);
   if (p.bytes > 0 && (!workspace || !on16(workspace) || workspace_bytes < p.bytes))
@@ -940,17 +1155,26 @@ int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8
     });
     return check_launch("plx_mx4_product");
   }
-  const int tiles_n = static_cast<int>(div_up(outputs, kTile));
-  const int64_t rows = (kMaxGroups / tiles_n > 0 ? kMaxGroups / tiles_n : 1) * kTile;  // of one launch
+  const Tiles t = tiles_of(tokens, outputs, inputs, 256);
+  const int tiles_n = static_cast<int>(div_up(outputs, t.ts));
+  const int64_t groups = kMaxGroups / (4 * t.splits);
+  const int64_t rows = (groups / tiles_n > 0 ? groups / tiles_n : 1) * t.ts;  // of one launch
   hipStream_t s = static_cast<hipStream_t>(stream);
-  with_type(dtype, [&](auto* t) {
-    using T = PLX_TYPE(t);
-    for (int64_t m = 0; m < tokens; m += rows) {
+  with_type(dtype, [&](auto* e) {
+    using T = PLX_TYPE(e);
+    for (int64_t m = 0; m < tokens; m += rows) {  // (more than one launch only without splits)
       const int64_t now = tokens - m < rows ? tokens - m : rows;
-      k_mx4_gemm<T><<<static_cast<unsigned>(div_up(now, kTile) * tiles_n), 256, 0, s>>>(
-          static_cast<int>(now), static_cast<int>(outputs), blocks, x_codes + m * blocks * 16, x_scales + m * blocks,
-          w_codes, w_scales, static_cast<T*>(out) + m * outputs, tiles_n);
+      const dim3 grid(static_cast<unsigned>(div_up(now, t.ts) * tiles_n), static_cast<unsigned>(t.splits));
+      with_tiles(t, [&](auto ts, auto ks) {
+        constexpr int TS = decltype(ts)::value, KS = decltype(ks)::value;
+        k_mx4_gemm<T, TS, KS><<<grid, 256 * KS, 0, s>>>(
+            static_cast<int>(now), static_cast<int>(outputs), static_cast<int>(blocks), x_codes + m * blocks * 16,
+            x_scales + m * blocks, w_codes, w_scales, static_cast<T*>(out) + m * outputs,
+            static_cast<float*>(workspace), tiles_n, t.kper / 32);
+      });
     }
+    if (t.splits > 1)
+      launch_join(tokens * outputs, t.splits, static_cast<const float*>(workspace), static_cast<T*>(out), s);
   });
   return check_launch("plx_mx4_product");
 }

@@ -41,58 +41,50 @@ __device__ __forceinline__ T from_f32(float v) {
   return static_cast<T>(v);  // to the nearest, ties to even
 }
 
-// v[0..8) = p[0..8), p on 16 bytes.
-__device__ __forceinline__ void load8v(const float* p, float v[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
+// Eight consecutive values as they are in memory, and as a load that needs
+// no more than the values' own alignment (the memory pipeline takes 16 bytes
+// from any address: rows of an odd length need no loads of single values).
 template <typename T>
-__device__ __forceinline__ void load8v(const T* p, float v[8]) {
-  typedef T t8 __attribute__((ext_vector_type(8)));
-  const t8 a = *reinterpret_cast<const t8*>(p);
+struct Unit {
+  typedef T type __attribute__((ext_vector_type(8)));
+  typedef T load __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
+// p[i * stride], i < n; zeros from there on.
+template <typename T>
+__device__ __forceinline__ typename Unit<T>::type load_unit(const T* p, int64_t stride, int n) {
+  if (stride == 1 && n >= 8) return *reinterpret_cast<const typename Unit<T>::load*>(p);
+  typename Unit<T>::type r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_f32(a[i]);
+  for (int i = 0; i < 8; ++i) r[i] = i < n ? p[i * stride] : from_f32<T>(0.0f);
+  return r;
+}
+// The same as float32.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int64_t stride, int n, float v[8]) {
+  const typename Unit<T>::type r = load_unit(p, stride, n);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_f32(r[i]);
 }
 
-// v[i] = p[i * stride] for i < n, zero from there on.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int64_t stride, int n, bool wide, float v[8]) {
-  if (wide && n >= 8) {
-    load8v(p, v);
-    return;
-  }
+__device__ __forceinline__ void store8(T* p, int n, const float v[8]) {
+  if (n >= 8) {
+    typename Unit<T>::load r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i * stride]) : 0.0f;
-}
-
-__device__ __forceinline__ void store8v(float* p, const float v[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-template <typename T>
-__device__ __forceinline__ void store8v(T* p, const float v[8]) {
-  typedef T t8 __attribute__((ext_vector_type(8)));
-  t8 a;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = from_f32<T>(v[i]);
-  *reinterpret_cast<t8*>(p) = a;
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int64_t stride, int n, bool wide, const float v[8]) {
-  if (wide && n >= 8) {
-    store8v(p, v);
+    for (int i = 0; i < 8; ++i) r[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<typename Unit<T>::load*>(p) = r;
     return;
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (i < n) p[i * stride] = from_f32<T>(v[i]);
+    if (i < n) p[i] = from_f32<T>(v[i]);
 }
 
-// Four consecutive results of a row of n, `left` of them inside it.
+// Four consecutive results of a row, `left` of them inside it.
 template <typename T>
-__device__ __forceinline__ void store4(T* p, int n, int left, f32x4 v) {
-  typedef T t4 __attribute__((ext_vector_type(4)));
-  if (left >= 4 && (n & 3) == 0) {  // (rows start on a multiple of 4)
+__device__ __forceinline__ void store4(T* p, int left, f32x4 v) {
+  typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (left >= 4) {
     t4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = from_f32<T>(v[i]);

@@ -115,9 +115,9 @@ __device__ __forceinline__ void big_store(const f32x4 acc[8][4], void* out, floa
       const int n = n0 + j * 16;
       const int64_t at = static_cast<int64_t>(m) * N + n;
       if (gridDim.y > 1)
-        store4(part + static_cast<int64_t>(blockIdx.y) * M * N + at, N, N - n, acc[i][j]);
+        store4(part + static_cast<int64_t>(blockIdx.y) * M * N + at, N - n, acc[i][j]);
       else
-        store4(static_cast<OT*>(out) + at, N, N - n, acc[i][j]);
+        store4(static_cast<OT*>(out) + at, N - n, acc[i][j]);
     }
   }
 }

@@ -67,6 +67,14 @@ class Mx4:
         _check_codes("Mx4", codes, scales, codes.shape[0], -(-n // 128) * 4, 16)
         self.codes, self.scales, self.shape = codes, scales, (codes.shape[0], n)
 
+    @classmethod
+    def _empty(cls, lines: int, n: int, device: torch.device) -> Mx4:
+        m, b = object.__new__(cls), -(-n // 128) * 4
+        m.codes = torch.empty((lines, 16 * b), dtype=torch.uint8, device=device)
+        m.scales = torch.empty((lines, b), dtype=torch.uint8, device=device)
+        m.shape = lines, n
+        return m
+
     @property
     def device(self) -> torch.device:
         return self.codes.device
@@ -91,6 +99,14 @@ class Mx8:
             raise ValueError(f"Mx8: axis 0 or 1 and a shape of two dimensions expected, got {axis} and {shape}")
         _check_codes("Mx8", codes, scales, shape[1 - axis], -(-shape[axis] // 32), 32)
         self.codes, self.scales, self.shape, self.axis = codes, scales, (shape[0], shape[1]), axis
+
+    @classmethod
+    def _empty(cls, shape: tuple[int, int], axis: int, device: torch.device) -> Mx8:
+        m, lines, b = object.__new__(cls), shape[1 - axis], -(-shape[axis] // 32)
+        m.codes = torch.empty((lines, 32 * b), dtype=torch.uint8, device=device)
+        m.scales = torch.empty((lines, b), dtype=torch.uint8, device=device)
+        m.shape, m.axis = shape, axis
+        return m
 
     @property
     def device(self) -> torch.device:
@@ -125,11 +141,13 @@ def _on_gpu(who: str, device: torch.device, *others: torch.device) -> None:
 def _launch(device: torch.device, name: str, *args: object) -> None:
     """The entry point on torch's current stream of ``device`` (the kernels
     launch on the current device)."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
+    index = device.index
+    # (current_stream(device).cuda_stream without its Stream object, 2 us of a 10 us call)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch.cuda.current_device():
         _lib.call(name, *args, stream)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             _lib.call(name, *args, stream)
 
 
@@ -148,12 +166,10 @@ def quantise4(x: torch.Tensor) -> Mx4:
     _check("quantise4", x)
     _on_gpu("quantise4", x.device)
     lines, n = x.shape
-    b = -(-n // 128) * 4
-    codes = torch.empty((lines, 16 * b), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((lines, b), dtype=torch.uint8, device=x.device)
+    m = Mx4._empty(lines, n, x.device)
     _launch(x.device, "plx_mx4_quantise", lines, n, DTYPES[x.dtype], x.data_ptr(), x.stride(0), x.stride(1),
-            codes.data_ptr(), scales.data_ptr())
-    return Mx4(codes, scales, n)
+            m.codes.data_ptr(), m.scales.data_ptr())
+    return m
 
 
 def activate(h: torch.Tensor, fn: str, axis: int = 1) -> tuple[torch.Tensor, Mx8]:
@@ -167,14 +183,11 @@ def activate(h: torch.Tensor, fn: str, axis: int = 1) -> tuple[torch.Tensor, Mx8
     if axis not in (0, 1):
         raise ValueError(f"activate: axis 0 or 1 expected, got {axis}")
     _on_gpu("activate", h.device)
-    lines, n = h.shape[1 - axis], h.shape[axis]
-    y = torch.empty_like(h)
-    b = -(-n // 32)
-    codes = torch.empty((lines, 32 * b), dtype=torch.uint8, device=h.device)
-    scales = torch.empty((lines, b), dtype=torch.uint8, device=h.device)
-    _launch(h.device, "plx_mx8_activate", lines, n, DTYPES[h.dtype], FUNCTIONS[fn], h.data_ptr(), h.stride(1 - axis),
-            h.stride(axis), y.data_ptr(), y.stride(1 - axis), y.stride(axis), codes.data_ptr(), scales.data_ptr())
-    return y, Mx8(codes, scales, tuple(h.shape), axis)
+    y, kept = torch.empty_like(h), Mx8._empty(tuple(h.shape), axis, h.device)
+    _launch(h.device, "plx_mx8_activate", h.shape[1 - axis], h.shape[axis], DTYPES[h.dtype], FUNCTIONS[fn],
+            h.data_ptr(), h.stride(1 - axis), h.stride(axis), y.data_ptr(), y.stride(1 - axis), y.stride(axis),
+            kept.codes.data_ptr(), kept.scales.data_ptr())
+    return y, kept
 
 
 def activate_grad(dy: torch.Tensor, kept: Mx8, fn: str) -> torch.Tensor:

@@ -23,6 +23,10 @@ SHAPES = [(1, 1, 1), (1, 33, 17), (2, 128, 64), (3, 129, 65), (15, 31, 128), (16
           (1, 4096, 1024), (33, 2048, 2049)]
 
 
+# large products: whole and odd tiles, lines of whole, odd and half steps, ranges of k over workgroups
+LARGE = [(2056, 2120, 2304), (1100, 2049, 4608), (264, 9600, 4104), (4104, 257, 9601), (2304, 16704, 264)]
+
+
 def _gen(*key: int) -> torch.Generator:
     seed = 0
     for k in key:
@@ -179,6 +183,29 @@ def test_product_and_its_gradient(shape, dtype, layout) -> None:
     dy = plain.layouts(_spread((tokens, outputs), g, -4, 4).to(dtype))[layout]
     dx = lowbit.product_grad(dy, w)
     plain.assert_product(dx, dy.double(), _w64(w).t())
+
+
+@pytest.mark.parametrize("layout", ["rows", "columns", "offset"])
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("shape", LARGE)
+def test_large_products(shape, dtype, layout) -> None:
+    tokens, inputs, outputs = shape
+    _say("large", shape, dtype, layout)
+    g = _gen(*shape, 5)
+    w = _weights(outputs, inputs, g)
+    w64 = _w64(w)
+    x = plain.layouts(_spread((tokens, inputs), g, -4, 4).to(dtype))[layout]
+    plain.assert_product(lowbit.product(x, w), x.double(), w64)
+    dy = plain.layouts(_spread((tokens, outputs), g, -4, 4).to(dtype))[layout]
+    plain.assert_product(lowbit.product_grad(dy, w), dy.double(), w64.t().contiguous())
+    for axis in (0, 1):
+        _, kept = lowbit.activate(x, "relu", axis=axis)
+        x8 = plain.values8(kept.codes, kept.scales, (tokens, inputs)[axis])
+        x8 = x8.t().contiguous() if axis else x8
+        plain.assert_product(lowbit.weight_grad(dy, kept), dy.double().t().contiguous(), x8)
+    if layout == "rows":
+        x4 = lowbit.quantise4(x)
+        plain.assert_product(lowbit.product(x4, w, dtype=dtype), plain.values4(x4.codes, x4.scales, inputs), w64)
 
 
 @pytest.mark.parametrize("dtype", plain.DTYPES)

@@ -138,12 +138,12 @@ def test_entry_points_check_before_they_launch(lib) -> None:
     assert lib.plx_mx_product(0, 4, -4, 4, 0, p, 4, 1, p, p, p, None, 0, None) == 1
     assert lib.plx_mx_product(0, 4, 4, 4, 0, None, 4, 1, p, p, p, None, 0, None) == 1
     assert lib.plx_mx_product(0, 0, 4, 4, 0, None, 4, 1, p, p, None, None, 0, None) == 0
-    assert lib.plx_mx_product(0, 512, 512, 512, 1, p, 512, 1, p, p, p, None, 0, None) == 1
+    assert lib.plx_mx_product(0, 4096, 4096, 4096, 1, p, 4096, 1, p, p, p, None, 0, None) == 1
     assert b"plx_mx_workspace" in lib.plx_last_error()
     assert lib.plx_mx4_product(4, 4, 4, p, p, p, p, 9, p, None, 0, None) == 3
     assert lib.plx_mx4_product(4, 4, 4, p, p, p, None, 0, p, None, 0, None) == 1
     assert lib.plx_mx4_product(4, 4, 0, None, None, None, None, 0, None, None, 0, None) == 0
-    assert lib.plx_mx4_product(512, 512, 512, p, p, p, p, 0, p, None, 0, None) == 1
+    assert lib.plx_mx4_product(4096, 4096, 4096, p, p, p, p, 0, p, None, 0, None) == 1
     assert b"plx_mx4_workspace" in lib.plx_last_error()
     assert lib.plx_mx_workspace(0, -1, 4, 4, 0, p, 4, 1) == -1
     assert lib.plx_mx_workspace(9, 4, 4, 4, 0, p, 4, 1) == -1
