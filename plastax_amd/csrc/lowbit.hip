@@ -760,11 +760,14 @@ inline unsigned groups_across(int64_t lines, int64_t blocks) {
   return static_cast<unsigned>(g < kMaxGroups ? g : kMaxGroups);
 }
 
-// A large product: 256 x 256 tiles have enough rows, columns and k, and the
-// operands' way through memory pays.
-constexpr double kBigLeast = 10e9;
-inline bool large(int64_t m, int64_t n, int64_t k) {
-  return m >= 256 && n >= 256 && k >= 256 && static_cast<double>(m) * n * k >= kBigLeast;
+// A large product: 256 x 256 tiles have enough rows, columns and k (counted
+// over a's pieces), and the operands' way through memory pays. Products of
+// 8.6e9 in bf16 take 34 to 56 us either way, 12.9e9 in float32 47 to 69 us
+// large and 68 to 77 in small tiles, 17.2e9 in bf16 45 to 65 and 68 to 87; in
+// 4 bits 17.2e9 take 41 us large and 26 to 30 in small tiles.
+constexpr double kBigLeast = 9e9, kBig4Least = 25e9;
+inline bool large(int64_t m, int64_t n, int64_t k, double least) {
+  return m >= 256 && n >= 256 && k >= 256 && static_cast<double>(m) * n * k >= least;
 }
 
 // How a product in small tiles runs: tiles of ts x ts, ks groups of waves in a
@@ -834,7 +837,7 @@ int big_splits(int64_t m, int64_t n, int64_t steps) {
 Plan plan_of(int kind, const Shape& s, int dtype, const void* a, int64_t sm, int64_t sk) {
   Plan p{};
   const int pieces = dtype == PLX_LB_F32 ? 3 : dtype == PLX_LB_F16 ? 2 : 1;
-  p.big = large(s.m, s.n, s.k * pieces);
+  p.big = large(s.m, s.n, s.k * pieces, kBigLeast);
   if (!p.big) {
     if (kind == PLX_LB_PRODUCT && s.m <= kFew) return p;
     p.splits = tiles_of(s.m, s.n, s.k, 64).splits;
@@ -899,9 +902,9 @@ void launch_big(const GemmArgs& g, const Plan& p, char* work, hipStream_t s) {
   b.tiles_m = static_cast<int>(div_up(g.M, kBig)), b.tiles_n = static_cast<int>(div_up(g.N, kBig));
   const dim3 grid(static_cast<unsigned>(b.tiles_m) * b.tiles_n, static_cast<unsigned>(p.splits));
   if (p.across_a)
-    k_big_gemm<true, BA, OT><<<grid, kBigThreads, 0, s>>>(b);
+    k_big_gemm<true, BA, false, OT><<<grid, kBigThreads, 0, s>>>(b);
   else
-    k_big_gemm<false, BA, OT><<<grid, kBigThreads, 0, s>>>(b);
+    k_big_gemm<false, BA, false, OT><<<grid, kBigThreads, 0, s>>>(b);
   if (p.splits > 1) launch_join(static_cast<int64_t>(g.M) * g.N, p.splits, b.part, static_cast<OT*>(g.out), s);
 }
 
@@ -913,7 +916,7 @@ struct Plan4 {
 };
 Plan4 plan4_of(int64_t m, int64_t n, int64_t k) {
   Plan4 p{};
-  p.big = large(m, n, k) && k <= 8 * kBigLine;
+  p.big = large(m, n, k, kBig4Least) && k <= 8 * kBigLine;
   if (!p.big) {
     p.splits = tiles_of(m, n, k, 256).splits;
     p.bytes = p.splits > 1 ? 4 * p.splits * m * n : 0;
@@ -921,7 +924,7 @@ Plan4 plan4_of(int64_t m, int64_t n, int64_t k) {
   }
   p.steps = static_cast<int>(div_up(k, 256));
   p.splits = big_splits(m, n, p.steps);
-  p.bytes_a = div_up(m, 128) * p.steps * 64 * 16, p.bytes_b = div_up(n, 64) * p.steps * 64 * 8;
+  p.bytes_a = div_up(m, kBig) * p.steps * 2048, p.bytes_b = div_up(n, kBig) * p.steps * 2048;
   p.bytes = p.bytes_a + p.bytes_b + (p.splits > 1 ? 4 * p.splits * m * n : 0);
   return p;
 }
@@ -1136,21 +1139,21 @@ int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8
   if (p.big) {
     hipStream_t s = static_cast<hipStream_t>(stream);
     char* work = static_cast<char*>(workspace);
-    Big4Args g{};
+    BigArgs g{};
     g.a = reinterpret_cast<const char*>(x_codes), g.b = reinterpret_cast<const char*>(w_codes);
-    g.sa = reinterpret_cast<const uint4*>(work), g.sb = reinterpret_cast<const uint2*>(work + p.bytes_a);
+    g.sa = work, g.sb = work + p.bytes_a;
     g.out = out, g.part = reinterpret_cast<float*>(work + p.bytes_a + p.bytes_b);
-    g.M = static_cast<int>(tokens), g.N = static_cast<int>(outputs), g.line = blocks * 16;
-    g.steps = p.steps, g.split = static_cast<int>(div_up(p.steps, p.splits));
+    g.M = g.rows_a = static_cast<int>(tokens), g.N = g.rows_b = static_cast<int>(outputs);
+    g.lda = g.ldb = blocks * 16;
+    g.steps = g.wrap = p.steps, g.split = static_cast<int>(div_up(p.steps, p.splits));
     g.tiles_m = static_cast<int>(div_up(tokens, kBig)), g.tiles_n = static_cast<int>(div_up(outputs, kBig));
-    const int64_t groups = div_up(p.bytes_a / 16 + p.bytes_b / 8, 256);
-    k_big_scales<<<static_cast<unsigned>(groups < kMaxGroups ? groups : kMaxGroups), 256, 0, s>>>(
+    k_big_scales<<<static_cast<unsigned>((g.tiles_m + g.tiles_n) * div_up(p.steps, 8)), 256, 0, s>>>(
         g.M, g.N, blocks, p.steps, x_scales, w_scales, reinterpret_cast<uint8_t*>(work),
         reinterpret_cast<uint8_t*>(work + p.bytes_a));
     with_type(dtype, [&](auto* t) {
       using T = PLX_TYPE(t);
       const dim3 grid(static_cast<unsigned>(g.tiles_m) * g.tiles_n, static_cast<unsigned>(p.splits));
-      k_big4_gemm<T><<<grid, kBigThreads, 0, s>>>(g);
+      k_big_gemm<false, false, true, T><<<grid, kBigThreads, 0, s>>>(g);
       if (p.splits > 1) launch_join(tokens * outputs, p.splits, g.part, static_cast<T*>(out), s);
     });
     return check_launch("plx_mx4_product");

@@ -20,6 +20,8 @@ struct BigArgs {
   int rows_a, rows_b;  // m and n that are in memory (M and N, or padded for "across")
   int steps;         // of 64 k, over all of a's pieces
   int wrap;          // steps of b, which starts again after them
+  const char* sa;    // 4 bits: the scales in the waves' order (k_big_scales)
+  const char* sb;
   int split;         // steps of one k range
   int tiles_m, tiles_n;
 };
@@ -30,41 +32,40 @@ constexpr int kBigBytes = kBig * 128;     // of one operand's step in LDS
 
 typedef __attribute__((address_space(3))) char lds_char;
 typedef const __attribute__((address_space(1))) char glb_char;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// The four 16-byte loads of a lane for one operand's step, in LDS order (a
-// wave's 64 lanes write 1 KB in a row), so that the swizzle is in the global
-// addresses. Along: 256 rows of 8 chunks, chunk c of row r at c ^ (r & 7).
-// Across: 64 rows (k) of 32 chunks, pair p of row k at p ^ (k & 3 | k / 8 % 4 * 4).
-template <bool ACROSS>
+// One operand's step in LDS: two halves of 128 rows (of m or n), 16 KB each.
+// Along: 128 lines of 8 chunks of 16 bytes, chunk c of line r at c ^ (r & 7).
+// Across: 64 lines (k) of 16 chunks, pair p of line k at p ^ (k & 3 | k / 8 % 2
+// * 4). A lane's loads are in LDS order (a wave's 64 lanes write 1 KB in a
+// row), so the swizzle is in the global addresses: off[2 h + i] of half h.
+template <bool ACROSS, bool F4 = false>
 __device__ __forceinline__ void big_offsets(int tid, int first, int rows, int64_t ld, uint32_t off[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int slot = i * kBigThreads + tid;
+    const int slot = (i & 1) * kBigThreads + tid, half = i >> 1;
     if (ACROSS) {
-      const int k = slot >> 5, cp = slot & 31;
-      const int c = ((cp >> 1) ^ ((k & 3) | ((k >> 3) & 3) << 2)) << 1 | (cp & 1);
+      const int k = slot >> 4, cp = slot & 15;
+      const int c = half * 16 + (((cp >> 1) ^ ((k & 3) | ((k >> 3) & 1) << 2)) << 1 | (cp & 1));
       const int last = (rows - first) / 8 - 1;  // (rows is a multiple of 8)
       off[i] = static_cast<uint32_t>(k * ld + (c < last ? c : last) * 16);
     } else {
-      const int r = slot >> 3, c = (slot & 7) ^ (r & 7);
+      const int r = half * 128 + (slot >> 3), c = (slot & 7) ^ (r & 7) ^ (F4 ? (r >> 4) & 1 : 0);
       const int last = rows - first - 1;
       off[i] = static_cast<uint32_t>((r < last ? r : last) * ld + c * 16);
     }
   }
 }
 
-__device__ __forceinline__ void big_load(const char* base, const uint32_t off[4], lds_char* lds, int wave) {
+__device__ __forceinline__ void big_load(const char* base, const uint32_t* off, lds_char* lds, int wave) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 2; ++i)
     __builtin_amdgcn_global_load_lds((glb_char*)(base + off[i]),
                                      (__attribute__((address_space(3))) void*)(lds + (i * kBigThreads + wave * 64) * 16),
                                      16, 0, 0);
 }
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-
-// LDS addresses of a lane's fragments of F x 16 rows from `row`.
+// LDS addresses of a lane's fragments of F x 16 rows from `row` of a half.
 template <bool ACROSS, int F>
 struct BigFrags {
   int at[ACROSS ? F : 2];
@@ -72,7 +73,7 @@ struct BigFrags {
     if (ACROSS) {
 #pragma unroll
       for (int f = 0; f < F; ++f)
-        at[f] = (q * 8 + (l15 >> 2)) * 512 + (((row >> 4) + f) ^ ((l15 >> 2) | q << 2)) * 32 + (l15 & 3) * 8;
+        at[f] = (q * 8 + (l15 >> 2)) * 256 + (((row >> 4) + f) ^ ((l15 >> 2) | (q & 1) << 2)) * 32 + (l15 & 3) * 8;
     } else {
 #pragma unroll
       for (int s = 0; s < 2; ++s) at[s] = (row + l15) * 128 + ((s * 4 + q) ^ (l15 & 7)) * 16;
@@ -81,8 +82,8 @@ struct BigFrags {
   __device__ __forceinline__ bf16x8 get(const lds_char* lds, int f, int s) const {
     if (ACROSS) {
       typedef __attribute__((address_space(3))) s16x4* p4;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lds + at[f] + s * 16384));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lds + at[f] + s * 16384 + 2048));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lds + at[f] + s * 8192));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((p4)(lds + at[f] + s * 8192 + 1024));
       return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
     return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8*>(lds + at[s] + f * 2048);
@@ -102,223 +103,327 @@ __device__ __forceinline__ void big_tile(int wg, int tiles_m, int tiles_n, int* 
   *tn = r / high;
 }
 
-// A wave's 128 x 64 results: with b's rows as the matrix instruction's first
-// operand a lane holds four consecutive n of one m.
-template <typename OT>
-__device__ __forceinline__ void big_store(const f32x4 acc[8][4], void* out, float* part, int M, int N, int m0, int n0) {
+// The same of the scaled 4-bit instruction, 32 rows by 64 k: a lane has row
+// l & 31 and one block of a step's eight, 2 s + l / 32.
+template <int F>
+struct Big4Frags {
+  int at[4];
+  __device__ __forceinline__ void init(int row, int lane) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int m = m0 + i * 16;
-    if (m >= M) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + j * 16;
-      const int64_t at = static_cast<int64_t>(m) * N + n;
-      if (gridDim.y > 1)
-        store4(part + static_cast<int64_t>(blockIdx.y) * M * N + at, N - n, acc[i][j]);
-      else
-        store4(static_cast<OT*>(out) + at, N - n, acc[i][j]);
-    }
+    for (int s = 0; s < 4; ++s) at[s] = (row + (lane & 31)) * 128 + ((s * 2 + (lane >> 5)) ^ (lane & 7) ^ ((lane >> 4) & 1)) * 16;
   }
-}
-
-template <bool AA, bool BA, typename OT>
-__global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
-  __shared__ __align__(16) char lds[4 * kBigBytes];
-  lds_char* l = (lds_char*)lds;
-  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int tm, tn;
-  big_tile(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
-  const int m0 = tm * kBig, n0 = tn * kBig, wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
-
-  uint32_t oa[4], ob[4];
-  big_offsets<AA>(tid, m0, g.rows_a, g.lda, oa);
-  big_offsets<BA>(tid, n0, g.rows_b, g.ldb, ob);
-  const int64_t sa = AA ? 64 * g.lda : 128, sb = BA ? 64 * g.ldb : 128;
-  const char* a = g.a + (AA ? int64_t{2} * m0 : m0 * g.lda);
-  const char* b = g.b + (BA ? int64_t{2} * n0 : n0 * g.ldb);
-  const int beg = blockIdx.y * g.split, end = beg + g.split < g.steps ? beg + g.split : g.steps;
-  int bt = beg % g.wrap;
-  a += beg * sa;
-
-  BigFrags<AA, 8> fa;
-  BigFrags<BA, 4> fb;
-  fa.init(wm, l15, q);
-  fb.init(wn, l15, q);
-
-  f32x4 acc[8][4] = {};
-  auto load = [&](int buf) {
-    big_load(a, oa, l + buf * 2 * kBigBytes, wave);
-    big_load(b + bt * sb, ob, l + buf * 2 * kBigBytes + kBigBytes, wave);
-    a += sa;
-    bt = bt + 1 == g.wrap ? 0 : bt + 1;
-  };
-  auto compute = [&](int buf) {
-    const lds_char* la = l + buf * 2 * kBigBytes;
-    const lds_char* lb = la + kBigBytes;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf16x8 xb[4], xa[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xb[i] = fb.get(lb, i, s);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) xa[i] = fa.get(la, i, s);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[j], xa[i], acc[i][j], 0, 0, 0);
-    }
-  };
-  load(0);
-  int buf = 0;
-  for (int t = beg; t < end; ++t) {
-    __syncthreads();
-    if (t + 1 < end) load(buf ^ 1);
-    compute(buf);
-    buf ^= 1;
+  __device__ __forceinline__ bf16x8 get(const lds_char* lds, int f, int s) const {
+    return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8*>(lds + at[s] + f * 4096);
   }
-
-  big_store<OT>(acc, g.out, g.part, g.M, g.N, m0 + wm + l15, n0 + wn + q * 4);
-}
-
-// The same with both operands in 4-bit blocks along k: a row's 128 bytes are
-// 8 blocks, and a lane's 16 bytes one of them with its scale byte, so that
-// the LDS layout and the fragments' addresses are the bf16 kernel's. A wave
-// finds the scales of its rows' blocks of a step side by side in `sa` and
-// `sb` (k_big_scales), a lane's own in 16 and 8 bytes.
-struct Big4Args {
-  const char* a;
-  const char* b;
-  const uint4* sa;  // [ceil(M / 128)][steps][64]
-  const uint2* sb;  // [ceil(N / 64)][steps][64]
-  void* out;
-  float* part;
-  int M, N;
-  int64_t line;  // bytes of a row, a multiple of 64
-  int steps, split, tiles_m, tiles_n;
 };
 
-template <int I>
-__device__ __forceinline__ uint32_t word(uint4 v) {
-  return I == 0 ? v.x : I == 1 ? v.y : I == 2 ? v.z : v.w;
+// The barrier between a wave's loads from LDS and its matrix instructions (the
+// reads are back before it, so that others may overwrite what they read) and
+// the one after those.
+__device__ __forceinline__ void big_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
 }
 
-template <typename OT>
-__global__ __launch_bounds__(kBigThreads, 2) void k_big4_gemm(Big4Args g) {
-  __shared__ __align__(16) char lds[4 * kBigBytes];
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// A wave's results, from its first row and column on: with b's rows as the
+// matrix instruction's first operand a lane holds runs of four consecutive n
+// of one m: one in a fragment of 16 x 16, in one of 32 x 32 four, 8 columns
+// apart, lanes l and l + 32 having neighbouring runs of the same row. Tiles
+// that are inside take the straight way.
+template <typename T>
+__device__ __forceinline__ void big_store(const f32x4 (&acc)[2][2][4][2], T* out, int M, int N, int m, int n,
+                                          bool whole) {
+#pragma unroll
+  for (int ha = 0; ha < 2; ++ha)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = m + ha * 128 + i * 16;
+      T* p = out + static_cast<int64_t>(row) * N + n;
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int col = hb * 128 + j * 16;
+          if (whole)
+            store4(p + col, 4, acc[ha][hb][i][j]);
+          else if (row < M)
+            store4(p + col, N - n - col, acc[ha][hb][i][j]);
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void big_store(const f32x16 (&acc)[2][2][2][1], T* out, int M, int N, int m, int n,
+                                          bool whole) {
+  const bool upper = (threadIdx.x & 32) != 0;
+#pragma unroll
+  for (int ha = 0; ha < 2; ++ha)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = m + ha * 128 + i * 32;
+      T* p = out + static_cast<int64_t>(row) * N + n;
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          // Runs r and r + 1 of both lanes, 16 columns: the lower lane gets
+          // the first 8, the upper one the others.
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[ha][hb][i][0][4 * r + k]),
+                                                            __float_as_uint(acc[ha][hb][i][0][4 * r + 4 + k]), false,
+                                                            false);
+            v[k] = __uint_as_float(t[0]), v[4 + k] = __uint_as_float(t[1]);
+          }
+          const int col = hb * 128 + r * 8 + (upper ? 4 : 0);  // (n is 4 more in the upper lane)
+          if (whole)
+            store8(p + col, 8, v);
+          else if (row < M)
+            store8(p + col, N - n - col, v);
+        }
+    }
+}
+
+// 256 x 256 of the output by 8 waves. A wave has 64 rows of m in each half of
+// its a and 32 of n in each half of b, so four quarters of 64 x 32, one a
+// phase: LDS reads and global loads, barrier, 16 matrix instructions,
+// barrier. The second four waves are one barrier behind the first, so that on
+// each SIMD one wave multiplies while the other one loads. A half of a buffer
+// is loaded for the step after next as soon as both have read it, nearly two
+// steps before it is needed. F4: both operands in 4-bit blocks along k, 8 of
+// them in a line's 128 bytes: a lane's 16 bytes are one block, and the LDS
+// layout and the fragments' addresses are the bf16 ones'. The scales of a step
+// come in the waves' order (k_big_scales) and by way of LDS too, a lane's own
+// in 16 and 8 bytes.
+template <bool AA, bool BA, bool F4, typename OT>
+__global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
+  __shared__ __align__(16) char lds[4 * kBigBytes + (F4 ? 2 * 4096 : 0)];
   lds_char* l = (lds_char*)lds;
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 2, wc = wave & 3;
   int tm, tn;
   big_tile(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
-  const int m0 = tm * kBig, n0 = tn * kBig, wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
+  const int m0 = tm * kBig, n0 = tn * kBig;
 
   uint32_t oa[4], ob[4];
-  big_offsets<false>(tid, m0, g.M, g.line, oa);
-  big_offsets<false>(tid, n0, g.N, g.line, ob);
+  big_offsets<AA, F4>(tid, m0, g.rows_a, g.lda, oa);
+  big_offsets<BA, F4>(tid, n0, g.rows_b, g.ldb, ob);
+  const int64_t sa = AA ? 64 * g.lda : 128, sb = BA ? 64 * g.ldb : 128;
   const int beg = blockIdx.y * g.split, end = beg + g.split < g.steps ? beg + g.split : g.steps;
-  const char* a = g.a + m0 * g.line + beg * 128;
-  const char* b = g.b + n0 * g.line + beg * 128;
-  // A line of an odd number of 64 bytes ends inside its last step, which then
-  // reads its first half twice and multiplies it once.
-  const bool odd = (g.line & 64) != 0;
-  const uint32_t back = (((tid & 7) ^ ((tid >> 3) & 7)) & 4) ? 64 : 0;
-  // (a wave past the last rows reads the last ones' scales)
-  const int ga = (m0 + wm) / 128, gb = (n0 + wn) / 64, la = (g.M - 1) / 128, lb = (g.N - 1) / 64;
-  const uint4* sa = g.sa + (static_cast<int64_t>(ga < la ? ga : la) * g.steps + beg) * 64 + lane;
-  const uint2* sb = g.sb + (static_cast<int64_t>(gb < lb ? gb : lb) * g.steps + beg) * 64 + lane;
+  const char* a = g.a + (AA ? int64_t{2} * m0 : m0 * g.lda) + beg * sa;
+  const char* b = g.b + (BA ? int64_t{2} * n0 : n0 * g.ldb);
+  int bt = beg % g.wrap;
+  // 4 bits: a line of an odd number of 64 bytes ends inside its last step,
+  // which then reads its first half twice and multiplies it once.
+  const bool odd = F4 && (g.lda & 64) != 0;
+  const uint32_t back = (((tid & 7) ^ ((tid >> 3) & 7) ^ ((tid >> 7) & 1)) & 4) ? 64 : 0;
+  // 4 KB of scales a step, by the first four waves: a's, then b's.
+  const char* gs = nullptr;
+  u32x4 xs = {};
+  u32x2 ws = {};
+  if (F4)
+    gs = (wave < 2 ? g.sa + (static_cast<int64_t>(tm) * g.steps + beg) * 2048
+                   : g.sb + (static_cast<int64_t>(tn) * g.steps + beg) * 2048) +
+         (wave & 1) * 1024 + lane * 16;
 
-  BigFrags<false, 8> fa;
-  BigFrags<false, 4> fb;
-  fa.init(wm, l15, q);
-  fb.init(wn, l15, q);
+  // Fragments: 16 rows by 32 k, or 32 rows by 64 k of 4 bits; of either a
+  // quarter's 64 x 32 take FA x FB, in S steps of k.
+  constexpr int FA = F4 ? 2 : 4, FB = F4 ? 1 : 2, S = F4 ? 4 : 2;
+  typedef typename std::conditional<F4, f32x16, f32x4>::type sums;
+  typename std::conditional<F4, Big4Frags<FA>, BigFrags<AA, FA>>::type fa;
+  typename std::conditional<F4, Big4Frags<FB>, BigFrags<BA, FB>>::type fb;
+  if constexpr (F4) {
+    fa.init(wr * 64, lane);
+    fb.init(wc * 32, lane);
+  } else {
+    fa.init(wr * 64, l15, q);
+    fb.init(wc * 32, l15, q);
+  }
+  sums acc[2][2][FA][FB] = {};
+  bf16x8 ra[FA][S], rb[2][FB][S];
 
-  f32x4 acc[8][4] = {};
-  uint4 xs = make_uint4(0, 0, 0, 0);
-  uint2 ws = make_uint2(0, 0);
-  auto load = [&](int t, int buf) {
+  // The next step's pointers; `t` is the step whose first load this is.
+  auto load_a0b0 = [&](int t, int buf) {
     if (odd && t + 1 == g.steps) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) oa[i] -= back, ob[i] -= back;
     }
     big_load(a, oa, l + buf * 2 * kBigBytes, wave);
-    big_load(b, ob, l + buf * 2 * kBigBytes + kBigBytes, wave);
-    a += 128, b += 128;
-    xs = *sa, ws = *sb;
-    sa += 64, sb += 64;
+    big_load(b + bt * sb, ob, l + buf * 2 * kBigBytes + kBigBytes, wave);
   };
-  auto half = [&](int buf, auto step, uint4 s_a, uint2 s_b) {
-    constexpr int s = decltype(step)::value;
-    const lds_char* pa = l + buf * 2 * kBigBytes;
-    const lds_char* pb = pa + kBigBytes;
-    i32x8 xb[4], xa[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) xb[i] = as_i32x8(fb.get(pb, i, s));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) xa[i] = as_i32x8(fa.get(pa, i, s));
-#define PX_BIG4_MFMA(i, j)                                                                          \
-  acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(                                     \
-      xb[j], xa[i], acc[i][j], 4, 4, ((j) * 2 + s) & 3, static_cast<int>((j) < 2 ? s_b.x : s_b.y),  \
-      ((i) * 2 + s) & 3, static_cast<int>(word<(i) / 2>(s_a)))
-#define PX_BIG4_ROW(i) PX_BIG4_MFMA(i, 0), PX_BIG4_MFMA(i, 1), PX_BIG4_MFMA(i, 2), PX_BIG4_MFMA(i, 3)
-    PX_BIG4_ROW(0), PX_BIG4_ROW(1), PX_BIG4_ROW(2), PX_BIG4_ROW(3);
-    PX_BIG4_ROW(4), PX_BIG4_ROW(5), PX_BIG4_ROW(6), PX_BIG4_ROW(7);
-#undef PX_BIG4_ROW
-#undef PX_BIG4_MFMA
+  auto load_b1 = [&](int buf) { big_load(b + bt * sb, ob + 2, l + buf * 2 * kBigBytes + kBigBytes + kBigBytes / 2, wave); };
+  auto load_a1 = [&](int buf) {
+    big_load(a, oa + 2, l + buf * 2 * kBigBytes + kBigBytes / 2, wave);
+    if (F4 && wave < 4) {
+      __builtin_amdgcn_global_load_lds(
+          (glb_char*)gs, (__attribute__((address_space(3))) void*)(l + 4 * kBigBytes + buf * 4096 + wave * 1024), 16, 0, 0);
+      gs += 2048;
+    }
+    a += sa;
+    bt = bt + 1 == g.wrap ? 0 : bt + 1;
   };
-  load(beg, 0);
-  int buf = 0;
-  for (int t = beg; t < end; ++t) {
-    const uint4 s_a = xs;
-    const uint2 s_b = ws;
-    __syncthreads();
-    if (t + 1 < end) load(t + 1, buf ^ 1);
-    half(buf, std::integral_constant<int, 0>{}, s_a, s_b);
-    if (!(odd && t + 1 == g.steps)) half(buf, std::integral_constant<int, 1>{}, s_a, s_b);
-    buf ^= 1;
+  auto read_a = [&](int buf, int h) {
+    const lds_char* p = l + buf * 2 * kBigBytes + h * (kBigBytes / 2);
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int s = 0; s < S; ++s) ra[i][s] = fa.get(p, i, s);
+  };
+  auto read_b = [&](int buf, auto half) {
+    constexpr int h = decltype(half)::value;
+    const lds_char* p = l + buf * 2 * kBigBytes + kBigBytes + h * (kBigBytes / 2);
+#pragma unroll
+    for (int i = 0; i < FB; ++i)
+#pragma unroll
+      for (int s = 0; s < S; ++s) rb[h][i][s] = fb.get(p, i, s);
+  };
+  auto multiply = [&](auto half_a, auto half_b, bool both) {
+    constexpr int ha = decltype(half_a)::value, hb = decltype(half_b)::value;
+    __builtin_amdgcn_s_setprio(1);
+    if constexpr (F4) {
+#define PX_F4(i, s)                                                                                            \
+  acc[ha][hb][i][0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                         \
+      as_i32x8(rb[hb][0][s]), as_i32x8(ra[i][s]), acc[ha][hb][i][0], 4, 4, s, static_cast<int>(ws[hb]), s,     \
+      static_cast<int>(xs[ha * 2 + (i)]))
+      PX_F4(0, 0), PX_F4(1, 0), PX_F4(0, 1), PX_F4(1, 1);
+      if (both) PX_F4(0, 2), PX_F4(1, 2), PX_F4(0, 3), PX_F4(1, 3);
+#undef PX_F4
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            acc[ha][hb][i][j] =
+                __builtin_amdgcn_mfma_f32_16x16x32_bf16(rb[hb][j][s], ra[i][s], acc[ha][hb][i][j], 0, 0, 0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  constexpr std::integral_constant<int, 0> k0{};
+  constexpr std::integral_constant<int, 1> k1{};
+
+  // All but the newest step's loads are back.
+  auto wait_older = [&]() {
+    if (F4 && wave < 4)
+      asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  };
+  load_a0b0(beg, 0);
+  load_b1(0);
+  load_a1(0);
+  if (beg + 1 < end) {
+    load_a0b0(beg + 1, 1);
+    load_b1(1);
+    load_a1(1);
+    wait_older();
+  } else {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
-  big_store<OT>(acc, g.out, g.part, g.M, g.N, m0 + wm + l15, n0 + wn + q * 4);
+  big_barrier();
+  if (wr) big_barrier();
+  for (int t = beg; t < end; ++t) {
+    const int buf = (t - beg) & 1;
+    const bool more = t + 2 < end, both = !(odd && t + 1 == g.steps);
+    read_b(buf, k0);
+    read_a(buf, 0);
+    if (F4) {
+      const lds_char* p = l + 4 * kBigBytes + buf * 4096;
+      // (Written out, and waited for in place: the compiler would wait for
+      // every load under way before it.)
+      asm volatile(
+          "ds_read_b128 %0, %2\n\tds_read_b64 %1, %3 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+          : "=&v"(xs), "=&v"(ws)
+          : "v"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p + wr * 1024 + lane * 16))),
+            "v"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p + wc * 512 + lane * 8)))
+          : "memory");
+    }
+    big_barrier();
+    multiply(k0, k0, both);
+    big_barrier();
+    read_b(buf, k1);
+    if (more) load_a0b0(t + 2, buf);
+    big_barrier();
+    multiply(k0, k1, both);
+    big_barrier();
+    read_a(buf, 1);
+    if (more) load_b1(buf);
+    big_barrier();
+    multiply(k1, k1, both);
+    big_barrier();
+    if (more) {
+      load_a1(buf);
+      wait_older();
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    big_barrier();
+    multiply(k1, k0, both);
+    big_barrier();
+  }
+  if (!wr) big_barrier();
+
+  const int m = m0 + wr * 64 + (F4 ? lane & 31 : l15), n = n0 + wc * 32 + (F4 ? (lane >> 5) * 4 : q * 4);
+  const bool whole = m0 + kBig <= g.M && n0 + kBig <= g.N;
+  if (gridDim.y > 1)
+    big_store(acc, g.part + static_cast<int64_t>(blockIdx.y) * g.M * g.N, g.M, g.N, m, n, false);
+  else if (whole)
+    big_store(acc, static_cast<OT*>(g.out), g.M, g.N, m, n, true);
+  else
+    big_store(acc, static_cast<OT*>(g.out), g.M, g.N, m, n, false);
 }
 
-// Scale bytes [rows][blocks] as k_big4_gemm reads them: of group r / (16 F),
-// step and lane (l15, q), byte 2 f + s is row 16 f + l15's block 8 step + 4 s
-// + q. Rows and blocks past the end get the scale 1.
+// Scale bytes [rows][blocks] as the waves of k_big_gemm read them: W waves
+// share a tile's 256 rows, each with F fragments of 32 rows in each half. Of
+// tile, step, wave and lane, byte 4 (F h + f) + s is the scale of row
+// 128 h + 32 (F wave + f) + lane % 32 in block 8 step + 2 s + lane / 32. Rows and
+// blocks past the end get the scale 1. A workgroup takes 8 steps of a tile
+// through LDS.
+constexpr int kScaleRow = 68;  // bytes of 8 steps of a row in LDS, and 4 that move the rows over the banks
 template <int F>
-__device__ __forceinline__ void big_scales(int64_t at, int rows, int64_t blocks, int steps, const uint8_t* in,
-                                           uint8_t* out) {
-  const int lane = at & 63;
-  const int64_t w = at >> 6;
-  const int step = static_cast<int>(w % steps), group = static_cast<int>(w / steps);
-  const int64_t b = int64_t{8} * step + (lane >> 4);
-  uint32_t r[F / 2];
+__device__ __forceinline__ void big_scales(int tile, int step0, int steps, int rows, int64_t blocks, const uint8_t* in,
+                                           uint8_t* out, uint8_t* lds) {
+  constexpr int W = 4 / F;
+  const int tid = threadIdx.x;
 #pragma unroll
-  for (int i = 0; i < F / 2; ++i) r[i] = 0;
+  for (int i = 0; i < 16; ++i) {
+    const int at = i * 256 + tid, r = at >> 4, c = (at & 15) * 4;
+    const int row = tile * 256 + r;
+    uint32_t v = 0x7F7F7F7Fu;
+    if (row < rows && int64_t{8} * step0 + c < blocks)
+      v = *reinterpret_cast<const uint32_t*>(in + row * blocks + int64_t{8} * step0 + c);
+    *reinterpret_cast<uint32_t*>(lds + r * kScaleRow + c) = v;
+  }
+  __syncthreads();
+  for (int at = tid; at < 8 * W * 64; at += 256) {
+    const int step = at / (W * 64), wave = at / 64 % W, lane = at & 63;
+    if (step0 + step >= steps) break;
+    uint32_t* o = reinterpret_cast<uint32_t*>(out) + ((static_cast<int64_t>(tile) * steps + step0) * W * 64 + at) * 2 * F;
 #pragma unroll
-  for (int f = 0; f < F; ++f) {
-    const int row = group * 16 * F + f * 16 + (lane & 15);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const uint32_t v = row < rows && b + 4 * s < blocks ? in[row * blocks + b + 4 * s] : 127u;
-      r[f / 2] |= v << (8 * ((f * 2 + s) & 3));
+    for (int f = 0; f < 2 * F; ++f) {
+      const int row = f / F * 128 + (wave * F + f % F) * 32 + (lane & 31);
+      const uint8_t* p = lds + row * kScaleRow + step * 8 + (lane >> 5);
+      o[f] = p[0] | p[2] << 8 | p[4] << 16 | static_cast<uint32_t>(p[6]) << 24;
     }
   }
-  uint32_t* o = reinterpret_cast<uint32_t*>(out) + at * (F / 2);
-#pragma unroll
-  for (int i = 0; i < F / 2; ++i) o[i] = r[i];
 }
 
 __global__ __launch_bounds__(256) void k_big_scales(int M, int N, int64_t blocks, int steps, const uint8_t* xs,
                                                     const uint8_t* ws, uint8_t* sa, uint8_t* sb) {
-  const int64_t na = static_cast<int64_t>((M + 127) / 128) * steps * 64;
-  const int64_t nb = static_cast<int64_t>((N + 63) / 64) * steps * 64;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < na + nb;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    if (i < na)
-      big_scales<8>(i, M, blocks, steps, xs, sa);
-    else
-      big_scales<4>(i - na, N, blocks, steps, ws, sb);
-  }
+  __shared__ uint8_t lds[256 * kScaleRow];
+  const int runs = (steps + 7) / 8, tile = blockIdx.x / runs, step0 = blockIdx.x % runs * 8, tiles_m = (M + 255) / 256;
+  if (tile < tiles_m)
+    big_scales<2>(tile, step0, steps, M, blocks, xs, sa, lds);
+  else
+    big_scales<1>(tile - tiles_m, step0, steps, N, blocks, ws, sb, lds);
 }
 
 }  // namespace px

@@ -24,7 +24,7 @@ SHAPES = [(1, 1, 1), (1, 33, 17), (2, 128, 64), (3, 129, 65), (15, 31, 128), (16
 
 
 # large products: whole and odd tiles, lines of whole, odd and half steps, ranges of k over workgroups
-LARGE = [(2056, 2120, 2304), (1100, 2049, 4608), (264, 9600, 4104), (4104, 257, 9601), (2304, 16704, 264)]
+LARGE = [(2056, 2120, 2304), (1100, 2049, 4608), (264, 9600, 4104), (4104, 257, 9601), (2304, 16704, 264), (256, 36864, 1024)]
 
 
 def _gen(*key: int) -> torch.Generator:
@@ -203,9 +203,18 @@ def test_large_products(shape, dtype, layout) -> None:
         x8 = plain.values8(kept.codes, kept.scales, (tokens, inputs)[axis])
         x8 = x8.t().contiguous() if axis else x8
         plain.assert_product(lowbit.weight_grad(dy, kept), dy.double().t().contiguous(), x8)
-    if layout == "rows":
-        x4 = lowbit.quantise4(x)
-        plain.assert_product(lowbit.product(x4, w, dtype=dtype), plain.values4(x4.codes, x4.scales, inputs), w64)
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("shape", [(2056, 2120, 6000), (1100, 5000, 4608), (264, 9600, 10000), (3001, 1300, 6500),
+                                   (256, 131072, 768)])
+def test_large_products_of_two_in_4_bits(shape, dtype) -> None:
+    tokens, inputs, outputs = shape
+    _say("large4", shape, dtype)
+    g = _gen(*shape, 6)
+    w, x = _weights(outputs, inputs, g), lowbit.quantise4(_spread((tokens, inputs), g, -4, 4))
+    got = lowbit.product(x, w, dtype=dtype)
+    plain.assert_product(got, plain.values4(x.codes, x.scales, inputs), _w64(w))
 
 
 @pytest.mark.parametrize("dtype", plain.DTYPES)
