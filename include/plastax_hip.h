@@ -1211,7 +1211,7 @@ PLX_EXPORT int plx_mx4_quantise(int64_t lines, int64_t n, int32_t dtype, const v
 PLX_EXPORT int plx_mx_values(int32_t bits, int64_t lines, int64_t n, const uint8_t* codes, const uint8_t* scales,
                              int32_t dtype, void* out, void* stream);
 
-/* y = fn(h), and h in 8-bit blocks along its lines. */
+/* y = fn(h) (null: none), and h in 8-bit blocks along its lines. */
 PLX_EXPORT int plx_mx8_activate(int64_t lines, int64_t n, int32_t dtype, int32_t fn, const void* h, int64_t h_line,
                                 int64_t h_elem, void* y, int64_t y_line, int64_t y_elem, uint8_t* codes,
                                 uint8_t* scales, void* stream);

@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kBlock) void k_act_along(int64_t lines, int64_t n, 
         m = a < kInfBits && a > m ? a : m;
         f[i] = act<FN>(v[i]);
       }
-      store8(y + line * sy + c * 8, left, f);
+      if (y) store8(y + line * sy + c * 8, left, f);
       const int e = exponent8(max4(m));
       reinterpret_cast<uint2*>(codes)[line * chunks + c] = codes8(v, pow2(-e));
       if ((tx & 3) == 0) scales[line * (chunks / 4) + c / 4] = static_cast<uint8_t>(e + 127);
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(kBlock) void k_act_across(int64_t lines, int64_t n,
     scales[line * blocks + b] = static_cast<uint8_t>(e + 127);
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      if (i < left) o[i * ye] = from_f32<T>(act<FN>(v[i / 8][i % 8]));
+      if (y && i < left) o[i * ye] = from_f32<T>(act<FN>(v[i / 8][i % 8]));
   }
 }
 
@@ -1023,7 +1023,7 @@ int plx_mx8_activate(int64_t lines, int64_t n, int32_t dtype, int32_t fn, const 
   if (!known(dtype)) return fail(PLX_ERR_UNSUPPORTED, "plx_mx8_activate: unknown element type");
   if (fn < PLX_LB_RELU || fn > PLX_LB_SILU) return fail(PLX_ERR_UNSUPPORTED, "plx_mx8_activate: unknown activation");
   if (lines == 0 || n == 0) return PLX_OK;
-  if (!h || !y || !codes || !scales) return fail(PLX_ERR_INVALID, "plx_mx8_activate: null pointer");
+  if (!h || !codes || !scales) return fail(PLX_ERR_INVALID, "plx_mx8_activate: null pointer");
   if (!on16(codes)) return fail(PLX_ERR_INVALID, "plx_mx8_activate: codes not on 16 bytes");
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_type(dtype, [&](auto* t) {

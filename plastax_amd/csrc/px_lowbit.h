@@ -182,19 +182,37 @@ __device__ __forceinline__ uint4 bf16_of8(uint2 c, float scale) {
 template <int P>
 __device__ __forceinline__ void pieces8(const float in[8], uint4 out[P]) {
   float v[8];
+  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = in[i];
+  for (int i = 0; i < 8; ++i) v[i] = in[i], m = m > abs_bits(in[i]) ? m : abs_bits(in[i]);
+  if (m >= kInfBits) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      uint32_t h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t u = __float_as_uint(v[i]);
+        if ((u & 0x7FFFFFFFu) > kInfBits) u |= 0x00400000u;  // a NaN stays one when its low bits go
+        h[i] = u & 0xFFFF0000u;
+        v[i] = (u & kInfBits) == kInfBits ? 0.0f : v[i] - __uint_as_float(h[i]);
+      }
+      out[p] = make_uint4((h[0] >> 16) | h[1], (h[2] >> 16) | h[3], (h[4] >> 16) | h[5], (h[6] >> 16) | h[7]);
+    }
+    return;
+  }
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    uint32_t h[8];
+    uint32_t r[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t u = __float_as_uint(v[i]);
-      if ((u & 0x7FFFFFFFu) > kInfBits) u |= 0x00400000u;  // a NaN stays one when its low bits go
-      h[i] = u & 0xFFFF0000u;
-      if (p + 1 < P) v[i] = (u & kInfBits) == kInfBits ? 0.0f : v[i] - __uint_as_float(h[i]);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = __float_as_uint(v[2 * i]), b = __float_as_uint(v[2 * i + 1]);
+      r[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);  // the high halves
+      if (p + 1 < P) {
+        v[2 * i] -= __uint_as_float(a & 0xFFFF0000u);
+        v[2 * i + 1] -= __uint_as_float(b & 0xFFFF0000u);
+      }
     }
-    out[p] = make_uint4((h[0] >> 16) | h[1], (h[2] >> 16) | h[3], (h[4] >> 16) | h[5], (h[6] >> 16) | h[7]);
+    out[p] = make_uint4(r[0], r[1], r[2], r[3]);
   }
 }
 template <typename T>

@@ -6,7 +6,7 @@ next) is a matrix ``[outputs, inputs]``. Here it is held in 4 bits
 (:func:`product`), and gives its input's gradient (:func:`product_grad`); the
 activation between two pairs keeps its argument in 8 bits for the backward
 (:func:`activate`, :class:`Mx8`, :func:`activate_grad`), and so does the
-weights' own gradient (:func:`weight_grad`).
+weights' own gradient its pair's input (:func:`quantise8`, :func:`weight_grad`).
 
 Formats. 32 consecutive values of a line share a scale ``2^(s - 127)``, ``s``
 one byte: the least power of two under which the block's largest value is not
@@ -40,7 +40,7 @@ _PRODUCT, _PRODUCT_GRAD, _WEIGHT_GRAD, _WEIGHT_GRAD_COLUMNS = range(4)
 
 
 def _check_codes(who: str, codes: torch.Tensor, scales: torch.Tensor, lines: int, blocks: int, size: int) -> None:
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
         raise TypeError(f"{who}: codes and scales are uint8, got {codes.dtype} and {scales.dtype}")
     if codes.shape != (lines, blocks * size) or scales.shape != (lines, blocks):
         raise ValueError(f"{who}: codes {(lines, blocks * size)} and scales {(lines, blocks)} expected, "
@@ -71,7 +71,7 @@ class Mx4:
     def _empty(cls, lines: int, n: int, device: torch.device) -> Mx4:
         m, b = object.__new__(cls), -(-n // 128) * 4
         m.codes = torch.empty((lines, 16 * b), dtype=torch.uint8, device=device)
-        m.scales = torch.empty((lines, b), dtype=torch.uint8, device=device)
+        m.scales = m.codes.new_empty((lines, b))
         m.shape = lines, n
         return m
 
@@ -104,7 +104,7 @@ class Mx8:
     def _empty(cls, shape: tuple[int, int], axis: int, device: torch.device) -> Mx8:
         m, lines, b = object.__new__(cls), shape[1 - axis], -(-shape[axis] // 32)
         m.codes = torch.empty((lines, 32 * b), dtype=torch.uint8, device=device)
-        m.scales = torch.empty((lines, b), dtype=torch.uint8, device=device)
+        m.scales = m.codes.new_empty((lines, b))
         m.shape, m.axis = shape, axis
         return m
 
@@ -144,11 +144,14 @@ def _launch(device: torch.device, name: str, *args: object) -> None:
     index = device.index
     # (current_stream(device).cuda_stream without its Stream object, 2 us of a 10 us call)
     stream = torch._C._cuda_getCurrentRawStream(index)
+    fn = getattr(_lib.load(), name)
     if index == torch.cuda.current_device():
-        _lib.call(name, *args, stream)
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(index):
-            _lib.call(name, *args, stream)
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, name)
 
 
 def _values(m: Mx4 | Mx8, bits: int, shape: tuple[int, int], dtype: torch.dtype) -> torch.Tensor:
@@ -190,6 +193,20 @@ def activate(h: torch.Tensor, fn: str, axis: int = 1) -> tuple[torch.Tensor, Mx8
     return y, kept
 
 
+def quantise8(x: torch.Tensor, axis: int = 1) -> Mx8:
+    """``x`` ``[tokens, units]`` in 8-bit blocks along ``axis``: a level pair's
+    input, kept for :func:`weight_grad`."""
+    _check("quantise8", x)
+    if axis not in (0, 1):
+        raise ValueError(f"quantise8: axis 0 or 1 expected, got {axis}")
+    _on_gpu("quantise8", x.device)
+    kept = Mx8._empty(tuple(x.shape), axis, x.device)
+    _launch(x.device, "plx_mx8_activate", x.shape[1 - axis], x.shape[axis], DTYPES[x.dtype], FUNCTIONS["relu"],
+            x.data_ptr(), x.stride(1 - axis), x.stride(axis), None, 1, 1, kept.codes.data_ptr(),
+            kept.scales.data_ptr())
+    return kept
+
+
 def activate_grad(dy: torch.Tensor, kept: Mx8, fn: str) -> torch.Tensor:
     """``dy * fn'(q)``, q the values that :func:`activate` kept; dy's type and
     layout."""
@@ -207,21 +224,22 @@ def activate_grad(dy: torch.Tensor, kept: Mx8, fn: str) -> torch.Tensor:
     return dh
 
 
-def _workspace(device: torch.device, name: str, *args: object) -> tuple[torch.Tensor | None, int | None, int]:
-    """(the workspace that keeps the memory, its address, its bytes)."""
+def _workspace(device: torch.device, name: str, *args: object) -> torch.Tensor | None:
     need = getattr(_lib.load(), name)(*args)
-    if need <= 0:
-        _lib.check(int(need < 0), name)
-        return None, None, 0
-    work = torch.empty(need, dtype=torch.uint8, device=device)
-    return work, work.data_ptr(), need
+    if need > 0:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if need < 0:
+        raise ValueError(f"{name}: sizes past 2^30")
+    return None
 
 
 def _product(kind: int, a: torch.Tensor, m: Mx4 | Mx8, inputs: int, outputs: int, out: torch.Tensor) -> torch.Tensor:
-    of_a = DTYPES[a.dtype], a.data_ptr(), a.stride(0), a.stride(1)
-    _work, at, need = _workspace(a.device, "plx_mx_workspace", kind, a.shape[0], inputs, outputs, *of_a)
-    _launch(a.device, "plx_mx_product", kind, a.shape[0], inputs, outputs, *of_a, m.codes.data_ptr(),
-            m.scales.data_ptr(), out.data_ptr(), at, need)
+    device, tokens = a.device, a.shape[0]
+    of_a = (DTYPES[a.dtype], a.data_ptr(), *a.stride())
+    work = _workspace(device, "plx_mx_workspace", kind, tokens, inputs, outputs, *of_a)
+    at, need = (None, 0) if work is None else (work.data_ptr(), work.numel())
+    _launch(device, "plx_mx_product", kind, tokens, inputs, outputs, *of_a, m.codes.data_ptr(), m.scales.data_ptr(),
+            out.data_ptr(), at, need)
     return out
 
 
@@ -240,7 +258,8 @@ def product(x: torch.Tensor | Mx4, w: Mx4, dtype: torch.dtype | None = None) -> 
             raise TypeError(f"product: float32, bfloat16 or float16 expected, got {dtype}")
         _on_gpu("product", x.device, w.device)
         out = torch.empty((x.shape[0], outputs), dtype=dtype, device=x.device)
-        _work, at, need = _workspace(x.device, "plx_mx4_workspace", x.shape[0], inputs, outputs)
+        work = _workspace(x.device, "plx_mx4_workspace", x.shape[0], inputs, outputs)
+        at, need = (None, 0) if work is None else (work.data_ptr(), work.numel())
         _launch(x.device, "plx_mx4_product", x.shape[0], inputs, outputs, x.codes.data_ptr(), x.scales.data_ptr(),
                 w.codes.data_ptr(), w.scales.data_ptr(), DTYPES[dtype], out.data_ptr(), at, need)
         return out
@@ -250,8 +269,7 @@ def product(x: torch.Tensor | Mx4, w: Mx4, dtype: torch.dtype | None = None) -> 
     if x.shape[1] != inputs:
         raise ValueError(f"product: {inputs} inputs expected, got {x.shape[1]}")
     _on_gpu("product", x.device, w.device)
-    out = torch.empty((x.shape[0], outputs), dtype=x.dtype, device=x.device)
-    return _product(_PRODUCT, x, w, inputs, outputs, out)
+    return _product(_PRODUCT, x, w, inputs, outputs, x.new_empty((x.shape[0], outputs)))
 
 
 def product_grad(g: torch.Tensor, w: Mx4) -> torch.Tensor:
@@ -262,8 +280,7 @@ def product_grad(g: torch.Tensor, w: Mx4) -> torch.Tensor:
     if g.shape[1] != outputs:
         raise ValueError(f"product_grad: {outputs} outputs expected, got {g.shape[1]}")
     _on_gpu("product_grad", g.device, w.device)
-    return _product(_PRODUCT_GRAD, g, w, inputs, outputs,
-                    torch.empty((g.shape[0], inputs), dtype=g.dtype, device=g.device))
+    return _product(_PRODUCT_GRAD, g, w, inputs, outputs, g.new_empty((g.shape[0], inputs)))
 
 
 def weight_grad(g: torch.Tensor, kept: Mx8) -> torch.Tensor:

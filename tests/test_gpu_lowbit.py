@@ -116,6 +116,8 @@ def test_activate_and_its_gradient(shape, dtype, layout, axis) -> None:
         codes, scales = plain.quantise8(h if axis else h.t())
         assert torch.equal(kept.scales, scales)
         nan = (codes & 127) == 127  # (NaN has two codes)
+        alone = lowbit.quantise8(h, axis=axis)
+        assert torch.equal(alone.codes, kept.codes) and torch.equal(alone.scales, kept.scales)
         assert torch.equal(torch.where(nan, 0, kept.codes), torch.where(nan, 0, codes))
         assert bool(((kept.codes & 127) == 127)[nan].all())
         # an elementary function is good to 2 steps, 1 / (1 + e) adds a step, the product half of one: 4 steps
@@ -425,3 +427,17 @@ def test_offsets_past_32_bits() -> None:
     want = g[-80:].double().t() @ q
     # (the other lines add zeros)
     assert bool(((dw.double() - want).abs() <= size * plain.sum_bound(lines)).all())
+
+
+def test_the_example_learns_and_its_answers_are_the_arenas() -> None:
+    import pathlib
+    import sys
+
+    sys.path.insert(0, str(pathlib.Path(__file__).resolve().parents[1] / "examples"))
+    import lowbit_mlp
+
+    first, last, worst = lowbit_mlp.main(steps=120, samples=2)
+    assert last < first / 2
+    # tanh of sums of at most 256 terms through 3 levels: each sum is off by its bound times the terms' sizes (below
+    # 64 for weights of this size), each tanh by 2 steps
+    assert worst <= 3 * (64 * plain.sum_bound(256) + 256 * 64 * plain.U)

@@ -71,7 +71,7 @@ def test_formats_are_checked() -> None:
 
 def test_arguments_are_checked() -> None:
     x, w, kept = torch.zeros(5, 70), _mx4(9, 70), _mx8((5, 70), 1)
-    calls = [lambda t: lowbit.quantise4(t), lambda t: lowbit.activate(t, "relu"),
+    calls = [lambda t: lowbit.quantise4(t), lambda t: lowbit.quantise8(t), lambda t: lowbit.activate(t, "relu"),
              lambda t: lowbit.activate_grad(t, kept, "relu"), lambda t: lowbit.product(t, w),
              lambda t: lowbit.product_grad(t, _mx4(70, 9)), lambda t: lowbit.weight_grad(t, kept)]
     for call in calls:
@@ -104,6 +104,8 @@ def test_arguments_are_checked() -> None:
             lowbit.activate_grad(x, kept, fn)
     with pytest.raises(ValueError, match="axis"):
         lowbit.activate(x, "relu", axis=-1)
+    with pytest.raises(ValueError, match="axis"):
+        lowbit.quantise8(x, axis=2)
     with pytest.raises(TypeError):
         lowbit.product(x, w, dtype=torch.bfloat16)
     with pytest.raises(TypeError):
@@ -129,7 +131,8 @@ def test_entry_points_check_before_they_launch(lib) -> None:
     assert lib.plx_mx_values(4, 4, 4, p, None, 0, p, None) == 1
     assert lib.plx_mx_values(8, 4, 0, None, None, 0, None, None) == 0
     assert lib.plx_mx8_activate(4, 4, 0, 4, p, 4, 1, p, 4, 1, p, p, None) == 3
-    assert lib.plx_mx8_activate(4, 4, 0, 0, p, 4, 1, None, 4, 1, p, p, None) == 1
+    assert lib.plx_mx8_activate(4, 4, 0, 0, None, 4, 1, p, 4, 1, p, p, None) == 1
+    assert lib.plx_mx8_activate(4, 4, 0, 0, p, 4, 1, None, 4, 1, None, p, None) == 1
     assert lib.plx_mx8_activate(4, 0, 0, 0, None, 4, 1, None, 4, 1, None, None, None) == 0
     assert lib.plx_mx8_activate_grad(4, 4, 0, -1, p, 4, 1, p, p, p, 4, 1, None) == 3
     assert lib.plx_mx8_activate_grad(4, 4, 7, 0, p, 4, 1, p, p, p, 4, 1, None) == 3
