@@ -704,17 +704,17 @@ __global__ __launch_bounds__(kBlock) void k_big_pieces(int64_t lines, int64_t n,
   }
 }
 
+// Lines of n codes as bf16, out_n values each.
 template <int BITS>
 __global__ __launch_bounds__(kBlock) void k_big_values(int64_t lines, int64_t n, const uint8_t* codes,
-                                                       const uint8_t* scales, uint16_t* out, int64_t out_lines,
-                                                       int64_t out_n, int lx) {
+                                                       const uint8_t* scales, uint16_t* out, int64_t out_n, int lx) {
   const int64_t kept = BITS == 4 ? div_up(n, 128) * 16 : div_up(n, 32) * 4;
   const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
-  for (int64_t line = static_cast<int64_t>(blockIdx.x) * ly + ty; line < out_lines;
+  for (int64_t line = static_cast<int64_t>(blockIdx.x) * ly + ty; line < lines;
        line += static_cast<int64_t>(gridDim.x) * ly) {
     for (int64_t c = tx; c < out_n / 8; c += lx) {
       uint4 r = make_uint4(0, 0, 0, 0);
-      if (line < lines && c < kept) {
+      if (c < kept) {
         const float scale = scale_value(scales[line * (kept / 4) + c / 4]);
         r = BITS == 4 ? bf16_of4(reinterpret_cast<const uint32_t*>(codes)[line * kept + c], scale)
                       : bf16_of8(reinterpret_cast<const uint2*>(codes)[line * kept + c], scale);
@@ -728,7 +728,7 @@ __global__ __launch_bounds__(kBlock) void k_big_values(int64_t lines, int64_t n,
 // Host side
 // ---------------------------------------------------------------------------
 constexpr int64_t kMaxDim = int64_t{1} << 30;
-constexpr int64_t kBigLine = int64_t{1} << 22;  // elements of its lines: 256 of them stay below 2^32 bytes
+constexpr int64_t kBigLine = int64_t{1} << 22;  // elements of a large product's lines: 256 of them stay below 2^32 bytes
 
 inline bool dims_fit(int64_t a, int64_t b) { return a >= 0 && b >= 0 && a <= kMaxDim && b <= kMaxDim; }
 inline bool known(int dtype) { return dtype == PLX_LB_F32 || dtype == PLX_LB_BF16 || dtype == PLX_LB_F16; }
@@ -819,10 +819,9 @@ constexpr int64_t round_up(int64_t a, int64_t b) { return div_up(a, b) * b; }
 struct Plan {
   bool big;
   int splits;
-  bool across_a, across_b, direct;
-  int64_t kp;       // k padded to whole steps
-  int64_t mp, np;   // padded rows' lengths of "across" operands
-  int64_t bytes_a, bytes_b, bytes;
+  bool across, direct;  // a in lines of m; as it is
+  int64_t kp, mp;       // padded k, and lines of m
+  int64_t bytes_w, bytes_u, bytes;
 };
 
 // Workgroups that a large product should fill: one per CU.
@@ -837,23 +836,22 @@ int big_splits(int64_t m, int64_t n, int64_t steps) {
 Plan plan_of(int kind, const Shape& s, int dtype, const void* a, int64_t sm, int64_t sk) {
   Plan p{};
   const int pieces = dtype == PLX_LB_F32 ? 3 : dtype == PLX_LB_F16 ? 2 : 1;
-  p.big = large(s.m, s.n, s.k * pieces, kBigLeast);
+  p.big = large(s.m, s.n, s.k * pieces, kBigLeast) && s.k * pieces <= kBigLine && s.m <= kBigLine;
   if (!p.big) {
     if (kind == PLX_LB_PRODUCT && s.m <= kFew) return p;
     p.splits = tiles_of(s.m, s.n, s.k, 64).splits;
     p.bytes = p.splits > 1 ? int64_t{4} * p.splits * s.m * s.n : 0;
     return p;
   }
-  p.across_a = sm == 1 && sk != 1;
-  p.across_b = kind == PLX_LB_PRODUCT_GRAD || kind == PLX_LB_WEIGHT_GRAD;
-  p.kp = round_up(s.k, 64), p.mp = round_up(s.m, 8), p.np = round_up(s.n, 8);
-  const int64_t line = p.across_a ? sk : sm;
+  p.across = sm == 1 && sk != 1;
+  p.kp = round_up(s.k, 64), p.mp = round_up(s.m, 8);
+  const int64_t line = p.across ? sk : sm;
   p.direct = dtype == PLX_LB_BF16 && s.k % 64 == 0 && on16(a) && line % 8 == 0 && line <= kBigLine &&
-             (p.across_a ? s.m % 8 == 0 : sk == 1);
-  p.bytes_a = p.direct ? 0 : round_up(2 * pieces * p.kp * (p.across_a ? p.mp : s.m), 256);
-  p.bytes_b = round_up(2 * p.kp * (p.across_b ? p.np : s.n), 256);
+             (p.across ? s.m % 8 == 0 : sk == 1);
+  p.bytes_w = round_up(2 * p.kp * s.n, 256);
+  p.bytes_u = p.direct ? 0 : round_up(2 * pieces * p.kp * (p.across ? p.mp : s.m), 256);
   p.splits = big_splits(s.m, s.n, pieces * p.kp / 64);
-  p.bytes = p.bytes_a + p.bytes_b + (p.splits > 1 ? int64_t{4} * p.splits * s.m * s.n : 0);
+  p.bytes = p.bytes_w + p.bytes_u + (p.splits > 1 ? int64_t{4} * p.splits * s.m * s.n : 0);
   return p;
 }
 
@@ -867,44 +865,47 @@ void launch_join(int64_t n, int splits, const float* part, OT* out, hipStream_t 
 template <typename T, int KIND, typename OT>
 void launch_big(const GemmArgs& g, const Plan& p, char* work, hipStream_t s) {
   constexpr int P = Pieces<T>::n;
-  constexpr bool BA = KIND == kWT || KIND == kX;
+  constexpr int BITS = KIND == kW || KIND == kWT ? 4 : 8;
   BigArgs b{};
-  if (p.direct) {
-    b.a = static_cast<const char*>(g.a);
-    b.lda = 2 * (p.across_a ? g.sk : g.sm);
-    b.rows_a = g.M;
+  uint16_t* w = reinterpret_cast<uint16_t*>(work);
+  if (KIND == kWT || KIND == kX) {
+    const int tiles_n = static_cast<int>(div_up(g.N, 128));
+    k_big_turned<BITS><<<static_cast<unsigned>(p.kp / 64 * tiles_n), 256, 0, s>>>(g.K, g.N, g.blocks, g.codes, g.scales,
+                                                                                 w, p.kp, tiles_n);
   } else {
-    uint16_t* out = reinterpret_cast<uint16_t*>(work);
-    const int64_t lines = p.across_a ? g.K : g.M, n = p.across_a ? g.M : g.K;
-    const int64_t sl = p.across_a ? g.sk : g.sm, se = p.across_a ? g.sm : g.sk;
-    const int64_t out_lines = p.across_a ? p.kp : g.M, out_n = p.across_a ? p.mp : p.kp;
-    const int64_t out_line = p.across_a ? p.mp : P * p.kp, piece = p.across_a ? p.kp * p.mp : p.kp;
+    const int lx = lanes_along(p.kp / 8);
+    k_big_values<BITS><<<groups_along(g.N, lx), kBlock, 0, s>>>(g.N, g.K, g.codes, g.scales, w, p.kp, lx);
+  }
+  b.w = work;
+  b.ldw = 2 * p.kp;
+  b.wrap = static_cast<int>(p.kp / 64), b.steps = P * b.wrap;
+  if (p.direct) {
+    b.u = static_cast<const char*>(g.a);
+    b.ldu = 2 * (p.across ? g.sk : g.sm);
+    b.rows_u = g.M;
+  } else {
+    uint16_t* out = reinterpret_cast<uint16_t*>(work + p.bytes_w);
+    const int64_t lines = p.across ? g.K : g.M, n = p.across ? g.M : g.K;
+    const int64_t sl = p.across ? g.sk : g.sm, se = p.across ? g.sm : g.sk;
+    const int64_t out_lines = p.across ? p.kp : g.M, out_n = p.across ? p.mp : p.kp;
+    const int64_t out_line = p.across ? p.mp : P * p.kp, piece = p.across ? p.kp * p.mp : p.kp;
     const int lx = lanes_along(out_n / 8);
     k_big_pieces<T><<<groups_along(out_lines, lx), kBlock, 0, s>>>(lines, n, static_cast<const T*>(g.a), sl, se,
                                                                    out, out_lines, out_n, out_line, piece, lx);
-    b.a = work;
-    b.lda = 2 * out_line;
-    b.rows_a = static_cast<int>(p.across_a ? p.mp : g.M);
+    b.u = work + p.bytes_w;
+    b.ldu = 2 * out_line;
+    b.rows_u = static_cast<int>(p.across ? p.mp : g.M);
   }
-  uint16_t* vb = reinterpret_cast<uint16_t*>(work + p.bytes_a);
-  const int64_t lines = BA ? g.K : g.N, out_lines = BA ? p.kp : g.N, out_n = BA ? p.np : p.kp;
-  const int lx = lanes_along(out_n / 8);
-  k_big_values<KIND == kW || KIND == kWT ? 4 : 8><<<groups_along(out_lines, lx), kBlock, 0, s>>>(
-      lines, BA ? g.N : g.K, g.codes, g.scales, vb, out_lines, out_n, lx);
-  b.b = reinterpret_cast<const char*>(vb);
-  b.ldb = 2 * out_n;
-  b.rows_b = static_cast<int>(BA ? p.np : g.N);
   b.out = g.out;
-  b.part = reinterpret_cast<float*>(work + p.bytes_a + p.bytes_b);
+  b.part = reinterpret_cast<float*>(work + p.bytes_w + p.bytes_u);
   b.M = g.M, b.N = g.N;
-  b.wrap = static_cast<int>(p.kp / 64), b.steps = P * b.wrap;
   b.split = static_cast<int>(div_up(b.steps, p.splits));
   b.tiles_m = static_cast<int>(div_up(g.M, kBig)), b.tiles_n = static_cast<int>(div_up(g.N, kBig));
   const dim3 grid(static_cast<unsigned>(b.tiles_m) * b.tiles_n, static_cast<unsigned>(p.splits));
-  if (p.across_a)
-    k_big_gemm<true, BA, false, OT><<<grid, kBigThreads, 0, s>>>(b);
+  if (p.across)
+    k_big_gemm<true, false, OT><<<grid, kBigThreads, 0, s>>>(b);
   else
-    k_big_gemm<false, BA, false, OT><<<grid, kBigThreads, 0, s>>>(b);
+    k_big_gemm<false, false, OT><<<grid, kBigThreads, 0, s>>>(b);
   if (p.splits > 1) launch_join(static_cast<int64_t>(g.M) * g.N, p.splits, b.part, static_cast<OT*>(g.out), s);
 }
 
@@ -912,7 +913,7 @@ void launch_big(const GemmArgs& g, const Plan& p, char* work, hipStream_t s) {
 struct Plan4 {
   bool big;
   int steps, splits;
-  int64_t bytes_a, bytes_b, bytes;
+  int64_t bytes_w, bytes_u, bytes;
 };
 Plan4 plan4_of(int64_t m, int64_t n, int64_t k) {
   Plan4 p{};
@@ -924,8 +925,8 @@ Plan4 plan4_of(int64_t m, int64_t n, int64_t k) {
   }
   p.steps = static_cast<int>(div_up(k, 256));
   p.splits = big_splits(m, n, p.steps);
-  p.bytes_a = div_up(m, kBig) * p.steps * 2048, p.bytes_b = div_up(n, kBig) * p.steps * 2048;
-  p.bytes = p.bytes_a + p.bytes_b + (p.splits > 1 ? 4 * p.splits * m * n : 0);
+  p.bytes_w = div_up(n, kBig) * p.steps * 2048, p.bytes_u = div_up(m, kBig) * p.steps * 2048;
+  p.bytes = p.bytes_w + p.bytes_u + (p.splits > 1 ? 4 * p.splits * m * n : 0);
   return p;
 }
 
@@ -1140,20 +1141,20 @@ int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8
     hipStream_t s = static_cast<hipStream_t>(stream);
     char* work = static_cast<char*>(workspace);
     BigArgs g{};
-    g.a = reinterpret_cast<const char*>(x_codes), g.b = reinterpret_cast<const char*>(w_codes);
-    g.sa = work, g.sb = work + p.bytes_a;
-    g.out = out, g.part = reinterpret_cast<float*>(work + p.bytes_a + p.bytes_b);
-    g.M = g.rows_a = static_cast<int>(tokens), g.N = g.rows_b = static_cast<int>(outputs);
-    g.lda = g.ldb = blocks * 16;
+    g.w = reinterpret_cast<const char*>(w_codes), g.u = reinterpret_cast<const char*>(x_codes);
+    g.sw = work, g.su = work + p.bytes_w;
+    g.out = out, g.part = reinterpret_cast<float*>(work + p.bytes_w + p.bytes_u);
+    g.M = g.rows_u = static_cast<int>(tokens), g.N = static_cast<int>(outputs);
+    g.ldw = g.ldu = blocks * 16;
     g.steps = g.wrap = p.steps, g.split = static_cast<int>(div_up(p.steps, p.splits));
     g.tiles_m = static_cast<int>(div_up(tokens, kBig)), g.tiles_n = static_cast<int>(div_up(outputs, kBig));
     k_big_scales<<<static_cast<unsigned>((g.tiles_m + g.tiles_n) * div_up(p.steps, 8)), 256, 0, s>>>(
-        g.M, g.N, blocks, p.steps, x_scales, w_scales, reinterpret_cast<uint8_t*>(work),
-        reinterpret_cast<uint8_t*>(work + p.bytes_a));
+        g.N, g.M, blocks, p.steps, w_scales, x_scales, reinterpret_cast<uint8_t*>(work),
+        reinterpret_cast<uint8_t*>(work + p.bytes_w));
     with_type(dtype, [&](auto* t) {
       using T = PLX_TYPE(t);
       const dim3 grid(static_cast<unsigned>(g.tiles_m) * g.tiles_n, static_cast<unsigned>(p.splits));
-      k_big_gemm<false, false, true, T><<<grid, kBigThreads, 0, s>>>(g);
+      k_big_gemm<false, true, T><<<grid, kBigThreads, 0, s>>>(g);
       if (p.splits > 1) launch_join(tokens * outputs, p.splits, g.part, static_cast<T*>(out), s);
     });
     return check_launch("plx_mx4_product");

@@ -8,25 +8,26 @@
 
 namespace px {
 
-// out[m][n] = sum over k of a(m, k) b(n, k). An operand is kept "along" (rows
-// of k next to each other) or "across" (rows of m or n, one for each k).
+// out[m][n] = sum over k of u(m, k) w(n, k): w from codes, in lines of k
+// ("along": next to each other in memory), u the user's, in lines of k or of m
+// ("across"). w is the side of whose rows a wave has more.
 struct BigArgs {
-  const char* a;
-  const char* b;
-  int64_t lda, ldb;  // bytes of a row
-  void* out;         // [M][N]
-  float* part;       // [splits][M][N], where splits > 1
+  const char* w;
+  const char* u;
+  int64_t ldw, ldu;    // bytes of a line
+  void* out;           // [M][N]
+  float* part;         // [splits][M][N], where splits > 1
   int M, N;
-  int rows_a, rows_b;  // m and n that are in memory (M and N, or padded for "across")
-  int steps;         // of 64 k, over all of a's pieces
-  int wrap;          // steps of b, which starts again after them
-  const char* sa;    // 4 bits: the scales in the waves' order (k_big_scales)
-  const char* sb;
-  int split;         // steps of one k range
+  int rows_u;          // m that are in memory (M, or padded for "across")
+  int steps;           // of 64 k, over all of u's pieces
+  int wrap;            // steps of w, which starts again after them
+  const char* sw;      // 4 bits: the scales in the waves' order (k_big_scales)
+  const char* su;
+  int split;           // steps of one k range
   int tiles_m, tiles_n;
 };
 
-constexpr int kBig = 256;                 // rows and columns of a workgroup's tile
+constexpr int kBig = 256;              // rows and columns of a workgroup's tile
 constexpr int kBigThreads = 512;
 constexpr int kBigBytes = kBig * 128;     // of one operand's step in LDS
 
@@ -132,7 +133,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// A wave's results, from its first row and column on: with b's rows as the
+// A wave's results, from its first row and column on: with w's rows as the
 // matrix instruction's first operand a lane holds runs of four consecutive n
 // of one m: one in a fragment of 16 x 16, in one of 32 x 32 four, 8 columns
 // apart, lanes l and l + 32 having neighbouring runs of the same row. Tiles
@@ -141,20 +142,20 @@ template <typename T>
 __device__ __forceinline__ void big_store(const f32x4 (&acc)[2][2][4][2], T* out, int M, int N, int m, int n,
                                           bool whole) {
 #pragma unroll
-  for (int ha = 0; ha < 2; ++ha)
+  for (int hu = 0; hu < 2; ++hu)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = m + ha * 128 + i * 16;
+    for (int j = 0; j < 2; ++j) {
+      const int row = m + hu * 128 + j * 16;
       T* p = out + static_cast<int64_t>(row) * N + n;
 #pragma unroll
-      for (int hb = 0; hb < 2; ++hb)
+      for (int hw = 0; hw < 2; ++hw)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int col = hb * 128 + j * 16;
+        for (int i = 0; i < 4; ++i) {
+          const int col = hw * 128 + i * 16;
           if (whole)
-            store4(p + col, 4, acc[ha][hb][i][j]);
+            store4(p + col, 4, acc[hw][hu][i][j]);
           else if (row < M)
-            store4(p + col, N - n - col, acc[ha][hb][i][j]);
+            store4(p + col, N - n - col, acc[hw][hu][i][j]);
         }
     }
 }
@@ -163,13 +164,13 @@ __device__ __forceinline__ void big_store(const f32x16 (&acc)[2][2][2][1], T* ou
                                           bool whole) {
   const bool upper = (threadIdx.x & 32) != 0;
 #pragma unroll
-  for (int ha = 0; ha < 2; ++ha)
+  for (int hu = 0; hu < 2; ++hu) {
+    const int row = m + hu * 128;
+    T* p = out + static_cast<int64_t>(row) * N + n;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = m + ha * 128 + i * 32;
-      T* p = out + static_cast<int64_t>(row) * N + n;
+    for (int hw = 0; hw < 2; ++hw)
 #pragma unroll
-      for (int hb = 0; hb < 2; ++hb)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
           // Runs r and r + 1 of both lanes, 16 columns: the lower lane gets
@@ -177,121 +178,121 @@ __device__ __forceinline__ void big_store(const f32x16 (&acc)[2][2][2][1], T* ou
           float v[8];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[ha][hb][i][0][4 * r + k]),
-                                                            __float_as_uint(acc[ha][hb][i][0][4 * r + 4 + k]), false,
+            const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[hw][hu][i][0][4 * r + k]),
+                                                            __float_as_uint(acc[hw][hu][i][0][4 * r + 4 + k]), false,
                                                             false);
             v[k] = __uint_as_float(t[0]), v[4 + k] = __uint_as_float(t[1]);
           }
-          const int col = hb * 128 + r * 8 + (upper ? 4 : 0);  // (n is 4 more in the upper lane)
+          const int col = hw * 128 + i * 32 + r * 8 + (upper ? 4 : 0);  // (n is 4 more in the upper lane)
           if (whole)
             store8(p + col, 8, v);
           else if (row < M)
             store8(p + col, N - n - col, v);
         }
-    }
+  }
 }
 
-// 256 x 256 of the output by 8 waves. A wave has 64 rows of m in each half of
-// its a and 32 of n in each half of b, so four quarters of 64 x 32, one a
-// phase: LDS reads and global loads, barrier, 16 matrix instructions,
-// barrier. The second four waves are one barrier behind the first, so that on
-// each SIMD one wave multiplies while the other one loads. A half of a buffer
-// is loaded for the step after next as soon as both have read it, nearly two
-// steps before it is needed. F4: both operands in 4-bit blocks along k, 8 of
-// them in a line's 128 bytes: a lane's 16 bytes are one block, and the LDS
-// layout and the fragments' addresses are the bf16 ones'. The scales of a step
-// come in the waves' order (k_big_scales) and by way of LDS too, a lane's own
-// in 16 and 8 bytes.
-template <bool AA, bool BA, bool F4, typename OT>
+// 256 x 256 of the output by 8 waves. A wave has 64 rows in each half of its w
+// and 32 in each half of u, so four quarters of 64 x 32, one a phase: LDS
+// reads and global loads, barrier, 16 matrix instructions, barrier. The second
+// four waves are one barrier behind the first, so that on each SIMD one wave
+// multiplies while the other one loads. A half of a buffer is loaded for the
+// step after next as soon as both have read it, nearly two steps before it is
+// needed. F4: both operands in 4-bit blocks along k, 8 of them in a line's 128
+// bytes: a lane's 16 bytes are one block, and the LDS layout is the bf16 one.
+// The scales of a step come in the waves' order (k_big_scales) and by way of
+// LDS too, a lane's own in 16 and 8 bytes.
+template <bool UA, bool F4, typename OT>
 __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
   __shared__ __align__(16) char lds[4 * kBigBytes + (F4 ? 2 * 4096 : 0)];
   lds_char* l = (lds_char*)lds;
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 2, wc = wave & 3;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), ww = wave >> 2, wu = wave & 3;
   int tm, tn;
   big_tile(blockIdx.x, g.tiles_m, g.tiles_n, &tm, &tn);
   const int m0 = tm * kBig, n0 = tn * kBig;
 
-  uint32_t oa[4], ob[4];
-  big_offsets<AA, F4>(tid, m0, g.rows_a, g.lda, oa);
-  big_offsets<BA, F4>(tid, n0, g.rows_b, g.ldb, ob);
-  const int64_t sa = AA ? 64 * g.lda : 128, sb = BA ? 64 * g.ldb : 128;
+  uint32_t ow[4], ou[4];
+  big_offsets<false, F4>(tid, n0, g.N, g.ldw, ow);
+  big_offsets<UA, F4>(tid, m0, g.rows_u, g.ldu, ou);
+  const int64_t su = UA ? 64 * g.ldu : 128;
   const int beg = blockIdx.y * g.split, end = beg + g.split < g.steps ? beg + g.split : g.steps;
-  const char* a = g.a + (AA ? int64_t{2} * m0 : m0 * g.lda) + beg * sa;
-  const char* b = g.b + (BA ? int64_t{2} * n0 : n0 * g.ldb);
-  int bt = beg % g.wrap;
+  const char* w = g.w + n0 * g.ldw;
+  const char* u = g.u + (UA ? int64_t{2} * m0 : m0 * g.ldu) + beg * su;
+  int wt = beg % g.wrap;
   // 4 bits: a line of an odd number of 64 bytes ends inside its last step,
   // which then reads its first half twice and multiplies it once.
-  const bool odd = F4 && (g.lda & 64) != 0;
+  const bool odd = F4 && (g.ldw & 64) != 0;
   const uint32_t back = (((tid & 7) ^ ((tid >> 3) & 7) ^ ((tid >> 7) & 1)) & 4) ? 64 : 0;
-  // 4 KB of scales a step, by the first four waves: a's, then b's.
+  // 4 KB of scales a step, by the first four waves: w's, then u's.
   const char* gs = nullptr;
-  u32x4 xs = {};
-  u32x2 ws = {};
+  u32x4 ws = {};
+  u32x2 us = {};
   if (F4)
-    gs = (wave < 2 ? g.sa + (static_cast<int64_t>(tm) * g.steps + beg) * 2048
-                   : g.sb + (static_cast<int64_t>(tn) * g.steps + beg) * 2048) +
+    gs = (wave < 2 ? g.sw + (static_cast<int64_t>(tn) * g.steps + beg) * 2048
+                   : g.su + (static_cast<int64_t>(tm) * g.steps + beg) * 2048) +
          (wave & 1) * 1024 + lane * 16;
 
   // Fragments: 16 rows by 32 k, or 32 rows by 64 k of 4 bits; of either a
-  // quarter's 64 x 32 take FA x FB, in S steps of k.
-  constexpr int FA = F4 ? 2 : 4, FB = F4 ? 1 : 2, S = F4 ? 4 : 2;
+  // quarter's 64 x 32 take FW x FU, in S steps of k.
+  constexpr int FW = F4 ? 2 : 4, FU = F4 ? 1 : 2, S = F4 ? 4 : 2;
   typedef typename std::conditional<F4, f32x16, f32x4>::type sums;
-  typename std::conditional<F4, Big4Frags<FA>, BigFrags<AA, FA>>::type fa;
-  typename std::conditional<F4, Big4Frags<FB>, BigFrags<BA, FB>>::type fb;
+  typename std::conditional<F4, Big4Frags<FW>, BigFrags<false, FW>>::type fw;
+  typename std::conditional<F4, Big4Frags<FU>, BigFrags<UA, FU>>::type fu;
   if constexpr (F4) {
-    fa.init(wr * 64, lane);
-    fb.init(wc * 32, lane);
+    fw.init(ww * 64, lane);
+    fu.init(wu * 32, lane);
   } else {
-    fa.init(wr * 64, l15, q);
-    fb.init(wc * 32, l15, q);
+    fw.init(ww * 64, l15, q);
+    fu.init(wu * 32, l15, q);
   }
-  sums acc[2][2][FA][FB] = {};
-  bf16x8 ra[FA][S], rb[2][FB][S];
+  sums acc[2][2][FW][FU] = {};
+  bf16x8 rw[FW][S], ru[2][FU][S];
 
-  // The next step's pointers; `t` is the step whose first load this is.
-  auto load_a0b0 = [&](int t, int buf) {
+  // A step's four loads, of w's and u's first halves (the step is t), u's and
+  // w's second ones; the last of them moves on to the next step.
+  auto load_w0u0 = [&](int t, int buf) {
     if (odd && t + 1 == g.steps) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) oa[i] -= back, ob[i] -= back;
+      for (int i = 0; i < 4; ++i) ow[i] -= back, ou[i] -= back;
     }
-    big_load(a, oa, l + buf * 2 * kBigBytes, wave);
-    big_load(b + bt * sb, ob, l + buf * 2 * kBigBytes + kBigBytes, wave);
+    big_load(w + static_cast<int64_t>(wt) * 128, ow, l + buf * 2 * kBigBytes, wave);
+    big_load(u, ou, l + buf * 2 * kBigBytes + kBigBytes, wave);
   };
-  auto load_b1 = [&](int buf) { big_load(b + bt * sb, ob + 2, l + buf * 2 * kBigBytes + kBigBytes + kBigBytes / 2, wave); };
-  auto load_a1 = [&](int buf) {
-    big_load(a, oa + 2, l + buf * 2 * kBigBytes + kBigBytes / 2, wave);
+  auto load_u1 = [&](int buf) { big_load(u, ou + 2, l + buf * 2 * kBigBytes + kBigBytes + kBigBytes / 2, wave); };
+  auto load_w1 = [&](int buf) {
+    big_load(w + static_cast<int64_t>(wt) * 128, ow + 2, l + buf * 2 * kBigBytes + kBigBytes / 2, wave);
     if (F4 && wave < 4) {
       __builtin_amdgcn_global_load_lds(
           (glb_char*)gs, (__attribute__((address_space(3))) void*)(l + 4 * kBigBytes + buf * 4096 + wave * 1024), 16, 0, 0);
       gs += 2048;
     }
-    a += sa;
-    bt = bt + 1 == g.wrap ? 0 : bt + 1;
+    u += su;
+    wt = wt + 1 == g.wrap ? 0 : wt + 1;
   };
-  auto read_a = [&](int buf, int h) {
+  auto read_w = [&](int buf, int h) {
     const lds_char* p = l + buf * 2 * kBigBytes + h * (kBigBytes / 2);
 #pragma unroll
-    for (int i = 0; i < FA; ++i)
+    for (int i = 0; i < FW; ++i)
 #pragma unroll
-      for (int s = 0; s < S; ++s) ra[i][s] = fa.get(p, i, s);
+      for (int s = 0; s < S; ++s) rw[i][s] = fw.get(p, i, s);
   };
-  auto read_b = [&](int buf, auto half) {
+  auto read_u = [&](int buf, auto half) {
     constexpr int h = decltype(half)::value;
     const lds_char* p = l + buf * 2 * kBigBytes + kBigBytes + h * (kBigBytes / 2);
 #pragma unroll
-    for (int i = 0; i < FB; ++i)
+    for (int i = 0; i < FU; ++i)
 #pragma unroll
-      for (int s = 0; s < S; ++s) rb[h][i][s] = fb.get(p, i, s);
+      for (int s = 0; s < S; ++s) ru[h][i][s] = fu.get(p, i, s);
   };
-  auto multiply = [&](auto half_a, auto half_b, bool both) {
-    constexpr int ha = decltype(half_a)::value, hb = decltype(half_b)::value;
+  auto multiply = [&](auto half_w, auto half_u, bool both) {
+    constexpr int hw = decltype(half_w)::value, hu = decltype(half_u)::value;
     __builtin_amdgcn_s_setprio(1);
     if constexpr (F4) {
 #define PX_F4(i, s)                                                                                            \
-  acc[ha][hb][i][0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                         \
-      as_i32x8(rb[hb][0][s]), as_i32x8(ra[i][s]), acc[ha][hb][i][0], 4, 4, s, static_cast<int>(ws[hb]), s,     \
-      static_cast<int>(xs[ha * 2 + (i)]))
+  acc[hw][hu][i][0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                         \
+      as_i32x8(rw[i][s]), as_i32x8(ru[hu][0][s]), acc[hw][hu][i][0], 4, 4, s,                                  \
+      static_cast<int>(ws[hw * 2 + (i)]), s, static_cast<int>(us[hu]))
       PX_F4(0, 0), PX_F4(1, 0), PX_F4(0, 1), PX_F4(1, 1);
       if (both) PX_F4(0, 2), PX_F4(1, 2), PX_F4(0, 3), PX_F4(1, 3);
 #undef PX_F4
@@ -302,8 +303,8 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            acc[ha][hb][i][j] =
-                __builtin_amdgcn_mfma_f32_16x16x32_bf16(rb[hb][j][s], ra[i][s], acc[ha][hb][i][j], 0, 0, 0);
+            acc[hw][hu][i][j] =
+                __builtin_amdgcn_mfma_f32_16x16x32_bf16(rw[i][s], ru[hu][j][s], acc[hw][hu][i][j], 0, 0, 0);
     }
     __builtin_amdgcn_s_setprio(0);
   };
@@ -317,50 +318,50 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
     else
       asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
   };
-  load_a0b0(beg, 0);
-  load_b1(0);
-  load_a1(0);
+  load_w0u0(beg, 0);
+  load_u1(0);
+  load_w1(0);
   if (beg + 1 < end) {
-    load_a0b0(beg + 1, 1);
-    load_b1(1);
-    load_a1(1);
+    load_w0u0(beg + 1, 1);
+    load_u1(1);
+    load_w1(1);
     wait_older();
   } else {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   big_barrier();
-  if (wr) big_barrier();
+  if (ww) big_barrier();
   for (int t = beg; t < end; ++t) {
     const int buf = (t - beg) & 1;
     const bool more = t + 2 < end, both = !(odd && t + 1 == g.steps);
-    read_b(buf, k0);
-    read_a(buf, 0);
+    read_u(buf, k0);
+    read_w(buf, 0);
     if (F4) {
       const lds_char* p = l + 4 * kBigBytes + buf * 4096;
       // (Written out, and waited for in place: the compiler would wait for
       // every load under way before it.)
       asm volatile(
           "ds_read_b128 %0, %2\n\tds_read_b64 %1, %3 offset:2048\n\ts_waitcnt lgkmcnt(0)"
-          : "=&v"(xs), "=&v"(ws)
-          : "v"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p + wr * 1024 + lane * 16))),
-            "v"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p + wc * 512 + lane * 8)))
+          : "=&v"(ws), "=&v"(us)
+          : "v"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p + ww * 1024 + lane * 16))),
+            "v"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p + wu * 512 + lane * 8)))
           : "memory");
     }
     big_barrier();
     multiply(k0, k0, both);
     big_barrier();
-    read_b(buf, k1);
-    if (more) load_a0b0(t + 2, buf);
+    read_u(buf, k1);
+    if (more) load_w0u0(t + 2, buf);
     big_barrier();
     multiply(k0, k1, both);
     big_barrier();
-    read_a(buf, 1);
-    if (more) load_b1(buf);
+    read_w(buf, 1);
+    if (more) load_u1(buf);
     big_barrier();
     multiply(k1, k1, both);
     big_barrier();
     if (more) {
-      load_a1(buf);
+      load_w1(buf);
       wait_older();
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -369,9 +370,9 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
     multiply(k1, k0, both);
     big_barrier();
   }
-  if (!wr) big_barrier();
+  if (!ww) big_barrier();
 
-  const int m = m0 + wr * 64 + (F4 ? lane & 31 : l15), n = n0 + wc * 32 + (F4 ? (lane >> 5) * 4 : q * 4);
+  const int m = m0 + wu * 32 + (F4 ? lane & 31 : l15), n = n0 + ww * 64 + (F4 ? (lane >> 5) * 4 : q * 4);
   const bool whole = m0 + kBig <= g.M && n0 + kBig <= g.N;
   if (gridDim.y > 1)
     big_store(acc, g.part + static_cast<int64_t>(blockIdx.y) * g.M * g.N, g.M, g.N, m, n, false);
@@ -416,14 +417,49 @@ __device__ __forceinline__ void big_scales(int tile, int step0, int steps, int r
   }
 }
 
-__global__ __launch_bounds__(256) void k_big_scales(int M, int N, int64_t blocks, int steps, const uint8_t* xs,
-                                                    const uint8_t* ws, uint8_t* sa, uint8_t* sb) {
+__global__ __launch_bounds__(256) void k_big_scales(int N, int M, int64_t blocks, int steps, const uint8_t* ws,
+                                                    const uint8_t* us, uint8_t* sw, uint8_t* su) {
   __shared__ uint8_t lds[256 * kScaleRow];
-  const int runs = (steps + 7) / 8, tile = blockIdx.x / runs, step0 = blockIdx.x % runs * 8, tiles_m = (M + 255) / 256;
-  if (tile < tiles_m)
-    big_scales<2>(tile, step0, steps, M, blocks, xs, sa, lds);
+  const int runs = (steps + 7) / 8, tile = blockIdx.x / runs, step0 = blockIdx.x % runs * 8, tiles_n = (N + 255) / 256;
+  if (tile < tiles_n)
+    big_scales<2>(tile, step0, steps, N, blocks, ws, sw, lds);
   else
-    big_scales<1>(tile - tiles_m, step0, steps, N, blocks, ws, sb, lds);
+    big_scales<1>(tile - tiles_n, step0, steps, M, blocks, us, su, lds);
+}
+
+// Lines of k in codes (k_big_gemm's "across") to bf16 lines of n, kp values
+// each: 64 k by 128 n go through LDS in k_big_gemm's layout and come back
+// transposed. k past `lines` are zeros.
+template <int BITS>
+__global__ __launch_bounds__(256) void k_big_turned(int lines, int n, int64_t blocks, const uint8_t* codes,
+                                                    const uint8_t* scales, uint16_t* out, int64_t kp, int tiles_n) {
+  __shared__ __align__(16) char lds[64 * 256];
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q = lane >> 4, wave = tid >> 6;
+  const int k0 = (blockIdx.x / tiles_n) * 64, n0 = (blockIdx.x % tiles_n) * 128;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int u = i * 256 + tid, line = u >> 4, c = u & 15, pos = n0 + c * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (k0 + line < lines && pos < blocks * 32) {
+      const int64_t at = (k0 + line) * blocks * 4 + pos / 8;
+      const float scale = scale_value(scales[at / 4]);
+      v = BITS == 4 ? bf16_of4(reinterpret_cast<const uint32_t*>(codes)[at], scale)
+                    : bf16_of8(reinterpret_cast<const uint2*>(codes)[at], scale);
+    }
+    *reinterpret_cast<uint4*>(lds + line * 256 + ((c >> 1) ^ ((line & 3) | ((line >> 3) & 1) << 2)) * 32 + (c & 1) * 16) = v;
+  }
+  __syncthreads();
+  BigFrags<true, 2> f;
+  f.init(wave * 32, l15, q);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = n0 + wave * 32 + i * 16 + l15;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const bf16x8 v = f.get((const lds_char*)lds, i, s);
+      if (row < n) *reinterpret_cast<bf16x8*>(out + row * kp + k0 + s * 32 + q * 8) = v;
+    }
+  }
 }
 
 }  // namespace px
