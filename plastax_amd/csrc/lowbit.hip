@@ -681,56 +681,16 @@ __global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks,
 }
 
 // ---------------------------------------------------------------------------
-// Operands of the large products: bf16 lines padded with zeros.
-// ---------------------------------------------------------------------------
-// Piece p of line l at out + p * piece + l * out_line.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void k_big_pieces(int64_t lines, int64_t n, const T* x, int64_t sl, int64_t se,
-                                                       uint16_t* out, int64_t out_lines, int64_t out_n,
-                                                       int64_t out_line, int64_t piece, int lx) {
-  constexpr int P = Pieces<T>::n;
-  const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
-  for (int64_t line = static_cast<int64_t>(blockIdx.x) * ly + ty; line < out_lines;
-       line += static_cast<int64_t>(gridDim.x) * ly) {
-    for (int64_t c = tx; c < out_n / 8; c += lx) {
-      const int64_t left = line < lines ? n - c * 8 : 0;
-      float v[8];
-      load8(x + line * sl + c * 8 * se, se, left > 8 ? 8 : left < 0 ? 0 : static_cast<int>(left), v);
-      uint4 p[P];
-      pieces8<P>(v, p);
-#pragma unroll
-      for (int i = 0; i < P; ++i) *reinterpret_cast<uint4*>(out + i * piece + line * out_line + c * 8) = p[i];
-    }
-  }
-}
-
-// Lines of n codes as bf16, out_n values each.
-template <int BITS>
-__global__ __launch_bounds__(kBlock) void k_big_values(int64_t lines, int64_t n, const uint8_t* codes,
-                                                       const uint8_t* scales, uint16_t* out, int64_t out_n, int lx) {
-  const int64_t kept = BITS == 4 ? div_up(n, 128) * 16 : div_up(n, 32) * 4;
-  const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
-  for (int64_t line = static_cast<int64_t>(blockIdx.x) * ly + ty; line < lines;
-       line += static_cast<int64_t>(gridDim.x) * ly) {
-    for (int64_t c = tx; c < out_n / 8; c += lx) {
-      uint4 r = make_uint4(0, 0, 0, 0);
-      if (c < kept) {
-        const float scale = scale_value(scales[line * (kept / 4) + c / 4]);
-        r = BITS == 4 ? bf16_of4(reinterpret_cast<const uint32_t*>(codes)[line * kept + c], scale)
-                      : bf16_of8(reinterpret_cast<const uint2*>(codes)[line * kept + c], scale);
-      }
-      *reinterpret_cast<uint4*>(out + line * out_n + c * 8) = r;
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 constexpr int64_t kMaxDim = int64_t{1} << 30;
 constexpr int64_t kBigLine = int64_t{1} << 22;  // elements of a large product's lines: 256 of them stay below 2^32 bytes
 
 inline bool dims_fit(int64_t a, int64_t b) { return a >= 0 && b >= 0 && a <= kMaxDim && b <= kMaxDim; }
+constexpr int64_t kMaxUnits = int64_t{1} << 24;  // of a level in products: a launch's tiles stay below 2^30 lanes
+inline bool product_fits(int64_t tokens, int64_t inputs, int64_t outputs) {
+  return tokens >= 0 && inputs >= 0 && outputs >= 0 && tokens <= kMaxDim && inputs <= kMaxUnits && outputs <= kMaxUnits;
+}
 inline bool known(int dtype) { return dtype == PLX_LB_F32 || dtype == PLX_LB_BF16 || dtype == PLX_LB_F16; }
 
 template <typename F>
@@ -766,8 +726,10 @@ inline unsigned groups_across(int64_t lines, int64_t blocks) {
 // large and 68 to 77 in small tiles, 17.2e9 in bf16 45 to 65 and 68 to 87; in
 // 4 bits 17.2e9 take 41 us large and 26 to 30 in small tiles.
 constexpr double kBigLeast = 9e9, kBig4Least = 25e9;
+// (Beyond 2^30 lanes of a launch, products go in small tiles, cut into launches.)
 inline bool large(int64_t m, int64_t n, int64_t k, double least) {
-  return m >= 256 && n >= 256 && k >= 256 && static_cast<double>(m) * n * k >= least;
+  return m >= 256 && n >= 256 && k >= 256 && static_cast<double>(m) * n * k >= least &&
+         div_up(m, kBig) * div_up(n, kBig) <= int64_t{1} << 21 && n * k <= int64_t{1} << 34;
 }
 
 // How a product in small tiles runs: tiles of ts x ts, ks groups of waves in a
@@ -866,36 +828,36 @@ template <typename T, int KIND, typename OT>
 void launch_big(const GemmArgs& g, const Plan& p, char* work, hipStream_t s) {
   constexpr int P = Pieces<T>::n;
   constexpr int BITS = KIND == kW || KIND == kWT ? 4 : 8;
+  constexpr bool turned = KIND == kWT || KIND == kX;
   BigArgs b{};
-  uint16_t* w = reinterpret_cast<uint16_t*>(work);
-  if (KIND == kWT || KIND == kX) {
-    const int tiles_n = static_cast<int>(div_up(g.N, 128));
-    k_big_turned<BITS><<<static_cast<unsigned>(p.kp / 64 * tiles_n), 256, 0, s>>>(g.K, g.N, g.blocks, g.codes, g.scales,
-                                                                                 w, p.kp, tiles_n);
-  } else {
-    const int lx = lanes_along(p.kp / 8);
-    k_big_values<BITS><<<groups_along(g.N, lx), kBlock, 0, s>>>(g.N, g.K, g.codes, g.scales, w, p.kp, lx);
-  }
+  BigValues v{};
+  v.lines = turned ? g.K : g.N, v.n = turned ? g.N : g.K, v.blocks = g.blocks;
+  v.codes = g.codes, v.scales = g.scales, v.out = reinterpret_cast<uint16_t*>(work), v.kp = p.kp;
+  v.tiles_n = static_cast<int>(div_up(g.N, 128)), v.lx = lanes_along(p.kp / 8);
+  const unsigned groups = turned ? static_cast<unsigned>(p.kp / 64 * v.tiles_n) : groups_along(g.N, v.lx);
   b.w = work;
   b.ldw = 2 * p.kp;
   b.wrap = static_cast<int>(p.kp / 64), b.steps = P * b.wrap;
+  BigPieces u{};
+  unsigned more = 0;
   if (p.direct) {
     b.u = static_cast<const char*>(g.a);
     b.ldu = 2 * (p.across ? g.sk : g.sm);
     b.rows_u = g.M;
   } else {
-    uint16_t* out = reinterpret_cast<uint16_t*>(work + p.bytes_w);
-    const int64_t lines = p.across ? g.K : g.M, n = p.across ? g.M : g.K;
-    const int64_t sl = p.across ? g.sk : g.sm, se = p.across ? g.sm : g.sk;
-    const int64_t out_lines = p.across ? p.kp : g.M, out_n = p.across ? p.mp : p.kp;
-    const int64_t out_line = p.across ? p.mp : P * p.kp, piece = p.across ? p.kp * p.mp : p.kp;
-    const int lx = lanes_along(out_n / 8);
-    k_big_pieces<T><<<groups_along(out_lines, lx), kBlock, 0, s>>>(lines, n, static_cast<const T*>(g.a), sl, se,
-                                                                   out, out_lines, out_n, out_line, piece, lx);
+    u.x = g.a;
+    u.lines = p.across ? g.K : g.M, u.n = p.across ? g.M : g.K;
+    u.sl = p.across ? g.sk : g.sm, u.se = p.across ? g.sm : g.sk;
+    u.out = reinterpret_cast<uint16_t*>(work + p.bytes_w);
+    u.out_lines = p.across ? p.kp : g.M, u.out_n = p.across ? p.mp : p.kp;
+    u.out_line = p.across ? p.mp : P * p.kp, u.piece = p.across ? p.kp * p.mp : p.kp;
+    u.lx = lanes_along(u.out_n / 8);
+    more = groups_along(u.out_lines, u.lx);
     b.u = work + p.bytes_w;
-    b.ldu = 2 * out_line;
+    b.ldu = 2 * u.out_line;
     b.rows_u = static_cast<int>(p.across ? p.mp : g.M);
   }
+  k_big_operands<T, BITS, turned><<<groups + more, 256, 0, s>>>(v, u, groups);
   b.out = g.out;
   b.part = reinterpret_cast<float*>(work + p.bytes_w + p.bytes_u);
   b.M = g.M, b.N = g.N;
@@ -1076,8 +1038,8 @@ int plx_mx8_activate_grad(int64_t lines, int64_t n, int32_t dtype, int32_t fn, c
 
 int64_t plx_mx_workspace(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs, int32_t dtype, const void* a,
                          int64_t token_stride, int64_t unit_stride) {
-  if (kind < PLX_LB_PRODUCT || kind > PLX_LB_WEIGHT_GRAD_COLUMNS || !known(dtype) || !dims_fit(tokens, inputs) ||
-      !dims_fit(outputs, outputs))
+  if (kind < PLX_LB_PRODUCT || kind > PLX_LB_WEIGHT_GRAD_COLUMNS || !known(dtype) ||
+      !product_fits(tokens, inputs, outputs))
     return -1;
   const bool grad = kind >= PLX_LB_WEIGHT_GRAD;
   return plan_of(kind, shape_of(kind, tokens, inputs, outputs), dtype, a, grad ? unit_stride : token_stride,
@@ -1090,7 +1052,7 @@ int plx_mx_product(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs
                    void* workspace, int64_t workspace_bytes, void* stream) {
   if (kind < PLX_LB_PRODUCT || kind > PLX_LB_WEIGHT_GRAD_COLUMNS)
     return fail(PLX_ERR_UNSUPPORTED, "plx_mx_product: unknown kind");
-  if (!dims_fit(tokens, inputs) || !dims_fit(outputs, outputs)) return fail(PLX_ERR_INVALID, "plx_mx_product: bad size");
+  if (!product_fits(tokens, inputs, outputs)) return fail(PLX_ERR_INVALID, "plx_mx_product: bad size");
   if (!known(dtype)) return fail(PLX_ERR_UNSUPPORTED, "plx_mx_product: unknown element type");
   const Shape sh = shape_of(kind, tokens, inputs, outputs);
   if (sh.m == 0 || sh.n == 0) return PLX_OK;
@@ -1119,15 +1081,14 @@ int plx_mx_product(int32_t kind, int64_t tokens, int64_t inputs, int64_t outputs
 }
 
 int64_t plx_mx4_workspace(int64_t tokens, int64_t inputs, int64_t outputs) {
-  if (!dims_fit(tokens, inputs) || !dims_fit(outputs, outputs)) return -1;
+  if (!product_fits(tokens, inputs, outputs)) return -1;
   return plan4_of(tokens, outputs, inputs).bytes;
 }
 
 int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8_t* x_codes, const uint8_t* x_scales,
                     const uint8_t* w_codes, const uint8_t* w_scales, int32_t dtype, void* out, void* workspace,
                     int64_t workspace_bytes, void* stream) {
-  if (!dims_fit(tokens, inputs) || !dims_fit(outputs, outputs))
-    return fail(PLX_ERR_INVALID, "plx_mx4_product: bad size");
+  if (!product_fits(tokens, inputs, outputs)) return fail(PLX_ERR_INVALID, "plx_mx4_product: bad size");
   if (!known(dtype)) return fail(PLX_ERR_UNSUPPORTED, "plx_mx4_product: unknown element type");
   if (tokens == 0 || outputs == 0) return PLX_OK;
   if (!out || (inputs > 0 && (!x_codes || !x_scales || !w_codes || !w_scales)))

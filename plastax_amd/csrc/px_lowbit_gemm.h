@@ -388,6 +388,7 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
 // 128 h + 32 (F wave + f) + lane % 32 in block 8 step + 2 s + lane / 32. Rows and
 // blocks past the end get the scale 1. A workgroup takes 8 steps of a tile
 // through LDS.
+typedef uint32_t u32_any __attribute__((aligned(1)));  // (scale bytes start anywhere)
 constexpr int kScaleRow = 68;  // bytes of 8 steps of a row in LDS, and 4 that move the rows over the banks
 template <int F>
 __device__ __forceinline__ void big_scales(int tile, int step0, int steps, int rows, int64_t blocks, const uint8_t* in,
@@ -400,7 +401,7 @@ __device__ __forceinline__ void big_scales(int tile, int step0, int steps, int r
     const int row = tile * 256 + r;
     uint32_t v = 0x7F7F7F7Fu;
     if (row < rows && int64_t{8} * step0 + c < blocks)
-      v = *reinterpret_cast<const uint32_t*>(in + row * blocks + int64_t{8} * step0 + c);
+      v = *reinterpret_cast<const u32_any*>(in + row * blocks + int64_t{8} * step0 + c);
     *reinterpret_cast<uint32_t*>(lds + r * kScaleRow + c) = v;
   }
   __syncthreads();
@@ -427,25 +428,49 @@ __global__ __launch_bounds__(256) void k_big_scales(int N, int M, int64_t blocks
     big_scales<1>(tile - tiles_n, step0, steps, M, blocks, us, su, lds);
 }
 
-// Lines of k in codes (k_big_gemm's "across") to bf16 lines of n, kp values
-// each: 64 k by 128 n go through LDS in k_big_gemm's layout and come back
-// transposed. k past `lines` are zeros.
+// Codes as bf16 lines of k for k_big_gemm, kp values each.
+struct BigValues {
+  int64_t lines, n, blocks;  // of the codes
+  const uint8_t* codes;
+  const uint8_t* scales;
+  uint16_t* out;
+  int64_t kp;
+  int tiles_n;  // turned
+  int lx;       // not turned: lanes beside each other along a line
+};
+
 template <int BITS>
-__global__ __launch_bounds__(256) void k_big_turned(int lines, int n, int64_t blocks, const uint8_t* codes,
-                                                    const uint8_t* scales, uint16_t* out, int64_t kp, int tiles_n) {
-  __shared__ __align__(16) char lds[64 * 256];
+__device__ __forceinline__ uint4 bf16_unit(const uint8_t* codes, const uint8_t* scales, int64_t at) {
+  const float scale = scale_value(scales[at / 4]);
+  return BITS == 4 ? bf16_of4(reinterpret_cast<const uint32_t*>(codes)[at], scale)
+                   : bf16_of8(reinterpret_cast<const uint2*>(codes)[at], scale);
+}
+
+// Lines of k: line by line, zeros behind their ends.
+template <int BITS>
+__device__ __forceinline__ void big_values(const BigValues& g, int64_t group, int64_t groups) {
+  const int tx = threadIdx.x & (g.lx - 1), ly = 256 / g.lx, ty = threadIdx.x / g.lx;
+  for (int64_t line = group * ly + ty; line < g.lines; line += groups * ly)
+    for (int64_t c = tx; c < g.kp / 8; c += g.lx) {
+      uint4 r = make_uint4(0, 0, 0, 0);
+      if (c < g.blocks * 4) r = bf16_unit<BITS>(g.codes, g.scales, line * g.blocks * 4 + c);
+      *reinterpret_cast<uint4*>(g.out + line * g.kp + c * 8) = r;
+    }
+}
+
+// Lines across, each of one k: 64 k by 128 n go through LDS in k_big_gemm's
+// layout and come back transposed. k past the lines are zeros.
+template <int BITS>
+__device__ __forceinline__ void big_turned(const BigValues& g, int64_t group, char* lds) {
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q = lane >> 4, wave = tid >> 6;
-  const int k0 = (blockIdx.x / tiles_n) * 64, n0 = (blockIdx.x % tiles_n) * 128;
+  const int64_t k0 = group / g.tiles_n * 64, n0 = group % g.tiles_n * 128;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int u = i * 256 + tid, line = u >> 4, c = u & 15, pos = n0 + c * 8;
+    const int u = i * 256 + tid, line = u >> 4, c = u & 15;
+    const int64_t pos = n0 + c * 8;
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (k0 + line < lines && pos < blocks * 32) {
-      const int64_t at = (k0 + line) * blocks * 4 + pos / 8;
-      const float scale = scale_value(scales[at / 4]);
-      v = BITS == 4 ? bf16_of4(reinterpret_cast<const uint32_t*>(codes)[at], scale)
-                    : bf16_of8(reinterpret_cast<const uint2*>(codes)[at], scale);
-    }
+    if (k0 + line < g.lines && pos < g.blocks * 32)
+      v = bf16_unit<BITS>(g.codes, g.scales, (k0 + line) * g.blocks * 4 + pos / 8);
     *reinterpret_cast<uint4*>(lds + line * 256 + ((c >> 1) ^ ((line & 3) | ((line >> 3) & 1) << 2)) * 32 + (c & 1) * 16) = v;
   }
   __syncthreads();
@@ -453,13 +478,52 @@ __global__ __launch_bounds__(256) void k_big_turned(int lines, int n, int64_t bl
   f.init(wave * 32, l15, q);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int row = n0 + wave * 32 + i * 16 + l15;
+    const int64_t row = n0 + wave * 32 + i * 16 + l15;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const bf16x8 v = f.get((const lds_char*)lds, i, s);
-      if (row < n) *reinterpret_cast<bf16x8*>(out + row * kp + k0 + s * 32 + q * 8) = v;
+      if (row < g.n) *reinterpret_cast<bf16x8*>(g.out + row * g.kp + k0 + s * 32 + q * 8) = v;
     }
   }
+}
+
+// The user's operand as bf16 pieces in padded lines: piece p of line l at
+// out + p * piece + l * out_line.
+struct BigPieces {
+  const void* x;
+  int64_t lines, n, sl, se;  // elements of line l at l * sl + i * se
+  uint16_t* out;
+  int64_t out_lines, out_n, out_line, piece;
+  int lx;
+};
+template <typename T>
+__device__ __forceinline__ void big_pieces(const BigPieces& g, int64_t group, int64_t groups) {
+  constexpr int P = Pieces<T>::n;
+  const T* x = static_cast<const T*>(g.x);
+  const int tx = threadIdx.x & (g.lx - 1), ly = 256 / g.lx, ty = threadIdx.x / g.lx;
+  for (int64_t line = group * ly + ty; line < g.out_lines; line += groups * ly)
+    for (int64_t c = tx; c < g.out_n / 8; c += g.lx) {
+      const int64_t left = line < g.lines ? g.n - c * 8 : 0;
+      float v[8];
+      load8(x + line * g.sl + c * 8 * g.se, g.se, left > 8 ? 8 : left < 0 ? 0 : static_cast<int>(left), v);
+      uint4 p[P];
+      pieces8<P>(v, p);
+#pragma unroll
+      for (int i = 0; i < P; ++i) *reinterpret_cast<uint4*>(g.out + i * g.piece + line * g.out_line + c * 8) = p[i];
+    }
+}
+
+// Both operands of a large product in one launch: the first `groups`
+// workgroups make w, the others u (none where it is taken as it is).
+template <typename T, int BITS, bool TURNED>
+__global__ __launch_bounds__(256) void k_big_operands(BigValues w, BigPieces u, unsigned groups) {
+  __shared__ __align__(16) char lds[TURNED ? 64 * 256 : 16];
+  if (blockIdx.x >= groups)
+    big_pieces<T>(u, blockIdx.x - groups, gridDim.x - groups);
+  else if (TURNED)
+    big_turned<BITS>(w, blockIdx.x, lds);
+  else
+    big_values<BITS>(w, blockIdx.x, groups);
 }
 
 }  // namespace px

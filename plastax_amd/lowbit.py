@@ -229,7 +229,7 @@ def _workspace(device: torch.device, name: str, *args: object) -> torch.Tensor |
     if need > 0:
         return torch.empty(need, dtype=torch.uint8, device=device)
     if need < 0:
-        raise ValueError(f"{name}: sizes past 2^30")
+        raise ValueError(f"{name}: at most 2^24 units a level and 2^30 tokens")
     return None
 
 

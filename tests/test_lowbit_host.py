@@ -152,3 +152,6 @@ def test_entry_points_check_before_they_launch(lib) -> None:
     assert lib.plx_mx_workspace(9, 4, 4, 4, 0, p, 4, 1) == -1
     assert lib.plx_mx_workspace(0, 4, 4, 4, 5, p, 4, 1) == -1
     assert lib.plx_mx4_workspace(4, -1, 4) == -1
+    assert lib.plx_mx4_workspace(4, 4, (1 << 24) + 1) == -1
+    assert lib.plx_mx_product(0, 4, (1 << 24) + 1, 4, 0, p, 4, 1, p, p, p, None, 0, None) == 1
+    assert lib.plx_mx4_product(4, 4, (1 << 24) + 1, p, p, p, p, 0, p, None, 0, None) == 1
