@@ -721,11 +721,14 @@ inline unsigned groups_across(int64_t lines, int64_t blocks) {
 }
 
 // A large product: 256 x 256 tiles have enough rows, columns and k (counted
-// over a's pieces), and the operands' way through memory pays. Products of
-// 8.6e9 in bf16 take 34 to 56 us either way, 12.9e9 in float32 47 to 69 us
-// large and 68 to 77 in small tiles, 17.2e9 in bf16 45 to 65 and 68 to 87; in
-// 4 bits 17.2e9 take 41 us large and 26 to 30 in small tiles.
-constexpr double kBigLeast = 9e9, kBig4Least = 25e9;
+// over a's pieces), and the operands' way through memory pays. Large against
+// small tiles, us, from the least to the largest of the four products: bf16
+// 8.6e9 (2048 cubed) 46 to 49 and 37 to 45, 10.1e9 (8192 x 4096 x 300) 48 to 67
+// and 63 to 138, 17.2e9 45 to 68 and 68 to 84. float32, where small tiles split
+// a in registers, 12.9e9 (1024 x 2048 x 2048, 32 tiles) 55 to 60 and 44 to 51,
+// with a tile for every CU (4096 x 4096 of 256 tokens) 41 to 44 and 50 to 55,
+// 14.7e9 62 and 62 to 85. In 4 bits 17.2e9 take 41 large and 26 to 30.
+constexpr double kBigLeast = 9e9, kBigPieces = 14e9, kBig4Least = 25e9;
 // (Beyond 2^30 lanes of a launch, products go in small tiles, cut into launches.)
 inline bool large(int64_t m, int64_t n, int64_t k, double least) {
   return m >= 256 && n >= 256 && k >= 256 && static_cast<double>(m) * n * k >= least &&
@@ -798,7 +801,8 @@ int big_splits(int64_t m, int64_t n, int64_t steps) {
 Plan plan_of(int kind, const Shape& s, int dtype, const void* a, int64_t sm, int64_t sk) {
   Plan p{};
   const int pieces = dtype == PLX_LB_F32 ? 3 : dtype == PLX_LB_F16 ? 2 : 1;
-  p.big = large(s.m, s.n, s.k * pieces, kBigLeast) && s.k * pieces <= kBigLine && s.m <= kBigLine;
+  const bool full = 2 * div_up(s.m, kBig) * div_up(s.n, kBig) >= cu_count();  // (no ranges of k)
+  p.big = large(s.m, s.n, s.k * pieces, pieces == 1 || full ? kBigLeast : kBigPieces) && s.k * pieces <= kBigLine && s.m <= kBigLine;
   if (!p.big) {
     if (kind == PLX_LB_PRODUCT && s.m <= kFew) return p;
     p.splits = tiles_of(s.m, s.n, s.k, 64).splits;
