@@ -67,7 +67,7 @@ __global__ __launch_bounds__(kBlock) void k_mx4_along(int64_t lines, int64_t n, 
     for (int64_t c = tx; c < chunks; c += lx) {
       const int64_t left = n - c * 8;
       float v[8];
-      load8(row + c * 8, 1, left > 8 ? 8 : left < 0 ? 0 : static_cast<int>(left), v);
+      load8<true>(row + c * 8, 1, left > 8 ? 8 : left < 0 ? 0 : static_cast<int>(left), v);
       uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = m > abs_bits(v[i]) ? m : abs_bits(v[i]);
@@ -110,22 +110,41 @@ __global__ __launch_bounds__(kBlock) void k_mx4_across(int64_t lines, int64_t n,
 }
 
 // BITS 4 or 8: the values that codes stand for, lines of n next to each other.
+// A lane writes 16 bytes, 4 values of float32 or 8 of the others, so that a
+// wave's store is whole lines (8192 x 8192 as float32 with 32 bytes a lane in
+// two stores 57 us, so 44).
 template <int BITS, typename T>
 __global__ __launch_bounds__(kBlock) void k_mx_values(int64_t lines, int64_t n, const uint8_t* codes,
                                                       const uint8_t* scales, T* out, int lx) {
-  const int64_t kept = BITS == 4 ? div_up(n, 128) * 16 : div_up(n, 32) * 4, chunks = div_up(n, 8);
+  constexpr int W = 16 / sizeof(T);
+  typedef T tw __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+  const int64_t blocks = BITS == 4 ? div_up(n, 128) * 4 : div_up(n, 32), chunks = div_up(n, W);
   const int tx = threadIdx.x & (lx - 1), ly = kBlock / lx, ty = threadIdx.x / lx;
   for (int64_t line = static_cast<int64_t>(blockIdx.x) * ly + ty; line < lines;
        line += static_cast<int64_t>(gridDim.x) * ly) {
     for (int64_t c = tx; c < chunks; c += lx) {
-      const float scale = scale_value(scales[line * (kept / 4) + c / 4]);
-      const int64_t left = n - c * 8;
+      const float scale = scale_value(scales[line * blocks + c * W / 32]);
+      const int64_t at = line * blocks * (32 / W) + c;
       float v[8];
       if (BITS == 4)
-        values4(reinterpret_cast<const uint32_t*>(codes)[line * kept + c], scale, v);
+        values4(W == 8 ? reinterpret_cast<const uint32_t*>(codes)[at] : reinterpret_cast<const uint16_t*>(codes)[at],
+                scale, v);
       else
-        values8(reinterpret_cast<const uint2*>(codes)[line * kept + c], scale, v);
-      store8(out + line * n + c * 8, left > 8 ? 8 : static_cast<int>(left), v);
+        values8(W == 8 ? reinterpret_cast<const uint2*>(codes)[at]
+                       : make_uint2(reinterpret_cast<const uint32_t*>(codes)[at], 0),
+                scale, v);
+      T* p = out + line * n + c * W;
+      const int64_t left = n - c * W;
+      if (left >= W) {
+        tw r;
+#pragma unroll
+        for (int i = 0; i < W; ++i) r[i] = from_f32<T>(v[i]);
+        __builtin_nontemporal_store(r, reinterpret_cast<tw*>(p));
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+          if (i < left) p[i] = from_f32<T>(v[i]);
+      }
     }
   }
 }
@@ -195,7 +214,7 @@ __global__ __launch_bounds__(kBlock) void k_act_along(int64_t lines, int64_t n, 
       const int64_t left64 = n - c * 8;
       const int left = left64 > 8 ? 8 : left64 < 0 ? 0 : static_cast<int>(left64);
       float v[8], f[8];
-      load8(h + line * sh + c * 8, 1, left, v);
+      load8<true>(h + line * sh + c * 8, 1, left, v);
       uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -203,7 +222,7 @@ __global__ __launch_bounds__(kBlock) void k_act_along(int64_t lines, int64_t n, 
         m = a < kInfBits && a > m ? a : m;
         f[i] = act<FN>(v[i]);
       }
-      if (y) store8(y + line * sy + c * 8, left, f);
+      if (y) store8<true>(y + line * sy + c * 8, left, f);
       const int e = exponent8(max4(m));
       reinterpret_cast<uint2*>(codes)[line * chunks + c] = codes8(v, pow2(-e));
       if ((tx & 3) == 0) scales[line * (chunks / 4) + c / 4] = static_cast<uint8_t>(e + 127);
@@ -254,12 +273,12 @@ __global__ __launch_bounds__(kBlock) void k_grad_along(int64_t lines, int64_t n,
       const int64_t left64 = n - c * 8;
       const int left = left64 > 8 ? 8 : static_cast<int>(left64);
       float v[8], q[8];
-      load8(dy + line * sy + c * 8, 1, left, v);
+      load8<true>(dy + line * sy + c * 8, 1, left, v);
       values8(reinterpret_cast<const uint2*>(codes)[line * kept + c], scale_value(scales[line * (kept / 4) + c / 4]),
               q);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= act_grad<FN>(q[i]);
-      store8(dh + line * sh + c * 8, left, v);
+      store8<true>(dh + line * sh + c * 8, left, v);
     }
   }
 }
@@ -971,7 +990,7 @@ int plx_mx_values(int32_t bits, int64_t lines, int64_t n, const uint8_t* codes, 
   if (!out || !codes || !scales) return fail(PLX_ERR_INVALID, "plx_mx_values: null pointer");
   if (!on16(codes)) return fail(PLX_ERR_INVALID, "plx_mx_values: codes not on 16 bytes");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int lx = lanes_along(div_up(n, 8));
+  const int lx = lanes_along(div_up(n, dtype == PLX_LB_F32 ? 4 : 8));
   with_type(dtype, [&](auto* t) {
     using T = PLX_TYPE(t);
     if (bits == 4)

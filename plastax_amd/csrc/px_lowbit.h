@@ -50,29 +50,39 @@ struct Unit {
   typedef T load __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 // p[i * stride], i < n; zeros from there on.
-template <typename T>
+// PASS: as in store8, of what a pass reads once.
+template <bool PASS = false, typename T>
 __device__ __forceinline__ typename Unit<T>::type load_unit(const T* p, int64_t stride, int n) {
-  if (stride == 1 && n >= 8) return *reinterpret_cast<const typename Unit<T>::load*>(p);
+  if (stride == 1 && n >= 8) {
+    if (PASS) return __builtin_nontemporal_load(reinterpret_cast<const typename Unit<T>::load*>(p));
+    return *reinterpret_cast<const typename Unit<T>::load*>(p);
+  }
   typename Unit<T>::type r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) r[i] = i < n ? p[i * stride] : from_f32<T>(0.0f);
   return r;
 }
 // The same as float32.
-template <typename T>
+template <bool PASS = false, typename T>
 __device__ __forceinline__ void load8(const T* p, int64_t stride, int n, float v[8]) {
-  const typename Unit<T>::type r = load_unit(p, stride, n);
+  const typename Unit<T>::type r = load_unit<PASS>(p, stride, n);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = to_f32(r[i]);
 }
 
-template <typename T>
+// PASS: the results of a pass over a large array, read by nothing in it: 16
+// bytes a lane go past the caches' replacement (of float32, whose two stores
+// would each leave half of every line, only whole lines may).
+template <bool PASS = false, typename T>
 __device__ __forceinline__ void store8(T* p, int n, const float v[8]) {
   if (n >= 8) {
     typename Unit<T>::load r;
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = from_f32<T>(v[i]);
-    *reinterpret_cast<typename Unit<T>::load*>(p) = r;
+    if (PASS && sizeof(T) == 2)
+      __builtin_nontemporal_store(r, reinterpret_cast<typename Unit<T>::load*>(p));
+    else
+      *reinterpret_cast<typename Unit<T>::load*>(p) = r;
     return;
   }
 #pragma unroll
