@@ -111,8 +111,8 @@ __global__ __launch_bounds__(kBlock) void k_mx4_across(int64_t lines, int64_t n,
 
 // BITS 4 or 8: the values that codes stand for, lines of n next to each other.
 // A lane writes 16 bytes, 4 values of float32 or 8 of the others, so that a
-// wave's store is whole lines (8192 x 8192 as float32 with 32 bytes a lane in
-// two stores 57 us, so 44).
+// wave's store is whole lines (8192 x 8192 as float32 50 us; with 32 bytes a
+// lane in two stores 57).
 template <int BITS, typename T>
 __global__ __launch_bounds__(kBlock) void k_mx_values(int64_t lines, int64_t n, const uint8_t* codes,
                                                       const uint8_t* scales, T* out, int lx) {
@@ -414,11 +414,11 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
   const T* a = static_cast<const T*>(g.a);
   typedef typename Unit<T>::type unit;
 
-  struct Regs {
+  struct {
     unit a[kU];
     uint2 b[kU];
     uint32_t s[kU];
-  } r0, r1;
+  } r;
   // The line and the chunk of this thread's i-th unit, and its place in LDS.
   auto place = [&](bool across, int i, int* line, int* chunk) {
     const int u = tid + 256 * KS * i;
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
     *line = u / (8 * KS), *chunk = u % (8 * KS);
     return (*chunk >> 3) * kSub + *line * 8 + ((*chunk & 7) ^ (*line & 7));
   };
-  auto load = [&](Regs& r, int k0) {
+  auto load = [&](int k0) {
     if (k0 >= kend) return;
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
@@ -458,7 +458,7 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
       }
     }
   };
-  auto put = [&](const Regs& r) {
+  auto put = [&]() {
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
       int line, chunk;
@@ -511,19 +511,13 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa[j][p], acc[i][j], 0, 0, 0);
     }
   };
-  // Two steps' loads in flight: a step is shorter than a load's way.
-  auto step = [&](Regs& r, int k0) {
+  load(kbeg);
+  for (int k0 = kbeg; k0 < kend; k0 += kStep) {
     __syncthreads();
-    put(r);
+    put();
     __syncthreads();
-    load(r, k0 + 2 * kStep);
+    load(k0 + kStep);
     compute();
-  };
-  load(r0, kbeg);
-  load(r1, kbeg + kStep);
-  for (int k0 = kbeg; k0 < kend; k0 += 2 * kStep) {
-    step(r0, k0);
-    if (k0 + kStep < kend) step(r1, k0 + kStep);
   }
   tile_store<TS, KS, OT>(acc, lds, group, wm, wn, m0, n0, g.M, g.N, static_cast<OT*>(g.out), g.part);
 }
@@ -633,11 +627,11 @@ __global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks,
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2;
   const int m0 = (blockIdx.x / tiles_n) * TS, n0 = (blockIdx.x % tiles_n) * TS;
   const int beg = blockIdx.y * per, end = beg + per < blocks ? beg + per : blocks;
-  struct Regs {
+  struct {
     uint4 c[2 * F];
     uint32_t s[2 * F];
-  } r0, r1;
-  auto load = [&](Regs& r, int b0) {
+  } r;
+  auto load = [&](int b0) {
     if (b0 >= end) return;
 #pragma unroll
     for (int i = 0; i < 2 * F; ++i) {  // x's, then w's
@@ -651,7 +645,7 @@ __global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks,
       }
     }
   };
-  auto put = [&](const Regs& r) {
+  auto put = [&]() {
 #pragma unroll
     for (int i = 0; i < 2 * F; ++i) {
       const int u = tid + 256 * KS * (i % F), line = u / kStep, b = u % kStep;
@@ -683,18 +677,13 @@ __global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks,
               __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[i], fx[j], acc[i][j], 4, 4, 0, sw[i], 0, sx[j]);
     }
   };
-  auto step = [&](Regs& r, int b0) {
+  load(beg);
+  for (int b0 = beg; b0 < end; b0 += kStep) {
     __syncthreads();
-    put(r);
+    put();
     __syncthreads();
-    load(r, b0 + 2 * kStep);
+    load(b0 + kStep);
     compute();
-  };
-  load(r0, beg);
-  load(r1, beg + kStep);
-  for (int b0 = beg; b0 < end; b0 += 2 * kStep) {
-    step(r0, b0);
-    if (b0 + kStep < end) step(r1, b0 + kStep);
   }
   tile_store<TS, KS, OT>(acc, lds, group, wm, wn, m0, n0, M, N, out, parts);
 }
