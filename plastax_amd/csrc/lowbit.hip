@@ -404,9 +404,12 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
   constexpr int F = TS / 32, kLine = TS / 8;                // (fragments a wave and side; chunks of a line across)
   constexpr int kStep = 64 * KS, kSub = TS * 8, kU = TS / 32;  // (16-byte chunks of TS x 64 values; units a thread)
   constexpr int kUints = (P + 1) * KS * kSub, kSums = KS * TS * TS / 4;
-  __shared__ uint4 lds[KS > 1 && kUints < kSums ? kSums : kUints];
-  uint4* la = lds;
-  uint4* lb = lds + P * KS * kSub;
+  // Two buffers where they fit: a step's stores to LDS then go beside the
+  // matrix instructions of the step before, with one barrier for both (bf16
+  // 512 x 4096 x 4096 44 -> 35 us). Not for one group of waves, where several
+  // workgroups of a CU do that already (float32 8192 x 512 x 512 25 -> 31).
+  constexpr int kBufs = KS == 4 && 2 * kUints * 16 <= 128 * 1024 ? 2 : 1;
+  __shared__ uint4 lds[KS > 1 && kBufs * kUints < kSums ? kSums : kBufs * kUints];
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2;
   const int m0 = (blockIdx.x / g.tiles_n) * TS, n0 = (blockIdx.x % g.tiles_n) * TS;
@@ -458,7 +461,9 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
       }
     }
   };
-  auto put = [&]() {
+  auto put = [&](int buf) {
+    uint4* la = lds + buf * kUints;
+    uint4* lb = la + P * KS * kSub;
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
       int line, chunk;
@@ -492,7 +497,9 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
 
   f32x4 acc[F][F] = {};
   const int wn = (wave & 1) * (TS / 2), wm = ((wave >> 1) & 1) * (TS / 2);
-  auto compute = [&]() {
+  auto compute = [&](int buf) {
+    const uint4* la = lds + buf * kUints;
+    const uint4* lb = la + P * KS * kSub;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       bf16x8 fb[F], fa[F][P];
@@ -512,12 +519,25 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
     }
   };
   load(kbeg);
-  for (int k0 = kbeg; k0 < kend; k0 += kStep) {
-    __syncthreads();
-    put();
-    __syncthreads();
-    load(k0 + kStep);
-    compute();
+  if (kBufs == 2) {
+    if (kbeg < kend) put(0);
+    load(kbeg + kStep);
+    int buf = 0;
+    for (int k0 = kbeg; k0 < kend; k0 += kStep) {
+      __syncthreads();
+      if (k0 + kStep < kend) put(buf ^ 1);
+      load(k0 + 2 * kStep);
+      compute(buf);
+      buf ^= 1;
+    }
+  } else {
+    for (int k0 = kbeg; k0 < kend; k0 += kStep) {
+      __syncthreads();
+      put(0);
+      __syncthreads();
+      load(k0 + kStep);
+      compute(0);
+    }
   }
   tile_store<TS, KS, OT>(acc, lds, group, wm, wn, m0, n0, g.M, g.N, static_cast<OT*>(g.out), g.part);
 }
