@@ -641,8 +641,9 @@ __global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks,
                                                        int tiles_n, int per) {
   constexpr int F = TS / 32, kSub = TS * 8, kStep = 8 * KS;  // blocks of a step
   constexpr int kUints = 2 * KS * kSub, kSums = KS * TS * TS / 4;
-  __shared__ uint4 lds[KS > 1 && kUints < kSums ? kSums : kUints];
-  __shared__ uint8_t lss[2 * KS * kSub];
+  constexpr int kBufs = KS == 4 ? 2 : 1;
+  __shared__ uint4 lds[KS > 1 && kBufs * kUints < kSums ? kSums : kBufs * kUints];
+  __shared__ uint8_t lss[kBufs * kUints];
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2;
   const int m0 = (blockIdx.x / tiles_n) * TS, n0 = (blockIdx.x % tiles_n) * TS;
@@ -665,18 +666,18 @@ __global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks,
       }
     }
   };
-  auto put = [&]() {
+  auto put = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < 2 * F; ++i) {
       const int u = tid + 256 * KS * (i % F), line = u / kStep, b = u % kStep;
-      const int at = ((i < F ? 0 : KS) + (b >> 3)) * kSub + line * 8 + ((b & 7) ^ (line & 7));
+      const int at = buf * kUints + ((i < F ? 0 : KS) + (b >> 3)) * kSub + line * 8 + ((b & 7) ^ (line & 7));
       lds[at] = r.c[i];
       lss[at] = static_cast<uint8_t>(r.s[i]);
     }
   };
   f32x4 acc[F][F] = {};
   const int wn = (wave & 1) * (TS / 2), wm = ((wave >> 1) & 1) * (TS / 2);
-  auto compute = [&]() {
+  auto compute = [&](int buf) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       i32x8 fx[F], fw[F];
@@ -684,8 +685,8 @@ __global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks,
 #pragma unroll
       for (int i = 0; i < F; ++i) {
         const int rm = wm + i * 16 + l15, rn = wn + i * 16 + l15;
-        const int am = group * kSub + rm * 8 + ((h * 4 + q) ^ (rm & 7));
-        const int an = (KS + group) * kSub + rn * 8 + ((h * 4 + q) ^ (rn & 7));
+        const int am = buf * kUints + group * kSub + rm * 8 + ((h * 4 + q) ^ (rm & 7));
+        const int an = buf * kUints + (KS + group) * kSub + rn * 8 + ((h * 4 + q) ^ (rn & 7));
         fx[i] = as_i32x8(as_bf16x8(lds[am])), sx[i] = lss[am];
         fw[i] = as_i32x8(as_bf16x8(lds[an])), sw[i] = lss[an];
       }
@@ -698,12 +699,25 @@ __global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks,
     }
   };
   load(beg);
-  for (int b0 = beg; b0 < end; b0 += kStep) {
-    __syncthreads();
-    put();
-    __syncthreads();
-    load(b0 + kStep);
-    compute();
+  if (kBufs == 2) {
+    if (beg < end) put(0);
+    load(beg + kStep);
+    int buf = 0;
+    for (int b0 = beg; b0 < end; b0 += kStep) {
+      __syncthreads();
+      if (b0 + kStep < end) put(buf ^ 1);
+      load(b0 + 2 * kStep);
+      compute(buf);
+      buf ^= 1;
+    }
+  } else {
+    for (int b0 = beg; b0 < end; b0 += kStep) {
+      __syncthreads();
+      put(0);
+      __syncthreads();
+      load(b0 + kStep);
+      compute(0);
+    }
   }
   tile_store<TS, KS, OT>(acc, lds, group, wm, wn, m0, n0, M, N, out, parts);
 }
