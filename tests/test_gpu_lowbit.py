@@ -429,6 +429,37 @@ def test_offsets_past_32_bits() -> None:
     assert bool(((dw.double() - want).abs() <= size * plain.sum_bound(lines)).all())
 
 
+def test_large_products_with_offsets_past_32_bits() -> None:
+    """The same through the large products: 70,000 lines of 32,768 against 260 and 256 units."""
+    lines, n = 70_000, 32_768
+    x = torch.zeros((lines, n), dtype=torch.bfloat16, device=DEV)
+    tail = (_randn((80, n), _gen(16)) * 2).bfloat16()
+    x[-80:] = tail
+    w = lowbit.quantise4(_randn((260, n), _gen(17)))
+    y = lowbit.product(x, w)
+    plain.assert_product(y[-80:], tail.double(), _w64(w))
+    assert not y[:1000].any()
+    y = lowbit.product(lowbit.quantise4(x), w)
+    q = plain.quantise4(tail)
+    plain.assert_product(y[-80:], plain.values4(*q, n), _w64(w))
+    assert not y[:1000].any()
+    kept = lowbit.quantise8(x)
+    g = torch.zeros((lines, 256), dtype=torch.bfloat16, device=DEV)
+    g[-80:] = _randn((80, 256), _gen(18))
+    dw = lowbit.weight_grad(g, kept)
+    q = plain.values8(kept.codes[-80:], kept.scales[-80:], n)
+    size = g[-80:].double().t().contiguous().abs() @ q.abs()
+    want = g[-80:].double().t().contiguous() @ q
+    assert bool(((dw.double() - want).abs() <= size * plain.sum_bound(lines)).all())
+    wide = lowbit.quantise4(_randn((lines, 256), _gen(19)))
+    dx = torch.zeros((300, lines), dtype=torch.bfloat16, device=DEV)
+    dx[:, -80:] = _randn((300, 80), _gen(20))
+    got = lowbit.product_grad(dx, wide)
+    w64 = plain.values4(wide.codes[-80:], wide.scales[-80:], 256)
+    want, size = dx[:, -80:].double() @ w64, dx[:, -80:].double().abs() @ w64.abs()
+    assert bool(((got.double() - want).abs() <= size * plain.sum_bound(lines) + want.abs() * 2.0**-8).all())
+
+
 def test_the_example_learns_and_its_answers_are_the_arenas() -> None:
     import pathlib
     import sys
