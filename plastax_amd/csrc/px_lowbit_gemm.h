@@ -136,8 +136,9 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 // A wave's results, from its first row and column on: with w's rows as the
 // matrix instruction's first operand a lane holds runs of four consecutive n
 // of one m: one in a fragment of 16 x 16, in one of 32 x 32 four, 8 columns
-// apart, lanes l and l + 32 having neighbouring runs of the same row. Tiles
-// that are inside take the straight way.
+// apart, lanes l and l + 32 having neighbouring runs of the same row. Rows are
+// written 64 bytes and more at a time (32 left lines of 16-bit results that were
+// written twice: 183 MB for 134). Tiles that are inside take the straight way.
 template <typename T>
 __device__ __forceinline__ void big_store(const f32x4 (&acc)[2][2][4][2], T* out, int M, int N, int m, int n,
                                           bool whole) {
@@ -147,6 +148,30 @@ __device__ __forceinline__ void big_store(const f32x4 (&acc)[2][2][4][2], T* out
     for (int j = 0; j < 2; ++j) {
       const int row = m + hu * 128 + j * 16;
       T* p = out + static_cast<int64_t>(row) * N + n;
+      if (sizeof(T) == 2) {
+        // Two fragments' runs, 32 columns: of lanes 16 apart the first gets 8
+        // columns of the first fragment, the second 8 of the second one, so
+        // that a row is written 64 bytes at a time.
+        const int q = (threadIdx.x >> 4) & 3, to = (q & 1) * 16 + (q >> 1) * 8 - q * 4;
+#pragma unroll
+        for (int hw = 0; hw < 2; ++hw)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[hw][hu][i][j][k]),
+                                                              __float_as_uint(acc[hw][hu][i + 1][j][k]), false, false);
+              v[k] = __uint_as_float(t[0]), v[4 + k] = __uint_as_float(t[1]);
+            }
+            const int col = hw * 128 + i * 16 + to;
+            if (whole)
+              store8(p + col, 8, v);
+            else if (row < M)
+              store8(p + col, N - n - col, v);
+          }
+        continue;
+      }
 #pragma unroll
       for (int hw = 0; hw < 2; ++hw)
 #pragma unroll
@@ -162,34 +187,45 @@ __device__ __forceinline__ void big_store(const f32x4 (&acc)[2][2][4][2], T* out
 template <typename T>
 __device__ __forceinline__ void big_store(const f32x16 (&acc)[2][2][2][1], T* out, int M, int N, int m, int n,
                                           bool whole) {
-  const bool upper = (threadIdx.x & 32) != 0;
+  // Neighbouring runs of lanes 32 apart, then those of lanes 16 apart: a lane
+  // gets 8 columns of rows l % 16 and l % 16 + 16, and a fragment's 32 columns
+  // of a row are written at once.
+  const int lane = threadIdx.x & 63, q = lane >> 4;
+  const int row0 = m - (lane & 31) + (lane & 15), to = (q & 1) * 16 + (q >> 1) * 8 - (lane >> 5) * 4;
 #pragma unroll
-  for (int hu = 0; hu < 2; ++hu) {
-    const int row = m + hu * 128;
-    T* p = out + static_cast<int64_t>(row) * N + n;
+  for (int hu = 0; hu < 2; ++hu)
 #pragma unroll
     for (int hw = 0; hw < 2; ++hw)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
+        float v[2][8];
 #pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          // Runs r and r + 1 of both lanes, 16 columns: the lower lane gets
-          // the first 8, the upper one the others.
-          float v[8];
+        for (int k = 0; k < 4; ++k) {
+          uint32_t r[2][2];  // runs 2 p and 2 p + 1 after the first exchange
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[hw][hu][i][0][4 * r + k]),
-                                                            __float_as_uint(acc[hw][hu][i][0][4 * r + 4 + k]), false,
+          for (int p = 0; p < 2; ++p) {
+            const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[hw][hu][i][0][8 * p + k]),
+                                                            __float_as_uint(acc[hw][hu][i][0][8 * p + 4 + k]), false,
                                                             false);
-            v[k] = __uint_as_float(t[0]), v[4 + k] = __uint_as_float(t[1]);
+            r[p][0] = t[0], r[p][1] = t[1];
           }
-          const int col = hw * 128 + i * 32 + r * 8 + (upper ? 4 : 0);  // (n is 4 more in the upper lane)
-          if (whole)
-            store8(p + col, 8, v);
-          else if (row < M)
-            store8(p + col, N - n - col, v);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const auto t = __builtin_amdgcn_permlane16_swap(r[0][h], r[1][h], false, false);
+            v[0][4 * h + k] = __uint_as_float(t[0]), v[1][4 * h + k] = __uint_as_float(t[1]);
+          }
         }
-  }
+        const int col = hw * 128 + i * 32 + to;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int row = row0 + hu * 128 + b * 16;
+          T* p = out + static_cast<int64_t>(row) * N + n + col;
+          if (whole)
+            store8(p, 8, v[b]);
+          else if (row < M)
+            store8(p, N - n - col, v[b]);
+        }
+      }
 }
 
 // 256 x 256 of the output by 8 waves. A wave has 64 rows in each half of its w
