@@ -10,7 +10,7 @@ fallback.
 
 from __future__ import annotations
 
-from plastax_amd import monoid, nn, numpy, optim, rng, topo
+from plastax_amd import lowbit, monoid, nn, numpy, optim, rng, topo
 from plastax_amd._expr import UnsupportedPolicyError
 from plastax_amd._types import (
     ACTIVATION,
@@ -118,6 +118,7 @@ __all__ = [
     "live_conn_count",
     "live_unit_count",
     "live_unit_mask",
+    "lowbit",
     "make_empty_state",
     "make_step",
     "monoid",
