@@ -1188,11 +1188,12 @@ PLX_EXPORT int plx_count_ids(int64_t n, const int32_t* ids, const uint8_t* skip,
  * bits) or 448 (8 bits), and at least 2^-125 or 2^-117. Values are rounded to
  * the nearest, ties to the even code.
  *   4 bits: e2m1 codes, two to a byte, the earlier value low; a line holds
- *     ceil(n / 128) * 4 blocks of 16 bytes, zero codes past its end. A block
- *     with an infinity or a NaN has s = 255 and stands for NaN.
+ *     ceil(n / 128) * 4 blocks of 16 bytes, zero codes past its end (scales of
+ *     blocks past it count for nothing). A block with an infinity or a NaN has
+ *     s = 255 and stands for NaN.
  *   8 bits: e4m3 codes without infinities, one to a byte; a line holds
- *     ceil(n / 32) blocks of 32 bytes. An infinity or a NaN is kept as NaN in
- *     its own place.
+ *     ceil(n / 32) blocks of 32 bytes; codes past its end count for nothing.
+ *     An infinity or a NaN is kept as NaN in its own place.
  * codes start on 16 bytes. Sizes are at most 2^30, in products 2^24 inputs and
  * outputs. Strides are in elements. */
 #define PLX_LB_F32 0

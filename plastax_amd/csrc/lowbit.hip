@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
       const int64_t l = BA ? k0 + line : n0 + line;
       const int pos = (BA ? n0 : k0) + chunk * 8;
       r.b[i] = make_uint2(0, 0), r.s[i] = 127;
-      if (l < (BA ? kend : g.N) && pos < g.blocks * 32) {
+      if (l < (BA ? kend : g.N) && pos < (BA ? g.N : kend)) {
         const int64_t at = l * g.blocks * 4 + pos / 8;
         if (BITS == 4)
           r.b[i].x = reinterpret_cast<const uint32_t*>(g.codes)[at];
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
       }
     }
   };
-  auto put = [&](int buf) {
+  auto put = [&](int buf, int k0) {  // (k0: the loads' first k)
     uint4* la = lds + buf * kUints;
     uint4* lb = la + P * KS * kSub;
 #pragma unroll
@@ -484,6 +484,7 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
       int line, chunk;
       const int at = place(BA, i, &line, &chunk);
       const float scale = scale_value(r.s[i]);
+      if (KIND == kXT) r.b[i] = first_codes8(r.b[i], kend - k0 - chunk * 8);
       lb[at] = BITS == 4 ? bf16_of4(r.b[i].x, scale) : bf16_of8(r.b[i], scale);
     }
   };
@@ -526,12 +527,12 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
   };
   load(kbeg);
   if (kBufs == 2) {
-    if (kbeg < kend) put(0);
+    if (kbeg < kend) put(0, kbeg);
     load(kbeg + kStep);
     int buf = 0;
     for (int k0 = kbeg; k0 < kend; k0 += kStep) {
       __syncthreads();
-      if (k0 + kStep < kend) put(buf ^ 1);
+      if (k0 + kStep < kend) put(buf ^ 1, k0 + kStep);
       load(k0 + 2 * kStep);
       compute(buf);
       buf ^= 1;
@@ -539,7 +540,7 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
   } else {
     for (int k0 = kbeg; k0 < kend; k0 += kStep) {
       __syncthreads();
-      put(0);
+      put(0, k0);
       __syncthreads();
       load(k0 + kStep);
       compute(0);
@@ -589,7 +590,7 @@ __global__ __launch_bounds__(64 * kFewWaves<ALONG>) void k_mx_few(GemmArgs g) {
   const T* x = static_cast<const T*>(g.a) + l15 * g.sm;
   const uint4* codes = reinterpret_cast<const uint4*>(g.codes) + n * g.blocks;
   const uint8_t* scales = g.scales + n * g.blocks;
-  const int blocks = static_cast<int>(g.blocks);
+  const int blocks = static_cast<int>(div_up(g.K, 32));  // (what is behind a line's end counts for nothing)
   f32x4 acc = {};
   for (int b0 = wave * 4 + q; b0 - q < blocks; b0 += kAhead * W * 4) {
     uint4 c[kAhead];
@@ -644,9 +645,9 @@ __global__ __launch_bounds__(64 * kFewWaves<ALONG>) void k_mx_few(GemmArgs g) {
 // and LDS as in k_mx_gemm, a chunk of 16 bytes being one block here: a step is
 // 256 k a group.
 template <typename OT, int TS, int KS>
-__global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks, const uint8_t* xc, const uint8_t* xs,
-                                                       const uint8_t* wc, const uint8_t* ws, OT* out, float* parts,
-                                                       int tiles_n, int per) {
+__global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int K, int blocks, const uint8_t* xc,
+                                                       const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, OT* out,
+                                                       float* parts, int tiles_n, int per) {
   constexpr int F = TS / 32, kSub = TS * 8, kStep = 8 * KS;  // blocks of a step
   constexpr int kUints = 2 * KS * kSub, kSums = KS * TS * TS / 4;
   constexpr int kBufs = KS == 4 ? 2 : 1;
@@ -655,7 +656,8 @@ __global__ __launch_bounds__(256 * KS) void k_mx4_gemm(int M, int N, int blocks,
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2;
   const int m0 = (blockIdx.x / tiles_n) * TS, n0 = (blockIdx.x % tiles_n) * TS;
-  const int beg = blockIdx.y * per, end = beg + per < blocks ? beg + per : blocks;
+  const int used = (K + 31) / 32;  // blocks that hold values
+  const int beg = blockIdx.y * per, end = beg + per < used ? beg + per : used;
   struct {
     uint4 c[2 * F];
     uint32_t s[2 * F];
@@ -1173,7 +1175,7 @@ int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8
     g.steps = g.wrap = p.steps, g.split = static_cast<int>(div_up(p.steps, p.splits));
     g.tiles_m = static_cast<int>(div_up(tokens, kBig)), g.tiles_n = static_cast<int>(div_up(outputs, kBig));
     k_big_scales<<<static_cast<unsigned>((g.tiles_m + g.tiles_n) * div_up(p.steps, 8)), 256, 0, s>>>(
-        g.N, g.M, blocks, p.steps, w_scales, x_scales, reinterpret_cast<uint8_t*>(work),
+        g.N, g.M, blocks, div_up(inputs, 32), p.steps, w_scales, x_scales, reinterpret_cast<uint8_t*>(work),
         reinterpret_cast<uint8_t*>(work + p.bytes_w));
     with_type(dtype, [&](auto* t) {
       using T = PLX_TYPE(t);
@@ -1196,8 +1198,8 @@ int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8
       with_tiles(t, [&](auto ts, auto ks) {
         constexpr int TS = decltype(ts)::value, KS = decltype(ks)::value;
         k_mx4_gemm<T, TS, KS><<<grid, 256 * KS, 0, s>>>(
-            static_cast<int>(now), static_cast<int>(outputs), static_cast<int>(blocks), x_codes + m * blocks * 16,
-            x_scales + m * blocks, w_codes, w_scales, static_cast<T*>(out) + m * outputs,
+            static_cast<int>(now), static_cast<int>(outputs), static_cast<int>(inputs), static_cast<int>(blocks),
+            x_codes + m * blocks * 16, x_scales + m * blocks, w_codes, w_scales, static_cast<T*>(out) + m * outputs,
             static_cast<float*>(workspace), tiles_n, t.kper / 32);
       });
     }

@@ -179,6 +179,13 @@ __device__ __forceinline__ uint4 bf16_of4(uint32_t c, float scale) {
   r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3));
   return r;
 }
+// The first `left` of 8 codes of 8 bits, zeros in place of the others: what is
+// behind a line's end may be NaN, which no other operand's zero takes out of a sum.
+__device__ __forceinline__ uint2 first_codes8(uint2 c, int64_t left) {
+  if (left >= 8) return c;
+  const uint64_t keep = left > 0 ? (uint64_t{1} << (8 * left)) - 1 : 0;
+  return make_uint2(c.x & static_cast<uint32_t>(keep), c.y & static_cast<uint32_t>(keep >> 32));
+}
 __device__ __forceinline__ uint4 bf16_of8(uint2 c, float scale) {
   float v[8];
   values8(c, scale, v);

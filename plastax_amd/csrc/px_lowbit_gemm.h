@@ -423,14 +423,14 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
 // Scale bytes [rows][blocks] as the waves of k_big_gemm read them: W waves
 // share a tile's 256 rows, each with F fragments of 32 rows in each half. Of
 // tile, step, wave and lane, byte 4 (F h + f) + s is the scale of row
-// 128 h + 32 (F wave + f) + lane % 32 in block 8 step + 2 s + lane / 32. Rows and
-// blocks past the end get the scale 1. A workgroup takes 8 steps of a tile
+// 128 h + 32 (F wave + f) + lane % 32 in block 8 step + 2 s + lane / 32. Rows
+// past the end and blocks that hold no values (from `used` on) get the scale 1. A workgroup takes 8 steps of a tile
 // through LDS (two of 8192 x 8192 values 8 us).
 typedef uint32_t u32_any __attribute__((aligned(1)));  // (scale bytes start anywhere)
 constexpr int kScaleRow = 68;  // bytes of 8 steps of a row in LDS, and 4 that move the rows over the banks
 template <int F>
-__device__ __forceinline__ void big_scales(int tile, int step0, int steps, int rows, int64_t blocks, const uint8_t* in,
-                                           uint8_t* out, uint8_t* lds) {
+__device__ __forceinline__ void big_scales(int tile, int step0, int steps, int rows, int64_t blocks, int64_t used,
+                                           const uint8_t* in, uint8_t* out, uint8_t* lds) {
   constexpr int W = 4 / F;
   const int tid = threadIdx.x;
 #pragma unroll
@@ -438,8 +438,11 @@ __device__ __forceinline__ void big_scales(int tile, int step0, int steps, int r
     const int at = i * 256 + tid, r = at >> 4, c = (at & 15) * 4;
     const int row = tile * 256 + r;
     uint32_t v = 0x7F7F7F7Fu;
-    if (row < rows && int64_t{8} * step0 + c < blocks)
-      v = *reinterpret_cast<const u32_any*>(in + row * blocks + int64_t{8} * step0 + c);
+    const int64_t left = used - (int64_t{8} * step0 + c);
+    if (row < rows && left > 0) {
+      const uint32_t keep = left < 4 ? (1u << (8 * left)) - 1u : ~0u;
+      v = (*reinterpret_cast<const u32_any*>(in + row * blocks + int64_t{8} * step0 + c) & keep) | (v & ~keep);
+    }
     *reinterpret_cast<uint32_t*>(lds + r * kScaleRow + c) = v;
   }
   __syncthreads();
@@ -456,14 +459,14 @@ __device__ __forceinline__ void big_scales(int tile, int step0, int steps, int r
   }
 }
 
-__global__ __launch_bounds__(256) void k_big_scales(int N, int M, int64_t blocks, int steps, const uint8_t* ws,
-                                                    const uint8_t* us, uint8_t* sw, uint8_t* su) {
+__global__ __launch_bounds__(256) void k_big_scales(int N, int M, int64_t blocks, int64_t used, int steps,
+                                                    const uint8_t* ws, const uint8_t* us, uint8_t* sw, uint8_t* su) {
   __shared__ uint8_t lds[256 * kScaleRow];
   const int runs = (steps + 7) / 8, tile = blockIdx.x / runs, step0 = blockIdx.x % runs * 8, tiles_n = (N + 255) / 256;
   if (tile < tiles_n)
-    big_scales<2>(tile, step0, steps, N, blocks, ws, sw, lds);
+    big_scales<2>(tile, step0, steps, N, blocks, used, ws, sw, lds);
   else
-    big_scales<1>(tile - tiles_n, step0, steps, M, blocks, us, su, lds);
+    big_scales<1>(tile - tiles_n, step0, steps, M, blocks, used, us, su, lds);
 }
 
 // Codes as bf16 lines of k for k_big_gemm, kp values each.
@@ -477,11 +480,13 @@ struct BigValues {
   int lx;       // not turned: lanes beside each other along a line
 };
 
+// The first `left` of 8 codes from the at-th eight on, as bf16 (in 4 bits the
+// codes behind a line's end are zeros).
 template <int BITS>
-__device__ __forceinline__ uint4 bf16_unit(const uint8_t* codes, const uint8_t* scales, int64_t at) {
+__device__ __forceinline__ uint4 bf16_unit(const uint8_t* codes, const uint8_t* scales, int64_t at, int64_t left = 8) {
   const float scale = scale_value(scales[at / 4]);
   return BITS == 4 ? bf16_of4(reinterpret_cast<const uint32_t*>(codes)[at], scale)
-                   : bf16_of8(reinterpret_cast<const uint2*>(codes)[at], scale);
+                   : bf16_of8(first_codes8(reinterpret_cast<const uint2*>(codes)[at], left), scale);
 }
 
 // Lines of k: line by line, zeros behind their ends.
@@ -491,7 +496,7 @@ __device__ __forceinline__ void big_values(const BigValues& g, int64_t group, in
   for (int64_t line = group * ly + ty; line < g.lines; line += groups * ly)
     for (int64_t c = tx; c < g.kp / 8; c += g.lx) {
       uint4 r = make_uint4(0, 0, 0, 0);
-      if (c < g.blocks * 4) r = bf16_unit<BITS>(g.codes, g.scales, line * g.blocks * 4 + c);
+      if (c * 8 < g.n) r = bf16_unit<BITS>(g.codes, g.scales, line * g.blocks * 4 + c, g.n - c * 8);
       *reinterpret_cast<uint4*>(g.out + line * g.kp + c * 8) = r;
     }
 }

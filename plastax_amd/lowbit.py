@@ -15,10 +15,11 @@ go to the nearest, ties to the even code.
 
 - 4 bits (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign): two values to a byte, the
   earlier one in the low half; a line holds ``ceil(n / 128) * 4`` blocks, zero
-  codes past its end. A block with an infinity or a NaN has ``s = 255`` and
-  stands for NaN.
+  codes past its end (the scales of blocks past it count for nothing). A block
+  with an infinity or a NaN has ``s = 255`` and stands for NaN.
 - 8 bits (e4m3, no infinities): one value to a byte; a line holds
-  ``ceil(n / 32)`` blocks. An infinity or a NaN is kept as NaN in its place.
+  ``ceil(n / 32)`` blocks, and codes past its end count for nothing. An
+  infinity or a NaN is kept as NaN in its place.
 
 Arguments are 2-dimensional GPU tensors of float32, bfloat16 or float16 with
 any strides; batches are ``[tokens, units]``. Work goes to torch's current

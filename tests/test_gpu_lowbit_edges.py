@@ -1,0 +1,75 @@
+"""plastax_amd.lowbit where its forms meet their limits: what lies behind a
+line's end, views, the ends of float32's range, infinities, and the large
+products (each case's form pinned by its workspace)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import lowbit_plain as plain
+from plastax_amd import lowbit
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+
+
+def _gen(seed: int) -> torch.Generator:
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _randn(shape, g) -> torch.Tensor:
+    return torch.randn(shape, generator=g, device=DEV)
+
+
+def _say(*what) -> None:
+    print(*what, flush=True)
+
+
+# ---------------------------------------------------------------------------
+# Behind a line's end
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("shape", [(1, 40, 24), (33, 130, 70), (70, 300, 200), (257, 770, 520), (1003, 64, 64),
+                                   (8190, 1100, 1100)])
+def test_codes_of_8_bits_behind_a_lines_end_count_for_nothing(shape, dtype) -> None:
+    tokens, inputs, outputs = shape
+    _say("padding8", shape, dtype)
+    g = _gen(1)
+    x, dy = _randn((tokens, inputs), g), _randn((tokens, outputs), g).to(dtype)
+    for axis in (0, 1):
+        n = (tokens, inputs)[axis]
+        kept = lowbit.quantise8(x, axis=axis)
+        want, values = lowbit.weight_grad(dy, kept), kept.values()
+        slopes = lowbit.activate_grad(x, kept, "silu")
+        for byte in (0x7F, 0xFF, 0x38):
+            codes = kept.codes.clone()
+            codes[:, n:] = byte
+            other = lowbit.Mx8(codes, kept.scales, (tokens, inputs), axis)
+            assert torch.equal(lowbit.weight_grad(dy, other), want)
+            assert torch.equal(other.values(), values)
+            assert torch.equal(lowbit.activate_grad(x, other, "silu"), slopes)
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 70), (3, 31, 70), (16, 1000, 100), (40, 33, 65), (300, 1003, 777),
+                                   (1100, 2049, 4608), (1100, 5000, 4700)])
+def test_scales_of_4_bits_behind_a_lines_end_count_for_nothing(shape) -> None:
+    tokens, inputs, outputs = shape
+    _say("padding4", shape)
+    g = _gen(2)
+
+    def with_nan_scales(m: lowbit.Mx4) -> lowbit.Mx4:
+        scales = m.scales.clone()
+        scales[:, -(-m.shape[1] // 32):] = 255
+        return lowbit.Mx4(m.codes, scales, m.shape[1])
+
+    w = lowbit.quantise4(_randn((outputs, inputs), g))
+    other = with_nan_scales(w)
+    assert torch.equal(other.values(), w.values())
+    for dtype in plain.DTYPES:
+        x, dy = _randn((tokens, inputs), g).to(dtype), _randn((tokens, outputs), g).to(dtype)
+        assert torch.equal(lowbit.product(x, other), lowbit.product(x, w))
+        assert torch.equal(lowbit.product_grad(dy, other), lowbit.product_grad(dy, w))
+        x4 = lowbit.quantise4(x)
+        assert torch.equal(lowbit.product(with_nan_scales(x4), other, dtype=dtype), lowbit.product(x4, w, dtype=dtype))
