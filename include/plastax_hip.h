@@ -1195,7 +1195,7 @@ PLX_EXPORT int plx_count_ids(int64_t n, const int32_t* ids, const uint8_t* skip,
  *     ceil(n / 32) blocks of 32 bytes; codes past its end count for nothing.
  *     An infinity or a NaN is kept as NaN in its own place.
  * codes start on 16 bytes. Sizes are at most 2^30, in products 2^24 inputs and
- * outputs. Strides are in elements. */
+ * outputs. Strides are in elements, of either sign or zero. */
 #define PLX_LB_F32 0
 #define PLX_LB_BF16 1
 #define PLX_LB_F16 2

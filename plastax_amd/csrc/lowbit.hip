@@ -873,7 +873,7 @@ Plan plan_of(int kind, const Shape& s, int dtype, const void* a, int64_t sm, int
   p.across = sm == 1 && sk != 1;
   p.kp = round_up(s.k, 64), p.mp = round_up(s.m, 8);
   const int64_t line = p.across ? sk : sm;
-  p.direct = dtype == PLX_LB_BF16 && s.k % 64 == 0 && on16(a) && line % 8 == 0 && line <= kBigLine &&
+  p.direct = dtype == PLX_LB_BF16 && s.k % 64 == 0 && on16(a) && line % 8 == 0 && line >= 0 && line <= kBigLine &&
              (p.across ? s.m % 8 == 0 : sk == 1);
   p.bytes_w = round_up(2 * p.kp * s.n, 256);
   p.bytes_u = p.direct ? 0 : round_up(2 * pieces * p.kp * (p.across ? p.mp : s.m), 256);

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import lowbit_plain as plain
-from plastax_amd import lowbit
+from plastax_amd import _lib, lowbit
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,27 @@ def test_scales_of_4_bits_behind_a_lines_end_count_for_nothing(shape) -> None:
         assert torch.equal(lowbit.product_grad(dy, other), lowbit.product_grad(dy, w))
         x4 = lowbit.quantise4(x)
         assert torch.equal(lowbit.product(with_nan_scales(x4), other, dtype=dtype), lowbit.product(x4, w, dtype=dtype))
+
+
+# ---------------------------------------------------------------------------
+# Lines that run backwards (of C callers: torch has no such views)
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("shape", [(5, 256, 70), (70, 300, 200), (2304, 2112, 2304)])
+def test_products_of_lines_that_run_backwards(shape, dtype) -> None:
+    tokens, inputs, outputs = shape
+    _say("backwards", shape, dtype)
+    g = _gen(3)
+    w = lowbit.quantise4(_randn((outputs, inputs), g))
+    x = _randn((tokens, inputs), g).to(dtype)
+    lib, size, stream = _lib.load(), x.element_size(), torch.cuda.current_stream().cuda_stream
+    back, columns = x.flip(0).contiguous(), x.t().flip(0).contiguous()
+    for at, strides in ((back.data_ptr() + (tokens - 1) * inputs * size, (-inputs, 1)),
+                        (columns.data_ptr() + (inputs - 1) * tokens * size, (1, -tokens))):
+        args = (0, tokens, inputs, outputs, lowbit.DTYPES[dtype], at, *strides)
+        need = lib.plx_mx_workspace(*args)
+        work = torch.empty(need, dtype=torch.uint8, device=DEV)
+        out = torch.empty((tokens, outputs), dtype=dtype, device=DEV)
+        _lib.check(lib.plx_mx_product(*args, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
+                                      work.data_ptr(), need, stream), "plx_mx_product")
+        assert torch.equal(out, lowbit.product(x, w))
