@@ -121,14 +121,16 @@ class Mx8:
         return _values(self, 8, (self.shape[1], self.shape[0]), dtype).t()
 
 
-def _check(who: str, *tensors: torch.Tensor) -> None:
-    for t in tensors:
-        if t.dim() != 2:
-            raise ValueError(f"{who}: a matrix expected, got {t.dim()} dimensions")
-        if t.dtype not in DTYPES:
-            raise TypeError(f"{who}: float32, bfloat16 or float16 expected, got {t.dtype}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{who}: no autograd here; detach the argument and call the gradients")
+def _check(who: str, t: torch.Tensor) -> torch.Tensor:
+    """``t`` checked, with the values that it stands for in its memory (the
+    imaginary part of a conjugate view holds them with the other sign)."""
+    if t.dim() != 2:
+        raise ValueError(f"{who}: a matrix expected, got {t.dim()} dimensions")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{who}: float32, bfloat16 or float16 expected, got {t.dtype}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{who}: no autograd here; detach the argument and call the gradients")
+    return t.resolve_neg() if t.is_neg() else t
 
 
 def _on_gpu(who: str, device: torch.device, *others: torch.device) -> None:
@@ -167,7 +169,7 @@ def _values(m: Mx4 | Mx8, bits: int, shape: tuple[int, int], dtype: torch.dtype)
 
 def quantise4(x: torch.Tensor) -> Mx4:
     """``x`` in 4-bit blocks along its second dimension."""
-    _check("quantise4", x)
+    x = _check("quantise4", x)
     _on_gpu("quantise4", x.device)
     lines, n = x.shape
     m = Mx4._empty(lines, n, x.device)
@@ -181,7 +183,7 @@ def activate(h: torch.Tensor, fn: str, axis: int = 1) -> tuple[torch.Tensor, Mx8
     "silu" of a batch ``[tokens, units]``, and what its gradient needs. Blocks
     along 1 suit a token-major batch, along 0 one kept unit-major; the result
     has h's layout."""
-    _check("activate", h)
+    h = _check("activate", h)
     if fn not in FUNCTIONS:
         raise ValueError(f"activate: one of {sorted(FUNCTIONS)} expected, got {fn!r}")
     if axis not in (0, 1):
@@ -197,7 +199,7 @@ def activate(h: torch.Tensor, fn: str, axis: int = 1) -> tuple[torch.Tensor, Mx8
 def quantise8(x: torch.Tensor, axis: int = 1) -> Mx8:
     """``x`` ``[tokens, units]`` in 8-bit blocks along ``axis``: a level pair's
     input, kept for :func:`weight_grad`."""
-    _check("quantise8", x)
+    x = _check("quantise8", x)
     if axis not in (0, 1):
         raise ValueError(f"quantise8: axis 0 or 1 expected, got {axis}")
     _on_gpu("quantise8", x.device)
@@ -211,7 +213,7 @@ def quantise8(x: torch.Tensor, axis: int = 1) -> Mx8:
 def activate_grad(dy: torch.Tensor, kept: Mx8, fn: str) -> torch.Tensor:
     """``dy * fn'(q)``, q the values that :func:`activate` kept; dy's type and
     layout."""
-    _check("activate_grad", dy)
+    dy = _check("activate_grad", dy)
     if fn not in FUNCTIONS:
         raise ValueError(f"activate_grad: one of {sorted(FUNCTIONS)} expected, got {fn!r}")
     if tuple(dy.shape) != kept.shape:
@@ -264,7 +266,7 @@ def product(x: torch.Tensor | Mx4, w: Mx4, dtype: torch.dtype | None = None) -> 
         _launch(x.device, "plx_mx4_product", x.shape[0], inputs, outputs, x.codes.data_ptr(), x.scales.data_ptr(),
                 w.codes.data_ptr(), w.scales.data_ptr(), DTYPES[dtype], out.data_ptr(), at, need)
         return out
-    _check("product", x)
+    x = _check("product", x)
     if dtype is not None and dtype != x.dtype:
         raise TypeError(f"product: the result has x's type, {x.dtype}, not {dtype}")
     if x.shape[1] != inputs:
@@ -277,7 +279,7 @@ def product_grad(g: torch.Tensor, w: Mx4) -> torch.Tensor:
     """``g w`` ``[tokens, inputs]``: the gradient of :func:`product` for its
     input, from the gradient ``[tokens, outputs]`` of its result."""
     outputs, inputs = w.shape
-    _check("product_grad", g)
+    g = _check("product_grad", g)
     if g.shape[1] != outputs:
         raise ValueError(f"product_grad: {outputs} outputs expected, got {g.shape[1]}")
     _on_gpu("product_grad", g.device, w.device)
@@ -288,7 +290,7 @@ def weight_grad(g: torch.Tensor, kept: Mx8) -> torch.Tensor:
     """``g^T x`` ``[outputs, inputs]`` in float32: the gradient of a level
     pair's weights, from its result's gradient ``[tokens, outputs]`` and its
     input kept in 8 bits."""
-    _check("weight_grad", g)
+    g = _check("weight_grad", g)
     tokens, inputs = kept.shape
     if g.shape[0] != tokens:
         raise ValueError(f"weight_grad: {tokens} tokens expected, got {g.shape[0]}")

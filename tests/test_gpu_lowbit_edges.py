@@ -97,3 +97,26 @@ def test_products_of_lines_that_run_backwards(shape, dtype) -> None:
         _lib.check(lib.plx_mx_product(*args, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(),
                                       work.data_ptr(), need, stream), "plx_mx_product")
         assert torch.equal(out, lowbit.product(x, w))
+
+
+# ---------------------------------------------------------------------------
+# Views
+# ---------------------------------------------------------------------------
+def test_conjugate_parts_are_the_values_that_they_stand_for() -> None:
+    """Their memory holds them with the other sign."""
+    g = _gen(4)
+    z = torch.complex(_randn((40, 70), g), _randn((40, 70), g))
+    x = z.conj().imag
+    assert x.is_neg()
+    same = x.clone()
+    w, wt = lowbit.quantise4(_randn((9, 70), g)), lowbit.quantise4(_randn((70, 9), g))
+    assert torch.equal(lowbit.quantise4(x).codes, lowbit.quantise4(same).codes)
+    assert torch.equal(lowbit.product(x, w), lowbit.product(same, w))
+    assert torch.equal(lowbit.product_grad(x, wt), lowbit.product_grad(same, wt))
+    for axis in (0, 1):
+        y, kept = lowbit.activate(x, "silu", axis=axis)
+        want, other = lowbit.activate(same, "silu", axis=axis)
+        assert torch.equal(y, want) and torch.equal(kept.codes, other.codes)
+        assert torch.equal(lowbit.quantise8(x, axis=axis).codes, kept.codes)
+        assert torch.equal(lowbit.activate_grad(x, kept, "silu"), lowbit.activate_grad(same, kept, "silu"))
+        assert torch.equal(lowbit.weight_grad(x, kept), lowbit.weight_grad(same, kept))

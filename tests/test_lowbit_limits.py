@@ -3,9 +3,12 @@ no kernel is launched)."""
 
 from __future__ import annotations
 
-import pytest
+import ctypes
 
-from plastax_amd import _lib
+import pytest
+import torch
+
+from plastax_amd import _lib, lowbit
 
 P = 4096  # a pointer that is never followed
 F32, BF16, F16 = range(3)
@@ -30,3 +33,41 @@ def test_lines_that_run_backwards_are_copied_before_a_large_product(lib, kind) -
         assert lib.plx_mx_workspace(kind, n, n, n, BF16, P, *strides) == weights
     for strides in ((-n, 1), (1, -n), (-2 * n, 1), (-8, 1), (n, -1), (-1, n)):
         assert lib.plx_mx_workspace(kind, n, n, n, BF16, P, *strides) == 2 * weights, strides
+
+
+def _mx4(lines: int, n: int) -> lowbit.Mx4:
+    b = -(-n // 128) * 4
+    return lowbit.Mx4(torch.zeros((lines, 16 * b), dtype=torch.uint8), torch.full((lines, b), 127, dtype=torch.uint8), n)
+
+
+def _mx8(shape: tuple[int, int]) -> lowbit.Mx8:
+    b = -(-shape[1] // 32)
+    return lowbit.Mx8(torch.zeros((shape[0], 32 * b), dtype=torch.uint8),
+                      torch.full((shape[0], b), 127, dtype=torch.uint8), shape, 1)
+
+
+def _calls():
+    """Every function that takes a tensor [5, 70]."""
+    w, wt, kept = _mx4(9, 70), _mx4(70, 9), _mx8((5, 70))
+    return [lowbit.quantise4, lowbit.quantise8, lambda t: lowbit.activate(t, "tanh"),
+            lambda t: lowbit.activate_grad(t, kept, "tanh"), lambda t: lowbit.product(t, w),
+            lambda t: lowbit.product_grad(t, wt), lambda t: lowbit.weight_grad(t, kept)]
+
+
+def test_views_are_given_as_the_values_that_they_stand_for(monkeypatch) -> None:
+    """What a kernel finds where each call points it: the imaginary part of a conjugate is kept with the other sign."""
+    seen = []
+
+    def launch(device, name, *args):
+        at = next(i for i, a in enumerate(args) if a > 1 << 20)  # the argument's address; its strides follow
+        seen.append(torch.tensor([[ctypes.c_float.from_address(args[at] + 4 * (r * args[at + 1] + c * args[at + 2])).value
+                                   for c in range(70)] for r in range(5)]))
+
+    monkeypatch.setattr(lowbit, "_launch", launch)
+    monkeypatch.setattr(lowbit, "_on_gpu", lambda *a: None)
+    z = torch.complex(torch.randn(5, 70), torch.randn(5, 70))
+    for x in (z.conj().imag, z.conj().imag[:, :], z.imag, z.real):
+        for call in _calls():
+            seen.clear()
+            call(x)
+            assert torch.equal(seen[0], x.clone())
