@@ -24,14 +24,15 @@ go to the nearest, ties to the even code.
 Arguments are 2-dimensional GPU tensors of float32, bfloat16 or float16 with
 any strides; batches are ``[tokens, units]``. Work goes to torch's current
 stream of the arguments' device, results and workspaces are allocated there.
-Sums are float32. Results carry no autograd graph: an argument that asks for
-one is refused, the gradients are calls of their own. The reference has no
+Sums are float32. Results carry no autograd graph and no tangent: an argument
+that asks for one is refused, the gradients are calls of their own. The reference has no
 counterpart: its weights and activations are float32.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from plastax_amd import _lib
 
@@ -130,6 +131,9 @@ def _check(who: str, t: torch.Tensor) -> torch.Tensor:
         raise TypeError(f"{who}: float32, bfloat16 or float16 expected, got {t.dtype}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{who}: no autograd here; detach the argument and call the gradients")
+    # (the level is -1 outside of dual_level(), where no tensor has a tangent)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{who}: no forward-mode autograd here; unpack the argument and its tangent")
     return t.resolve_neg() if t.is_neg() else t
 
 

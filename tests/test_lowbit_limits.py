@@ -7,6 +7,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from plastax_amd import _lib, lowbit
 
@@ -71,3 +72,19 @@ def test_views_are_given_as_the_values_that_they_stand_for(monkeypatch) -> None:
             seen.clear()
             call(x)
             assert torch.equal(seen[0], x.clone())
+
+
+def test_tangents_are_refused() -> None:
+    """A result without the tangent would be a derivative of zero."""
+    x = torch.randn(5, 70)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in _calls():
+            with pytest.raises(ValueError, match="forward-mode"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                call(dual)
+            with pytest.raises(ValueError, match="GPU"):  # none of its own: as outside of the level
+                call(forward_ad.unpack_dual(dual).primal)
+            with pytest.raises(ValueError, match="GPU"):
+                call(x)
