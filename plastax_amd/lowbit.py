@@ -145,18 +145,21 @@ def _on_gpu(who: str, device: torch.device, *others: torch.device) -> None:
             raise ValueError(f"{who}: arguments are on different devices, {device} and {d}")
 
 
-def _launch(device: torch.device, name: str, *args: object) -> None:
-    """The entry point on torch's current stream of ``device`` (the kernels
-    launch on the current device)."""
-    index = device.index
-    # (current_stream(device).cuda_stream without its Stream object, 2 us of a 10 us call)
-    stream = torch._C._cuda_getCurrentRawStream(index)
+def _call(device: torch.device, name: str, *args: object) -> int:
+    """The entry point with ``device`` as the current one: kernels launch on
+    it, and plans go by its CUs."""
     fn = getattr(_lib.load(), name)
-    if index == torch.cuda.current_device():
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, stream)
+    # (a tensor is there, so the device is set up: current_device() without its check for that)
+    if device.index == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(device.index):
+        return fn(*args)
+
+
+def _launch(device: torch.device, name: str, *args: object) -> None:
+    """The entry point on torch's current stream of ``device``."""
+    # (current_stream(device).cuda_stream without its Stream object, 2 us of a 10 us call)
+    rc = _call(device, name, *args, torch._C._cuda_getCurrentRawStream(device.index))
     if rc:
         _lib.check(rc, name)
 
@@ -232,7 +235,7 @@ def activate_grad(dy: torch.Tensor, kept: Mx8, fn: str) -> torch.Tensor:
 
 
 def _workspace(device: torch.device, name: str, *args: object) -> torch.Tensor | None:
-    need = getattr(_lib.load(), name)(*args)
+    need = _call(device, name, *args)
     if need > 0:
         return torch.empty(need, dtype=torch.uint8, device=device)
     if need < 0:

@@ -3,7 +3,9 @@ no kernel is launched)."""
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import types
 
 import pytest
 import torch
@@ -66,6 +68,7 @@ def test_views_are_given_as_the_values_that_they_stand_for(monkeypatch) -> None:
 
     monkeypatch.setattr(lowbit, "_launch", launch)
     monkeypatch.setattr(lowbit, "_on_gpu", lambda *a: None)
+    monkeypatch.setattr(lowbit, "_workspace", lambda *a: None)
     z = torch.complex(torch.randn(5, 70), torch.randn(5, 70))
     for x in (z.conj().imag, z.conj().imag[:, :], z.imag, z.real):
         for call in _calls():
@@ -88,3 +91,33 @@ def test_tangents_are_refused() -> None:
                 call(forward_ad.unpack_dual(dual).primal)
             with pytest.raises(ValueError, match="GPU"):
                 call(x)
+
+
+def test_plans_and_launches_run_with_the_arguments_device_current(monkeypatch) -> None:
+    """Both count the current device's CUs: a size query on another one's plan is a workspace too small."""
+    current, seen = [0], []
+
+    @contextlib.contextmanager
+    def device(index):
+        was, current[0] = current[0], index
+        yield
+        current[0] = was
+
+    def entry(name, result):
+        return lambda *args: seen.append((name, current[0])) or result
+
+    lib = types.SimpleNamespace(**{n: entry(n, 0) for n in ("plx_mx_workspace", "plx_mx_product", "plx_mx4_workspace",
+                                                            "plx_mx4_product")})
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    for index in (0, 1):
+        at = torch.device("cuda", index)
+        for name in ("plx_mx_workspace", "plx_mx4_workspace"):
+            assert lowbit._workspace(at, name) is None
+        for name in ("plx_mx_product", "plx_mx4_product"):
+            lowbit._launch(at, name)
+        assert [i for _, i in seen] == [index] * 4 and current == [0]
+        seen.clear()
