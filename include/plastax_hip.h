@@ -1193,7 +1193,8 @@ PLX_EXPORT int plx_count_ids(int64_t n, const int32_t* ids, const uint8_t* skip,
  *     s = 255 and stands for NaN.
  *   8 bits: e4m3 codes without infinities, one to a byte; a line holds
  *     ceil(n / 32) blocks of 32 bytes; codes past its end count for nothing.
- *     An infinity or a NaN is kept as NaN in its own place.
+ *     An infinity or a NaN is kept as NaN in its own place, 0xff for a
+ *     negative infinity and 0x7f for the others.
  * codes start on 16 bytes. Sizes are at most 2^30, in products 2^24 inputs and
  * outputs. Strides are in elements, of either sign or zero. */
 #define PLX_LB_F32 0
@@ -1218,7 +1219,8 @@ PLX_EXPORT int plx_mx8_activate(int64_t lines, int64_t n, int32_t dtype, int32_t
                                 int64_t h_elem, void* y, int64_t y_line, int64_t y_elem, uint8_t* codes,
                                 uint8_t* scales, void* stream);
 
-/* dh = dy fn'(q), q the values of plx_mx8_activate's blocks. */
+/* dh = dy fn'(q), q the values of plx_mx8_activate's blocks (the rectifier's
+ * slope is 1 at the code 0x7f and 0 at 0xff, the others' NaN at both). */
 PLX_EXPORT int plx_mx8_activate_grad(int64_t lines, int64_t n, int32_t dtype, int32_t fn, const void* dy,
                                      int64_t y_line, int64_t y_elem, const uint8_t* codes, const uint8_t* scales,
                                      void* dh, int64_t h_line, int64_t h_elem, void* stream);

@@ -199,12 +199,28 @@ __device__ __forceinline__ float act(float h) {
 // silu' = sigmoid(q) + q sigmoid'(q).
 template <int FN>
 __device__ __forceinline__ float act_grad(float q) {
-  if (FN == PLX_LB_RELU) return q > 0.0f ? 1.0f : 0.0f;
   const float a = fabsf(q);
   const float t = exp_neg(FN == PLX_LB_TANH ? 2.0f * a : a), r = inverse(1.0f + t), d = t * r * r;
   if (FN == PLX_LB_TANH) return 4.0f * d;
   if (FN == PLX_LB_SIGMOID) return d;
   return (q >= 0.0f ? r : t * r) + (t == 0.0f ? 0.0f : q * d);  // (an infinite q has the slope 0 or 1)
+}
+// The slopes at 8 kept values. The rectifier's goes by the codes: 1 unless the
+// sign is set or all else is zero, so 1 at a kept infinity or NaN (0x7f), whose
+// result the forward passed on, and 0 at a negative infinity (0xff).
+template <int FN>
+__device__ __forceinline__ void act_grads8(uint2 c, float scale, float d[8]) {
+  if (FN == PLX_LB_RELU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int32_t top = static_cast<int32_t>((i < 4 ? c.x : c.y) << (24 - i % 4 * 8)) >> 24;  // (as a signed byte)
+      d[i] = top > 0 ? 1.0f : 0.0f;
+    }
+    return;
+  }
+  values8(c, scale, d);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) d[i] = act_grad<FN>(d[i]);
 }
 
 template <int FN, typename T>
@@ -276,12 +292,12 @@ __global__ __launch_bounds__(kBlock) void k_grad_along(int64_t lines, int64_t n,
     for (int64_t c = tx; c < chunks; c += lx) {
       const int64_t left64 = n - c * 8;
       const int left = left64 > 8 ? 8 : static_cast<int>(left64);
-      float v[8], q[8];
+      float v[8], d[8];
       load8<true>(dy + line * sy + c * 8, 1, left, v);
-      values8(reinterpret_cast<const uint2*>(codes)[line * kept + c], scale_value(scales[line * (kept / 4) + c / 4]),
-              q);
+      act_grads8<FN>(reinterpret_cast<const uint2*>(codes)[line * kept + c],
+                     scale_value(scales[line * (kept / 4) + c / 4]), d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= act_grad<FN>(q[i]);
+      for (int i = 0; i < 8; ++i) v[i] *= d[i];
       store8<true>(dh + line * sh + c * 8, left, v);
     }
   }
@@ -304,11 +320,11 @@ __global__ __launch_bounds__(kBlock) void k_grad_across(int64_t lines, int64_t n
     T* o = dh + line * hl + b * 32 * he;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float q[8];
-      values8(c[i], scale, q);
+      float d[8];
+      act_grads8<FN>(c[i], scale, d);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (i * 8 + j < left) o[(i * 8 + j) * he] = from_f32<T>(to_f32(p[(i * 8 + j) * se]) * act_grad<FN>(q[j]));
+        if (i * 8 + j < left) o[(i * 8 + j) * he] = from_f32<T>(to_f32(p[(i * 8 + j) * se]) * d[j]);
     }
   }
 }

@@ -137,17 +137,30 @@ __device__ __forceinline__ uint32_t codes4(const float v[8], float scale) {
   return c;
 }
 
-// 8 values times inv = 2^-e as e4m3 codes; a value that is not finite is NaN.
+// 8 values times inv = 2^-e as e4m3 codes; one that is not finite is NaN, with
+// the sign bit of a negative infinity alone.
 __device__ __forceinline__ uint2 codes8(const float v[8], float inv) {
   float m[8];
+  bool fine = true;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m[i] = abs_bits(v[i]) >= kInfBits ? __builtin_nanf("") : v[i] * inv;
+  for (int i = 0; i < 8; ++i) {
+    const bool in = abs_bits(v[i]) < kInfBits;
+    m[i] = in ? v[i] * inv : 0.0f;
+    fine = fine && in;
+  }
   int a = 0, b = 0;
   a = __builtin_amdgcn_cvt_pk_fp8_f32(m[0], m[1], a, false);
   a = __builtin_amdgcn_cvt_pk_fp8_f32(m[2], m[3], a, true);
   b = __builtin_amdgcn_cvt_pk_fp8_f32(m[4], m[5], b, false);
   b = __builtin_amdgcn_cvt_pk_fp8_f32(m[6], m[7], b, true);
-  return make_uint2(static_cast<uint32_t>(a), static_cast<uint32_t>(b));
+  uint2 c = make_uint2(static_cast<uint32_t>(a), static_cast<uint32_t>(b));
+  if (!fine) {  // (the conversion of a NaN would lose its sign)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (abs_bits(v[i]) >= kInfBits)
+        (i < 4 ? c.x : c.y) |= (__float_as_uint(v[i]) == (0x80000000u | kInfBits) ? 0xFFu : 0x7Fu) << (i % 4 * 8);
+  }
+  return c;
 }
 
 // The float32 values of 8 codes under a scale (exact: 2 or 4 significant

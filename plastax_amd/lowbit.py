@@ -19,7 +19,8 @@ go to the nearest, ties to the even code.
   with an infinity or a NaN has ``s = 255`` and stands for NaN.
 - 8 bits (e4m3, no infinities): one value to a byte; a line holds
   ``ceil(n / 32)`` blocks, and codes past its end count for nothing. An
-  infinity or a NaN is kept as NaN in its place.
+  infinity or a NaN is kept as NaN in its place, with the sign bit of a
+  negative infinity alone.
 
 Arguments are 2-dimensional GPU tensors of float32, bfloat16 or float16 with
 any strides; batches are ``[tokens, units]``. Work goes to torch's current
@@ -219,7 +220,8 @@ def quantise8(x: torch.Tensor, axis: int = 1) -> Mx8:
 
 def activate_grad(dy: torch.Tensor, kept: Mx8, fn: str) -> torch.Tensor:
     """``dy * fn'(q)``, q the values that :func:`activate` kept; dy's type and
-    layout."""
+    layout. At a kept infinity or NaN the rectifier's slope is 1 (0 at a
+    negative infinity), the others' is NaN."""
     dy = _check("activate_grad", dy)
     if fn not in FUNCTIONS:
         raise ValueError(f"activate_grad: one of {sorted(FUNCTIONS)} expected, got {fn!r}")

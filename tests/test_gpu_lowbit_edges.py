@@ -120,3 +120,35 @@ def test_conjugate_parts_are_the_values_that_they_stand_for() -> None:
         assert torch.equal(lowbit.quantise8(x, axis=axis).codes, kept.codes)
         assert torch.equal(lowbit.activate_grad(x, kept, "silu"), lowbit.activate_grad(same, kept, "silu"))
         assert torch.equal(lowbit.weight_grad(x, kept), lowbit.weight_grad(same, kept))
+
+
+# ---------------------------------------------------------------------------
+# Infinities and NaN in kept activations
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("axis", [0, 1])
+@pytest.mark.parametrize("layout", ["rows", "columns", "steps"])
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+def test_the_rectifiers_gradient_passes_where_its_result_does(dtype, layout, axis) -> None:
+    """At an infinity and a NaN, not at a negative infinity, as torch's own; the other slopes are NaN at all three."""
+    g = _gen(5)
+    h = _randn((70, 131), g) * 3
+    places = torch.rand((70, 131), generator=g, device=DEV)
+    h[places < 0.15] = torch.inf
+    h[places < 0.10] = -torch.inf
+    h[places < 0.05] = torch.nan
+    h[places < 0.02] = -torch.tensor(torch.nan, device=DEV).abs()  # a NaN whose sign bit is set
+    h[:, 64:96] = torch.where(places[:, 64:96] < 0.5, torch.inf, -torch.inf)  # blocks without a finite value
+    h = h.to(dtype)
+    dy = plain.layouts(_randn((70, 131), g).to(dtype))[layout]
+    x = plain.layouts(h)[layout]
+    y, kept = lowbit.activate(x, "relu", axis=axis)
+    finite = torch.isfinite(h)
+    assert torch.equal(torch.isposinf(y), torch.isposinf(h)) and torch.equal(torch.isnan(y), torch.isnan(h))
+    q = kept.values(torch.float32)
+    assert torch.equal(torch.isnan(q), ~finite)
+    codes = (kept.codes[:, :131] if axis else kept.codes[:, :70].t())[~finite]
+    assert torch.equal(codes == 0xFF, torch.isneginf(h)[~finite]) and bool(((codes & 0x7F) == 0x7F).all())
+    passes = torch.where(finite, q > 0, ~torch.isneginf(h))
+    assert torch.equal(lowbit.activate_grad(dy, kept, "relu"), torch.where(passes, dy, 0 * dy))
+    for fn in ("tanh", "sigmoid", "silu"):
+        assert torch.equal(torch.isnan(lowbit.activate_grad(dy, kept, fn)), ~finite)
