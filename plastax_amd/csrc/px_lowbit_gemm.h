@@ -531,7 +531,8 @@ __device__ __forceinline__ void big_turned(const BigValues& g, int64_t group, ch
 }
 
 // The user's operand as bf16 pieces in padded lines: piece p of line l at
-// out + p * piece + l * out_line.
+// out + (P - 1 - p) * piece + l * out_line. k goes over the least pieces first:
+// added to the sums of the largest ones they would be rounded off one by one.
 struct BigPieces {
   const void* x;
   int64_t lines, n, sl, se;  // elements of line l at l * sl + i * se
@@ -552,7 +553,8 @@ __device__ __forceinline__ void big_pieces(const BigPieces& g, int64_t group, in
       uint4 p[P];
       pieces8<P>(v, p);
 #pragma unroll
-      for (int i = 0; i < P; ++i) *reinterpret_cast<uint4*>(g.out + i * g.piece + line * g.out_line + c * 8) = p[i];
+      for (int i = 0; i < P; ++i)
+        *reinterpret_cast<uint4*>(g.out + (P - 1 - i) * g.piece + line * g.out_line + c * 8) = p[i];
     }
 }
 

@@ -27,6 +27,30 @@ def _say(*what) -> None:
     print(*what, flush=True)
 
 
+def _ranges(kind: str, w: lowbit.Mx4 | lowbit.Mx8, a: torch.Tensor) -> int:
+    """The ranges of k that a product of ``a`` runs in as a large one, 0 if it runs in small tiles: by its workspace,
+    which holds the codes as bf16, a's pieces (a itself where it is bf16 already) and the ranges' sums."""
+    lib = _lib.load()
+    tokens = a.shape[0]
+    if kind == "weight_grad":
+        number, inputs, outputs = 2 if w.axis else 3, w.shape[1], a.shape[1]
+        m, n, k = outputs, inputs, tokens
+    else:
+        number, (outputs, inputs) = ("product", "product_grad").index(kind), w.shape
+        m, n, k = (tokens, outputs, inputs) if number == 0 else (tokens, inputs, outputs)
+    need = lib.plx_mx_workspace(number, tokens, inputs, outputs, lowbit.DTYPES[a.dtype], a.data_ptr(), *a.stride())
+    padded = -(-k // 64) * 64
+    pieces = {torch.float32: 3, torch.float16: 2, torch.bfloat16: 1}[a.dtype]
+    along_m = (a.stride(1) if number >= 2 else a.stride(0)) == 1
+    codes, copy = -(-2 * padded * n // 256) * 256, -(-2 * pieces * padded * (-(-m // 8) * 8 if along_m else m) // 256) * 256
+    for size in (codes, codes + copy) if pieces == 1 else (codes + copy,):
+        if need == size:
+            return 1
+        if need > size and (need - size) % (4 * m * n) == 0 and (need - size) // (4 * m * n) > 1:
+            return (need - size) // (4 * m * n)
+    return 0
+
+
 # ---------------------------------------------------------------------------
 # Behind a line's end
 # ---------------------------------------------------------------------------
@@ -152,3 +176,32 @@ def test_the_rectifiers_gradient_passes_where_its_result_does(dtype, layout, axi
     assert torch.equal(lowbit.activate_grad(dy, kept, "relu"), torch.where(passes, dy, 0 * dy))
     for fn in ("tanh", "sigmoid", "silu"):
         assert torch.equal(torch.isnan(lowbit.activate_grad(dy, kept, fn)), ~finite)
+
+
+# ---------------------------------------------------------------------------
+# The pieces of float32
+# ---------------------------------------------------------------------------
+def _forms(tokens, inputs, outputs, x, dy):
+    """(name, k, function, codes, tensor) of the products of x and dy with weights and kept inputs of ones."""
+    w = lowbit.quantise4(torch.ones((outputs, inputs), device=DEV))
+    yield "product", inputs, lowbit.product, w, x
+    yield "product_grad", outputs, lowbit.product_grad, w, dy
+    for axis in (0, 1):
+        yield "weight_grad", tokens, lowbit.weight_grad, lowbit.quantise8(torch.ones((tokens, inputs), device=DEV), axis), dy
+
+
+@pytest.mark.parametrize("layout", ["rows", "columns", "offset"])
+@pytest.mark.parametrize("shape", [(4096, 4096, 4096), (8192, 4096, 2048)])
+def test_large_sums_keep_what_float32_can_hold(shape, layout) -> None:
+    """k times 1 + 2^-23 is one step above k, and its low pieces, half a step of the sum and less each, count together
+    (in one range of k: two ranges may halve the step between them)."""
+    tokens, inputs, outputs = shape
+    _say("low pieces", shape, layout)
+    x = plain.layouts(torch.full((tokens, inputs), 1 + 2.0**-23, device=DEV))[layout]
+    dy = plain.layouts(torch.full((tokens, outputs), 1 + 2.0**-23, device=DEV))[layout]
+    large = 0
+    for kind, k, call, codes, a in _forms(*shape, x, dy):
+        if _ranges(kind, codes, a) == 1:
+            large += 1
+            assert call(a, codes).eq(k * (1 + 2.0**-23)).all().item(), kind
+    assert large == (4 if tokens == 4096 else 2)
