@@ -213,8 +213,9 @@ __device__ __forceinline__ void act_grads8(uint2 c, float scale, float d[8]) {
   if (FN == PLX_LB_RELU) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int32_t top = static_cast<int32_t>((i < 4 ? c.x : c.y) << (24 - i % 4 * 8)) >> 24;  // (as a signed byte)
-      d[i] = top > 0 ? 1.0f : 0.0f;
+      const uint32_t w = i < 4 ? c.x : c.y;
+      const uint32_t set = (((w & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) & ~w & 0x80808080u) >> 7;  // (1 in those bytes)
+      d[i] = static_cast<float>(set >> (i % 4 * 8) & 0xFFu);
     }
     return;
   }
@@ -235,16 +236,16 @@ __global__ __launch_bounds__(kBlock) void k_act_along(int64_t lines, int64_t n, 
       const int left = left64 > 8 ? 8 : left64 < 0 ? 0 : static_cast<int>(left64);
       float v[8], f[8];
       load8<true>(h + line * sh + c * 8, 1, left, v);
-      uint32_t m = 0;
+      uint32_t m = largest8<false>(0, v);
+      const bool fine = m < kInfBits;
+      if (!fine) m = largest8<true>(0, v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t a = abs_bits(v[i]);
-        m = a < kInfBits && a > m ? a : m;
-        f[i] = act<FN>(v[i]);
-      }
+      for (int i = 0; i < 8; ++i) f[i] = act<FN>(v[i]);
       if (y) store8<true>(y + line * sy + c * 8, left, f);
       const int e = exponent8(max4(m));
-      reinterpret_cast<uint2*>(codes)[line * chunks + c] = codes8(v, pow2(-e));
+      uint2 k = codes8(v, pow2(-e));
+      if (!fine) k = mark8(k, v);
+      reinterpret_cast<uint2*>(codes)[line * chunks + c] = k;
       if ((tx & 3) == 0) scales[line * (chunks / 4) + c / 4] = static_cast<uint8_t>(e + 127);
     }
   }
@@ -265,15 +266,29 @@ __global__ __launch_bounds__(kBlock) void k_act_across(int64_t lines, int64_t n,
     float v[4][8];
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      v[i / 8][i % 8] = i < left ? to_f32(p[i * se]) : 0.0f;
-      const uint32_t a = abs_bits(v[i / 8][i % 8]);
-      m = a < kInfBits && a > m ? a : m;
+    for (int i = 0; i < 32; ++i) {  // (loads without a condition, 32 in flight)
+      const float at = to_f32(p[(i < left ? i : left - 1) * se]);
+      v[i / 8][i % 8] = i < left ? at : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = largest8<false>(m, v[i]);
+    const bool fine = m < kInfBits;
+    if (!fine) {
+      m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = largest8<true>(m, v[i]);
     }
     const int e = exponent8(m);
+    uint2 k[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = codes8(v[i], pow2(-e));
+    if (!fine) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] = mark8(k[i], v[i]);
+    }
     uint2* c = reinterpret_cast<uint2*>(codes) + (line * blocks + b) * 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = codes8(v[i], pow2(-e));
+    for (int i = 0; i < 4; ++i) c[i] = k[i];
     scales[line * blocks + b] = static_cast<uint8_t>(e + 127);
 #pragma unroll
     for (int i = 0; i < 32; ++i)

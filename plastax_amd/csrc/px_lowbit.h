@@ -137,30 +137,36 @@ __device__ __forceinline__ uint32_t codes4(const float v[8], float scale) {
   return c;
 }
 
-// 8 values times inv = 2^-e as e4m3 codes; one that is not finite is NaN, with
-// the sign bit of a negative infinity alone.
+// 8 values times inv = 2^-e as e4m3 codes; one that is not finite is some NaN.
 __device__ __forceinline__ uint2 codes8(const float v[8], float inv) {
-  float m[8];
-  bool fine = true;
+  int a = 0, b = 0;
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, a, false);
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, a, true);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, b, false);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, b, true);
+  return make_uint2(static_cast<uint32_t>(a), static_cast<uint32_t>(b));
+}
+// The codes of values that are not finite: 0xff for a negative infinity, 0x7f
+// for the others.
+__device__ __forceinline__ uint2 mark8(uint2 c, const float v[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (abs_bits(v[i]) >= kInfBits) {
+      const uint32_t code = __float_as_uint(v[i]) == (0x80000000u | kInfBits) ? 0xFFu : 0x7Fu;
+      uint32_t& w = i < 4 ? c.x : c.y;
+      w = (w & ~(0xFFu << (i % 4 * 8))) | code << (i % 4 * 8);
+    }
+  return c;
+}
+// The largest of m and 8 |values| as bits, of all of them or of the finite ones.
+template <bool FINITE>
+__device__ __forceinline__ uint32_t largest8(uint32_t m, const float v[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const bool in = abs_bits(v[i]) < kInfBits;
-    m[i] = in ? v[i] * inv : 0.0f;
-    fine = fine && in;
+    const uint32_t a = abs_bits(v[i]);
+    m = a > m && (!FINITE || a < kInfBits) ? a : m;
   }
-  int a = 0, b = 0;
-  a = __builtin_amdgcn_cvt_pk_fp8_f32(m[0], m[1], a, false);
-  a = __builtin_amdgcn_cvt_pk_fp8_f32(m[2], m[3], a, true);
-  b = __builtin_amdgcn_cvt_pk_fp8_f32(m[4], m[5], b, false);
-  b = __builtin_amdgcn_cvt_pk_fp8_f32(m[6], m[7], b, true);
-  uint2 c = make_uint2(static_cast<uint32_t>(a), static_cast<uint32_t>(b));
-  if (!fine) {  // (the conversion of a NaN would lose its sign)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (abs_bits(v[i]) >= kInfBits)
-        (i < 4 ? c.x : c.y) |= (__float_as_uint(v[i]) == (0x80000000u | kInfBits) ? 0xFFu : 0x7Fu) << (i % 4 * 8);
-  }
-  return c;
+  return m;
 }
 
 // The float32 values of 8 codes under a scale (exact: 2 or 4 significant
