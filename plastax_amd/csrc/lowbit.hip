@@ -353,7 +353,8 @@ __global__ __launch_bounds__(kBlock) void k_grad_across(int64_t lines, int64_t n
 //   kXT   8-bit values, lines n, blocks along k       (the same, unit-major)
 // Every b is exact in bf16, and a is split into the bf16 pieces that hold it
 // exactly (pieces8), so every product is exact and only the float32 sums of
-// the matrix instruction round.
+// the matrix instruction round. Pieces of different units have sums of their own,
+// joined at the end.
 // ---------------------------------------------------------------------------
 enum { kW = 0, kWT = 1, kX = 2, kXT = 3 };
 
@@ -433,9 +434,11 @@ __device__ __forceinline__ void tile_store(const f32x4 (&acc)[TS / 32][TS / 32],
 // fragments are read transposed. What bounds it is that a step's phases follow
 // each other: bf16 256 x 4096 x 4096 takes 20 us, 36 % of a CU's cycles
 // conversions and addresses, 33 % LDS, 16 % matrix instructions.
+// Four waves a SIMD at least: float32's sums for each unit would leave three
+// (1 x 4096 x 4096's weight gradient 22.4 us, so 19.0).
 template <typename T, int KIND, typename OT, int TS, int KS, bool AA>
-__global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
-  constexpr int P = Pieces<T>::n;
+__global__ __launch_bounds__(256 * KS, 4) void k_mx_gemm(GemmArgs g) {
+  constexpr int P = Pieces<T>::n, S = Pieces<T>::sums;
   constexpr bool BA = KIND == kWT || KIND == kX;
   constexpr int BITS = KIND == kW || KIND == kWT ? 4 : 8;
   constexpr int F = TS / 32, kLine = TS / 8;                // (fragments a wave and side; chunks of a line across)
@@ -533,13 +536,14 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
     return as_bf16x8(t[r * 8 + ((s * 4 + q) ^ (r & 7))]);
   };
 
-  f32x4 acc[F][F] = {};
+  f32x4 acc[F][F][S] = {};
   const int wn = (wave & 1) * (TS / 2), wm = ((wave >> 1) & 1) * (TS / 2);
-  auto compute = [&](int buf) {
+  auto compute = [&](int buf, int k0) {
     const uint4* la = lds + buf * kUints;
     const uint4* lb = la + P * KS * kSub;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
+      if (KS == 1 && k0 + s * 32 >= kend) break;  // (zeros from there on)
       bf16x8 fb[F], fa[F][P];
 #pragma unroll
       for (int i = 0; i < F; ++i) {
@@ -553,7 +557,7 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
         for (int i = 0; i < F; ++i)
 #pragma unroll
           for (int j = 0; j < F; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa[j][p], acc[i][j], 0, 0, 0);
+            acc[i][j][p % S] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[i], fa[j][p], acc[i][j][p % S], 0, 0, 0);
     }
   };
   load(kbeg);
@@ -565,7 +569,7 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
       __syncthreads();
       if (k0 + kStep < kend) put(buf ^ 1, k0 + kStep);
       load(k0 + 2 * kStep);
-      compute(buf);
+      compute(buf, k0);
       buf ^= 1;
     }
   } else {
@@ -574,10 +578,15 @@ __global__ __launch_bounds__(256 * KS) void k_mx_gemm(GemmArgs g) {
       put(0, k0);
       __syncthreads();
       load(k0 + kStep);
-      compute(0);
+      compute(0, k0);
     }
   }
-  tile_store<TS, KS, OT>(acc, lds, group, wm, wn, m0, n0, g.M, g.N, static_cast<OT*>(g.out), g.part);
+  f32x4 sums[F][F];
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int j = 0; j < F; ++j) sums[i][j] = join_sums(acc[i][j]);
+  tile_store<TS, KS, OT>(sums, lds, group, wm, wn, m0, n0, g.M, g.N, static_cast<OT*>(g.out), g.part);
 }
 
 // out = the partial sums of the k ranges, in their order.
@@ -596,7 +605,8 @@ __global__ __launch_bounds__(kBlock) void k_mx_join(int64_t n, int splits, const
 // inputs of one token, straight into the matrix instruction, and the waves'
 // sums are added in order. Weights are read once, so what counts is how many
 // loads are in flight: one token through 4096 x 4096 takes 5.6 us (8.9 MB),
-// with 8 waves 8.3; small tiles take 10.5 and the sum of their ranges 3.7.
+// with 8 waves 8.3; small tiles take 10.5 and the sum of their ranges 3.7 (in a
+// captured graph 5.1, in float32 8.4).
 constexpr int kFew = 16;
 template <bool ALONG>
 constexpr int kFewWaves = ALONG ? 16 : 8;
@@ -614,7 +624,7 @@ __device__ __forceinline__ typename Unit<T>::type load_tail(const T* p, int left
 // ALONG: inputs next to each other, 8 of them or more.
 template <typename T, bool ALONG>
 __global__ __launch_bounds__(64 * kFewWaves<ALONG>) void k_mx_few(GemmArgs g) {
-  constexpr int W = kFewWaves<ALONG>, P = Pieces<T>::n, kAhead = ALONG ? 2 : 1;
+  constexpr int W = kFewWaves<ALONG>, P = Pieces<T>::n, S = Pieces<T>::sums, kAhead = ALONG ? 2 : 1;
   __shared__ f32x4 sums[W][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, q = lane >> 4;
   const int n = blockIdx.x * 16 + l15;
@@ -622,7 +632,7 @@ __global__ __launch_bounds__(64 * kFewWaves<ALONG>) void k_mx_few(GemmArgs g) {
   const uint4* codes = reinterpret_cast<const uint4*>(g.codes) + n * g.blocks;
   const uint8_t* scales = g.scales + n * g.blocks;
   const int blocks = static_cast<int>(div_up(g.K, 32));  // (what is behind a line's end counts for nothing)
-  f32x4 acc = {};
+  f32x4 of[S] = {};
   for (int b0 = wave * 4 + q; b0 - q < blocks; b0 += kAhead * W * 4) {
     uint4 c[kAhead];
     uint32_t s[kAhead];
@@ -657,10 +667,12 @@ __global__ __launch_bounds__(64 * kFewWaves<ALONG>) void k_mx_few(GemmArgs g) {
         unit_pieces(v[i][j], p);
         const bf16x8 fw = as_bf16x8(bf16_of4(w[j], scale));
 #pragma unroll
-        for (int h = P - 1; h >= 0; --h) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, as_bf16x8(p[h]), acc, 0, 0, 0);
+        for (int h = P - 1; h >= 0; --h)
+          of[h % S] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, as_bf16x8(p[h]), of[h % S], 0, 0, 0);
       }
     }
   }
+  f32x4 acc = join_sums(of);
   sums[wave][lane] = acc;
   __syncthreads();
   if (wave != 0 || l15 >= g.M) return;
@@ -881,11 +893,12 @@ struct Plan {
   int64_t bytes_w, bytes_u, bytes;
 };
 
-// Workgroups that a large product should fill: one per CU.
-int big_splits(int64_t m, int64_t n, int64_t steps) {
+// Workgroups that a large product should fill: one per CU, each with 8 steps
+// or more, `each` of them from one of its range.
+int big_splits(int64_t m, int64_t n, int64_t steps, int64_t each) {
   const int64_t tiles = div_up(m, kBig) * div_up(n, kBig);
   int64_t s = cu_count() / (tiles > 0 ? tiles : 1);
-  s = s < steps / 8 ? s : steps / 8;
+  s = s < steps * each / 8 ? s : steps * each / 8;
   if (s < 2) return 1;
   return static_cast<int>(div_up(steps, div_up(steps, s)));  // (no range is empty)
 }
@@ -908,7 +921,7 @@ Plan plan_of(int kind, const Shape& s, int dtype, const void* a, int64_t sm, int
              (p.across ? s.m % 8 == 0 : sk == 1);
   p.bytes_w = round_up(2 * p.kp * s.n, 256);
   p.bytes_u = p.direct ? 0 : round_up(2 * pieces * p.kp * (p.across ? p.mp : s.m), 256);
-  p.splits = big_splits(s.m, s.n, pieces * p.kp / 64);
+  p.splits = pieces == 3 ? big_splits(s.m, s.n, p.kp / 64, 3) : big_splits(s.m, s.n, pieces * p.kp / 64, 1);
   p.bytes = p.bytes_w + p.bytes_u + (p.splits > 1 ? int64_t{4} * p.splits * s.m * s.n : 0);
   return p;
 }
@@ -933,7 +946,9 @@ void launch_big(const GemmArgs& g, const Plan& p, char* work, hipStream_t s) {
   const unsigned groups = turned ? static_cast<unsigned>(p.kp / 64 * v.tiles_n) : groups_along(g.N, v.lx);
   b.w = work;
   b.ldw = 2 * p.kp;
-  b.wrap = static_cast<int>(p.kp / 64), b.steps = P * b.wrap;
+  b.wrap = static_cast<int>(p.kp / 64), b.units = Pieces<T>::sums;
+  b.steps = P / b.units * b.wrap;
+  b.down[0] = kPiece2, b.down[1] = kPiece1;
   BigPieces u{};
   unsigned more = 0;
   if (p.direct) {
@@ -982,7 +997,7 @@ Plan4 plan4_of(int64_t m, int64_t n, int64_t k) {
     return p;
   }
   p.steps = static_cast<int>(div_up(k, 256));
-  p.splits = big_splits(m, n, p.steps);
+  p.splits = big_splits(m, n, p.steps, 1);
   p.bytes_w = div_up(n, kBig) * p.steps * 2048, p.bytes_u = div_up(m, kBig) * p.steps * 2048;
   p.bytes = p.bytes_w + p.bytes_u + (p.splits > 1 ? 4 * p.splits * m * n : 0);
   return p;
@@ -1203,7 +1218,7 @@ int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, const uint8
     g.out = out, g.part = reinterpret_cast<float*>(work + p.bytes_w + p.bytes_u);
     g.M = g.rows_u = static_cast<int>(tokens), g.N = static_cast<int>(outputs);
     g.ldw = g.ldu = blocks * 16;
-    g.steps = g.wrap = p.steps, g.split = static_cast<int>(div_up(p.steps, p.splits));
+    g.steps = g.wrap = p.steps, g.units = 1, g.split = static_cast<int>(div_up(p.steps, p.splits));
     g.tiles_m = static_cast<int>(div_up(tokens, kBig)), g.tiles_n = static_cast<int>(div_up(outputs, kBig));
     k_big_scales<<<static_cast<unsigned>((g.tiles_m + g.tiles_n) * div_up(p.steps, 8)), 256, 0, s>>>(
         g.N, g.M, blocks, div_up(inputs, 32), p.steps, w_scales, x_scales, reinterpret_cast<uint8_t*>(work),

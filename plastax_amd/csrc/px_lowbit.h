@@ -211,57 +211,78 @@ __device__ __forceinline__ uint4 bf16_of8(uint2 c, float scale) {
   return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
 }
 
-// 8 values as a sum of P bf16 pieces each, by cutting off 8 significant bits
-// at a time: exact for P = 1 (bf16), 2 (float16, 11 bits) and 3 (float32, 24
-// bits) down to bf16's least subnormal. An infinity or a NaN is its own first
-// piece and its others are zero.
+// bf16 of two values, to the nearest, and its halves as float32.
+__device__ __forceinline__ uint32_t round_bf16(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
+__device__ __forceinline__ float low_bf16(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float high_bf16(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
+// The high halves of two values: bf16 by cutting off.
+__device__ __forceinline__ uint32_t cut_bf16(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+// 8 values as sums of P bf16 pieces, exactly. P = 1: bf16. P = 2: float16's 11
+// significant bits, the first 8 cut off. P = 3: float32, v = p0 + 2^-7 p1 +
+// 2^-16 p2: p0 the first 8 bits (a multiple of 2^-133, bf16's least step), p1
+// 2^7 times what is left of v, rounded to the nearest 8 bits, and p2 2^9 times
+// what is then left, which is 8 bits at most. Scaled so, the pieces of the
+// least values keep all bits (p2's steps stand for 2^-149, float32's own), and
+// none is larger than v, so their sums stay finite where those of |v| do. An
+// infinity or a NaN is its own first piece and its others are zero.
+constexpr float kPiece1 = 0x1p-7f, kPiece2 = 0x1p-9f;  // p1's unit in p0's, p2's in p1's
 template <int P>
-__device__ __forceinline__ void pieces8(const float in[8], uint4 out[P]) {
-  float v[8];
-  uint32_t m = 0;
+__device__ __forceinline__ void pieces8(const float v[8], uint4 out[P]) {
+  uint32_t r[P][4];
+  float rest[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = in[i], m = m > abs_bits(in[i]) ? m : abs_bits(in[i]);
-  if (m >= kInfBits) {
+  for (int i = 0; i < 4; ++i) {
+    r[0][i] = cut_bf16(v[2 * i], v[2 * i + 1]);
+    rest[2 * i] = v[2 * i] - low_bf16(r[0][i]), rest[2 * i + 1] = v[2 * i + 1] - high_bf16(r[0][i]);
+  }
+  // (The rest of a value that is not finite is NaN, and stays so in a sum; the
+  // others' rests are far from float32's largest.)
+  const float sum = ((rest[0] + rest[1]) + (rest[2] + rest[3])) + ((rest[4] + rest[5]) + (rest[6] + rest[7]));
+  if (P > 1 && sum != sum) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      uint32_t h[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t u = __float_as_uint(v[i]);
-        if ((u & 0x7FFFFFFFu) > kInfBits) u |= 0x00400000u;  // a NaN stays one when its low bits go
-        h[i] = u & 0xFFFF0000u;
-        v[i] = (u & kInfBits) == kInfBits ? 0.0f : v[i] - __uint_as_float(h[i]);
-      }
-      out[p] = make_uint4((h[0] >> 16) | h[1], (h[2] >> 16) | h[3], (h[4] >> 16) | h[5], (h[6] >> 16) | h[7]);
+    for (int i = 0; i < 8; ++i) {
+      if (abs_bits(v[i]) >= kInfBits) rest[i] = 0.0f;
+      if (abs_bits(v[i]) > kInfBits) r[0][i / 2] |= i % 2 ? 0x00400000u : 0x00000040u;  // (a NaN stays one)
     }
-    return;
   }
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    uint32_t r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t a = __float_as_uint(v[2 * i]), b = __float_as_uint(v[2 * i + 1]);
-      r[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);  // the high halves
-      if (p + 1 < P) {
-        v[2 * i] -= __uint_as_float(a & 0xFFFF0000u);
-        v[2 * i + 1] -= __uint_as_float(b & 0xFFFF0000u);
-      }
+  for (int i = 0; i < 4; ++i) {
+    float a = rest[2 * i], b = rest[2 * i + 1];
+    if (P == 2) r[P - 1][i] = cut_bf16(a, b);
+    if (P == 3) {
+      a *= 1.0f / kPiece1, b *= 1.0f / kPiece1;
+      const uint32_t p = round_bf16(a, b);
+      r[P - 2][i] = p;
+      r[P - 1][i] = cut_bf16((a - low_bf16(p)) * (1.0f / kPiece2), (b - high_bf16(p)) * (1.0f / kPiece2));
     }
-    out[p] = make_uint4(r[0], r[1], r[2], r[3]);
   }
+#pragma unroll
+  for (int p = 0; p < P; ++p) out[p] = make_uint4(r[p][0], r[p][1], r[p][2], r[p][3]);
 }
 template <typename T>
 struct Pieces {
-  static constexpr int n = 3;
+  static constexpr int n = 3, sums = 3;  // (of different units, so with sums of their own)
 };
 template <>
 struct Pieces<__bf16> {
-  static constexpr int n = 1;
+  static constexpr int n = 1, sums = 1;
 };
 template <>
 struct Pieces<_Float16> {
-  static constexpr int n = 2;
+  static constexpr int n = 2, sums = 1;
 };
+template <typename V>
+__device__ __forceinline__ V join_sums(const V (&s)[1]) {
+  return s[0];
+}
+template <typename V>
+__device__ __forceinline__ V join_sums(const V (&s)[3]) {
+  return s[0] + kPiece1 * (s[1] + kPiece2 * s[2]);
+}
 
 }  // namespace px

@@ -19,11 +19,13 @@ struct BigArgs {
   float* part;         // [splits][M][N], where splits > 1
   int M, N;
   int rows_u;          // m that are in memory (M, or padded for "across")
-  int steps;           // of 64 k, over all of u's pieces
-  int wrap;            // steps of w, which starts again after them
+  int wrap;            // steps of w's lines, 64 k each (256 in 4 bits), which start again with u's next piece
+  int units;           // pieces of u that have units of their own (the others have one and follow each other)
+  int steps;           // of u's lines in one unit
+  float down[2];       // the first unit in the second one, and the second in the third
   const char* sw;      // 4 bits: the scales in the waves' order (k_big_scales)
   const char* su;
-  int split;           // steps of one k range
+  int split;           // steps of one k range, in every unit
   int tiles_m, tiles_n;
 };
 
@@ -255,9 +257,14 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
   big_offsets<UA, F4>(tid, m0, g.rows_u, g.ldu, ou);
   const int64_t su = UA ? 64 * g.ldu : 128;
   const int beg = blockIdx.y * g.split, end = beg + g.split < g.steps ? beg + g.split : g.steps;
+  const int count = F4 ? end - beg : (end - beg) * g.units;
   const char* w = g.w + n0 * g.ldw;
   const char* u = g.u + (UA ? int64_t{2} * m0 : m0 * g.ldu) + beg * su;
-  int wt = beg % g.wrap;
+  // Where w's steps start again, after which one, and u's way to its next piece.
+  const bool alone = F4 || g.units == 1;
+  const int again = alone ? 0 : beg, last = (alone ? g.wrap : end) - 1;
+  const int64_t next_piece = alone ? su : (g.steps - last + again) * su;
+  int wt = alone ? beg % g.wrap : beg;
   // 4 bits: a line of an odd number of 64 bytes ends inside its last step,
   // which then reads its first half twice and multiplies it once.
   const bool odd = F4 && (g.ldw & 64) != 0;
@@ -287,10 +294,10 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
   sums acc[2][2][FW][FU] = {};
   bf16x8 rw[FW][S], ru[2][FU][S];
 
-  // A step's four loads, of w's and u's first halves (the step is t), u's and
-  // w's second ones; the last of them moves on to the next step.
-  auto load_w0u0 = [&](int t, int buf) {
-    if (odd && t + 1 == g.steps) {
+  // A step's four loads, of w's and u's first halves, u's and w's second ones;
+  // the last of them moves on to the next step.
+  auto load_w0u0 = [&](int buf) {
+    if (odd && wt + 1 == g.wrap) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) ow[i] -= back, ou[i] -= back;
     }
@@ -305,8 +312,9 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
           (glb_char*)gs, (__attribute__((address_space(3))) void*)(l + 4 * kBigBytes + buf * 4096 + wave * 1024), 16, 0, 0);
       gs += 2048;
     }
-    u += su;
-    wt = wt + 1 == g.wrap ? 0 : wt + 1;
+    const bool over = wt == last;
+    u += over ? next_piece : su;
+    wt = over ? again : wt + 1;
   };
   auto read_w = [&](int buf, int h) {
     const lds_char* p = l + buf * 2 * kBigBytes + h * (kBigBytes / 2);
@@ -356,11 +364,11 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
     else
       asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
   };
-  load_w0u0(beg, 0);
+  load_w0u0(0);
   load_u1(0);
   load_w1(0);
-  if (beg + 1 < end) {
-    load_w0u0(beg + 1, 1);
+  if (count > 1) {
+    load_w0u0(1);
     load_u1(1);
     load_w1(1);
     wait_older();
@@ -369,9 +377,9 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
   }
   big_barrier();
   if (ww) big_barrier();
-  for (int t = beg; t < end; ++t) {
-    const int buf = (t - beg) & 1;
-    const bool more = t + 2 < end, both = !(odd && t + 1 == g.steps);
+  auto step = [&](int t) {
+    const int buf = t & 1;
+    const bool more = t + 2 < count, both = !(odd && beg + t + 1 == g.steps);
     read_u(buf, k0);
     read_w(buf, 0);
     if (F4) {
@@ -389,7 +397,7 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
     multiply(k0, k0, both);
     big_barrier();
     read_u(buf, k1);
-    if (more) load_w0u0(t + 2, buf);
+    if (more) load_w0u0(buf);
     big_barrier();
     multiply(k0, k1, both);
     big_barrier();
@@ -407,6 +415,23 @@ __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
     big_barrier();
     multiply(k1, k0, both);
     big_barrier();
+  };
+  // At the end of a piece the sums change to the next one's unit.
+  int left = end - beg, piece = 0;
+  for (int t = 0; t < count; ++t) {
+    step(t);
+    if (!F4 && --left == 0 && t + 1 < count) {
+      const float by = g.down[piece++];
+      left = end - beg;
+#pragma unroll
+      for (int hw = 0; hw < 2; ++hw)
+#pragma unroll
+        for (int hu = 0; hu < 2; ++hu)
+#pragma unroll
+          for (int i = 0; i < FW; ++i)
+#pragma unroll
+            for (int j = 0; j < FU; ++j) acc[hw][hu][i][j] *= by;
+    }
   }
   if (!ww) big_barrier();
 

@@ -205,3 +205,82 @@ def test_large_sums_keep_what_float32_can_hold(shape, layout) -> None:
             large += 1
             assert call(a, codes).eq(k * (1 + 2.0**-23)).all().item(), kind
     assert large == (4 if tokens == 4096 else 2)
+
+
+def _numbers(n, dtype, g) -> torch.Tensor:
+    """``n`` values of the type's whole range, subnormal ones among them, all of their bits drawn."""
+    bits = {torch.float32: 32, torch.bfloat16: 16, torch.float16: 16}[dtype]
+    as_int = {32: torch.int32, 16: torch.int16}[bits]
+    v = torch.randint(-(1 << (bits - 1)), 1 << (bits - 1), (n,), generator=g, device=DEV).to(as_int).view(dtype)
+    least = torch.arange(1, 9, device=DEV).to(as_int).view(dtype)  # the least ones of all, each kind once at least
+    top = torch.finfo(dtype)
+    ends = torch.tensor([top.tiny, top.max, -top.max, top.tiny * (2 - top.eps), top.tiny * (1 - top.eps)], device=DEV,
+                        dtype=torch.float64).to(dtype)
+    v = torch.where(torch.isfinite(v), v, torch.ones_like(v))
+    some = torch.cat([least, ends])[:n]
+    v[: some.numel()] = some
+    return v
+
+
+# few tokens; tiles of 32 and 64, k in one and four groups, in ranges; large ones, in ranges
+ONES = [(1, 40, 33), (16, 300, 200), (70, 300, 200), (70, 4096, 130), (300, 1003, 777), (2048, 512, 512),
+        (33, 2048, 2049), (4096, 2112, 2304), (512, 4200, 4608), (256, 32768, 1024), (8192, 256, 2048)]
+
+
+@pytest.mark.parametrize("layout", ["rows", "columns", "offset", "steps"])
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("shape", ONES)
+def test_single_products_keep_every_bit(shape, dtype, layout) -> None:
+    """One value a sum, anywhere along k, times powers of two from 2^-110 to 2^110: wherever the type holds the result,
+    that is it, and one below its normal numbers is off by its least step at most."""
+    tokens, inputs, outputs = shape
+    _say("single", shape, dtype, layout)
+    g = _gen(7)
+
+    def check(got, want):
+        size = torch.finfo(got.dtype)
+        held = (want.to(got.dtype).double() == want) & ((want.abs() >= size.smallest_normal) | (want == 0))
+        off = (got.double() - want).abs()
+        assert bool((off == 0)[held].all()), f"{int((off != 0)[held].sum())} of {int(held.sum())} off"
+        small = ~held & (want.abs() < size.smallest_normal)
+        assert bool((off[small] <= size.smallest_normal * size.eps).all())
+
+    # weights and kept inputs: a power of two for each line and 32 of its values, of either sign
+    def signed(lines, n):
+        e = torch.randint(-110, 111, (lines, -(-n // 32)), generator=g, device=DEV).repeat_interleave(32, 1)[:, :n]
+        sign = torch.randint(0, 2, (lines, n), generator=g, device=DEV) * 2 - 1
+        return sign.double() * torch.exp2(e.double())
+
+    wide = signed(outputs, inputs)
+    w = lowbit.quantise4(wide.float())
+    assert torch.equal(w.values().double(), wide)
+    for k, call in ((inputs, lowbit.product), (outputs, lowbit.product_grad)):
+        at = torch.randint(0, k, (tokens,), generator=g, device=DEV)
+        v = _numbers(tokens, dtype, g)
+        a = torch.zeros((tokens, k), dtype=dtype, device=DEV)
+        a[torch.arange(tokens, device=DEV), at] = v
+        lines = wide.t()[at] if call is lowbit.product else wide[at]
+        check(call(plain.layouts(a)[layout], w), v.double()[:, None] * lines)
+    v = _numbers(outputs, dtype, g)
+    at = torch.randint(0, tokens, (outputs,), generator=g, device=DEV)
+    dy = torch.zeros((tokens, outputs), dtype=dtype, device=DEV)
+    dy[at, torch.arange(outputs, device=DEV)] = v
+    for axis in (0, 1):
+        x = signed(tokens, inputs) if axis else signed(inputs, tokens).t()
+        kept = lowbit.quantise8(x.float(), axis=axis)
+        assert torch.equal(kept.values(torch.float32).double(), x)
+        check(lowbit.weight_grad(plain.layouts(dy)[layout], kept), v.double()[:, None] * x[at])
+
+
+def test_single_products_run_in_every_form() -> None:
+    """The shapes above, by their plans: small tiles whole and in ranges, large ones whole and in ranges."""
+    lib, small, large = _lib.load(), set(), set()
+    for tokens, inputs, outputs in ONES:
+        x = torch.empty((tokens, inputs), device=DEV)
+        w = lowbit.Mx4._empty(outputs, inputs, DEV)
+        ranges = _ranges("product", w, x)
+        if ranges:
+            large.add(min(ranges, 2))
+        elif tokens > 16:
+            small.add(lib.plx_mx_workspace(0, tokens, inputs, outputs, 0, x.data_ptr(), inputs, 1) > 0)
+    assert small == {False, True} and large == {1, 2}
