@@ -284,3 +284,150 @@ def test_single_products_run_in_every_form() -> None:
         elif tokens > 16:
             small.add(lib.plx_mx_workspace(0, tokens, inputs, outputs, 0, x.data_ptr(), inputs, 1) > 0)
     assert small == {False, True} and large == {1, 2}
+
+
+# ---------------------------------------------------------------------------
+# Large products
+# ---------------------------------------------------------------------------
+def _spread(shape, g) -> torch.Tensor:
+    """Values from 2^-4 to 2^4, a tenth of them zeros."""
+    x = _randn(shape, g) * torch.exp2(torch.randint(-4, 4, shape, generator=g, device=DEV).float())
+    return torch.where(torch.rand(shape, generator=g, device=DEV) < 0.1, 0.0, x)
+
+
+@pytest.mark.parametrize("layout", ["rows", "columns", "offset_columns", "steps"])
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+def test_infinities_and_nan_in_large_products(dtype, layout) -> None:
+    tokens, inputs, outputs = 2056, 2120, 3300
+    _say("large nan", dtype, layout)
+    g = _gen(8)
+    wf = _randn((outputs, inputs), g)
+    wf[7, 40], wf[3001, 2119] = torch.nan, torch.inf  # their blocks of 32 become NaN, the last one of 8 values
+    w = lowbit.quantise4(wf)
+    w64 = plain.values4(w.codes, w.scales, inputs)
+    assert int(torch.isnan(w64).sum()) == 40
+
+    def places(n):
+        a = _randn((tokens, n), g).to(dtype)
+        a[0, 3], a[300, n - 1], a[1999, 9] = torch.inf, -torch.inf, torch.nan
+        a[2000, 64:72] = torch.tensor([torch.nan, torch.inf, -torch.inf, 1, 0, -1, torch.nan, torch.inf]).to(dtype)
+        return a
+
+    def same(got, want):
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        inf = torch.isinf(want)
+        assert torch.equal(torch.isinf(got), inf) and torch.equal(got.double()[inf], want[inf])
+
+    x, dy = places(inputs), places(outputs)
+    a = plain.layouts(x)[layout]
+    assert _ranges("product", w, a)
+    same(lowbit.product(a, w), x.double() @ w64.t())
+    a = plain.layouts(dy)[layout]
+    assert _ranges("product_grad", w, a)
+    same(lowbit.product_grad(a, w), dy.double() @ w64)
+    h = _randn((tokens, inputs), g)
+    h[0, 8], h[500, 2119], h[2055, 77] = torch.nan, torch.inf, -torch.inf
+    for axis in (0, 1):
+        kept = lowbit.quantise8(h, axis=axis)
+        x8 = kept.values(torch.float32).double()
+        assert _ranges("weight_grad", kept, a)
+        same(lowbit.weight_grad(a, kept), dy.double().t() @ x8)
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+def test_infinities_and_nan_in_large_products_of_two_in_4_bits(dtype) -> None:
+    tokens, inputs, outputs = 2056, 2120, 6000
+    g = _gen(9)
+    wf, xf = _randn((outputs, inputs), g), _randn((tokens, inputs), g)
+    wf[7, 40], wf[5999, 2119], xf[300, 2], xf[2055, 64] = torch.nan, torch.inf, -torch.inf, torch.nan
+    w, x = lowbit.quantise4(wf), lowbit.quantise4(xf)
+    assert _large4(tokens, inputs, outputs)
+    want = plain.values4(x.codes, x.scales, inputs) @ plain.values4(w.codes, w.scales, inputs).t()
+    got = lowbit.product(x, w, dtype=dtype)
+    assert int(torch.isnan(want).sum()) == 2 * tokens + 2 * outputs - 4
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+
+
+def _large4(tokens, inputs, outputs) -> bool:
+    """Whether a product of two in 4 bits runs as a large one: its workspace then holds the scales of whole tiles."""
+    scales = (-(-tokens // 256) + -(-outputs // 256)) * -(-inputs // 256) * 2048
+    need = _lib.load().plx_mx4_workspace(tokens, inputs, outputs)
+    return need >= scales and (need - scales) % (4 * tokens * outputs) == 0
+
+
+@pytest.mark.parametrize("layout", ["offset_columns", "steps"])
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+def test_large_products_of_other_layouts(dtype, layout) -> None:
+    tokens, inputs, outputs = 2056, 2120, 3300
+    _say("large layouts", dtype, layout)
+    g = _gen(10)
+    w = lowbit.quantise4(_spread((outputs, inputs), g))
+    w64 = plain.values4(w.codes, w.scales, inputs)
+    x = plain.layouts(_spread((tokens, inputs), g).to(dtype))[layout]
+    assert _ranges("product", w, x)
+    plain.assert_product(lowbit.product(x, w), x.double(), w64)
+    dy = plain.layouts(_spread((tokens, outputs), g).to(dtype))[layout]
+    assert _ranges("product_grad", w, dy)
+    plain.assert_product(lowbit.product_grad(dy, w), dy.double(), w64.t().contiguous())
+    for axis in (0, 1):
+        kept = lowbit.quantise8(x, axis=axis)
+        assert _ranges("weight_grad", kept, dy)
+        plain.assert_product(lowbit.weight_grad(dy, kept), dy.double().t().contiguous(),
+                             kept.values(torch.float32).double().t().contiguous())
+
+
+@pytest.mark.parametrize("shape", [(2304, 2176, 4700), (256, 36864, 1024)])
+def test_large_products_on_another_stream_and_in_a_graph(shape) -> None:
+    tokens, inputs, outputs = shape
+    g = _gen(11)
+    w = lowbit.quantise4(_randn((outputs, inputs), g))
+    wide = lowbit.quantise4(_randn((6200, inputs), g))
+    x, dy = _randn((tokens, inputs), g).bfloat16(), _randn((tokens, outputs), g).bfloat16()
+
+    def step():
+        kept = lowbit.quantise8(x)
+        low = lowbit.product(lowbit.quantise4(x), wide, dtype=torch.bfloat16)
+        return (lowbit.product(x, w), lowbit.product(x.float(), w), lowbit.product_grad(dy, w),
+                lowbit.product_grad(dy.half(), w), lowbit.weight_grad(dy, kept), lowbit.weight_grad(dy.float(), kept), low)
+
+    assert _ranges("product", w, x) and _large4(tokens, inputs, 6200)
+    want = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(3):
+        x.copy_(_randn((tokens, inputs), g))
+        want = [t.clone() for t in step()]  # eager work between the replays
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert torch.equal(a, b), k
+
+
+def test_products_of_more_tiles_than_a_launch_holds() -> None:
+    """2^26 rows are a launch of 64 x 64 tiles; results go past 2^32 elements."""
+    border, tokens, inputs, outputs = 1 << 26, (1 << 26) + 100, 8, 64
+    g = _gen(12)
+    w = lowbit.quantise4(_randn((outputs, inputs), g))
+    w64 = plain.values4(w.codes, w.scales, inputs)
+    x = torch.zeros((tokens, inputs), dtype=torch.bfloat16, device=DEV)
+    parts = [slice(0, 70), slice(border // 2 - 50, border // 2 + 50), slice(border - 70, tokens)]
+    for part in parts:
+        x[part] = _randn((part.stop - part.start, inputs), g)
+    for y, values in ((lowbit.product(x, w), lambda v: v.double()),
+                      (lowbit.product(lowbit.quantise4(x), w, dtype=torch.bfloat16),
+                       lambda v: plain.values4(*plain.quantise4(v), inputs))):
+        for part in parts:
+            plain.assert_product(y[part], values(x[part]), w64)
+        assert not y[border // 4 : border // 4 + 1000].any() and not y[border - 1000 : border - 70].any()
+        del y

@@ -121,3 +121,25 @@ def test_plans_and_launches_run_with_the_arguments_device_current(monkeypatch) -
             lowbit._launch(at, name)
         assert [i for _, i in seen] == [index] * 4 and current == [0]
         seen.clear()
+
+
+def test_the_shapes_of_the_large_products_tests_are_large(lib) -> None:
+    """Each holds its codes as bf16, for each of the four products, types and layouts; some run in ranges of k."""
+    from test_gpu_lowbit import LARGE
+
+    ranges = set()
+    for tokens, inputs, outputs in LARGE:
+        for kind in (PRODUCT, PRODUCT_GRAD, WEIGHT_GRAD, WEIGHT_GRAD_COLUMNS):
+            m, n, k = ((tokens, outputs, inputs), (tokens, inputs, outputs), (outputs, inputs, tokens))[min(kind, 2)]
+            units = inputs if kind == PRODUCT else outputs
+            for dtype in (F32, BF16, F16):
+                for at, strides in ((P, (units, 1)), (P, (1, tokens)), (P + 2, (units + 3, 1))):
+                    need = lib.plx_mx_workspace(kind, tokens, inputs, outputs, dtype, at, *strides)
+                    assert need >= 2 * -(-k // 64) * 64 * n, (kind, tokens, inputs, outputs, dtype)
+                    ranges.add(need >= 2 * -(-k // 64) * 64 * (n + 3 * m) + 8 * m * n)
+    assert ranges == {False, True}
+    for tokens, inputs, outputs in ((2056, 2120, 6000), (1100, 5000, 4608), (264, 9600, 10000), (3001, 1300, 6500),
+                                    (256, 131072, 768)):
+        scales = (-(-tokens // 256) + -(-outputs // 256)) * -(-inputs // 256) * 2048
+        parts = lib.plx_mx4_workspace(tokens, inputs, outputs) - scales
+        assert parts >= 0 and parts % (4 * tokens * outputs) == 0
