@@ -237,7 +237,11 @@ def activate_grad(dy: torch.Tensor, kept: Mx8, fn: str) -> torch.Tensor:
 
 
 def _workspace(device: torch.device, name: str, *args: object) -> torch.Tensor | None:
-    need = _call(device, name, *args)
+    # (without _call's frame in the usual case: every product asks)
+    if device.index == torch._C._cuda_getDevice():
+        need = getattr(_lib.load(), name)(*args)
+    else:
+        need = _call(device, name, *args)
     if need > 0:
         return torch.empty(need, dtype=torch.uint8, device=device)
     if need < 0:
