@@ -154,7 +154,8 @@ __global__ __launch_bounds__(kBlock) void k_mx_values(int64_t lines, int64_t n, 
 // ---------------------------------------------------------------------------
 // Activations. y = fn(h) from h itself; fn'(q) from what was kept. Bound by
 // memory as long as a value costs below some 30 instructions: silu of 8192 x
-// 8192 bf16 65 us and its gradient 63, 338 MB each, 5.3 TB/s.
+// 8192 bf16 72 us on average and its gradient 74 (62 and 64 at least), 338 MB
+// each, 4.6 TB/s (5.4).
 // ---------------------------------------------------------------------------
 // exp(-a), a >= 0, to 2 steps: the hardware's 2^f (1 step) of the fraction of
 // -a log2(e), whose rounding error goes on as a factor 1 + r ln 2, and ldexp,
@@ -432,7 +433,7 @@ __device__ __forceinline__ void tile_store(const f32x4 (&acc)[TS / 32][TS / 32],
 // that the rows of a fragment's read fall on different banks; lines of m or n
 // ("across") are rows too, pairs of chunks at p ^ (k & 3) (k & 1 of 32), and their
 // fragments are read transposed. What bounds it is that a step's phases follow
-// each other: bf16 256 x 4096 x 4096 takes 20 us, 36 % of a CU's cycles
+// each other: bf16 256 x 4096 x 4096 takes 19 us, 36 % of a CU's cycles
 // conversions and addresses, 33 % LDS, 16 % matrix instructions.
 // Four waves a SIMD at least: float32's sums for each unit would leave three
 // (1 x 4096 x 4096's weight gradient 22.4 us, so 19.0).
@@ -684,7 +685,7 @@ __global__ __launch_bounds__(64 * kFewWaves<ALONG>) void k_mx_few(GemmArgs g) {
 
 // 4-bit times 4-bit blocks: the scaled matrix instruction takes 128 k of both
 // operands as they are kept, a block and its scale byte per lane (256 x 4096 x
-// 4096 9.7 us; with fragments straight from memory 24). Tiles, groups
+// 4096 9.6 us; with fragments straight from memory 24). Tiles, groups
 // and LDS as in k_mx_gemm, a chunk of 16 bytes being one block here: a step is
 // 256 k a group.
 template <typename OT, int TS, int KS>
@@ -818,11 +819,11 @@ inline unsigned groups_across(int64_t lines, int64_t blocks) {
 // A large product: 256 x 256 tiles have enough rows, columns and k (counted
 // over a's pieces), and the operands' way through memory pays. Large against
 // small tiles, us, from the least to the largest of the four products: bf16
-// 8.6e9 (2048 cubed) 46 to 49 and 37 to 45, 10.1e9 (8192 x 4096 x 300) 48 to 67
-// and 63 to 138, 17.2e9 45 to 68 and 68 to 84. float32, where small tiles split
-// a in registers, 12.9e9 (1024 x 2048 x 2048, 32 tiles) 55 to 60 and 44 to 51,
-// with a tile for every CU (4096 x 4096 of 256 tokens) 41 to 44 and 50 to 55,
-// 14.7e9 62 and 62 to 85. In 4 bits 17.2e9 take 41 large and 26 to 30.
+// 8.6e9 (2048 cubed) 46 to 49 and 40 to 47, 10.1e9 (8192 x 4096 x 300) 39 to 67
+// and 59 to 116, 17.2e9 56 to 61 and 63 to 80. float32, where small tiles split
+// a in registers, 12.9e9 (1024 x 2048 x 2048, 32 tiles) 53 to 55 and 44 to 47,
+// with a tile for every CU (4096 x 4096 of 256 tokens) 41 to 42 and 46, 14.7e9
+// 59 to 60 and 52 to 68. In 4 bits 17.2e9 take 26 and 24, 25.2e9 31 and 34.
 constexpr double kBigLeast = 9e9, kBigPieces = 14e9, kBig4Least = 25e9;
 // (Beyond 2^30 lanes of a launch, products go in small tiles, cut into launches.)
 inline bool large(int64_t m, int64_t n, int64_t k, double least) {
@@ -832,7 +833,8 @@ inline bool large(int64_t m, int64_t n, int64_t k, double least) {
 
 // How a product in small tiles runs: tiles of ts x ts, ks groups of waves in a
 // workgroup, each with `share` of k in a step, and ranges of k over workgroups.
-// By measurement (us in a captured graph, bf16 and float32):
+// By measurement (us in a captured graph, bf16 and float32, which has taken up
+// to 5 % more on both sides since its pieces have units of their own):
 //   ts 32 where tiles of 64 leave half the CUs idle and steps are few (256 x
 //   777 of 1003 k: 5.6 and 7.5, with 64 8.2 and 13.0) or tiles very few (64 x
 //   1024 of 4096 k: 8.1 and 10.1, 10.0 and 15.2), but not in between (256 x

@@ -236,11 +236,12 @@ __device__ __forceinline__ void big_store(const f32x16 (&acc)[2][2][2][1], T* ou
 // four waves are one barrier behind the first, so that on each SIMD one wave
 // multiplies while the other one loads. A half of a buffer is loaded for the
 // step after next as soon as both have read it, nearly two steps before it is
-// needed. bf16 8192 cubed: 1400 TFLOP/s, matrix cores 74 to 78 % busy (two buffers
-// and one barrier a step: 58 %, 1250). F4: both operands in 4-bit blocks along k, 8 of them in a line's 128
+// needed. bf16 8192 cubed 702 us on average, 1570 TFLOP/s; 8192 x 4096 x 4096
+// 214 (184 at least), matrix cores 77 % busy (two buffers and one barrier a step:
+// 58 %, 270 us). F4: both operands in 4-bit blocks along k, 8 of them in a line's 128
 // bytes: a lane's 16 bytes are one block, and the LDS layout is the bf16 one.
 // The scales of a step come in the waves' order (k_big_scales) and by way of
-// LDS too, a lane's own in 16 and 8 bytes (8192 cubed 247 us; read by each lane
+// LDS too, a lane's own in 16 and 8 bytes (8192 cubed 242 us; read by each lane
 // for itself, every load under way would be waited for first).
 template <bool UA, bool F4, typename OT>
 __global__ __launch_bounds__(kBigThreads, 2) void k_big_gemm(BigArgs g) {
