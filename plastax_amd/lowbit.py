@@ -25,7 +25,9 @@ go to the nearest, ties to the even code.
 Arguments are 2-dimensional GPU tensors of float32, bfloat16 or float16 with
 any strides; batches are ``[tokens, units]``. Work goes to torch's current
 stream of the arguments' device, results and workspaces are allocated there.
-Sums are float32. Results carry no autograd graph and no tangent: an argument
+Products are exact over each type's whole range, sums are float32 (a value
+rounded up past float32's largest is an infinity, and sums with one are not
+finite). Results carry no autograd graph and no tangent: an argument
 that asks for one is refused, the gradients are calls of their own. The reference has no
 counterpart: its weights and activations are float32.
 """
