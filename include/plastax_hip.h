@@ -1254,6 +1254,84 @@ PLX_EXPORT int plx_mx4_product(int64_t tokens, int64_t inputs, int64_t outputs, 
                                const uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales, int32_t dtype,
                                void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* --------------------------------------------------------------------------
+ * Around dense level pairs: operators on batches [tokens][units] of float32,
+ * bfloat16 or float16 (PLX_LB_*). `line`: elements from one token to the next;
+ * a token's units lie next to each other. ids and starts are int32 (`wide` 0)
+ * or int64 (1). Results are whole batches. Tokens are at most 2^30, units and
+ * ids 2^24. workspace: as many bytes as the entry point's _workspace() says,
+ * on 16 bytes (null where it says 0; -1 from it is a bad argument).
+ * ------------------------------------------------------------------------ */
+
+/* out [tokens][units] = scale * table[ids[t]], zeros for an id outside of the
+ * table's rows. */
+PLX_EXPORT int plx_look_up(int64_t tokens, int64_t rows, int64_t units, const void* ids, int32_t wide, int32_t dtype,
+                           const void* table, int64_t line, float scale, void* out, void* stream);
+
+/* out [rows][units] (float32) = scale * the sums of g over the tokens of each
+ * id, in the tokens' order (zeros for a row without any). At most 2^28 tokens. */
+PLX_EXPORT int64_t plx_look_up_workspace(int64_t tokens, int64_t rows, int64_t units);
+PLX_EXPORT int plx_look_up_grad(int64_t tokens, int64_t rows, int64_t units, const void* ids, int32_t wide,
+                                int32_t dtype, const void* g, int64_t line, float scale, float* out, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
+/* y = (x - mean) r * weight + bias (null: none) over each token's units,
+ * r = 1 / sqrt(var + eps); kept [tokens][2] (float32) = mean, r. weight and
+ * bias are of type `params`: dtype, or float32. */
+PLX_EXPORT int plx_normalise(int64_t tokens, int64_t units, int32_t dtype, const void* x, int64_t line, int32_t params,
+                             const void* weight, const void* bias, float eps, void* y, float* kept, void* stream);
+
+/* dx, and dparams [2][units] (float32) = the gradients of weight and bias,
+ * from g, that of y. */
+PLX_EXPORT int64_t plx_normalise_workspace(int64_t tokens, int64_t units, int32_t dtype);
+PLX_EXPORT int plx_normalise_grad(int64_t tokens, int64_t units, int32_t dtype, const void* g, int64_t g_line,
+                                  const void* x, int64_t x_line, int32_t params, const void* weight, const float* kept,
+                                  void* dx, float* dparams, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* a = sigmoid(z), h[t] = a[t] h[t-1] + (1 - a[t]) x[t] along sequences; xz
+ * [tokens][2 units] is x beside z. Sequence s is the rows from starts[s] to
+ * before starts[s + 1] (rising; taken as 0 to tokens at least and at most), or
+ * all rows if starts is null (then sequences is 1). It goes on from state
+ * [sequences][units] (float32; null: zeros), and last [sequences][units] is
+ * its last h, or its state if it has no rows. Rows of no sequence have h = 0.
+ * kept [ceil(tokens / 64)][units] (float32) is for plx_recur_grad. `ragged`:
+ * whether starts is given. */
+#define PLX_RECUR_KEEP 64
+PLX_EXPORT int64_t plx_recur_workspace(int64_t tokens, int64_t units, int64_t sequences, int32_t ragged);
+PLX_EXPORT int plx_recur(int64_t tokens, int64_t units, int64_t sequences, int32_t dtype, const void* xz, int64_t line,
+                         const void* starts, int32_t wide, const float* state, void* h, float* last, float* kept,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/* dxz [tokens][2 units] and dstate [sequences][units] (float32) from the
+ * gradients of h and (g_last, null: zeros) of last. Rows of no sequence have
+ * the gradient 0. */
+PLX_EXPORT int plx_recur_grad(int64_t tokens, int64_t units, int64_t sequences, int32_t dtype, const void* g,
+                              int64_t g_line, const void* xz, int64_t line, const void* starts, int32_t wide,
+                              const float* state, const float* g_last, const float* kept, void* dxz, float* dstate,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One token a sequence: state (float32, state_line elements from one sequence
+ * to the next) becomes a state + (1 - a) x, which h [sequences][units] has in
+ * dtype. */
+PLX_EXPORT int plx_recur_step(int64_t sequences, int64_t units, int32_t dtype, const void* xz, int64_t line,
+                              float* state, int64_t state_line, void* h, void* stream);
+
+/* loss [tokens] (float32) = T^2 sum p (log p - log q), q = softmax(logits / T)
+ * over the token's outputs, p = softmax(top / T) over the outputs that
+ * ids [tokens][named] name; top [tokens][named] is of type `top_type`. A place
+ * whose id is no output, or whose top is -inf, counts for nothing; a token
+ * without any other has the loss 0. named is at most PLX_MAX_NAMED. */
+#define PLX_MAX_NAMED 1024
+PLX_EXPORT int plx_distil(int64_t tokens, int64_t outputs, int32_t named, int32_t dtype, const void* logits,
+                          int64_t line, const void* ids, int32_t wide, int32_t top_type, const void* top,
+                          float temperature, float* loss, void* stream);
+
+/* The losses, and dlogits [tokens][outputs] = the gradient of their sum
+ * weighted by g [tokens] (float32). */
+PLX_EXPORT int plx_distil_grad(int64_t tokens, int64_t outputs, int32_t named, const float* g, int32_t dtype,
+                               const void* logits, int64_t line, const void* ids, int32_t wide, int32_t top_type,
+                               const void* top, float temperature, float* loss, void* dlogits, void* stream);
+
 PLX_EXPORT int32_t plx_abi_version(void);
 
 #ifdef __cplusplus

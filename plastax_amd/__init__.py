@@ -10,7 +10,7 @@ fallback.
 
 from __future__ import annotations
 
-from plastax_amd import lowbit, monoid, nn, numpy, optim, rng, topo
+from plastax_amd import dense, lowbit, monoid, nn, numpy, optim, rng, topo
 from plastax_amd._expr import UnsupportedPolicyError
 from plastax_amd._types import (
     ACTIVATION,
@@ -114,6 +114,7 @@ __all__ = [
     "UnsupportedPolicyError",
     "UpdateConn",
     "UpdateUnit",
+    "dense",
     "grow_bucket",
     "live_conn_count",
     "live_unit_count",

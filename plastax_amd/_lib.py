@@ -18,7 +18,7 @@ LIB_PATH = pathlib.Path(
     or pathlib.Path(__file__).resolve().parent / "libplastax_hip.so"
 )
 
-ABI_VERSION = 30  # plx_abi_version() of the library these mirrors describe
+ABI_VERSION = 31  # plx_abi_version() of the library these mirrors describe
 
 PLX_MAX_INSTR = 48
 PLX_MAX_CONST = 32
@@ -572,6 +572,23 @@ _SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "plx_mx_product": (c_i32, [c_i32, c_i64, c_i64, c_i64, c_i32, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64,
                                c_vp]),
     "plx_mx4_product": (c_i32, [c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp]),
+    "plx_look_up": (c_i32, [c_i64, c_i64, c_i64, c_vp, c_i32, c_i32, c_vp, c_i64, c_f32, c_vp, c_vp]),
+    "plx_look_up_workspace": (c_i64, [c_i64, c_i64, c_i64]),
+    "plx_look_up_grad": (c_i32, [c_i64, c_i64, c_i64, c_vp, c_i32, c_i32, c_vp, c_i64, c_f32, c_vp, c_vp, c_i64,
+                                 c_vp]),
+    "plx_normalise": (c_i32, [c_i64, c_i64, c_i32, c_vp, c_i64, c_i32, c_vp, c_vp, c_f32, c_vp, c_vp, c_vp]),
+    "plx_normalise_workspace": (c_i64, [c_i64, c_i64, c_i32]),
+    "plx_normalise_grad": (c_i32, [c_i64, c_i64, c_i32, c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                   c_i64, c_vp]),
+    "plx_recur_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i32]),
+    "plx_recur": (c_i32, [c_i64, c_i64, c_i64, c_i32, c_vp, c_i64, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64,
+                          c_vp]),
+    "plx_recur_grad": (c_i32, [c_i64, c_i64, c_i64, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_i32, c_vp, c_vp, c_vp,
+                               c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "plx_recur_step": (c_i32, [c_i64, c_i64, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp]),
+    "plx_distil": (c_i32, [c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_i32, c_i32, c_vp, c_f32, c_vp, c_vp]),
+    "plx_distil_grad": (c_i32, [c_i64, c_i64, c_i32, c_vp, c_i32, c_vp, c_i64, c_vp, c_i32, c_i32, c_vp, c_f32, c_vp,
+                                c_vp, c_vp]),
 }
 
 # Entry points the header declares (checked by the CPU test suite).

@@ -24,7 +24,8 @@ PKG = pathlib.Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libplastax_hip.so"
-SOURCES = ("plastax_hip.hip", "structural.hip", "layout.hip", "lowbit.hip")
+SOURCES = ("plastax_hip.hip", "structural.hip", "layout.hip", "lowbit.hip", "lookup.hip", "normalise.hip", "recur.hip",
+           "distil.hip")
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -1,0 +1,446 @@
+// normalise.hip -- layer norm of what goes from one level pair to the next,
+// and its gradients. No counterpart in the reference.
+//
+// Over a token's units: n = (x - mean) r, r = 1 / sqrt(var + eps),
+// y = n w + b. With u = g w: dx = r (u - mean(u) - n mean(u n)); dw and db are
+// the sums of g n and g over the tokens, by workgroup and then over the
+// workgroups, always in the same order.
+
+#include "px_dense.h"
+
+using plx_detail::check_launch;
+using plx_detail::cu_count;
+using plx_detail::fail;
+
+namespace {
+
+using namespace px;
+
+struct NormArgs {
+  int64_t tokens, x_line, g_line;
+  int units;
+  float eps;
+  const void* x;
+  const void* g;
+  const void* weight;
+  const void* bias;
+  void* y;       // or dx
+  float* kept;   // [tokens][2]: mean, r
+  float* part;   // [workgroups][2][units]
+};
+
+// Two sums over the WAVES waves that share a row. One barrier: the next sums
+// take another `part`.
+template <int WAVES>
+__device__ __forceinline__ float2 row_sum2(float a, float b, float2* part) {
+  a = wave_sum(a), b = wave_sum(b);
+  if (WAVES == 1) return make_float2(a, b);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) part[wave] = make_float2(a, b);
+  __syncthreads();
+  float2 s = part[wave / WAVES * WAVES + (threadIdx.x & (WAVES - 1))];
+#pragma unroll
+  for (int d = 1; d < WAVES; d *= 2) s.x += __shfl_xor(s.x, d, 64), s.y += __shfl_xor(s.y, d, 64);
+  return s;
+}
+
+// ROWS rows a workgroup, each of WAVES waves, NC chunks of 16 bytes a lane.
+// The variance is the mean of the squares of x - mean, from registers.
+template <typename T, typename P, int ROWS, int WAVES, int NC>
+__global__ __launch_bounds__(ROWS* WAVES * 64) void k_normalise(NormArgs a) {
+  constexpr int W = kChunk<T>, NT = WAVES * 64;
+  __shared__ float2 part[2][ROWS * WAVES];
+  const int lane = threadIdx.x % NT;
+  const int64_t token = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / NT;
+  const bool there = token < a.tokens;
+  const T* row = static_cast<const T*>(a.x) + (there ? token : 0) * a.x_line;
+  float v[NC][W];
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const int at = (k * NT + lane) * W;
+    const typename Pack<T, W>::type x = load_pack<W>(row + at, a.units - at);
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[k][i] = to_f32(x[i]), sum += v[k][i];
+  }
+  const float inv = 1.0f / static_cast<float>(a.units);
+  const float mean = row_sum2<WAVES>(sum, 0.0f, part[0]).x * inv;
+  float square = 0.0f;
+#pragma unroll
+  for (int k = 0; k < NC; ++k)
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      v[k][i] = (k * NT + lane) * W + i < a.units ? v[k][i] - mean : 0.0f;
+      square = __builtin_fmaf(v[k][i], v[k][i], square);
+    }
+  const float var = row_sum2<WAVES>(square, 0.0f, part[1]).x * inv;
+  const float r = 1.0f / sqrtf(var + a.eps);
+  if (!there) return;
+  if (lane == 0) reinterpret_cast<float2*>(a.kept)[token] = make_float2(mean, r);
+  T* out = static_cast<T*>(a.y) + token * a.units;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const int at = (k * NT + lane) * W;
+    if (at >= a.units) break;
+    const typename Pack<P, W>::type w = load_pack<W>(static_cast<const P*>(a.weight) + at, a.units - at);
+    float y[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) y[i] = v[k][i] * r * to_f32(w[i]);
+    if (a.bias) {
+      const typename Pack<P, W>::type b = load_pack<W>(static_cast<const P*>(a.bias) + at, a.units - at);
+#pragma unroll
+      for (int i = 0; i < W; ++i) y[i] += to_f32(b[i]);
+    }
+    store_pack<W>(out + at, a.units - at, y);
+  }
+}
+
+// Levels that no registers hold: the row is read three times.
+template <typename T, typename P>
+__global__ __launch_bounds__(1024) void k_normalise_stream(NormArgs a) {
+  constexpr int W = kChunk<T>, WAVES = 16, STEP = 1024 * W;
+  __shared__ float2 part[2][WAVES];
+  const int64_t token = blockIdx.x;
+  const T* row = static_cast<const T*>(a.x) + token * a.x_line;
+  float sum = 0.0f, square = 0.0f;
+  for (int at = threadIdx.x * W; at < a.units; at += STEP) {
+    const typename Pack<T, W>::type x = load_pack<W>(row + at, a.units - at);
+#pragma unroll
+    for (int i = 0; i < W; ++i) sum += to_f32(x[i]);
+  }
+  const float inv = 1.0f / static_cast<float>(a.units);
+  const float mean = row_sum2<WAVES>(sum, 0.0f, part[0]).x * inv;
+  for (int at = threadIdx.x * W; at < a.units; at += STEP) {
+    const typename Pack<T, W>::type x = load_pack<W>(row + at, a.units - at);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float d = at + i < a.units ? to_f32(x[i]) - mean : 0.0f;
+      square = __builtin_fmaf(d, d, square);
+    }
+  }
+  const float var = row_sum2<WAVES>(square, 0.0f, part[1]).x * inv;
+  const float r = 1.0f / sqrtf(var + a.eps);
+  if (threadIdx.x == 0) reinterpret_cast<float2*>(a.kept)[token] = make_float2(mean, r);
+  T* out = static_cast<T*>(a.y) + token * a.units;
+  for (int at = threadIdx.x * W; at < a.units; at += STEP) {
+    const typename Pack<T, W>::type x = load_pack<W>(row + at, a.units - at);
+    const typename Pack<P, W>::type w = load_pack<W>(static_cast<const P*>(a.weight) + at, a.units - at);
+    float y[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) y[i] = (to_f32(x[i]) - mean) * r * to_f32(w[i]);
+    if (a.bias) {
+      const typename Pack<P, W>::type b = load_pack<W>(static_cast<const P*>(a.bias) + at, a.units - at);
+#pragma unroll
+      for (int i = 0; i < W; ++i) y[i] += to_f32(b[i]);
+    }
+    store_pack<W>(out + at, a.units - at, y);
+  }
+}
+
+// The gradients: a workgroup takes every gridDim.x-th group of ROWS rows and
+// keeps its lanes' sums of g n and g in registers; they are joined over the
+// rows' groups in LDS and written as the workgroup's part.
+template <typename T, typename P, int ROWS, int WAVES, int NC>
+__global__ __launch_bounds__(ROWS* WAVES * 64) void k_normalise_grad(NormArgs a) {
+  constexpr int W = kChunk<T>, NT = WAVES * 64;
+  __shared__ float2 part[2][ROWS * WAVES];
+  __shared__ float joined[ROWS > 1 ? NT * W : 1];
+  const int lane = threadIdx.x % NT, group = threadIdx.x / NT;
+  const float inv = 1.0f / static_cast<float>(a.units);
+  float w[NC][W], dw[NC][W], db[NC][W];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const int at = (k * NT + lane) * W;
+    const typename Pack<P, W>::type p = load_pack<W>(static_cast<const P*>(a.weight) + at, a.units - at);
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[k][i] = to_f32(p[i]), dw[k][i] = 0.0f, db[k][i] = 0.0f;
+  }
+  int slot = 0;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS; first < a.tokens;
+       first += static_cast<int64_t>(gridDim.x) * ROWS) {
+    const int64_t token = first + group;
+    const bool there = token < a.tokens;
+    const int64_t from = there ? token : 0;
+    const T* xr = static_cast<const T*>(a.x) + from * a.x_line;
+    const T* gr = static_cast<const T*>(a.g) + from * a.g_line;
+    const float2 kept = reinterpret_cast<const float2*>(a.kept)[from];
+    typename Pack<T, W>::type x[NC], g[NC];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int at = (k * NT + lane) * W;
+      const int64_t left = there ? a.units - at : 0;
+      x[k] = load_pack<W>(xr + at, left), g[k] = load_pack<W>(gr + at, left);
+    }
+    float s = 0.0f, sn = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {  // (past the row's end g and w are zeros, and n is finite or the row's NaN)
+        const float d = to_f32(g[k][i]), n = (to_f32(x[k][i]) - kept.x) * kept.y, u = d * w[k][i];
+        dw[k][i] = __builtin_fmaf(d, n, dw[k][i]);
+        db[k][i] += d;
+        s += u;
+        sn = __builtin_fmaf(u, n, sn);
+      }
+    }
+    const float2 sums = row_sum2<WAVES>(s, sn, part[slot]);
+    slot ^= 1;
+    if (!there) continue;
+    const float mean = sums.x * inv, mean_n = sums.y * inv;
+    T* out = static_cast<T*>(a.y) + token * a.units;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int at = (k * NT + lane) * W;
+      if (at >= a.units) break;
+      float d[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float n = (to_f32(x[k][i]) - kept.x) * kept.y;
+        d[i] = kept.y * (to_f32(g[k][i]) * w[k][i] - mean - n * mean_n);
+      }
+      store_pack<W>(out + at, a.units - at, d);
+    }
+  }
+  float* mine = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.units;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const int at = (k * NT + lane) * W;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float* v = h ? db[k] : dw[k];
+      for (int o = 1; o < ROWS; ++o) {
+        __syncthreads();
+        if (group == o) {
+#pragma unroll
+          for (int i = 0; i < W; ++i) joined[i * NT + lane] = v[i];
+        }
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+          for (int i = 0; i < W; ++i) v[i] += joined[i * NT + lane];
+        }
+      }
+      if (group == 0 && at < a.units) store_pack<W>(mine + h * a.units + at, a.units - at, v);
+    }
+  }
+}
+
+// Levels that no registers hold: first each row's two means, then dx and the
+// parts of dw and db by columns of units (blockIdx.y), rows in turn.
+template <typename T, typename P>
+__global__ __launch_bounds__(1024) void k_normalise_means(NormArgs a, float* means) {
+  constexpr int W = kChunk<T>, WAVES = 16;
+  __shared__ float2 part[WAVES];
+  const int64_t token = blockIdx.x;
+  const T* xr = static_cast<const T*>(a.x) + token * a.x_line;
+  const T* gr = static_cast<const T*>(a.g) + token * a.g_line;
+  const float2 kept = reinterpret_cast<const float2*>(a.kept)[token];
+  float s = 0.0f, sn = 0.0f;
+  for (int at = threadIdx.x * W; at < a.units; at += 1024 * W) {
+    const typename Pack<T, W>::type x = load_pack<W>(xr + at, a.units - at), d = load_pack<W>(gr + at, a.units - at);
+    const typename Pack<P, W>::type w = load_pack<W>(static_cast<const P*>(a.weight) + at, a.units - at);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float u = to_f32(d[i]) * to_f32(w[i]);
+      s += u;
+      sn += at + i < a.units ? u * ((to_f32(x[i]) - kept.x) * kept.y) : 0.0f;
+    }
+  }
+  const float2 sums = row_sum2<WAVES>(s, sn, part);
+  const float inv = 1.0f / static_cast<float>(a.units);
+  if (threadIdx.x == 0) reinterpret_cast<float2*>(means)[token] = make_float2(sums.x * inv, sums.y * inv);
+}
+template <typename T, typename P>
+__global__ __launch_bounds__(256) void k_normalise_columns(NormArgs a, const float* means) {
+  const int unit = blockIdx.y * 256 + threadIdx.x;
+  if (unit >= a.units) return;
+  const float w = to_f32(static_cast<const P*>(a.weight)[unit]);
+  float dw = 0.0f, db = 0.0f;
+  for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
+    const float2 kept = reinterpret_cast<const float2*>(a.kept)[token];
+    const float2 mean = reinterpret_cast<const float2*>(means)[token];
+    const float g = to_f32(static_cast<const T*>(a.g)[token * a.g_line + unit]);
+    const float n = (to_f32(static_cast<const T*>(a.x)[token * a.x_line + unit]) - kept.x) * kept.y;
+    dw += g * n;
+    db += g;
+    static_cast<T*>(a.y)[token * a.units + unit] = from_f32<T>(kept.y * (g * w - mean.x - n * mean.y));
+  }
+  float* mine = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.units;
+  mine[unit] = dw;
+  mine[a.units + unit] = db;
+}
+
+// out [2][units] = the sums of the workgroups' parts: 64 columns a workgroup,
+// the parts over its 4 waves.
+__global__ __launch_bounds__(256) void k_normalise_join(int parts, int64_t n, const float* part, float* out) {
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  float s = 0.0f;
+  if (at < n) {
+    const int per = (parts + 3) / 4, last = (wave + 1) * per < parts ? (wave + 1) * per : parts;
+#pragma unroll 8
+    for (int p = wave * per; p < last; ++p) s += part[p * n + at];
+  }
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && at < n) out[at] = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
+}
+
+// Workgroups of the gradients: enough for every CU, no more than there are
+// groups of rows.
+struct NormPlan {
+  int waves, chunks, rows, groups;  // chunks 0: the forms that hold no rows
+  int64_t bytes, means;
+};
+NormPlan norm_plan(int64_t tokens, int64_t units, int dtype) {
+  const int64_t chunks = div_up(units, dtype == PLX_LB_F32 ? 4 : 8);
+  NormPlan p{};
+  p.waves = chunks <= 64 ? 1 : chunks <= 128 ? 2 : chunks <= 256 ? 4 : chunks <= 512 ? 8 : 16;
+  p.chunks = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : 0;
+  p.rows = p.chunks ? 16 / p.waves : 1;
+  const int64_t groups = div_up(tokens, p.rows), most = cu_count();
+  p.groups = static_cast<int>(groups < most ? groups : most);
+  p.bytes = int64_t{8} * p.groups * units;
+  p.means = p.bytes;
+  if (!p.chunks) p.bytes += 8 * tokens;
+  return p;
+}
+
+template <typename F>
+void with_rows(const NormPlan& p, F f) {
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I4 = std::integral_constant<int, 4>;
+  using I8 = std::integral_constant<int, 8>;
+  using I16 = std::integral_constant<int, 16>;
+  if (p.waves == 1)
+    f(I1{}, I1{});
+  else if (p.waves == 2)
+    f(I2{}, I1{});
+  else if (p.waves == 4)
+    f(I4{}, I1{});
+  else if (p.waves == 8)
+    f(I8{}, I1{});
+  else if (p.chunks == 1)
+    f(I16{}, I1{});
+  else
+    f(I16{}, I2{});
+}
+
+template <typename T, typename P>
+void launch_normalise(const NormArgs& all, const NormPlan& p, hipStream_t s) {
+  constexpr int64_t most = int64_t{1} << 20;  // workgroups of a launch: at most 2^30 lanes
+  for (int64_t first = 0; first < all.tokens; first += most) {
+    NormArgs a = all;
+    a.tokens = all.tokens - first < most ? all.tokens - first : most;
+    a.x = static_cast<const T*>(all.x) + first * all.x_line;
+    a.y = static_cast<T*>(all.y) + first * all.units;
+    a.kept = all.kept + 2 * first;
+    if (!p.chunks) {
+      k_normalise_stream<T, P><<<static_cast<unsigned>(a.tokens), 1024, 0, s>>>(a);
+      continue;
+    }
+    with_rows(p, [&](auto waves, auto chunks) {
+      constexpr int WAVES = decltype(waves)::value, ROWS = WAVES < 4 ? 4 / WAVES : 1;
+      k_normalise<T, P, ROWS, WAVES, decltype(chunks)::value>
+          <<<static_cast<unsigned>(div_up(a.tokens, ROWS)), ROWS * WAVES * 64, 0, s>>>(a);
+    });
+  }
+}
+
+template <typename T, typename P>
+void launch_grad(const NormArgs& a, const NormPlan& p, hipStream_t s) {
+  if (!p.chunks) {
+    float* means = reinterpret_cast<float*>(reinterpret_cast<char*>(a.part) + p.means);
+    constexpr int64_t most = int64_t{1} << 20;
+    for (int64_t first = 0; first < a.tokens; first += most) {
+      NormArgs b = a;
+      b.x = static_cast<const T*>(a.x) + first * a.x_line;
+      b.g = static_cast<const T*>(a.g) + first * a.g_line;
+      b.kept = a.kept + 2 * first;
+      const int64_t now = a.tokens - first < most ? a.tokens - first : most;
+      k_normalise_means<T, P><<<static_cast<unsigned>(now), 1024, 0, s>>>(b, means + 2 * first);
+    }
+    const dim3 grid(static_cast<unsigned>(p.groups), static_cast<unsigned>(div_up(a.units, 256)));
+    k_normalise_columns<T, P><<<grid, 256, 0, s>>>(a, means);
+    return;
+  }
+  with_rows(p, [&](auto waves, auto chunks) {
+    constexpr int WAVES = decltype(waves)::value, ROWS = 16 / WAVES;
+    k_normalise_grad<T, P, ROWS, WAVES, decltype(chunks)::value>
+        <<<static_cast<unsigned>(p.groups), ROWS * WAVES * 64, 0, s>>>(a);
+  });
+}
+
+// F(T, P) by the types of the batch and of the parameters.
+template <typename F>
+void with_types(int dtype, int params, F f) {
+  with_type(dtype, [&](auto* e) {
+    if (params == PLX_LB_F32)
+      f(e, static_cast<float*>(nullptr));
+    else
+      f(e, e);
+  });
+}
+
+int check_norm(const char* who, int64_t tokens, int64_t units, int dtype, int params, float eps) {
+  if (!batch_fits(tokens, units)) return fail(PLX_ERR_INVALID, who);
+  if (!known_type(dtype) || (params != dtype && params != PLX_LB_F32)) return fail(PLX_ERR_UNSUPPORTED, who);
+  if (!(eps >= 0.0f && eps < INFINITY)) return fail(PLX_ERR_INVALID, who);
+  return PLX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int plx_normalise(int64_t tokens, int64_t units, int32_t dtype, const void* x, int64_t line, int32_t params,
+                  const void* weight, const void* bias, float eps, void* y, float* kept, void* stream) {
+  const char* who = "plx_normalise: bad size, type, eps or null pointer";
+  if (const int rc = check_norm(who, tokens, units, dtype, params, eps)) return rc;
+  if (tokens == 0 || units == 0) return PLX_OK;
+  if (!x || !weight || !y || !kept) return fail(PLX_ERR_INVALID, who);
+  NormArgs a{};
+  a.tokens = tokens, a.x_line = line, a.units = static_cast<int>(units), a.eps = eps;
+  a.x = x, a.weight = weight, a.bias = bias, a.y = y, a.kept = kept;
+  const NormPlan p = norm_plan(tokens, units, dtype);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  with_types(dtype, params, [&](auto* t, auto* q) {
+    launch_normalise<PLX_DENSE_TYPE(t), PLX_DENSE_TYPE(q)>(a, p, s);
+  });
+  return check_launch("plx_normalise");
+}
+
+int64_t plx_normalise_workspace(int64_t tokens, int64_t units, int32_t dtype) {
+  if (!batch_fits(tokens, units) || !known_type(dtype)) return -1;
+  return tokens == 0 || units == 0 ? 0 : norm_plan(tokens, units, dtype).bytes;
+}
+
+int plx_normalise_grad(int64_t tokens, int64_t units, int32_t dtype, const void* g, int64_t g_line, const void* x,
+                       int64_t x_line, int32_t params, const void* weight, const float* kept, void* dx,
+                       float* dparams, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "plx_normalise_grad: bad size, type or null pointer";
+  if (const int rc = check_norm(who, tokens, units, dtype, params, 0.0f)) return rc;
+  if (units == 0) return PLX_OK;
+  if (!dparams) return fail(PLX_ERR_INVALID, who);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t n = 2 * units;
+  if (tokens == 0) {
+    k_normalise_join<<<static_cast<unsigned>(div_up(n, 64)), 256, 0, s>>>(0, n, nullptr, dparams);
+    return check_launch("plx_normalise_grad");
+  }
+  const NormPlan p = norm_plan(tokens, units, dtype);
+  if (!g || !x || !weight || !kept || !dx) return fail(PLX_ERR_INVALID, who);
+  if (!workspace || !on_16(workspace) || workspace_bytes < p.bytes)
+    return fail(PLX_ERR_INVALID, "plx_normalise_grad: plx_normalise_workspace() bytes on 16 bytes needed");
+  NormArgs a{};
+  a.tokens = tokens, a.x_line = x_line, a.g_line = g_line, a.units = static_cast<int>(units);
+  a.x = x, a.g = g, a.weight = weight, a.y = dx, a.kept = const_cast<float*>(kept);
+  a.part = static_cast<float*>(workspace);
+  with_types(dtype, params, [&](auto* t, auto* q) { launch_grad<PLX_DENSE_TYPE(t), PLX_DENSE_TYPE(q)>(a, p, s); });
+  k_normalise_join<<<static_cast<unsigned>(div_up(n, 64)), 256, 0, s>>>(p.groups, n, a.part, dparams);
+  return check_launch("plx_normalise_grad");
+}
+
+}  // extern "C"

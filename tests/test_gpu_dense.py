@@ -1,0 +1,540 @@
+"""plastax_amd.dense on the GPU against the plain 64-bit forms, within bounds
+that count the roundings of float32 sums and of the results' types."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import dense_plain as plain
+from plastax_amd import dense
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+F32, BF16, F16 = plain.DTYPES
+
+
+def _gen(*key: int) -> torch.Generator:
+    seed = 0
+    for k in key:
+        seed = seed * 10007 + k
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _randn(shape, g) -> torch.Tensor:
+    return torch.randn(shape, generator=g, device=DEV)
+
+
+def _say(*what) -> None:
+    print(*what, flush=True)
+
+
+def _layout(t: torch.Tensor, layout: str) -> torch.Tensor:
+    """The same values: as they are, behind an odd offset with rows apart, or unit-major."""
+    if layout == "columns":
+        return t.t().contiguous().t()
+    if layout == "apart":
+        room = torch.full((t.shape[0] * (t.shape[1] + 3) + 1,), torch.nan, dtype=t.dtype, device=t.device)
+        v = room[1:].view(t.shape[0], t.shape[1] + 3)[:, : t.shape[1]]
+        v.copy_(t)
+        return v
+    return t
+
+
+LAYOUTS = ["rows", "apart", "columns"]
+
+
+# --------------------------------------------------------------------------
+# An input level by ids
+# --------------------------------------------------------------------------
+def _some_ids(tokens: int, rows: int, kind: str, wide: torch.dtype, g) -> torch.Tensor:
+    if kind == "one":
+        ids = torch.full((tokens,), rows // 2, device=DEV)
+    elif kind == "few":
+        ids = torch.randint(min(rows, 3), (tokens,), generator=g, device=DEV)
+    else:
+        ids = torch.randint(rows, (tokens,), generator=g, device=DEV)
+    if kind != "one":
+        ids[torch.rand((tokens,), generator=g, device=DEV) < 0.1] = -1
+        top = torch.iinfo(wide)
+        for i, bad in enumerate((rows, top.max, top.min)):
+            ids[i + 1 :: 41] = bad
+    return ids.to(wide)
+
+
+# tokens, rows, units: lanes of every width, columns past a slab, classes with several rows, more classes
+LOOKS = [(1, 1, 1), (3, 7, 5), (64, 10, 8), (65, 300, 33), (128, 5, 129), (129, 40, 260), (200, 1000, 513),
+         (1000, 70, 1003), (4100, 3000, 64), (700, 9, 2100), (5000, 20000, 24), (300, 2_100_000, 3)]
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("shape", LOOKS)
+def test_look_up(shape, dtype, layout) -> None:
+    tokens, rows, units = shape
+    _say("look_up", shape, dtype, layout)
+    g = _gen(*shape)
+    table = _layout((_randn((rows, units), g) * 3).to(dtype), layout)
+    for wide in (torch.int32, torch.int64):
+        ids = _some_ids(tokens, rows, "any", wide, g)
+        for scale in (1.0, 2.5):  # (exact in float32)
+            want = plain.look_up(ids, table, scale)
+            plain.near(dense.look_up(ids, table, scale), want, plain.EPS * want.abs() + plain.rounded(want, dtype))
+    assert torch.equal(dense.look_up(ids, table), torch.where((ids >= 0) & (ids < rows), table.t()[:, ids.clamp(0, rows - 1).long()], 0).t())
+
+
+@pytest.mark.parametrize("kind", ["any", "few", "one"])
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("shape", LOOKS)
+def test_look_up_grad(shape, dtype, kind) -> None:
+    tokens, rows, units = shape
+    _say("look_up_grad", shape, dtype, kind)
+    g = _gen(*shape, 1)
+    for wide, layout in ((torch.int32, "rows"), (torch.int64, "apart"), (torch.int64, "columns")):
+        ids, grad = _some_ids(tokens, rows, kind, wide, g), _layout(_randn((tokens, units), g).to(dtype), layout)
+        got = dense.look_up_grad(grad, ids, rows, 2.5)
+        want, off = plain.look_up_grad(grad, ids, rows, 2.5)
+        plain.near(got, want, off)
+        assert torch.equal(got, dense.look_up_grad(grad, ids, rows, 2.5))  # a fixed order
+
+
+@pytest.mark.parametrize("runs", [[64], [65], [63, 65, 64], [1, 64, 129, 63, 128, 2], [200, 1, 1, 300], [64] * 5 + [65] * 5])
+def test_rows_of_the_gradient_at_the_borders_of_parts(runs) -> None:
+    """Rows of a class lie behind each other in the list (ids 0, 256, 512, ...): runs of these lengths begin and end
+    at every place of a part."""
+    ids = torch.cat([torch.full((n,), 256 * i, device=DEV) for i, n in enumerate(runs)])
+    g = _gen(len(runs))
+    ids = ids[torch.randperm(ids.shape[0], generator=g, device=DEV)]
+    grad = torch.randint(-8, 9, (ids.shape[0], 70), generator=g, device=DEV).float()  # (whole numbers: exact sums)
+    got = dense.look_up_grad(grad, ids, 256 * len(runs))
+    want = torch.zeros((256 * len(runs), 70), dtype=torch.float64, device=DEV).index_add_(0, ids, grad.double())
+    assert torch.equal(got.double(), want)
+
+
+def test_infinities_and_nan_stay_in_their_rows() -> None:
+    ids = torch.tensor([2, -1, 4, 2, 9], device=DEV)
+    g = torch.ones((5, 40), device=DEV)
+    g[1], g[4], g[2, 3] = torch.nan, torch.inf, -torch.inf
+    got = dense.look_up_grad(g, ids, 6)
+    want = torch.zeros((6, 40), device=DEV)
+    want[2], want[4] = 2, 1
+    want[4, 3] = -torch.inf
+    assert torch.equal(got, want)
+    table = torch.ones((3, 40), device=DEV)
+    table[0] = torch.nan
+    assert torch.equal(dense.look_up(torch.tensor([-1, 1, 3], device=DEV), table), torch.tensor([0.0, 1.0, 0.0], device=DEV)[:, None].expand(3, 40))
+
+
+# --------------------------------------------------------------------------
+# Layer norm
+# --------------------------------------------------------------------------
+UNITS = [1, 2, 7, 64, 255, 256, 257, 512, 513, 1003, 1024, 2048, 2050, 4096, 4100, 8192, 8200, 16384, 16390, 20001]
+
+
+def _levels(tokens, units, dtype, g) -> torch.Tensor:
+    x = _randn((tokens, units), g) * torch.exp(_randn((tokens, 1), g)) + 3 * _randn((tokens, 1), g)
+    x[:, ::17] *= 10
+    if tokens > 2:
+        x[2] = 0.5  # a row without variance
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("units", UNITS)
+def test_normalise_and_its_gradients(units, dtype) -> None:
+    for tokens, layout, params, biased in ((1, "rows", F32, True), (3, "apart", dtype, True), (37, "columns", F32, False),
+                                           (700, "rows", dtype, True)):
+        _say("normalise", tokens, units, dtype, layout, params)
+        g = _gen(tokens, units)
+        x, d = _layout(_levels(tokens, units, dtype, g), layout), _layout(_randn((tokens, units), g).to(dtype), layout)
+        w, b = (1 + 0.3 * _randn((units,), g)).to(params), _randn((units,), g).to(params) if biased else None
+        (y, off), (dx, dx_off), (dw, dw_off), (db, db_off) = plain.normalise(x, w, b, 1e-3, d)
+        got, kept = dense.normalise(x, w, b, 1e-3)
+        plain.near(got, y, off + plain.rounded(y, dtype))
+        got = dense.normalise_grad(d, x, w, kept)
+        plain.near(got[0], dx, dx_off + plain.rounded(dx, dtype))
+        plain.near(got[1], dw, dw_off)
+        plain.near(got[2], db, db_off)
+        again = dense.normalise_grad(d, x, w, kept)
+        assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+
+@pytest.mark.parametrize("units", [100, 1003, 4096, 16384, 20001])
+def test_rows_that_are_not_finite_spoil_no_others(units) -> None:
+    g = _gen(units)
+    x, w, d = _randn((9, units), g), _randn((units,), g), _randn((9, units), g)
+    y, kept = dense.normalise(x, w)
+    dx, _, _ = dense.normalise_grad(d, x, w, kept)
+    bad = x.clone()
+    bad[3, units // 2], bad[6, 0], bad[8, -1] = torch.nan, torch.inf, -torch.inf
+    z, kept = dense.normalise(bad, w)
+    dz, _, _ = dense.normalise_grad(d, bad, w, kept)
+    fine = torch.tensor([0, 1, 2, 4, 5, 7], device=DEV)
+    assert torch.equal(z[fine], y[fine]) and torch.equal(dz[fine], dx[fine])
+    assert not torch.isfinite(z[[3, 6, 8]]).any() and not torch.isfinite(dz[[3, 6, 8]]).any()
+
+
+# --------------------------------------------------------------------------
+# A level carried along sequences
+# --------------------------------------------------------------------------
+def _xz(tokens, units, dtype, g) -> torch.Tensor:
+    xz = _randn((tokens, 2 * units), g)
+    xz[:, units:] = 3 * xz[:, units:] + 10 * torch.rand((units,), generator=g, device=DEV) - 1
+    return xz.to(dtype)
+
+
+def _check_recur(xz, starts, state, g, g_last, wide, layout="rows") -> None:
+    dtype = xz.dtype
+    (h, h_off), (last, last_off), (dxz, dxz_off), (ds, ds_off) = plain.recur(xz, starts, state, g, g_last)
+    xz, g = _layout(xz, layout), _layout(g, layout)
+    at = None if wide is None else torch.tensor(starts, dtype=wide, device=DEV)
+    got = dense.recur(xz, at, state)
+    plain.near(got[0], h, h_off + plain.rounded(h, dtype))
+    plain.near(got[1], last, last_off)
+    back = dense.recur_grad(g, xz, got[2], at, state, g_last)
+    plain.near(back[0], dxz, dxz_off + plain.rounded(dxz, dtype))
+    plain.near(back[1], ds, ds_off)
+    again = dense.recur_grad(g, xz, got[2], at, state, g_last)
+    assert torch.equal(back[0], again[0]) and torch.equal(back[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("tokens", [1, 2, 4, 7, 8, 9, 63, 64, 65, 127, 128, 129, 200, 700])
+def test_recur_of_one_sequence(tokens, dtype) -> None:
+    for units, layout in ((1, "rows"), (2, "apart"), (3, "columns"), (127, "rows"), (129, "apart"), (300, "rows")):
+        _say("recur", tokens, units, dtype, layout)
+        g = _gen(tokens, units)
+        xz, d = _xz(tokens, units, dtype, g), _randn((tokens, units), g).to(dtype)
+        _check_recur(xz, [0, tokens], None, d, None, None, layout)
+        state, g_last = _randn((1, units), g), _randn((1, units), g)
+        _check_recur(xz, [0, tokens], state, d, g_last, torch.int64, layout)
+
+
+RAGGED = {
+    "ones": list(range(41)),
+    "empty": [0, 0, 0, 5, 5, 5, 9, 40, 40, 40],
+    "inner": [3, 8, 20, 31],  # rows before the first and behind the last
+    "none": [17, 17, 17],
+    "steps": [0, 64, 128, 192, 256, 300],
+    "odd": [0, 1, 63, 127, 129, 130, 255, 300, 700],
+    "long": [5, 600, 601, 1100],
+}
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("name", list(RAGGED))
+def test_recur_of_ragged_sequences(name, dtype) -> None:
+    starts = RAGGED[name]
+    tokens = max(starts[-1], 40) + (0 if name in ("ones", "steps") else 7)
+    for units, wide in ((5, torch.int32), (130, torch.int64)):
+        _say("recur ragged", name, units, dtype)
+        g = _gen(len(name), units)
+        xz, d = _xz(tokens, units, dtype, g), _randn((tokens, units), g).to(dtype)
+        sequences = len(starts) - 1
+        _check_recur(xz, starts, None, d, None, wide)
+        _check_recur(xz, starts, _randn((sequences, units), g), d, _randn((sequences, units), g), wide)
+
+
+def test_recur_of_many_parts() -> None:
+    """Long enough for more rows than one step in a part, and for all parts that a level of few units is cut into."""
+    tokens, units = 20000, 5
+    g = _gen(tokens)
+    xz, d = _xz(tokens, units, F32, g), _randn((tokens, units), g)
+    starts = [0, 100, 100, 9000, 9064, 19990]
+    _check_recur(xz, starts, _randn((5, units), g), d, _randn((5, units), g), torch.int32)
+
+
+@pytest.mark.parametrize("tokens", [100, 1500])
+def test_what_is_not_finite_stays_in_its_sequence(tokens) -> None:
+    g = _gen(tokens)
+    units, starts = 70, torch.tensor([10, tokens // 3, tokens // 2, tokens - 5], device=DEV)
+    xz, d = _xz(tokens, units, F32, g), _randn((tokens, units), g)
+    state, g_last = _randn((3, units), g), _randn((3, units), g)
+    want = dense.recur(xz, starts, state)
+    want_back = dense.recur_grad(d, xz, want[2], starts, state, g_last)
+    bad, bad_d, bad_state, bad_last = xz.clone(), d.clone(), state.clone(), g_last.clone()
+    bad[:10], bad[-5:], bad_d[:10], bad_d[-5:] = torch.nan, torch.nan, torch.nan, torch.inf  # rows of no sequence
+    bad[tokens // 3 + 3, 5] = torch.nan
+    bad[tokens // 2 - 2, units + 9] = torch.nan
+    bad_state[1, 20], bad_last[1, 30], bad_d[tokens // 3 + 1, 40] = torch.inf, torch.nan, torch.nan
+    got = dense.recur(bad, starts, bad_state)
+    back = dense.recur_grad(bad_d, bad, got[2], starts, bad_state, bad_last)
+    rows = torch.ones(tokens, dtype=torch.bool, device=DEV)
+    rows[tokens // 3 : tokens // 2] = False
+    others = [0, 2]
+    assert torch.equal(got[0][rows], want[0][rows]) and torch.equal(got[1][others], want[1][others])
+    assert torch.equal(back[0][rows], want_back[0][rows]) and torch.equal(back[1][others], want_back[1][others])
+    assert not got[0][:10].any() and not got[0][-5:].any() and not back[0][:10].any() and not back[0][-5:].any()
+    assert torch.isnan(got[0][tokens // 3 + 3 : tokens // 2, 5]).all() and torch.isnan(got[1][1, 5])
+    assert not torch.isfinite(got[0][tokens // 3 : tokens // 2, 20]).any()
+    clean = [c for c in range(units) if c not in (5, 9, 20, 30, 40)]
+    assert torch.equal(got[0][:, clean], want[0][:, clean])
+    assert torch.equal(back[0][:, clean], want_back[0][:, clean])
+
+
+def test_starts_out_of_range_are_taken_to_the_range() -> None:
+    g = _gen(5)
+    xz, d = _xz(50, 6, F32, g), _randn((50, 6), g)
+    for wide, low, high in ((torch.int32, -7, 1000), (torch.int64, -(1 << 62), 1 << 62)):
+        out = torch.tensor([low, 20, high, high], dtype=wide, device=DEV)
+        same = torch.tensor([0, 20, 50, 50], dtype=wide, device=DEV)
+        state = _randn((3, 6), g)
+        got, want = dense.recur(xz, out, state), dense.recur(xz, same, state)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        got, want = (dense.recur_grad(d, xz, want[2], at, state, state) for at in (out, same))
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 2048), (5, 3), (64, 130), (300, 1003)])
+def test_recur_step(shape, dtype) -> None:
+    """One token at a time: the formula, and what recur gives for all of them."""
+    sequences, units = shape
+    _say("recur_step", shape, dtype)
+    g = _gen(*shape)
+    tokens = 6
+    xz = _xz(sequences * tokens, units, dtype, g)
+    room = torch.zeros((sequences, units + 2), device=DEV)
+    state = room[:, :units]
+    state.copy_(_randn((sequences, units), g))
+    start = state.clone()
+    starts = torch.arange(sequences + 1, device=DEV) * tokens
+    h, last, _ = dense.recur(xz, starts, start)
+    (want, off), (want_last, last_off) = plain.recur(xz, starts.tolist(), start)
+    for t in range(tokens):
+        step = dense.recur_step(xz[t::tokens], state)
+        plain.near(step, want[t::tokens], off[t::tokens] + plain.rounded(want[t::tokens], dtype))
+        assert torch.equal(step, state.to(dtype))
+    plain.near(state, want_last, last_off)
+    plain.near(last, want_last, last_off)
+    assert not room[:, units:].any()
+
+
+# --------------------------------------------------------------------------
+# An output level learned from a teacher
+# --------------------------------------------------------------------------
+# outputs of every form: a wave, 4, 8 and 16 waves, rows past the registers
+OUTPUTS = [1, 2, 10, 255, 257, 512, 1000, 2049, 4097, 8200, 16400, 32003, 70001, 140000]
+
+
+def _teacher(tokens, outputs, named, wide, g):
+    ids = torch.randint(outputs, (tokens, named), generator=g, device=DEV)
+    top = 2 * _randn((tokens, named), g)
+    if named > 1:
+        ids[:, 1::7] = ids[:, :1]  # an output named twice
+        ids[torch.rand((tokens, named), generator=g, device=DEV) < 0.1] = -1
+        limit = torch.iinfo(wide)
+        ids[:, 3::11], ids[:, 4::11], ids[:, 5::11] = outputs, limit.max, limit.min
+        top[torch.rand((tokens, named), generator=g, device=DEV) < 0.1] = -torch.inf
+    if tokens > 2:
+        ids[2] = -1
+    if tokens > 3:
+        top[3] = -torch.inf
+    return ids.to(wide), top
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("outputs", OUTPUTS)
+def test_distil_and_its_gradient(outputs, dtype) -> None:
+    for tokens, named, wide, layout, temperature in ((1, 1, torch.int32, "rows", 1.0), (5, 12, torch.int64, "apart", 2.0),
+                                                     (4, 70, torch.int32, "columns", 0.75), (2, 1024, torch.int64, "rows", 1.0),
+                                                     (3, 0, torch.int32, "rows", 1.0)):
+        _say("distil", tokens, outputs, named, dtype, layout)
+        g = _gen(tokens, outputs, named)
+        logits = (3 * _randn((tokens, outputs), g)).to(dtype)
+        if outputs > 5:
+            logits[:, 3::9] = -torch.inf
+            logits[:, 4::9] = torch.finfo(dtype).min
+        ids, top = _teacher(tokens, outputs, named, wide, g)
+        # (a named output of -inf has an infinite loss: some tokens keep theirs finite)
+        finite = torch.isfinite(torch.gather(logits, 1, ids.long().clamp(0, outputs - 1)))
+        if tokens > 1:
+            ids[1:][~finite[1:]] = -1
+        top = top.to(dtype) if wide is torch.int32 else top
+        weight = torch.rand((tokens,), generator=g, device=DEV)
+        (loss, off), (d, d_off) = plain.distil(logits, ids, top, temperature, weight)
+        x = _layout(logits, layout)
+        got = dense.distil_grad(weight, x, ids, top, temperature)
+        plain.near(got[0], loss, off)
+        plain.near(got[1], d, d_off + plain.rounded(d, dtype))
+        assert torch.equal(dense.distil(x, ids, top, temperature), got[0])
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES)
+@pytest.mark.parametrize("outputs", [40, 1000, 33000, 70001])
+def test_masks_that_leave_a_row_nothing(outputs, dtype) -> None:
+    """Rows of the type's lowest value alone are rows of equal logits; rows of -inf alone are not a number, but for a
+    token that nobody named an output of; and so are rows with an infinity or a NaN, and no others."""
+    low = torch.finfo(dtype).min
+    x = torch.full((6, outputs), low, dtype=dtype, device=DEV)
+    x[1:3] = -torch.inf
+    x[3, 1], x[4, 1], x[5, 2] = torch.inf, torch.nan, 0.0
+    ids = torch.tensor([[0, 1], [0, 1], [-1, outputs], [0, 1], [-1, 0], [2, -1]], device=DEV)
+    top = torch.zeros((6, 2), device=DEV)
+    weight = torch.ones(6, device=DEV)
+    loss, d = dense.distil_grad(weight, x, ids, top)
+    assert abs(float(loss[0]) - float(torch.tensor(outputs / 2.0).log())) < 1e-5
+    q = torch.full((outputs,), 1.0 / outputs, dtype=torch.float64, device=DEV)
+    q[:2] -= 0.5
+    plain.near(d[0], q, q.abs() * (1e-5 + plain.half(dtype)) + plain.rounded(q, dtype))
+    assert torch.isnan(d[1]).all() and torch.isnan(d[3]).all() and torch.isnan(d[4]).all()
+    assert torch.isnan(loss[[1, 3, 4]]).all()
+    assert float(loss[2]) == 0.0 and not d[2].any()
+    assert float(loss[5]) == 0.0 and not d[5].any()  # all of q and of p on one output
+
+
+# --------------------------------------------------------------------------
+# Nothing to do, streams, graphs, long arrays
+# --------------------------------------------------------------------------
+def test_nothing_to_do() -> None:
+    ids, none = torch.zeros(0, dtype=torch.int64, device=DEV), torch.zeros((0, 6), device=DEV)
+    three = torch.zeros(3, dtype=torch.int64, device=DEV)
+    assert dense.look_up(ids, torch.ones((4, 6), device=DEV)).shape == (0, 6)
+    assert torch.equal(dense.look_up(three, none), torch.zeros((3, 6), device=DEV))
+    assert dense.look_up(three, torch.ones((4, 0), device=DEV)).shape == (3, 0)
+    assert torch.equal(dense.look_up_grad(none, ids, 4), torch.zeros((4, 6), device=DEV))
+    assert dense.look_up_grad(torch.ones((3, 6), device=DEV), three, 0).shape == (0, 6)
+    w = torch.ones(6, device=DEV)
+    y, kept = dense.normalise(none, w)
+    dx, dw, db = dense.normalise_grad(none, none, w, kept)
+    assert y.shape == dx.shape == (0, 6) and not dw.any() and not db.any()
+    empty = torch.ones((3, 0), device=DEV)
+    y, kept = dense.normalise(empty, w[:0])
+    assert [t.shape for t in dense.normalise_grad(empty, empty, w[:0], kept)] == [(3, 0), (0,), (0,)]
+    state = torch.ones((1, 3), device=DEV)
+    h, last, kept = dense.recur(none, None, state)
+    assert h.shape == (0, 3) and torch.equal(last, state)
+    dxz, ds = dense.recur_grad(none[:, :3], none, kept, None, state, 2 * state)
+    assert dxz.shape == (0, 6) and torch.equal(ds, 2 * state)
+    h, last, kept = dense.recur(torch.ones((5, 6), device=DEV), three[:1])  # no sequences
+    assert not h.any() and last.shape == (0, 3)
+    dxz, ds = dense.recur_grad(torch.ones((5, 3), device=DEV), torch.ones((5, 6), device=DEV), kept, three[:1])
+    assert not dxz.any() and ds.shape == (0, 3)
+    assert dense.recur_step(none, torch.zeros((0, 3), device=DEV)).shape == (0, 3)
+    assert dense.distil(none, ids.view(0, 1), none[:, :1]).shape == (0,)
+    loss, d = dense.distil_grad(torch.ones(3, device=DEV), empty, three[:, None], torch.ones((3, 1), device=DEV))
+    assert not loss.any() and d.shape == (3, 0)
+
+
+def _together(s):
+    """A run of the operators as a net would call them."""
+    y = dense.look_up(s["ids"], s["table"], 8.0)
+    n, kept = dense.normalise(y, s["w"], s["b"])
+    h, last, walked = dense.recur(n, s["starts"], s["state"])
+    loss, d = dense.distil_grad(s["weight"], h, s["named"], s["top"], 2.0)
+    dn, ds = dense.recur_grad(d, n, walked, s["starts"], s["state"], last)
+    dy, dw, db = dense.normalise_grad(dn, y, s["w"], kept)
+    step = dense.recur_step(n[: s["now"].shape[0]], s["now"])
+    return y, n, h, last, loss, d, dn, ds, dy, dw, db, dense.look_up_grad(dy, s["ids"], s["table"].shape[0], 8.0), step
+
+
+def _inputs(seed: int, dtype=BF16, tokens=900, rows=50, units=256):
+    g = _gen(seed)
+    ids = torch.randint(-1, rows, (tokens,), generator=g, device=DEV)
+    named = torch.randint(-1, units // 2, (tokens, 9), generator=g, device=DEV)
+    cuts = torch.sort(torch.randint(tokens + 1, (8,), generator=g, device=DEV)).values
+    return {"ids": ids, "table": _randn((rows, units), g).to(dtype), "w": 1 + 0.1 * _randn((units,), g),
+            "b": _randn((units,), g), "starts": cuts, "state": _randn((7, units // 2), g), "named": named,
+            "top": _randn((tokens, 9), g), "weight": torch.rand((tokens,), generator=g, device=DEV) / tokens,
+            "now": torch.zeros((3, units // 2), device=DEV)}
+
+
+def test_on_another_stream() -> None:
+    s = _inputs(1)
+    want = _together(s)
+    torch.cuda.synchronize()
+    s["now"].zero_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _together(s)
+    side.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_in_graphs() -> None:
+    """Two captured graphs, replayed in turn on new inputs with eager calls between: every replay gives what the eager
+    call gives."""
+    graphs, states, outs = [], [], []
+    for k in range(2):
+        s = _inputs(10 + k)
+        _together(s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _together(s)
+        graphs.append(graph), states.append(s), outs.append(out)
+    for turn in range(4):
+        for k in range(2):
+            for name, v in _inputs(100 * turn + k).items():
+                states[k][name].copy_(v)
+            graphs[k].replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in outs[k]]
+            states[k]["now"].zero_()
+            want = _together(states[k])
+            assert all(torch.equal(p, q) for p, q in zip(got, want)), (turn, k)
+
+
+def test_gradients_are_the_differences() -> None:
+    """The gradients' products with a direction against differences of the 64-bit loss along it, for the run of all
+    operators in float32: a central difference with a step of 1e-5 is off by some 1e-10, float32's sums by their
+    bounds, far below 1e-5 of the magnitudes."""
+    tokens, rows, units = 150, 30, 16
+    s = _inputs(7, F32, tokens, rows, units)
+    s["named"] = s["named"].clamp_max(units // 2 - 1)
+    s["starts"][-1], s["starts"][0] = tokens, 0
+    out = _together(s)
+    last, grads = out[3], {"table": out[11], "w": out[9], "b": out[10], "state": out[7]}
+    starts = s["starts"].tolist()
+
+    def value(**changed):
+        v = {**s, **changed}
+        y = plain.look_up(v["ids"], v["table"], 8.0)
+        n = plain.normalise(y, v["w"], v["b"], 1e-5)[0][0]
+        (h, _), (end, _) = plain.recur(n, starts, v["state"])
+        return (plain.distil(h, v["named"], v["top"], 2.0)[0][0] * v["weight"].double()).sum() + (end * last.double()).sum()
+
+    for name, grad in grads.items():
+        x, v = s[name].double(), _randn(grad.shape, _gen(3)).double()
+        slope = float(value(**{name: x + 1e-5 * v}) - value(**{name: x - 1e-5 * v})) / 2e-5
+        size = float((grad.double() * v).abs().sum())
+        assert abs(slope - float((grad.double() * v).sum())) <= 1e-5 * size, name
+
+
+def test_offsets_past_32_bits() -> None:
+    """Batches of more than 2^32 values: their last rows are what the same rows give by themselves."""
+    g = _gen(9)
+    few = 3
+    table = torch.zeros((1 << 22, 1100), dtype=BF16, device=DEV)
+    table[-few:] = _randn((few, 1100), g).to(BF16)
+    ids = torch.arange((1 << 22) - few, 1 << 22, device=DEV)
+    assert torch.equal(dense.look_up(ids, table), table[-few:])
+    grad = _randn((few, 1100), g).to(BF16)
+    d = dense.look_up_grad(grad, ids, 1 << 22)
+    assert torch.equal(d[-few:], grad.float()) and not d[: 1 << 20].any()
+    del d
+    w = torch.ones(1100, device=DEV)
+    y, kept = dense.normalise(table, w)
+    z, few_kept = dense.normalise(table[-few:], w)
+    assert torch.equal(y[-few:], z) and torch.equal(kept[-few:], few_kept)
+    del y
+    dx, _, _ = dense.normalise_grad(table, table, w, kept)
+    dz, _, _ = dense.normalise_grad(table[-few:], table[-few:], w, few_kept)
+    assert torch.equal(dx[-few:], dz)
+    del dx
+    many = table.view(1 << 22, 1100)
+    starts = torch.tensor([0, (1 << 22) - few, 1 << 22], device=DEV)
+    h, last, walked = dense.recur(many, starts)
+    few_h, few_last, few_walked = dense.recur(many[-few:].clone())
+    assert torch.equal(h[-few:], few_h) and torch.equal(last[1], few_last[0])
+    dxz, ds = dense.recur_grad(h, many, walked, starts)
+    few_dxz, few_ds = dense.recur_grad(few_h, many[-few:].clone(), few_walked)
+    assert torch.equal(dxz[-few:], few_dxz) and torch.equal(ds[1], few_ds[0])
+    del dxz, h, walked
+    named, top = torch.zeros((1 << 22, 1), dtype=torch.int32, device=DEV), torch.zeros((1 << 22, 1), device=DEV)
+    weight = torch.ones(1 << 22, device=DEV)
+    loss, d = dense.distil_grad(weight, table, named, top)
+    few_loss, few_d = dense.distil_grad(weight[:few], table[-few:], named[:few], top[:few])
+    assert torch.equal(loss[-few:], few_loss) and torch.equal(d[-few:], few_d)
