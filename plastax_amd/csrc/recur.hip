@@ -7,32 +7,36 @@
 // last row plus its last state's gradient), dx = (1 - a) c,
 // dz = a (1 - a) (h[t-1] - x) c, and a c of its first row is the state's.
 //
-// Rows with h -> A h + H compose, so a row range can be summed up before what
-// comes in is known. A workgroup walks its part of the rows in steps of kStep,
-// a lane two units of a few rows, the step's waves behind each other: each
-// wave sums up its rows, the sums meet in LDS, and each wave walks its rows
-// again from what comes in. Where units alone do not fill the CUs the rows are
-// cut into parts, which a launch before sums up (the rows are read twice).
+// Rows as maps h -> A h + H compose, so rows can be summed up before what comes
+// in is known. A workgroup takes a tile, a few rows a wave of kSlab units, into
+// its registers, two units a lane; its waves' sums meet in LDS, the
+// tiles' in memory, and each wave walks its rows again from what comes in: xz
+// is read once. Tiles are taken in the order of a counter, and wait for
+// earlier ones only, which are under way: every wait ends (and is bounded, for
+// a caller who has two calls share a workspace). A tile waits for the sums of
+// the tiles before it in its group, and for what comes into the group, so that
+// a long sequence is a chain of groups; every sum has one order.
 
 #include "px_dense.h"
 
 using plx_detail::check_launch;
-using plx_detail::cu_count;
 using plx_detail::fail;
 
 namespace {
 
 using namespace px;
 
-constexpr int kWaves = 16, kRows = 8, kStep = kWaves * kRows;  // rows of a step
-constexpr int kBack = 4, kKeep = PLX_RECUR_KEEP;              // and of one of the gradients' (registers)
-static_assert(kKeep == kWaves * kBack && kStep % kKeep == 0, "a step begins where its state is kept");
+constexpr int kWaves = 8;                 // of a tile
+constexpr int kForth = 16, kBack = 8;     // rows of a wave forwards, and of the gradients' (registers)
+constexpr int kKeep = kWaves * kBack;     // rows of the gradients' tile: what comes into it is kept
+static_assert(kKeep == PLX_RECUR_KEEP && kKeep % kForth == 0, "a wave begins where its h is kept");
+constexpr int kGroup = 16;  // tiles of a group
 constexpr int kSlab = 128;                                     // units of a workgroup
 constexpr int64_t kMaxSequences = int64_t{1} << 30;
 
 struct RecurArgs {
-  int64_t tokens, sequences, line, g_line, part;  // part: rows of a part, a multiple of kStep
-  int units, wide;
+  int64_t tokens, sequences, line, g_line, tiles;
+  int units, wide, slabs;
   const void* xz;
   const void* starts;  // null: one sequence
   const int* of;       // [tokens]: the row's sequence, -1 outside of all (null: one sequence)
@@ -40,12 +44,15 @@ struct RecurArgs {
   void* h;
   float* last;
   float* kept;  // [ceil(tokens / kKeep)][units]: what comes into its rows
-  float* sums;  // [parts][3][units]
   // backwards
   const void* g;
   const float* g_last;  // null: zeros
   void* dxz;
   float* dstate;
+  // zeros at first, in the order in which tiles are taken
+  unsigned* ticket;
+  uint64_t* spans;    // [tiles][units]: the tile summed up
+  uint64_t* carries;  // [groups][units]: what comes out of the group
 };
 
 __device__ __forceinline__ int64_t start_of(const RecurArgs& a, int64_t s) {
@@ -53,64 +60,94 @@ __device__ __forceinline__ int64_t start_of(const RecurArgs& a, int64_t s) {
   return t < 0 ? 0 : t < a.tokens ? t : a.tokens;
 }
 
-// of[t]: the last sequence that starts at t or before, if t is before its end.
-__global__ __launch_bounds__(256) void k_recur_rows(RecurArgs a, int* of) {
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (t >= a.tokens) return;
-  int64_t lo = -1, hi = a.sequences;  // start_of(lo) <= t < start_of(hi), as far as they are sequences
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) / 2;
-    if (start_of(a, mid) <= t)
-      lo = mid;
-    else
-      hi = mid;
+// of[t]: the last sequence that starts at t or before, if t is before its end;
+// and the `words` of the tiles' sums, zeros.
+__global__ __launch_bounds__(256) void k_recur_setup(RecurArgs a, int* of, uint64_t* zeros, int64_t words) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, all = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t t = i; t < words; t += all) zeros[t] = 0;
+  if (!of) return;
+  for (int64_t t = i; t < a.tokens; t += all) {
+    int64_t lo = -1, hi = a.sequences;  // start_of(lo) <= t < start_of(hi), as far as they are sequences
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) / 2;
+      if (start_of(a, mid) <= t)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    of[t] = lo >= 0 && t < start_of(a, lo + 1) ? static_cast<int>(lo) : -1;
   }
-  of[t] = lo >= 0 && t < start_of(a, lo + 1) ? static_cast<int>(lo) : -1;
 }
 
-// The sequences of rows first - 1 to first + N, the same in all lanes.
+// The sequences of N rows from first - 1 on, the same in all lanes.
 template <int N>
-__device__ __forceinline__ void rows_of(const RecurArgs& a, int64_t first, int of[N + 2]) {
+__device__ __forceinline__ void rows_of(const RecurArgs& a, int64_t first, int (&of)[N]) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = first - 1 + lane;
+  const bool there = t >= 0 && t < a.tokens;
+  int mine = there ? 0 : -1;
+  if (a.of && there && lane < N) mine = a.of[t];
 #pragma unroll
-  for (int i = 0; i < N + 2; ++i) {
-    const int64_t t = first - 1 + i;
-    const bool there = t >= 0 && t < a.tokens;
-    of[i] = !there ? -1 : a.of ? __builtin_amdgcn_readfirstlane(a.of[t]) : 0;
-  }
+  for (int i = 0; i < N; ++i) of[i] = __builtin_amdgcn_readlane(mine, i);
 }
 
-// a = sigmoid(z) and b = 1 - a, both to a few steps: by exp(-|z|), with the
-// rounding error of its exponent carried on.
+// a = sigmoid(z) and b = 1 - a: the lesser is t / (1 + t), t = exp(-|z|) with
+// the rounding error of its exponent carried on, and the other one minus it, so
+// that what a row passes on and takes in make one.
 __device__ __forceinline__ void gate(float z, float& a, float& b) {
-  const float y = fabsf(z);
+  const float y = __builtin_elementwise_minimum(fabsf(z), 128.0f);  // (a NaN stays)
   const float hi = y * -1.44269502162933349609375f;
   float lo = __builtin_fmaf(y, -1.44269502162933349609375f, -hi);
   lo = __builtin_fmaf(y, -1.925963033500011e-8f, lo);
   float t = __builtin_amdgcn_exp2f(hi);
-  t = t > 0.0f ? __builtin_fmaf(t * lo, 0.693147182464599609375f, t) : t;
-  float r = __builtin_amdgcn_rcpf(1.0f + t);
-  r = __builtin_fmaf(__builtin_fmaf(-(1.0f + t), r, 1.0f), r, r);
-  const float s = t * r;
-  a = z < 0.0f ? s : r;
-  b = z < 0.0f ? r : s;
+  t = __builtin_fmaf(t * lo, 0.693147182464599609375f, t);
+  const float s = t * __builtin_amdgcn_rcpf(1.0f + t), l = 1.0f - s;
+  a = z < 0.0f ? s : l;
+  b = z < 0.0f ? l : s;
 }
 
 struct Pair {
   float v[2];
 };
-__device__ __forceinline__ Pair load_pair(const float* p, int n) {
-  Pair r;
-  r.v[0] = n > 0 ? p[0] : 0.0f, r.v[1] = n > 1 ? p[1] : 0.0f;
-  return r;
+// A lane's two units of a row, without a branch, for lanes past the row's end
+// read something of it: units `at` and `at + 1`, EVEN if a level's are even in
+// number (then both are one load), else one by one.
+struct Lane {
+  unsigned col, at, next;
+  int n;  // of the two, how many are there
+};
+__device__ __forceinline__ Lane lane_of(unsigned first, int units) {
+  Lane l;
+  l.col = first + (threadIdx.x & 63) * 2;
+  l.n = units - static_cast<int>(l.col);
+  l.at = l.n > 0 ? l.col : 0;
+  l.next = l.n > 1 ? l.col + 1 : 0;
+  return l;
 }
-__device__ __forceinline__ void store_pair(float* p, int n, const float v[2]) {
-  if (n > 0) p[0] = v[0];
-  if (n > 1) p[1] = v[1];
+template <bool EVEN, typename T>
+__device__ __forceinline__ typename Pack<T, 2>::type load_two(const T* row, const Lane& l) {
+  if (EVEN) return *reinterpret_cast<const typename Pack<T, 2>::load*>(row + l.at);
+  return typename Pack<T, 2>::type{row[l.at], row[l.next]};
+}
+template <bool EVEN, typename T>
+__device__ __forceinline__ void store_two(T* row, const Lane& l, const float v[2]) {
+  if (EVEN) {
+    if (l.n > 0) *reinterpret_cast<typename Pack<T, 2>::load*>(row + l.col) = {from_f32<T>(v[0]), from_f32<T>(v[1])};
+    return;
+  }
+  if (l.n > 0) row[l.col] = from_f32<T>(v[0]);
+  if (l.n > 1) row[l.col + 1] = from_f32<T>(v[1]);
+}
+template <bool EVEN>
+__device__ __forceinline__ Pair load_pair(const float* row, const Lane& l) {
+  const typename Pack<float, 2>::type v = load_two<EVEN>(row, l);
+  return {{v[0], v[1]}};
 }
 
-__device__ __forceinline__ Pair load_state(const RecurArgs& a, const float* states, int s, int col, int n) {
+template <bool EVEN>
+__device__ __forceinline__ Pair load_state(const RecurArgs& a, const float* states, int s, const Lane& l) {
   if (!states) return {{0.0f, 0.0f}};
-  return load_pair(states + static_cast<int64_t>(s) * a.units + col, n);
+  return load_pair<EVEN>(states + static_cast<int64_t>(s) * a.units, l);
 }
 
 // A row range as a map of what comes in, two units: v -> A v + H, or H alone
@@ -129,336 +166,345 @@ __device__ __forceinline__ void span_then(Span& s, const Span& next) {  // s, th
   }
   s.cut |= next.cut;
 }
-// The spans of a step's waves.
+// Spans in LDS, and which of them are cut.
+template <int N>
 struct Spans {
-  float4 v[kWaves][64];
-  int cut[kWaves];
-  __device__ __forceinline__ void put(int wave, int lane, const Span& s) {
-    v[wave][lane] = make_float4(s.A[0], s.A[1], s.H[0], s.H[1]);
-    if (lane == 0) cut[wave] = s.cut;
+  float4 v[N][64];
+  int cut[N];
+  __device__ __forceinline__ void put(int i, int lane, const Span& s) {
+    v[i][lane] = make_float4(s.A[0], s.A[1], s.H[0], s.H[1]);
+    if (lane == 0) cut[i] = s.cut;
   }
-  __device__ __forceinline__ Span get(int wave, int lane) const {
-    const float4 f = v[wave][lane];
-    return {{f.x, f.y}, {f.z, f.w}, __builtin_amdgcn_readfirstlane(cut[wave]) != 0};
-  }
-  __device__ __forceinline__ void pass(int wave, int lane, Pair& in) const {
-    const Span s = get(wave, lane);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) in.v[j] = s.cut ? s.H[j] : __builtin_fmaf(s.A[j], in.v[j], s.H[j]);
+  // The first `count`, one after another (what lies before the last cut counts
+  // for nothing).
+  __device__ __forceinline__ Span fold(int count, int lane) const {
+    const uint64_t cuts = __ballot(lane < count && cut[lane < N ? lane : 0] != 0);
+    Span s = span_none();
+    int i = 0;
+    if (cuts) {
+      i = 63 - __builtin_clzll(cuts);
+      const float4 f = v[i++][lane];
+      s = {{0.0f, 0.0f}, {f.z, f.w}, true};
+    }
+    for (; i < count; ++i) {
+      const float4 f = v[i][lane];
+      s.H[0] = __builtin_fmaf(f.x, s.H[0], f.z), s.H[1] = __builtin_fmaf(f.y, s.H[1], f.w);
+      s.A[0] *= f.x, s.A[1] *= f.y;
+    }
+    return s;
   }
 };
-
-// A part's span in memory: A, H, and cut (as a float) for each unit.
-__device__ __forceinline__ void store_span(const RecurArgs& a, int64_t part, int col, int n, const Span& s) {
-  float* out = a.sums + part * 3 * a.units + col;
-  const float cut[2] = {s.cut ? 1.0f : 0.0f, s.cut ? 1.0f : 0.0f};
-  store_pair(out, n, s.A);
-  store_pair(out + a.units, n, s.H);
-  store_pair(out + 2 * a.units, n, cut);
+__device__ __forceinline__ void span_into(const Span& s, Pair& in) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) in.v[j] = s.cut ? s.H[j] : __builtin_fmaf(s.A[j], in.v[j], s.H[j]);
 }
 
-// The parts before (or, backwards, behind) part p summed up to what comes into
-// it: over the waves, then over LDS.
-template <bool BACK>
-__device__ __forceinline__ Pair into_part(const RecurArgs& a, int64_t p, int64_t parts, int col, int n, Spans& spans) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t count = BACK ? parts - 1 - p : p, per = div_up(count, kWaves);
-  Span s = span_none();
-  for (int64_t i = wave * per; i < (wave + 1) * per && i < count; ++i) {
-    const float* q = a.sums + (BACK ? parts - 1 - i : i) * 3 * a.units;
-    const Pair A = load_pair(q + col, n), H = load_pair(q + a.units + col, n);
-    // (the first unit's: a slab's first column is there)
-    const bool cut = __builtin_amdgcn_readfirstlane(__float_as_int(q[2 * a.units + blockIdx.x * kSlab])) != 0;
-    span_then(s, {{A.v[0], A.v[1]}, {H.v[0], H.v[1]}, cut});
+// A unit's span as a word that is not 0: H above, A (never below 0) with its
+// sign set, or all ones for a cut. The word is its own flag: words go to memory
+// and from there past the caches that the chip's parts have to themselves.
+constexpr uint32_t kReady = 0x80000000u, kCut = 0xFFFFFFFFu;
+__device__ __forceinline__ void put_word(uint64_t* p, float h, uint32_t low) {
+  __hip_atomic_store(p, static_cast<uint64_t>(__float_as_uint(h)) << 32 | low, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint32_t span_low(float A, bool cut) {
+  if (cut) return kCut;
+  return A != A ? 0xFFC00000u : __float_as_uint(A) | kReady;
+}
+// A lane's two words, when all lanes' are there. (Some 2^20 polls of half a
+// microsecond and more, and then NaN.)
+__device__ __forceinline__ void wait_words(const uint64_t* row, const Lane& l, uint64_t w[2]) {
+#pragma unroll 1
+  for (int tries = 0; tries < 1 << 20; ++tries) {
+    w[0] = __hip_atomic_load(row + l.at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    w[1] = __hip_atomic_load(row + l.next, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__all((w[0] & w[1] & kReady) != 0)) return;
+    __builtin_amdgcn_s_sleep(1);
   }
-  spans.put(wave, lane, s);
+  w[0] = w[1] = uint64_t{0x7FC00000u} << 32 | 0xFFC00000u;
+}
+
+// What the waves of a workgroup share.
+struct Shared {
+  Spans<kWaves> waves;  // of the tile's waves
+  Spans<kGroup> tiles;  // of the tiles before it in its group
+  float2 into[64];     // what comes into the group
+  unsigned number;
+};
+// What comes into the tile that is walked as the `at`-th. Its span goes out (by
+// the last wave, `own` the wave's, `s` of the waves before it); the others wait
+// for the tiles before it, the last one for what comes into the group.
+__device__ __forceinline__ Pair into_tile(const RecurArgs& a, int64_t at, const Lane& l, int wave, const Span& s,
+                                          const Span& own, Shared& sh) {
+  const int lane = threadIdx.x & 63, place = static_cast<int>(at % kGroup);
+  const int64_t group = at / kGroup;
+  const bool last = wave == kWaves - 1, more = at + 1 < a.tiles;
+  Span whole = s;
+  if (last) {
+    span_then(whole, own);
+    if (more && place < kGroup - 1) {
+      uint64_t* out = a.spans + at * a.units;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (j < l.n) put_word(out + (l.col + j), whole.H[j], span_low(whole.A[j], whole.cut));
+    }
+    Pair in = {{0.0f, 0.0f}};
+    if (group > 0) {
+      uint64_t w[2];
+      wait_words(a.carries + (group - 1) * a.units, l, w);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) in.v[j] = __uint_as_float(static_cast<uint32_t>(w[j] >> 32));
+    }
+    sh.into[lane] = make_float2(in.v[0], in.v[1]);
+  }
+  for (int i = last ? place : wave; i < place; i += kWaves - 1) {
+    uint64_t w[2];
+    wait_words(a.spans + (at - place + i) * a.units, l, w);
+    Span tile;
+    tile.cut = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(w[0])) == kCut;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      tile.A[j] = __uint_as_float(static_cast<uint32_t>(w[j]) & ~kReady);
+      tile.H[j] = __uint_as_float(static_cast<uint32_t>(w[j] >> 32));
+    }
+    sh.tiles.put(i, lane, tile);
+  }
   __syncthreads();
-  Pair in = {{0.0f, 0.0f}};
-#pragma unroll 4
-  for (int w = 0; w < kWaves; ++w) spans.pass(w, lane, in);
-  __syncthreads();
+  Pair in = {{sh.into[lane].x, sh.into[lane].y}};
+  span_into(sh.tiles.fold(place, lane), in);
+  if (last && more && place == kGroup - 1) {
+    uint64_t* out = a.carries + group * a.units;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (j < l.n)
+        put_word(out + (l.col + j), whole.cut ? whole.H[j] : __builtin_fmaf(whole.A[j], in.v[j], whole.H[j]), kReady);
+  }
   return in;
 }
 
-// One row forwards: A and H as its map, from its z and x; `first` has the
-// sequence's state put in.
-__device__ __forceinline__ void row_forward(const RecurArgs& a, int q, bool first, int col, int n, float A[2],
-                                            float H[2]) {
-  if (q < 0) {
-    H[0] = H[1] = 0.0f;
-  } else if (first) {
-    const Pair in = load_state(a, a.state, q, col, n);
+// Whether no sequence begins or ends in a wave's rows, and all are of one: then
+// they are walked without looking.
+template <int N>
+__device__ __forceinline__ bool unbroken(const int (&of)[N]) {
+  bool same = of[0] >= 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) H[j] = __builtin_fmaf(A[j], in.v[j], H[j]);
-  }
+  for (int i = 0; i < N - 1; ++i) same &= of[i] == of[i + 1];
+  return same;
 }
 
-// Forwards: each part (but the last) as a span; a wave's rows lie behind each
-// other.
-template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void k_recur_parts(RecurArgs a) {
-  __shared__ Spans spans;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = blockIdx.x * kSlab + lane * 2, n = a.units - col;
-  const int64_t part = blockIdx.y, per = a.part / kWaves, begin = part * a.part + wave * per;
+// A wave's rows forwards, from their A and H: rows at which a sequence starts
+// get its state put into H.
+template <bool EVEN, int N>
+__device__ __forceinline__ Span sum_up(const RecurArgs& a, const int (&of)[N + 2], const Lane& l,
+                                       const float (&A)[N][2], float (&H)[N][2]) {
   Span s = span_none();
-  const T* xz = static_cast<const T*>(a.xz) + col;
-  for (int64_t t = begin; t < begin + per; t += kRows) {
-    int of[kRows + 2];
-    rows_of<kRows>(a, t, of);
-    typename Pack<T, 2>::type x[kRows], z[kRows];
+  if (unbroken(of)) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const bool there = t + i < a.tokens;
-      const T* row = xz + (there ? t + i : 0) * a.line;
-      x[i] = load_pack<2>(row, there ? n : 0), z[i] = load_pack<2>(row + a.units, there ? n : 0);
-    }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      Span row;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float b;
-        gate(to_f32(z[i][j]), row.A[j], b);
-        row.H[j] = b * to_f32(x[i][j]);
-      }
-      const int q = of[i + 1];
-      row.cut = q < 0 || of[i] != q;
-      row_forward(a, q, row.cut, col, n, row.A, row.H);
-      span_then(s, row);
-    }
+    for (int i = 0; i < N; ++i) span_then(s, {{A[i][0], A[i][1]}, {H[i][0], H[i][1]}, false});
+    return s;
   }
-  spans.put(wave, lane, s);
-  __syncthreads();
-  if (wave) return;
-  for (int w = 1; w < kWaves; ++w) span_then(s, spans.get(w, lane));
-  store_span(a, part, col, n, s);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int q = of[i + 1];
+    const bool cut = q < 0 || of[i] != q;
+    if (q < 0) {
+      H[i][0] = H[i][1] = 0.0f;
+    } else if (cut) {
+      const Pair in = load_state<EVEN>(a, a.state, q, l);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) H[i][j] = __builtin_fmaf(A[i][j], in.v[j], H[i][j]);
+    }
+    span_then(s, {{A[i][0], A[i][1]}, {H[i][0], H[i][1]}, cut});
+  }
+  return s;
 }
 
 // Sequences without rows: out = in (null: zeros), 64 of them at a time by the
 // waves of a slab's workgroups.
-__device__ __forceinline__ void pass_empty(const RecurArgs& a, const float* in, float* out, int col, int n) {
-  const int lane = threadIdx.x & 63;
+template <bool EVEN>
+__device__ __forceinline__ void pass_empty(const RecurArgs& a, int64_t tile, const float* in, float* out,
+                                           const Lane& l) {
   if (!a.starts && a.tokens > 0) return;
-  for (int64_t first = (static_cast<int64_t>(blockIdx.y) * kWaves + (threadIdx.x >> 6)) * 64; first < a.sequences;
-       first += static_cast<int64_t>(gridDim.y) * kWaves * 64) {
-    const int64_t s = first + lane;
+  const int64_t all = a.tiles > 0 ? a.tiles : 1;
+  for (int64_t first = (tile * kWaves + (threadIdx.x >> 6)) * 64; first < a.sequences; first += all * kWaves * 64) {
+    const int64_t s = first + (threadIdx.x & 63);
     const bool empty = s < a.sequences && (!a.starts || start_of(a, s) >= start_of(a, s + 1));
     for (uint64_t mask = __ballot(empty); mask; mask &= mask - 1) {
-      const int64_t at = (first + __builtin_ctzll(mask)) * a.units + col;
-      const Pair v = in ? load_pair(in + at, n) : Pair{{0.0f, 0.0f}};
-      store_pair(out + at, n, v.v);
+      const int at = static_cast<int>(first + __builtin_ctzll(mask));
+      store_two<EVEN>(out + static_cast<int64_t>(at) * a.units, l, load_state<EVEN>(a, in, at, l).v);
     }
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void k_recur(RecurArgs a) {
-  __shared__ Spans spans[2];
+// The workgroup's number in the order in which they are taken.
+__device__ __forceinline__ unsigned take(const RecurArgs& a, unsigned* shared) {
+  if (a.tiles <= 1) return blockIdx.x;
+  if (threadIdx.x == 0)
+    *shared = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(*shared);
+}
+
+template <typename T, bool EVEN>
+__global__ __launch_bounds__(64 * kWaves, 4) void k_recur(RecurArgs a) {
+  __shared__ Shared sh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = blockIdx.x * kSlab + lane * 2, n = a.units - col;
-  const int64_t part = blockIdx.y, begin = part * a.part;
-  const int64_t end = begin + a.part < a.tokens ? begin + a.part : a.tokens;
-  const T* xz = static_cast<const T*>(a.xz) + col;
-  T* out = static_cast<T*>(a.h) + col;
-  Pair in = {{0.0f, 0.0f}};
-  if (part > 0) in = into_part<false>(a, part, gridDim.y, col, n, spans[0]);
-  int slot = 0;
-  for (int64_t step = begin; step < end; step += kStep) {
-    const int64_t t = step + wave * kRows;
-    int of[kRows + 2];
-    rows_of<kRows>(a, t, of);
-    typename Pack<T, 2>::type x[kRows], z[kRows];
+  const unsigned taken = take(a, &sh.number), slabs = a.slabs;
+  const int64_t tile = taken / slabs, t = (tile * kWaves + wave) * kForth;
+  const Lane l = lane_of(taken % slabs * kSlab, a.units);
+  int of[kForth + 2];
+  float A[kForth][2], H[kForth][2];
+  if (a.tokens > 0) {
+    typename Pack<T, 2>::type x[kForth], z[kForth];
+    const int64_t first = t < a.tokens ? t : 0, rows = a.tokens - t;
+    const T* xz = static_cast<const T*>(a.xz) + first * a.line;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const bool there = t + i < a.tokens;
-      const T* row = xz + (there ? t + i : 0) * a.line;
-      x[i] = load_pack<2>(row, there ? n : 0), z[i] = load_pack<2>(row + a.units, there ? n : 0);
+    for (int i = 0; i < kForth; ++i) {
+      const T* row = xz + (i < rows ? i * a.line : 0);
+      x[i] = load_two<EVEN>(row, l), z[i] = load_two<EVEN>(row + a.units, l);
     }
-    float A[kRows][2], H[kRows][2];
-    Span s = span_none();
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < kForth; ++i) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float b;
         gate(to_f32(z[i][j]), A[i][j], b);
         H[i][j] = b * to_f32(x[i][j]);
       }
-      const int q = of[i + 1];
-      const bool cut = q < 0 || of[i] != q;
-      row_forward(a, q, cut, col, n, A[i], H[i]);
-      span_then(s, {{A[i][0], A[i][1]}, {H[i][0], H[i][1]}, cut});
     }
-    spans[slot].put(wave, lane, s);
-    __syncthreads();
-    Pair h = in;
-#pragma unroll 4
-    for (int w = 0; w < kWaves; ++w) {
-      if (w == wave) h = in;
-      spans[slot].pass(w, lane, in);
-    }
-    slot ^= 1;
-    if (t % kKeep == 0 && t < end) store_pair(a.kept + t / kKeep * a.units + col, n, h.v);
+  }
+  rows_of(a, t, of);
+  const Span own = sum_up<EVEN, kForth>(a, of, l, A, H);
+  sh.waves.put(wave, lane, own);
+  __syncthreads();
+  const Span s = sh.waves.fold(wave, lane);  // the waves before
+  Pair h = into_tile(a, tile, l, wave, s, own, sh);
+  span_into(s, h);
+  if (t % kKeep == 0 && t < a.tokens) store_two<EVEN>(a.kept + t / kKeep * a.units, l, h.v);
+  T* out = static_cast<T*>(a.h) + t * a.units;
+  if (unbroken(of)) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      if (t + i >= end) break;
+    for (int i = 0; i < kForth; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) h.v[j] = __builtin_fmaf(A[i][j], h.v[j], H[i][j]);
+      store_two<EVEN>(out + i * a.units, l, h.v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kForth; ++i) {
+      if (t + i >= a.tokens) continue;
       const int q = of[i + 1];
       const bool cut = q < 0 || of[i] != q;
 #pragma unroll
       for (int j = 0; j < 2; ++j) h.v[j] = cut ? H[i][j] : __builtin_fmaf(A[i][j], h.v[j], H[i][j]);
-      store_pack<2>(out + (t + i) * a.units, n, h.v);
-      if (q >= 0 && of[i + 2] != q) store_pair(a.last + static_cast<int64_t>(q) * a.units + col, n, h.v);
+      store_two<EVEN>(out + i * a.units, l, h.v);
+      if (q >= 0 && of[i + 2] != q) store_two<EVEN>(a.last + static_cast<int64_t>(q) * a.units, l, h.v);
     }
   }
-  pass_empty(a, a.state, a.last, col, n);
+  pass_empty<EVEN>(a, tile, a.state, a.last, l);
 }
 
-// Backwards, a row passes on what comes in from behind as u -> a (g + u); a
-// sequence's last row puts its last state's gradient in, its first row's goes
-// to its state and no further.
-template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void k_recur_grad_parts(RecurArgs a) {
-  __shared__ Spans spans;
+// The gradients, tiles from the last to the first. Backwards, a row passes on
+// what comes in from behind as u -> a (g + u); a sequence's last row puts its
+// last state's gradient in, its first row's goes to its state and no further.
+// h is walked again from what came into the tile, so that it is neither kept
+// nor rounded.
+template <typename T, bool EVEN>
+__global__ __launch_bounds__(64 * kWaves, 4) void k_recur_grad(RecurArgs a) {
+  __shared__ Shared sh;
+  __shared__ Spans<kWaves> forth;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = blockIdx.x * kSlab + lane * 2, n = a.units - col;
-  const int64_t part = blockIdx.y + 1, per = a.part / kWaves, begin = part * a.part + wave * per;
-  Span s = span_none();
-  const T* zs = static_cast<const T*>(a.xz) + a.units + col;
-  const T* gs = static_cast<const T*>(a.g) + col;
-  for (int64_t t = begin + per - kRows; t >= begin; t -= kRows) {
-    int of[kRows + 2];
-    rows_of<kRows>(a, t, of);
-    typename Pack<T, 2>::type z[kRows], g[kRows];
+  const unsigned taken = take(a, &sh.number), slabs = a.slabs;
+  const int64_t at = taken / slabs, tile = a.tiles > 0 ? a.tiles - 1 - at : 0, t = (tile * kWaves + wave) * kBack;
+  const Lane l = lane_of(taken % slabs * kSlab, a.units);
+  int of[kBack + 2];
+  typename Pack<T, 2>::type x[kBack], g[kBack];
+  float A[kBack][2], B[kBack][2];  // the gates
+  Pair h = {{0.0f, 0.0f}};
+  if (a.tokens > 0) {
+    typename Pack<T, 2>::type z[kBack];
+    const int64_t first = t < a.tokens ? t : 0, rows = a.tokens - t;
+    const T* xz = static_cast<const T*>(a.xz) + first * a.line;
+    const T* gs = static_cast<const T*>(a.g) + first * a.g_line;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const bool there = t + i < a.tokens;
-      z[i] = load_pack<2>(zs + (there ? t + i : 0) * a.line, there ? n : 0);
-      g[i] = load_pack<2>(gs + (there ? t + i : 0) * a.g_line, there ? n : 0);
+    for (int i = 0; i < kBack; ++i) {
+      const T* row = xz + (i < rows ? i * a.line : 0);
+      x[i] = load_two<EVEN>(row, l), z[i] = load_two<EVEN>(row + a.units, l);
+      g[i] = load_two<EVEN>(gs + (i < rows ? i * a.g_line : 0), l);
     }
+    h = load_pair<EVEN>(a.kept + tile * a.units, l);
 #pragma unroll
-    for (int i = kRows - 1; i >= 0; --i) {
-      const int q = of[i + 1];
-      const bool on = q >= 0 && of[i] == q, last = of[i + 2] != q;
-      const Pair more = on && last ? load_state(a, a.g_last, q, col, n) : Pair{{0.0f, 0.0f}};
-      Span row;
+    for (int i = 0; i < kBack; ++i) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float b;
-        gate(to_f32(z[i][j]), row.A[j], b);
-        row.H[j] = on ? row.A[j] * (to_f32(g[i][j]) + more.v[j]) : 0.0f;
-      }
-      row.cut = !on || last;
-      span_then(s, row);
+      for (int j = 0; j < 2; ++j) gate(to_f32(z[i][j]), A[i][j], B[i][j]);
     }
   }
-  spans.put(wave, lane, s);
+  rows_of(a, t, of);
+  const bool whole = unbroken(of);
+  Span u = span_none();
+  {
+    float H[kBack][2];
+#pragma unroll
+    for (int i = 0; i < kBack; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) H[i][j] = B[i][j] * to_f32(x[i][j]);
+    forth.put(wave, lane, sum_up<EVEN, kBack>(a, of, l, A, H));
+  }
+#pragma unroll
+  for (int i = kBack - 1; i >= 0; --i) {
+    const int q = of[i + 1];
+    const bool on = whole || (q >= 0 && of[i] == q), last = !whole && of[i + 2] != q;
+    Pair more = {{0.0f, 0.0f}};
+    if (on && last) more = load_state<EVEN>(a, a.g_last, q, l);
+    Span row;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      row.A[j] = A[i][j];
+      row.H[j] = on ? A[i][j] * (to_f32(g[i][j]) + more.v[j]) : 0.0f;
+    }
+    row.cut = !on || last;
+    span_then(u, row);
+  }
+  const int back = kWaves - 1 - wave;  // waves backwards
+  sh.waves.put(back, lane, u);
   __syncthreads();
-  if (wave < kWaves - 1) return;
-  for (int w = kWaves - 2; w >= 0; --w) span_then(s, spans.get(w, lane));
-  store_span(a, part, col, n, s);
-}
-
-// The gradients, steps from the last to the first. h is walked again from what
-// came into the step, so that it is neither kept nor rounded.
-template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void k_recur_grad(RecurArgs a) {
-  __shared__ Spans spans[2], backs[2];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = blockIdx.x * kSlab + lane * 2, n = a.units - col;
-  const int64_t part = blockIdx.y, begin = part * a.part;
-  const int64_t end = begin + a.part < a.tokens ? begin + a.part : a.tokens;
-  const T* xz = static_cast<const T*>(a.xz) + col;
-  const T* gs = static_cast<const T*>(a.g) + col;
-  T* out = static_cast<T*>(a.dxz) + col;
-  Pair back = {{0.0f, 0.0f}};
-  if (part + 1 < gridDim.y) back = into_part<true>(a, part, gridDim.y, col, n, spans[0]);
-  int slot = 0;
-  for (int64_t step = begin + (div_up(end - begin, kKeep) - 1) * kKeep; step >= begin; step -= kKeep) {
-    const int64_t t = step + wave * kBack;
-    int of[kBack + 2];
-    rows_of<kBack>(a, t, of);
-    typename Pack<T, 2>::type x[kBack], z[kBack], g[kBack];
+  const Span s = sh.waves.fold(back, lane);  // the waves behind
+  Pair c = into_tile(a, at, l, back, s, u, sh);
+  span_into(s, c);
+  span_into(forth.fold(wave, lane), h);
+  float before[kBack][2];  // h of the row before
 #pragma unroll
-    for (int i = 0; i < kBack; ++i) {
-      const bool there = t + i < a.tokens;
-      const T* row = xz + (there ? t + i : 0) * a.line;
-      x[i] = load_pack<2>(row, there ? n : 0), z[i] = load_pack<2>(row + a.units, there ? n : 0);
-      g[i] = load_pack<2>(gs + (there ? t + i : 0) * a.g_line, there ? n : 0);
-    }
-    Pair h = load_pair(a.kept + step / kKeep * a.units + col, n);
-    float A[kBack][2], B[kBack][2], d[kBack][2];  // d: g, with the last state's gradient at a last row
-    Span s = span_none(), u = span_none();
+  for (int i = 0; i < kBack; ++i) {
+    const int q = of[i + 1];
+    if (!whole && of[i] != q) h = q >= 0 ? load_state<EVEN>(a, a.state, q, l) : Pair{{0.0f, 0.0f}};
 #pragma unroll
-    for (int i = 0; i < kBack; ++i) {
-      const int q = of[i + 1];
-      Span row;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        gate(to_f32(z[i][j]), A[i][j], B[i][j]);
-        row.A[j] = A[i][j], row.H[j] = B[i][j] * to_f32(x[i][j]);
-      }
-      row.cut = q < 0 || of[i] != q;
-      row_forward(a, q, row.cut, col, n, row.A, row.H);
-      span_then(s, row);
-    }
-#pragma unroll
-    for (int i = kBack - 1; i >= 0; --i) {
-      const int q = of[i + 1];
-      const bool on = q >= 0 && of[i] == q, last = of[i + 2] != q;
-      const Pair more = q >= 0 && last ? load_state(a, a.g_last, q, col, n) : Pair{{0.0f, 0.0f}};
-      Span row;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        d[i][j] = to_f32(g[i][j]) + more.v[j];
-        row.A[j] = A[i][j], row.H[j] = on ? A[i][j] * d[i][j] : 0.0f;
-      }
-      row.cut = !on || last;
-      span_then(u, row);
-    }
-    spans[slot].put(wave, lane, s);
-    backs[slot].put(wave, lane, u);
-    __syncthreads();
-    Pair c = back;
-    for (int w = 0; w < wave; ++w) spans[slot].pass(w, lane, h);
-#pragma unroll 4
-    for (int w = kWaves - 1; w >= 0; --w) {
-      if (w == wave) c = back;
-      backs[slot].pass(w, lane, back);
-    }
-    slot ^= 1;
-    float before[kBack][2];  // h of the row before
-#pragma unroll
-    for (int i = 0; i < kBack; ++i) {
-      const int q = of[i + 1];
-      if (of[i] != q) h = q >= 0 ? load_state(a, a.state, q, col, n) : Pair{{0.0f, 0.0f}};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        before[i][j] = h.v[j];
-        h.v[j] = __builtin_fmaf(A[i][j], h.v[j], B[i][j] * to_f32(x[i][j]));
-      }
-    }
-#pragma unroll
-    for (int i = kBack - 1; i >= 0; --i) {
-      if (t + i >= end) continue;
-      const int q = of[i + 1];
-      float dx[2] = {0.0f, 0.0f}, dz[2] = {0.0f, 0.0f};
-      if (q >= 0) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float v = of[i + 2] != q ? d[i][j] : d[i][j] + c.v[j];
-          dx[j] = B[i][j] * v;
-          dz[j] = dx[j] * A[i][j] * (before[i][j] - to_f32(x[i][j]));
-          c.v[j] = A[i][j] * v;
-        }
-        if (of[i] != q) store_pair(a.dstate + static_cast<int64_t>(q) * a.units + col, n, c.v);
-      }
-      T* row = out + (t + i) * 2 * a.units;
-      store_pack<2>(row, n, dx);
-      store_pack<2>(row + a.units, n, dz);
+    for (int j = 0; j < 2; ++j) {
+      before[i][j] = h.v[j];
+      h.v[j] = __builtin_fmaf(A[i][j], h.v[j], B[i][j] * to_f32(x[i][j]));
     }
   }
-  pass_empty(a, a.g_last, a.dstate, col, n);
+  T* out = static_cast<T*>(a.dxz) + t * 2 * a.units;
+#pragma unroll
+  for (int i = kBack - 1; i >= 0; --i) {
+    if (t + i >= a.tokens) continue;
+    const int q = of[i + 1];
+    float dx[2] = {0.0f, 0.0f}, dz[2] = {0.0f, 0.0f};
+    if (whole || q >= 0) {
+      if (!whole && of[i + 2] != q) c = load_state<EVEN>(a, a.g_last, q, l);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float v = to_f32(g[i][j]) + c.v[j];
+        dx[j] = B[i][j] * v;
+        c.v[j] = A[i][j] * v;
+        dz[j] = B[i][j] * c.v[j] * (before[i][j] - to_f32(x[i][j]));
+      }
+      if (!whole && of[i] != q) store_two<EVEN>(a.dstate + static_cast<int64_t>(q) * a.units, l, c.v);
+    }
+    T* row = out + i * 2 * a.units;
+    store_two<EVEN>(row, l, dx);
+    store_two<EVEN>(row + a.units, l, dz);
+  }
+  pass_empty<EVEN>(a, at, a.g_last, a.dstate, l);
 }
 
 // One row a sequence, the state in place; a lane takes 4 units.
@@ -484,46 +530,40 @@ __global__ __launch_bounds__(256) void k_recur_step(int64_t sequences, int units
   }
 }
 
-// How the rows are cut: two workgroups a CU, parts of whole steps, few enough
-// that what comes into one is soon summed up.
 struct RecurPlan {
-  int64_t slabs, parts, part, steps, of, bytes;
+  int64_t tiles, slabs, spans, carries, words, bytes;  // words of 8 bytes, then the rows' sequences
 };
-constexpr int64_t kMaxParts = 128;
-RecurPlan recur_plan(int64_t tokens, int64_t units, bool ragged) {
+RecurPlan recur_plan(int64_t tokens, int64_t units, bool ragged, int rows) {
   RecurPlan p{};
-  p.slabs = div_up(units, kSlab);
-  p.steps = div_up(tokens, kStep);
-  int64_t parts = 2 * cu_count() / p.slabs;
-  parts = parts < kMaxParts ? parts : kMaxParts;
-  parts = parts < p.steps ? parts : p.steps;
-  parts = parts > 1 ? parts : 1;
-  p.part = div_up(p.steps, parts) * kStep;
-  p.part = p.part > 0 ? p.part : kStep;
-  p.parts = tokens > 0 ? div_up(tokens, p.part) : 1;
-  p.of = p.parts > 1 ? div_up(12 * p.parts * units, 16) * 16 : 0;
-  p.bytes = p.of + (ragged ? 4 * tokens : 0);
+  p.tiles = div_up(tokens, kWaves * rows), p.slabs = div_up(units, kSlab);
+  if (p.tiles > 1) {  // (the ticket comes first)
+    p.spans = 1;
+    p.carries = p.spans + p.tiles * units;
+    p.words = p.carries + p.tiles / kGroup * units;
+  }
+  p.bytes = 8 * p.words + (ragged ? 4 * tokens : 0);
   return p;
 }
 
+constexpr int64_t kMaxWork = int64_t{1} << 22;  // workgroups of a launch: at most 2^31 lanes
 bool recur_fits(int64_t tokens, int64_t units, int64_t sequences, int wide) {
   return batch_fits(tokens, units) && units <= kMaxLevel / 2 && sequences >= 0 && sequences <= kMaxSequences &&
-         (wide == 0 || wide == 1);
-}
-int64_t recur_bytes(int64_t tokens, int64_t units, int64_t sequences, bool ragged) {
-  if (units == 0 || (tokens == 0 && sequences == 0)) return 0;
-  return recur_plan(tokens, units, ragged).bytes;
+         (wide == 0 || wide == 1) && div_up(tokens, kKeep) * div_up(units, kSlab) <= kMaxWork;
 }
 
-// The plan into the arguments, and the rows' sequences.
+// The plan into the arguments, the rows' sequences and the words' zeros.
 void recur_setup(RecurArgs& a, const RecurPlan& p, void* workspace, hipStream_t s) {
-  a.part = p.part;
-  a.sums = static_cast<float*>(workspace);
-  if (!a.starts || a.tokens == 0) return;
-  int* of = reinterpret_cast<int*>(static_cast<char*>(workspace) + p.of);
+  uint64_t* words = static_cast<uint64_t*>(workspace);
+  a.tiles = p.tiles, a.slabs = static_cast<int>(p.slabs);
+  a.ticket = reinterpret_cast<unsigned*>(words), a.spans = words + p.spans, a.carries = words + p.carries;
+  int* of = a.starts && a.tokens > 0 ? reinterpret_cast<int*>(words + p.words) : nullptr;
   a.of = of;
-  k_recur_rows<<<static_cast<unsigned>(div_up(a.tokens, 256)), 256, 0, s>>>(a, of);
+  const int64_t rows = of ? a.tokens : 0, lanes = p.words > rows ? p.words : rows;
+  if (lanes == 0) return;
+  const int64_t groups = div_up(lanes, 256), most = int64_t{1} << 16;
+  k_recur_setup<<<static_cast<unsigned>(groups < most ? groups : most), 256, 0, s>>>(a, of, words, p.words);
 }
+unsigned recur_groups(const RecurPlan& p) { return static_cast<unsigned>((p.tiles > 0 ? p.tiles : 1) * p.slabs); }
 
 }  // namespace
 
@@ -531,7 +571,8 @@ extern "C" {
 
 int64_t plx_recur_workspace(int64_t tokens, int64_t units, int64_t sequences, int32_t ragged) {
   if (!recur_fits(tokens, units, sequences, 0)) return -1;
-  return recur_bytes(tokens, units, sequences, ragged != 0);
+  if (units == 0 || (tokens == 0 && sequences == 0)) return 0;
+  return recur_plan(tokens, units, ragged != 0, kBack).bytes;  // (the gradients' is the larger)
 }
 
 int plx_recur(int64_t tokens, int64_t units, int64_t sequences, int32_t dtype, const void* xz, int64_t line,
@@ -543,7 +584,7 @@ int plx_recur(int64_t tokens, int64_t units, int64_t sequences, int32_t dtype, c
   if (!starts && sequences != 1) return fail(PLX_ERR_INVALID, who);
   if (units == 0 || (tokens == 0 && sequences == 0)) return PLX_OK;
   if ((tokens > 0 && (!xz || !h || !kept)) || (sequences > 0 && !last)) return fail(PLX_ERR_INVALID, who);
-  const RecurPlan p = recur_plan(tokens, units, starts != nullptr);
+  const RecurPlan p = recur_plan(tokens, units, starts != nullptr, kForth);
   if (p.bytes > 0 && (!workspace || !on_16(workspace) || workspace_bytes < p.bytes))
     return fail(PLX_ERR_INVALID, "plx_recur: plx_recur_workspace() bytes on 16 bytes needed");
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -553,9 +594,10 @@ int plx_recur(int64_t tokens, int64_t units, int64_t sequences, int32_t dtype, c
   recur_setup(a, p, workspace, s);
   with_type(dtype, [&](auto* e) {
     using T = PLX_DENSE_TYPE(e);
-    const unsigned slabs = static_cast<unsigned>(p.slabs), parts = static_cast<unsigned>(p.parts);
-    if (parts > 1) k_recur_parts<T><<<dim3(slabs, parts - 1), 64 * kWaves, 0, s>>>(a);
-    k_recur<T><<<dim3(slabs, parts), 64 * kWaves, 0, s>>>(a);
+    if (units % 2)
+      k_recur<T, false><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
+    else
+      k_recur<T, true><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
   });
   return check_launch("plx_recur");
 }
@@ -570,7 +612,7 @@ int plx_recur_grad(int64_t tokens, int64_t units, int64_t sequences, int32_t dty
   if (!starts && sequences != 1) return fail(PLX_ERR_INVALID, who);
   if (units == 0 || (tokens == 0 && sequences == 0)) return PLX_OK;
   if ((tokens > 0 && (!xz || !g || !kept || !dxz)) || (sequences > 0 && !dstate)) return fail(PLX_ERR_INVALID, who);
-  const RecurPlan p = recur_plan(tokens, units, starts != nullptr);
+  const RecurPlan p = recur_plan(tokens, units, starts != nullptr, kBack);
   if (p.bytes > 0 && (!workspace || !on_16(workspace) || workspace_bytes < p.bytes))
     return fail(PLX_ERR_INVALID, "plx_recur_grad: plx_recur_workspace() bytes on 16 bytes needed");
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -581,9 +623,10 @@ int plx_recur_grad(int64_t tokens, int64_t units, int64_t sequences, int32_t dty
   recur_setup(a, p, workspace, s);
   with_type(dtype, [&](auto* e) {
     using T = PLX_DENSE_TYPE(e);
-    const unsigned slabs = static_cast<unsigned>(p.slabs), parts = static_cast<unsigned>(p.parts);
-    if (parts > 1) k_recur_grad_parts<T><<<dim3(slabs, parts - 1), 64 * kWaves, 0, s>>>(a);
-    k_recur_grad<T><<<dim3(slabs, parts), 64 * kWaves, 0, s>>>(a);
+    if (units % 2)
+      k_recur_grad<T, false><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
+    else
+      k_recur_grad<T, true><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
   });
   return check_launch("plx_recur_grad");
 }
