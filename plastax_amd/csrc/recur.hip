@@ -11,11 +11,12 @@
 // in is known. A workgroup takes a tile, a few rows a wave of kSlab units, into
 // its registers, two units a lane; its waves' sums meet in LDS, the
 // tiles' in memory, and each wave walks its rows again from what comes in: xz
-// is read once. Tiles are taken in the order of a counter, and wait for
+// is read once. Tiles are taken in the order of a counter (a slab's), and wait for
 // earlier ones only, which are under way: every wait ends (and is bounded, for
 // a caller who has two calls share a workspace). A tile waits for the sums of
-// the tiles before it in its group, and for what comes into the group, so that
-// a long sequence is a chain of groups; every sum has one order.
+// the tiles before it in its group of 8, for those of the groups before in the
+// row of 8 groups, and for what comes into the row: a long sequence is a chain
+// of rows of 64 tiles (a link takes some 3 us), and every sum has one order.
 
 #include "px_dense.h"
 
@@ -28,9 +29,11 @@ using namespace px;
 
 constexpr int kWaves = 8;                 // of a tile
 constexpr int kForth = 16, kBack = 8;     // rows of a wave forwards, and of the gradients' (registers)
+static_assert(kWaves >= 8, "a wave for each of a group's tiles before the last, and one");
 constexpr int kKeep = kWaves * kBack;     // rows of the gradients' tile: what comes into it is kept
 static_assert(kKeep == PLX_RECUR_KEEP && kKeep % kForth == 0, "a wave begins where its h is kept");
-constexpr int kGroup = 16;  // tiles of a group
+constexpr int kTicket = 64;  // (a counter takes an atomic addition each 20 ns: one for all slabs took longer than the rows)
+constexpr int kGroup = 8;  // tiles of a group, groups of a row
 constexpr int kSlab = 128;                                     // units of a workgroup
 constexpr int64_t kMaxSequences = int64_t{1} << 30;
 
@@ -50,9 +53,10 @@ struct RecurArgs {
   void* dxz;
   float* dstate;
   // zeros at first, in the order in which tiles are taken
-  unsigned* ticket;
+  unsigned* tickets;  // one a slab, kTicket apart
   uint64_t* spans;    // [tiles][units]: the tile summed up
-  uint64_t* carries;  // [groups][units]: what comes out of the group
+  uint64_t* groups;   // [groups][units]: the group
+  uint64_t* carries;  // [rows of groups][units]: what comes out of the row
 };
 
 __device__ __forceinline__ int64_t start_of(const RecurArgs& a, int64_t s) {
@@ -109,45 +113,47 @@ __device__ __forceinline__ void gate(float z, float& a, float& b) {
 struct Pair {
   float v[2];
 };
-// A lane's two units of a row, without a branch, for lanes past the row's end
-// read something of it: units `at` and `at + 1`, EVEN if a level's are even in
-// number (then both are one load), else one by one.
+// A lane's two units of a row, without a branch: lanes past the row's end read
+// something of it. FORM kEven: a level's units are even in number; kOdd: the
+// last lane reads the pair before its single unit, and takes the second; kOne:
+// a level of one unit, read alone.
+enum { kEven, kOdd, kOne };
 struct Lane {
-  unsigned col, at, next;
-  int n;  // of the two, how many are there
+  unsigned col, at, word, next;  // the first unit; where its pair, its word and the second's are read
+  int n;                         // of the two, how many are there
 };
+template <int FORM>
 __device__ __forceinline__ Lane lane_of(unsigned first, int units) {
   Lane l;
   l.col = first + (threadIdx.x & 63) * 2;
   l.n = units - static_cast<int>(l.col);
-  l.at = l.n > 0 ? l.col : 0;
-  l.next = l.n > 1 ? l.col + 1 : 0;
+  l.word = l.n > 0 ? l.col : 0, l.next = l.n > 1 ? l.col + 1 : 0;
+  l.at = FORM == kOdd && l.n == 1 ? l.col - 1 : l.word;
   return l;
 }
-template <bool EVEN, typename T>
+template <int FORM, typename T>
 __device__ __forceinline__ typename Pack<T, 2>::type load_two(const T* row, const Lane& l) {
-  if (EVEN) return *reinterpret_cast<const typename Pack<T, 2>::load*>(row + l.at);
-  return typename Pack<T, 2>::type{row[l.at], row[l.next]};
+  if (FORM == kOne) return typename Pack<T, 2>::type{row[0], row[0]};
+  typename Pack<T, 2>::type v = *reinterpret_cast<const typename Pack<T, 2>::load*>(row + l.at);
+  if (FORM == kOdd) v[0] = l.n == 1 ? v[1] : v[0];
+  return v;
 }
-template <bool EVEN, typename T>
+template <int FORM, typename T>
 __device__ __forceinline__ void store_two(T* row, const Lane& l, const float v[2]) {
-  if (EVEN) {
-    if (l.n > 0) *reinterpret_cast<typename Pack<T, 2>::load*>(row + l.col) = {from_f32<T>(v[0]), from_f32<T>(v[1])};
-    return;
-  }
-  if (l.n > 0) row[l.col] = from_f32<T>(v[0]);
-  if (l.n > 1) row[l.col + 1] = from_f32<T>(v[1]);
+  if (FORM != kOne && l.n > 1)
+    *reinterpret_cast<typename Pack<T, 2>::load*>(row + l.col) = {from_f32<T>(v[0]), from_f32<T>(v[1])};
+  if (FORM != kEven && l.n == 1) row[l.col] = from_f32<T>(v[0]);
 }
-template <bool EVEN>
+template <int FORM>
 __device__ __forceinline__ Pair load_pair(const float* row, const Lane& l) {
-  const typename Pack<float, 2>::type v = load_two<EVEN>(row, l);
+  const typename Pack<float, 2>::type v = load_two<FORM>(row, l);
   return {{v[0], v[1]}};
 }
 
-template <bool EVEN>
+template <int FORM>
 __device__ __forceinline__ Pair load_state(const RecurArgs& a, const float* states, int s, const Lane& l) {
   if (!states) return {{0.0f, 0.0f}};
-  return load_pair<EVEN>(states + static_cast<int64_t>(s) * a.units, l);
+  return load_pair<FORM>(states + static_cast<int64_t>(s) * a.units, l);
 }
 
 // A row range as a map of what comes in, two units: v -> A v + H, or H alone
@@ -216,7 +222,7 @@ __device__ __forceinline__ uint32_t span_low(float A, bool cut) {
 __device__ __forceinline__ void wait_words(const uint64_t* row, const Lane& l, uint64_t w[2]) {
 #pragma unroll 1
   for (int tries = 0; tries < 1 << 20; ++tries) {
-    w[0] = __hip_atomic_load(row + l.at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    w[0] = __hip_atomic_load(row + l.word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     w[1] = __hip_atomic_load(row + l.next, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (__all((w[0] & w[1] & kReady) != 0)) return;
     __builtin_amdgcn_s_sleep(1);
@@ -224,60 +230,78 @@ __device__ __forceinline__ void wait_words(const uint64_t* row, const Lane& l, u
   w[0] = w[1] = uint64_t{0x7FC00000u} << 32 | 0xFFC00000u;
 }
 
+__device__ __forceinline__ Span wait_span(const uint64_t* row, const Lane& l) {
+  uint64_t w[2];
+  wait_words(row, l, w);
+  Span s;
+  s.cut = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(w[0])) == kCut;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    s.A[j] = __uint_as_float(static_cast<uint32_t>(w[j]) & ~kReady);
+    s.H[j] = __uint_as_float(static_cast<uint32_t>(w[j] >> 32));
+  }
+  return s;
+}
+__device__ __forceinline__ void put_span(uint64_t* row, const Lane& l, const Span& s) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (j < l.n) put_word(row + (l.col + j), s.H[j], span_low(s.A[j], s.cut));
+}
+
 // What the waves of a workgroup share.
 struct Shared {
-  Spans<kWaves> waves;  // of the tile's waves
-  Spans<kGroup> tiles;  // of the tiles before it in its group
-  float2 into[64];     // what comes into the group
+  Spans<kWaves> waves;           // of the tile's waves
+  Spans<kGroup> tiles, groups;   // of the tiles before it in its group, the groups before in the row
+  float2 into[64];               // what comes into the row of groups
   unsigned number;
 };
 // What comes into the tile that is walked as the `at`-th. Its span goes out (by
-// the last wave, `own` the wave's, `s` of the waves before it); the others wait
-// for the tiles before it, the last one for what comes into the group.
+// the last wave, `own` the wave's, `s` of the waves before it), and its group's
+// if it is the last of it; the other waves wait for the tiles and groups
+// before it, the last one for what comes into the row.
 __device__ __forceinline__ Pair into_tile(const RecurArgs& a, int64_t at, const Lane& l, int wave, const Span& s,
                                           const Span& own, Shared& sh) {
-  const int lane = threadIdx.x & 63, place = static_cast<int>(at % kGroup);
-  const int64_t group = at / kGroup;
+  const int lane = threadIdx.x & 63;
+  const int tile = static_cast<int>(at % kGroup), group = static_cast<int>(at / kGroup % kGroup);
+  const int64_t row = at / (kGroup * kGroup);
   const bool last = wave == kWaves - 1, more = at + 1 < a.tiles;
   Span whole = s;
   if (last) {
     span_then(whole, own);
-    if (more && place < kGroup - 1) {
-      uint64_t* out = a.spans + at * a.units;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (j < l.n) put_word(out + (l.col + j), whole.H[j], span_low(whole.A[j], whole.cut));
+    if (more && tile < kGroup - 1) put_span(a.spans + at * a.units, l, whole);
+  } else if (wave < tile) {
+    sh.tiles.put(wave, lane, wait_span(a.spans + (at - tile + wave) * a.units, l));
+  }
+  if (more && tile == kGroup - 1 && group < kGroup - 1) {  // (the group's sum waits for no other group's)
+    __syncthreads();
+    if (last) {
+      Span all = sh.tiles.fold(tile, lane);
+      span_then(all, whole);
+      put_span(a.groups + at / kGroup * a.units, l, all);
     }
+  }
+  if (last) {
     Pair in = {{0.0f, 0.0f}};
-    if (group > 0) {
+    if (row > 0) {
       uint64_t w[2];
-      wait_words(a.carries + (group - 1) * a.units, l, w);
+      wait_words(a.carries + (row - 1) * a.units, l, w);
 #pragma unroll
       for (int j = 0; j < 2; ++j) in.v[j] = __uint_as_float(static_cast<uint32_t>(w[j] >> 32));
     }
     sh.into[lane] = make_float2(in.v[0], in.v[1]);
-  }
-  for (int i = last ? place : wave; i < place; i += kWaves - 1) {
-    uint64_t w[2];
-    wait_words(a.spans + (at - place + i) * a.units, l, w);
-    Span tile;
-    tile.cut = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(w[0])) == kCut;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      tile.A[j] = __uint_as_float(static_cast<uint32_t>(w[j]) & ~kReady);
-      tile.H[j] = __uint_as_float(static_cast<uint32_t>(w[j] >> 32));
-    }
-    sh.tiles.put(i, lane, tile);
+  } else if (wave < group) {
+    sh.groups.put(wave, lane, wait_span(a.groups + (at / kGroup - group + wave) * a.units, l));
   }
   __syncthreads();
   Pair in = {{sh.into[lane].x, sh.into[lane].y}};
-  span_into(sh.tiles.fold(place, lane), in);
-  if (last && more && place == kGroup - 1) {
-    uint64_t* out = a.carries + group * a.units;
+  span_into(sh.groups.fold(group, lane), in);
+  span_into(sh.tiles.fold(tile, lane), in);
+  if (last && more && tile == kGroup - 1 && group == kGroup - 1) {
+    Pair out = in;
+    span_into(whole, out);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-      if (j < l.n)
-        put_word(out + (l.col + j), whole.cut ? whole.H[j] : __builtin_fmaf(whole.A[j], in.v[j], whole.H[j]), kReady);
+      if (j < l.n) put_word(a.carries + row * a.units + (l.col + j), out.v[j], kReady);
   }
   return in;
 }
@@ -294,7 +318,7 @@ __device__ __forceinline__ bool unbroken(const int (&of)[N]) {
 
 // A wave's rows forwards, from their A and H: rows at which a sequence starts
 // get its state put into H.
-template <bool EVEN, int N>
+template <int FORM, int N>
 __device__ __forceinline__ Span sum_up(const RecurArgs& a, const int (&of)[N + 2], const Lane& l,
                                        const float (&A)[N][2], float (&H)[N][2]) {
   Span s = span_none();
@@ -310,7 +334,7 @@ __device__ __forceinline__ Span sum_up(const RecurArgs& a, const int (&of)[N + 2
     if (q < 0) {
       H[i][0] = H[i][1] = 0.0f;
     } else if (cut) {
-      const Pair in = load_state<EVEN>(a, a.state, q, l);
+      const Pair in = load_state<FORM>(a, a.state, q, l);
 #pragma unroll
       for (int j = 0; j < 2; ++j) H[i][j] = __builtin_fmaf(A[i][j], in.v[j], H[i][j]);
     }
@@ -321,7 +345,7 @@ __device__ __forceinline__ Span sum_up(const RecurArgs& a, const int (&of)[N + 2
 
 // Sequences without rows: out = in (null: zeros), 64 of them at a time by the
 // waves of a slab's workgroups.
-template <bool EVEN>
+template <int FORM>
 __device__ __forceinline__ void pass_empty(const RecurArgs& a, int64_t tile, const float* in, float* out,
                                            const Lane& l) {
   if (!a.starts && a.tokens > 0) return;
@@ -331,27 +355,35 @@ __device__ __forceinline__ void pass_empty(const RecurArgs& a, int64_t tile, con
     const bool empty = s < a.sequences && (!a.starts || start_of(a, s) >= start_of(a, s + 1));
     for (uint64_t mask = __ballot(empty); mask; mask &= mask - 1) {
       const int at = static_cast<int>(first + __builtin_ctzll(mask));
-      store_two<EVEN>(out + static_cast<int64_t>(at) * a.units, l, load_state<EVEN>(a, in, at, l).v);
+      store_two<FORM>(out + static_cast<int64_t>(at) * a.units, l, load_state<FORM>(a, in, at, l).v);
     }
   }
 }
 
-// The workgroup's number in the order in which they are taken.
-__device__ __forceinline__ unsigned take(const RecurArgs& a, unsigned* shared) {
-  if (a.tiles <= 1) return blockIdx.x;
+// The workgroup's slab of units, each as often as there are tiles: 8 workgroups
+// in a row, one on each of the chip's parts, take the same one. (A slab of a
+// row is 256 bytes, a channel of a part's cache; with slab after slab a part
+// had the same few of them all the time, 143 us in place of 122.)
+__device__ __forceinline__ unsigned slab_of(const RecurArgs& a) {
+  const unsigned slabs = a.slabs, i = blockIdx.x, whole = gridDim.x / (8 * slabs) * (8 * slabs);
+  return i < whole ? i / 8 % slabs : (i - whole) % slabs;
+}
+// The workgroup's tile in the order in which a slab's are taken.
+__device__ __forceinline__ int take(const RecurArgs& a, unsigned slab, unsigned* shared) {
+  if (a.tiles <= 1) return 0;
   if (threadIdx.x == 0)
-    *shared = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *shared = __hip_atomic_fetch_add(a.tickets + slab * kTicket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   return __builtin_amdgcn_readfirstlane(*shared);
 }
 
-template <typename T, bool EVEN>
+template <typename T, int FORM>
 __global__ __launch_bounds__(64 * kWaves, 4) void k_recur(RecurArgs a) {
   __shared__ Shared sh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned taken = take(a, &sh.number), slabs = a.slabs;
-  const int64_t tile = taken / slabs, t = (tile * kWaves + wave) * kForth;
-  const Lane l = lane_of(taken % slabs * kSlab, a.units);
+  const unsigned slab = slab_of(a);
+  const int64_t tile = take(a, slab, &sh.number), t = (tile * kWaves + wave) * kForth;
+  const Lane l = lane_of<FORM>(slab * kSlab, a.units);
   int of[kForth + 2];
   float A[kForth][2], H[kForth][2];
   if (a.tokens > 0) {
@@ -361,7 +393,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur(RecurArgs a) {
 #pragma unroll
     for (int i = 0; i < kForth; ++i) {
       const T* row = xz + (i < rows ? i * a.line : 0);
-      x[i] = load_two<EVEN>(row, l), z[i] = load_two<EVEN>(row + a.units, l);
+      x[i] = load_two<FORM>(row, l), z[i] = load_two<FORM>(row + a.units, l);
     }
 #pragma unroll
     for (int i = 0; i < kForth; ++i) {
@@ -374,20 +406,20 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur(RecurArgs a) {
     }
   }
   rows_of(a, t, of);
-  const Span own = sum_up<EVEN, kForth>(a, of, l, A, H);
+  const Span own = sum_up<FORM, kForth>(a, of, l, A, H);
   sh.waves.put(wave, lane, own);
   __syncthreads();
   const Span s = sh.waves.fold(wave, lane);  // the waves before
   Pair h = into_tile(a, tile, l, wave, s, own, sh);
   span_into(s, h);
-  if (t % kKeep == 0 && t < a.tokens) store_two<EVEN>(a.kept + t / kKeep * a.units, l, h.v);
+  if (t % kKeep == 0 && t < a.tokens) store_two<FORM>(a.kept + t / kKeep * a.units, l, h.v);
   T* out = static_cast<T*>(a.h) + t * a.units;
   if (unbroken(of)) {
 #pragma unroll
     for (int i = 0; i < kForth; ++i) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) h.v[j] = __builtin_fmaf(A[i][j], h.v[j], H[i][j]);
-      store_two<EVEN>(out + i * a.units, l, h.v);
+      store_two<FORM>(out + i * a.units, l, h.v);
     }
   } else {
 #pragma unroll
@@ -397,11 +429,11 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur(RecurArgs a) {
       const bool cut = q < 0 || of[i] != q;
 #pragma unroll
       for (int j = 0; j < 2; ++j) h.v[j] = cut ? H[i][j] : __builtin_fmaf(A[i][j], h.v[j], H[i][j]);
-      store_two<EVEN>(out + i * a.units, l, h.v);
-      if (q >= 0 && of[i + 2] != q) store_two<EVEN>(a.last + static_cast<int64_t>(q) * a.units, l, h.v);
+      store_two<FORM>(out + i * a.units, l, h.v);
+      if (q >= 0 && of[i + 2] != q) store_two<FORM>(a.last + static_cast<int64_t>(q) * a.units, l, h.v);
     }
   }
-  pass_empty<EVEN>(a, tile, a.state, a.last, l);
+  pass_empty<FORM>(a, tile, a.state, a.last, l);
 }
 
 // The gradients, tiles from the last to the first. Backwards, a row passes on
@@ -409,14 +441,14 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur(RecurArgs a) {
 // last state's gradient in, its first row's goes to its state and no further.
 // h is walked again from what came into the tile, so that it is neither kept
 // nor rounded.
-template <typename T, bool EVEN>
+template <typename T, int FORM>
 __global__ __launch_bounds__(64 * kWaves, 4) void k_recur_grad(RecurArgs a) {
   __shared__ Shared sh;
   __shared__ Spans<kWaves> forth;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned taken = take(a, &sh.number), slabs = a.slabs;
-  const int64_t at = taken / slabs, tile = a.tiles > 0 ? a.tiles - 1 - at : 0, t = (tile * kWaves + wave) * kBack;
-  const Lane l = lane_of(taken % slabs * kSlab, a.units);
+  const unsigned slab = slab_of(a);
+  const int64_t at = take(a, slab, &sh.number), tile = a.tiles > 0 ? a.tiles - 1 - at : 0, t = (tile * kWaves + wave) * kBack;
+  const Lane l = lane_of<FORM>(slab * kSlab, a.units);
   int of[kBack + 2];
   typename Pack<T, 2>::type x[kBack], g[kBack];
   float A[kBack][2], B[kBack][2];  // the gates
@@ -429,10 +461,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur_grad(RecurArgs a) {
 #pragma unroll
     for (int i = 0; i < kBack; ++i) {
       const T* row = xz + (i < rows ? i * a.line : 0);
-      x[i] = load_two<EVEN>(row, l), z[i] = load_two<EVEN>(row + a.units, l);
-      g[i] = load_two<EVEN>(gs + (i < rows ? i * a.g_line : 0), l);
+      x[i] = load_two<FORM>(row, l), z[i] = load_two<FORM>(row + a.units, l);
+      g[i] = load_two<FORM>(gs + (i < rows ? i * a.g_line : 0), l);
     }
-    h = load_pair<EVEN>(a.kept + tile * a.units, l);
+    h = load_pair<FORM>(a.kept + tile * a.units, l);
 #pragma unroll
     for (int i = 0; i < kBack; ++i) {
 #pragma unroll
@@ -448,14 +480,14 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur_grad(RecurArgs a) {
     for (int i = 0; i < kBack; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) H[i][j] = B[i][j] * to_f32(x[i][j]);
-    forth.put(wave, lane, sum_up<EVEN, kBack>(a, of, l, A, H));
+    forth.put(wave, lane, sum_up<FORM, kBack>(a, of, l, A, H));
   }
 #pragma unroll
   for (int i = kBack - 1; i >= 0; --i) {
     const int q = of[i + 1];
     const bool on = whole || (q >= 0 && of[i] == q), last = !whole && of[i + 2] != q;
     Pair more = {{0.0f, 0.0f}};
-    if (on && last) more = load_state<EVEN>(a, a.g_last, q, l);
+    if (on && last) more = load_state<FORM>(a, a.g_last, q, l);
     Span row;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -476,7 +508,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur_grad(RecurArgs a) {
 #pragma unroll
   for (int i = 0; i < kBack; ++i) {
     const int q = of[i + 1];
-    if (!whole && of[i] != q) h = q >= 0 ? load_state<EVEN>(a, a.state, q, l) : Pair{{0.0f, 0.0f}};
+    if (!whole && of[i] != q) h = q >= 0 ? load_state<FORM>(a, a.state, q, l) : Pair{{0.0f, 0.0f}};
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       before[i][j] = h.v[j];
@@ -490,7 +522,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur_grad(RecurArgs a) {
     const int q = of[i + 1];
     float dx[2] = {0.0f, 0.0f}, dz[2] = {0.0f, 0.0f};
     if (whole || q >= 0) {
-      if (!whole && of[i + 2] != q) c = load_state<EVEN>(a, a.g_last, q, l);
+      if (!whole && of[i + 2] != q) c = load_state<FORM>(a, a.g_last, q, l);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float v = to_f32(g[i][j]) + c.v[j];
@@ -498,13 +530,13 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur_grad(RecurArgs a) {
         c.v[j] = A[i][j] * v;
         dz[j] = B[i][j] * c.v[j] * (before[i][j] - to_f32(x[i][j]));
       }
-      if (!whole && of[i] != q) store_two<EVEN>(a.dstate + static_cast<int64_t>(q) * a.units, l, c.v);
+      if (!whole && of[i] != q) store_two<FORM>(a.dstate + static_cast<int64_t>(q) * a.units, l, c.v);
     }
     T* row = out + i * 2 * a.units;
-    store_two<EVEN>(row, l, dx);
-    store_two<EVEN>(row + a.units, l, dz);
+    store_two<FORM>(row, l, dx);
+    store_two<FORM>(row + a.units, l, dz);
   }
-  pass_empty<EVEN>(a, at, a.g_last, a.dstate, l);
+  pass_empty<FORM>(a, at, a.g_last, a.dstate, l);
 }
 
 // One row a sequence, the state in place; a lane takes 4 units.
@@ -531,15 +563,16 @@ __global__ __launch_bounds__(256) void k_recur_step(int64_t sequences, int units
 }
 
 struct RecurPlan {
-  int64_t tiles, slabs, spans, carries, words, bytes;  // words of 8 bytes, then the rows' sequences
+  int64_t tiles, slabs, spans, groups, carries, words, bytes;  // words of 8 bytes, then the rows' sequences
 };
 RecurPlan recur_plan(int64_t tokens, int64_t units, bool ragged, int rows) {
   RecurPlan p{};
   p.tiles = div_up(tokens, kWaves * rows), p.slabs = div_up(units, kSlab);
-  if (p.tiles > 1) {  // (the ticket comes first)
-    p.spans = 1;
-    p.carries = p.spans + p.tiles * units;
-    p.words = p.carries + p.tiles / kGroup * units;
+  if (p.tiles > 1) {  // (the tickets come first)
+    p.spans = p.slabs * kTicket / 2;
+    p.groups = p.spans + p.tiles * units;
+    p.carries = p.groups + p.tiles / kGroup * units;
+    p.words = p.carries + p.tiles / (kGroup * kGroup) * units;
   }
   p.bytes = 8 * p.words + (ragged ? 4 * tokens : 0);
   return p;
@@ -555,7 +588,8 @@ bool recur_fits(int64_t tokens, int64_t units, int64_t sequences, int wide) {
 void recur_setup(RecurArgs& a, const RecurPlan& p, void* workspace, hipStream_t s) {
   uint64_t* words = static_cast<uint64_t*>(workspace);
   a.tiles = p.tiles, a.slabs = static_cast<int>(p.slabs);
-  a.ticket = reinterpret_cast<unsigned*>(words), a.spans = words + p.spans, a.carries = words + p.carries;
+  a.tickets = reinterpret_cast<unsigned*>(words), a.spans = words + p.spans;
+  a.groups = words + p.groups, a.carries = words + p.carries;
   int* of = a.starts && a.tokens > 0 ? reinterpret_cast<int*>(words + p.words) : nullptr;
   a.of = of;
   const int64_t rows = of ? a.tokens : 0, lanes = p.words > rows ? p.words : rows;
@@ -594,10 +628,12 @@ int plx_recur(int64_t tokens, int64_t units, int64_t sequences, int32_t dtype, c
   recur_setup(a, p, workspace, s);
   with_type(dtype, [&](auto* e) {
     using T = PLX_DENSE_TYPE(e);
-    if (units % 2)
-      k_recur<T, false><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
+    if (units == 1)
+      k_recur<T, kOne><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
+    else if (units % 2)
+      k_recur<T, kOdd><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
     else
-      k_recur<T, true><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
+      k_recur<T, kEven><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
   });
   return check_launch("plx_recur");
 }
@@ -623,10 +659,12 @@ int plx_recur_grad(int64_t tokens, int64_t units, int64_t sequences, int32_t dty
   recur_setup(a, p, workspace, s);
   with_type(dtype, [&](auto* e) {
     using T = PLX_DENSE_TYPE(e);
-    if (units % 2)
-      k_recur_grad<T, false><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
+    if (units == 1)
+      k_recur_grad<T, kOne><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
+    else if (units % 2)
+      k_recur_grad<T, kOdd><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
     else
-      k_recur_grad<T, true><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
+      k_recur_grad<T, kEven><<<recur_groups(p), 64 * kWaves, 0, s>>>(a);
   });
   return check_launch("plx_recur_grad");
 }
