@@ -1269,7 +1269,7 @@ PLX_EXPORT int plx_look_up(int64_t tokens, int64_t rows, int64_t units, const vo
                            const void* table, int64_t line, float scale, void* out, void* stream);
 
 /* out [rows][units] (float32) = scale * the sums of g over the tokens of each
- * id, in the tokens' order (zeros for a row without any). At most 2^28 tokens. */
+ * id, in the tokens' order (zeros for a row without any). At most 2^25 tokens. */
 PLX_EXPORT int64_t plx_look_up_workspace(int64_t tokens, int64_t rows, int64_t units);
 PLX_EXPORT int plx_look_up_grad(int64_t tokens, int64_t rows, int64_t units, const void* ids, int32_t wide,
                                 int32_t dtype, const void* g, int64_t line, float scale, float* out, void* workspace,

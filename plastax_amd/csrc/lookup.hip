@@ -6,7 +6,8 @@
 // order (float32, no atomics on floats): three launches,
 //   k_group      ids to classes (id mod classes), a workgroup each: it reads
 //                all ids, counts those of lower classes, which gives its place
-//                in the list, and sorts its own by counting;
+//                in the list, and sorts its own by counting (bound by the
+//                caches that all of them read through: 65536 ids {KG} us);
 //   k_row_sums   every row of up to kPart tokens (zeros where it has none),
 //                and the parts of longer ones: kPart places of the list each;
 //   k_join_sums  the longer rows from their parts, in order.
@@ -20,9 +21,10 @@ namespace {
 
 using namespace px;
 
-constexpr int kPart = 64;      // places of the list that one part sums
-constexpr int kLocal = 8192;   // rows of a class at most (their counters are in LDS)
+constexpr int kPart = 16;      // places of the list that one part sums
+constexpr int kLocal = 4096;   // rows of a class at most (their counters are in LDS)
 constexpr int kGroupWaves = 16;
+constexpr int kFound = 256;    // tokens that a wave keeps in LDS
 
 struct LookArgs {
   int64_t tokens, line;
@@ -71,9 +73,24 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
                                    __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
 }
 
+// Ids 64 apart, -1 from `end` on: enough of them on their way at once.
+constexpr int kAhead = 16;
+template <typename I>
+__device__ __forceinline__ void load_ids(const LookArgs& a, int64_t t, int64_t end, I id[kAhead]) {
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int64_t at = t + 64 * i;
+    id[i] = static_cast<const I*>(a.ids)[at < end ? at : end - 1];
+  }
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) id[i] = t + 64 * i < end ? id[i] : I{-1};
+}
+
+template <typename I>  // the ids' type
 __global__ __launch_bounds__(64 * kGroupWaves) void k_group(LookArgs a) {
   constexpr int NT = 64 * kGroupWaves;
   __shared__ int cursor[kLocal];
+  __shared__ int2 found[kGroupWaves][kFound];  // a wave's tokens of the class, in order, as many as fit
   __shared__ int less[kGroupWaves], own[kGroupWaves], sums[kGroupWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = blockIdx.x;
   const int local = (a.rows + a.classes - 1) / a.classes;
@@ -81,16 +98,33 @@ __global__ __launch_bounds__(64 * kGroupWaves) void k_group(LookArgs a) {
   // A wave's tokens lie behind each other.
   const int64_t per = div_up(a.tokens, NT) * 64, begin = wave * per;
   const int64_t end = begin + per < a.tokens ? begin + per : a.tokens;
+  __syncthreads();
   int below = 0, hits = 0;
-#pragma unroll 8
-  for (int64_t t = begin + lane; t < end; t += 64) {
-    const int64_t id = load_id(a.ids, a.wide, t);
-    const bool there = id >= 0 && id < a.rows;
-    const int c = static_cast<int>(id & (a.classes - 1));
-    below += there && c < mine;
-    hits += there && c == mine;
-  }
-  below = wave_sum_int(below), hits = wave_sum_int(hits);
+  // The wave's tokens of the class, from place `at` of `out` on, the first
+  // `room` of them; below: those of lower classes.
+  auto search = [&](bool count, int2* out, int at, int room) {
+    for (int64_t first = begin; first < end; first += 64 * kAhead) {
+      I id[kAhead];
+      load_ids(a, first + lane, end, id);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const bool there = id[i] >= 0 && id[i] < a.rows;
+        const int c = static_cast<int>(id[i] & (a.classes - 1));
+        if (count) below += there && c < mine;
+        const bool hit = there && c == mine;
+        const uint64_t mask = __ballot(hit);
+        if (hit) {
+          const int row = static_cast<int>(id[i] >> a.shift), place = at + lanes_below(mask);
+          if (place < room) out[place] = make_int2(static_cast<int>(first + 64 * i) + lane, row);
+          if (count) atomicAdd(&cursor[row], 1);
+        }
+        at += __popcll(mask);
+      }
+    }
+    return at;
+  };
+  hits = search(true, found[wave], 0, kFound);
+  below = wave_sum_int(below);
   if (lane == 0) less[wave] = below, own[wave] = hits;
   __syncthreads();
   int base = 0, n = 0, at = 0;
@@ -102,18 +136,10 @@ __global__ __launch_bounds__(64 * kGroupWaves) void k_group(LookArgs a) {
   }
   if (mine == a.classes - 1 && threadIdx.x == 0) *a.total = base + n;
   int2* stage = a.stage + base;
-  if (hits > 0) {
-    for (int64_t first = begin; first < end; first += 64) {
-      const int64_t t = first + lane, id = t < end ? load_id(a.ids, a.wide, t) : -1;
-      const bool hit = id >= 0 && id < a.rows && (id & (a.classes - 1)) == mine;
-      const uint64_t mask = __ballot(hit);
-      if (hit) {
-        const int row = static_cast<int>(id >> a.shift);
-        stage[at + lanes_below(mask)] = make_int2(static_cast<int>(t), row);
-        atomicAdd(&cursor[row], 1);
-      }
-      at += __popcll(mask);
-    }
+  if (hits <= kFound) {
+    for (int i = lane; i < hits; i += 64) stage[at + i] = found[wave][i];
+  } else {
+    search(false, stage, at, n);  // (again: it has all the room)
   }
   __syncthreads();
   // The rows' places: an exclusive scan of the counts, kLocal / NT a lane.
@@ -147,23 +173,43 @@ __global__ __launch_bounds__(64 * kGroupWaves) void k_group(LookArgs a) {
     place += count[i];
   }
   __syncthreads();
-  // The tokens to their places, in order: 64 at a time by the first wave, equal
-  // rows found bit by bit.
-  if (wave > 0) return;
-  volatile int* next = cursor;
+  // The tokens to their places, in order: 64 at a time, 4 such blocks a wave.
+  // Equal rows of a block are found bit by bit by all waves at once; then the
+  // waves take their rows' places one after another.
+  constexpr int GO = 4, ROUND = NT * GO;
   int* list = a.list + base;
-  for (int first = 0; first < n; first += 64) {
-    const bool there = first + lane < n;
-    const int2 v = there ? stage[first + lane] : make_int2(0, 0);
-    uint64_t same = __ballot(there);
-    for (int b = 1; b < local; b *= 2) {
-      const uint64_t ones = __ballot(there && (v.y & b));
-      same &= (v.y & b) ? ones : ~ones;
+  for (int first = 0; first < n; first += ROUND) {
+    int2 v[GO];
+    uint64_t same[GO];
+    int from[GO];
+#pragma unroll
+    for (int k = 0; k < GO; ++k) {
+      const int i = first + (wave * GO + k) * 64 + lane;
+      v[k] = i < n ? stage[i] : make_int2(-1, 0);
     }
-    if (there) {
-      const int rank = lanes_below(same), from = next[v.y];
-      list[from + rank] = v.x;
-      if (rank == 0) next[v.y] = from + __popcll(same);
+#pragma unroll
+    for (int k = 0; k < GO; ++k) {
+      same[k] = __ballot(v[k].x >= 0);
+      for (int b = 1; b < local; b *= 2) {
+        const uint64_t ones = __ballot(v[k].y & b);
+        same[k] &= (v[k].y & b) ? ones : ~ones;
+      }
+    }
+    const int left = n - first, turns = left < ROUND ? (left + 64 * GO - 1) / (64 * GO) : kGroupWaves;
+    for (int turn = 0; turn < turns; ++turn) {
+      if (turn == wave) {
+#pragma unroll
+        for (int k = 0; k < GO; ++k) {
+          from[k] = 0;
+          if (v[k].x >= 0 && lanes_below(same[k]) == 0) from[k] = atomicAdd(&cursor[v[k].y], __popcll(same[k]));
+        }
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < GO; ++k) {
+      const int start = __shfl(from[k], v[k].x >= 0 ? __builtin_ctzll(same[k]) : 0, 64);
+      if (v[k].x >= 0) list[start + lanes_below(same[k])] = v[k].x;
     }
   }
 }
@@ -181,14 +227,22 @@ struct Columns {
       for (int i = 0; i < 4; ++i) v[k][i] = 0.0f;
   }
   template <typename T>
-  __device__ __forceinline__ void add(const T* row, int units, int at) {
+  struct Raw {
     typename Pack<T, 4>::type x[NC];
+  };
+  template <typename T>
+  __device__ __forceinline__ Raw<T> load(const T* row, int units, int at) const {
+    Raw<T> r;
 #pragma unroll
-    for (int k = 0; k < NC; ++k) x[k] = load_pack<4>(row + at + k * LX * 4, units - at - k * LX * 4);
+    for (int k = 0; k < NC; ++k) r.x[k] = load_pack<4>(row + at + k * LX * 4, units - at - k * LX * 4);
+    return r;
+  }
+  template <typename T>
+  __device__ __forceinline__ void add(const Raw<T>& r) {
 #pragma unroll
     for (int k = 0; k < NC; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[k][i] += to_f32(x[k][i]);
+      for (int i = 0; i < 4; ++i) v[k][i] += to_f32(r.x[k][i]);
   }
   template <bool PASS>
   __device__ __forceinline__ void store(float* row, int units, int at, float scale) {
@@ -204,7 +258,8 @@ struct Columns {
 
 // Workgroups of the first `part_groups` sum parts, the others rows; blockIdx.y
 // is the slab of columns. A row's lanes read its place and count, then its
-// tokens, then their gradients.
+// tokens, then their gradients: for kEach rows at once.
+constexpr int kEach = 4;
 template <typename T, int LX, int NC>
 __global__ __launch_bounds__(256) void k_row_sums(LookArgs a, int part_groups) {
   using Sum = Columns<LX, NC>;
@@ -226,56 +281,73 @@ __global__ __launch_bounds__(256) void k_row_sums(LookArgs a, int part_groups) {
       const int from = h ? row.x : static_cast<int>(begin), to = h || row.x + row.y > end ? end : row.x + row.y;
       sum.clear();
 #pragma unroll 4
-      for (int j = from; j < to; ++j) sum.add(g + a.list[j] * a.line, a.units, at);
+      for (int j = from; j < to; ++j) sum.add(sum.load(g + a.list[j] * a.line, a.units, at));
       sum.template store<false>(a.part + (2 * p + h) * a.units, a.units, at, 1.0f);
     }
     return;
   }
-  const int64_t r = static_cast<int64_t>(blockIdx.x - part_groups) * PER + threadIdx.x / LX;
-  if (r >= a.rows) return;
-  const int2 row = a.info[r];
-  if (row.y > kPart) return;
-  sum.clear();
-#pragma unroll 2
-  for (int j = row.x; j < row.x + row.y; ++j) sum.add(g + a.list[j] * a.line, a.units, at);
-  sum.template store<true>(static_cast<float*>(a.out) + r * a.units, a.units, at, a.scale);
+  const int64_t first = (static_cast<int64_t>(blockIdx.x - part_groups) * PER + threadIdx.x / LX) * kEach;
+  int2 row[kEach];
+  typename Sum::template Raw<T> x[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) row[i] = first + i < a.rows ? a.info[first + i] : make_int2(0, -1);
+  int token[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) token[i] = row[i].y > 0 ? a.list[row[i].x] : -1;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) x[i] = sum.load(g + (token[i] >= 0 ? token[i] : 0) * a.line, token[i] >= 0 ? a.units : 0, at);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (row[i].y < 0 || row[i].y > kPart) continue;
+    sum.clear();
+    sum.add(x[i]);
+#pragma unroll 4
+    for (int j = row[i].x + 1; j < row[i].x + row[i].y; ++j) sum.add(sum.load(g + a.list[j] * a.line, a.units, at));
+    sum.template store<true>(static_cast<float*>(a.out) + (first + i) * a.units, a.units, at, row[i].y > 0 ? a.scale : 0.0f);
+  }
 }
 
-// A workgroup for each part in which a longer row may begin: it is the row of
-// the part's last place. The row's parts go over the workgroup's groups of LX
-// lanes, then over LDS, both in order.
-template <int LX, int NC>
-__global__ __launch_bounds__(256) void k_join_sums(LookArgs a) {
-  using Sum = Columns<LX, NC>;
-  constexpr int PER = 256 / LX;
+// The longer rows. A workgroup looks at kJoin parts: a longer row that begins in a
+// part is the row of the part's last place. Its parts go over the workgroup's
+// groups of LX lanes, then over LDS, both in order.
+constexpr int kJoin = 8;
+template <int LX>
+__global__ __launch_bounds__(1024) void k_join_sums(LookArgs a) {
+  using Sum = Columns<LX, 1>;
+  constexpr int PER = 1024 / LX;
   __shared__ float joined[PER][Sum::kSlab];
-  const int total = *a.total;
-  const int64_t p = blockIdx.x, begin = p * kPart;
-  if (begin >= total) return;
-  const int end = static_cast<int>(begin + kPart < total ? begin + kPart : total);
-  const int64_t r = load_id(a.ids, a.wide, a.list[end - 1]);
-  const int2 row = a.info[r];
-  if (row.y <= kPart || row.x < begin) return;
+  const int total = *a.total, lane = threadIdx.x & 63;
   const int tx = threadIdx.x & (LX - 1), group = threadIdx.x / LX;
   const int at = static_cast<int>(blockIdx.y) * Sum::kSlab + tx * 4;
-  const int64_t last = (row.x + row.y - 1) / kPart;
-  Sum sum;
-  sum.clear();
+  const int64_t mine = static_cast<int64_t>(blockIdx.x) * kJoin + lane, begin = mine * kPart;
+  int row = -1, place = 0, count = 0;
+  if (lane < kJoin && begin < total) {
+    row = static_cast<int>(load_id(a.ids, a.wide, a.list[begin + kPart < total ? begin + kPart - 1 : total - 1]));
+    const int2 info = a.info[row];
+    place = info.x, count = info.y;
+    if (count <= kPart || place < begin) row = -1;
+  }
+  for (uint64_t found = __ballot(row >= 0); found; found &= found - 1) {  // (the same in all waves)
+    const int from = __builtin_ctzll(found);
+    const int64_t p = static_cast<int64_t>(blockIdx.x) * kJoin + from;
+    const int r = __builtin_amdgcn_readlane(row, from), first = __builtin_amdgcn_readlane(place, from);
+    const int64_t last = (first + __builtin_amdgcn_readlane(count, from) - 1) / kPart;
+    Sum sum;
+    sum.clear();
 #pragma unroll 4
-  for (int64_t q = p + group; q <= last; q += PER)
-    sum.add(a.part + (2 * q + (q == p && row.x > begin)) * a.units, a.units, at);
+    for (int64_t q = p + group; q <= last; q += PER)
+      sum.add(sum.load(a.part + (2 * q + (q == p && first > p * kPart)) * a.units, a.units, at));
+    __syncthreads();
 #pragma unroll
-  for (int k = 0; k < NC; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) joined[group][(k * 4 + i) * LX + tx] = sum.v[k][i];
-  __syncthreads();
-  if (group) return;
-#pragma unroll
-  for (int k = 0; k < NC; ++k)
+    for (int i = 0; i < 4; ++i) joined[group][i * LX + tx] = sum.v[0][i];
+    __syncthreads();
+    if (group) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      for (int o = 1; o < PER; ++o) sum.v[k][i] += joined[o][(k * 4 + i) * LX + tx];
-  sum.template store<true>(static_cast<float*>(a.out) + r * a.units, a.units, at, a.scale);
+#pragma unroll 4
+      for (int o = 1; o < PER; ++o) sum.v[0][i] += joined[o][i * LX + tx];
+    sum.template store<true>(static_cast<float*>(a.out) + static_cast<int64_t>(r) * a.units, a.units, at, a.scale);
+  }
 }
 
 struct LookPlan {
@@ -301,12 +373,15 @@ void launch_sums(const LookArgs& a, const LookPlan& p, hipStream_t s) {
   constexpr int PER = 256 / LX;
   const unsigned slabs = static_cast<unsigned>(div_up(a.units, Columns<LX, NC>::kSlab));
   const int part_groups = static_cast<int>(div_up(p.parts, PER));
-  const dim3 grid(static_cast<unsigned>(part_groups + div_up(a.rows, PER)), slabs);
+  const dim3 grid(static_cast<unsigned>(part_groups + div_up(a.rows, PER * kEach)), slabs);
   k_row_sums<T, LX, NC><<<grid, 256, 0, s>>>(a, part_groups);
-  if (p.parts) k_join_sums<LX, NC><<<dim3(static_cast<unsigned>(p.parts), slabs), 256, 0, s>>>(a);
+  if (p.parts) {
+    const dim3 join(static_cast<unsigned>(div_up(p.parts, kJoin)), static_cast<unsigned>(div_up(a.units, Columns<LX, 1>::kSlab)));
+    k_join_sums<LX><<<join, 1024, 0, s>>>(a);
+  }
 }
 
-constexpr int64_t kMaxSorted = int64_t{1} << 28;  // tokens of a gradient: a launch's parts stay below 2^30 lanes
+constexpr int64_t kMaxSorted = int64_t{1} << 25;  // tokens of a gradient: a launch's parts stay below 2^31 lanes
 inline bool look_fits(int64_t tokens, int64_t rows, int64_t units, int wide) {
   return batch_fits(tokens, units) && rows >= 0 && rows <= kMaxLevel && (wide == 0 || wide == 1);
 }
@@ -361,7 +436,10 @@ int plx_look_up_grad(int64_t tokens, int64_t rows, int64_t units, const void* id
   a.stage = reinterpret_cast<int2*>(work + p.stage);
   a.part = reinterpret_cast<float*>(work + p.part);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  k_group<<<static_cast<unsigned>(p.classes), 64 * kGroupWaves, 0, s>>>(a);
+  if (wide)
+    k_group<int64_t><<<static_cast<unsigned>(p.classes), 64 * kGroupWaves, 0, s>>>(a);
+  else
+    k_group<int32_t><<<static_cast<unsigned>(p.classes), 64 * kGroupWaves, 0, s>>>(a);
   with_type(dtype, [&](auto* e) {
     using T = PLX_DENSE_TYPE(e);
     if (units <= 32)

@@ -182,8 +182,8 @@ def test_entry_points_check_before_they_launch(lib) -> None:
     assert b"plx_look_up_workspace" in lib.plx_last_error()
     assert lib.plx_look_up_grad(5, 7, 8, P, 0, 0, P, 8, 1.0, None, P, 1 << 30, None) == bad
     assert lib.plx_look_up_grad(5, 0, 8, P, 0, 0, P, 8, 1.0, P, None, 0, None) == 0
-    assert lib.plx_look_up_grad((1 << 28) + 1, 7, 8, P, 0, 0, P, 8, 1.0, P, P, 1 << 62, None) == bad
-    assert lib.plx_look_up_workspace(-1, 7, 8) == -1 and lib.plx_look_up_workspace((1 << 28) + 1, 7, 8) == -1
+    assert lib.plx_look_up_grad((1 << 25) + 1, 7, 8, P, 0, 0, P, 8, 1.0, P, P, 1 << 62, None) == bad
+    assert lib.plx_look_up_workspace(-1, 7, 8) == -1 and lib.plx_look_up_workspace((1 << 25) + 1, 7, 8) == -1
     assert lib.plx_look_up_workspace(5, big, 8) == -1
     assert lib.plx_normalise(5, big, 0, P, 8, 0, P, P, 1e-5, P, P, None) == bad
     assert lib.plx_normalise(5, 8, 1, P, 8, 2, P, P, 1e-5, P, P, None) == unknown
