@@ -7,7 +7,7 @@
 //   k_group      ids to classes (id mod classes), a workgroup each: it reads
 //                all ids, counts those of lower classes, which gives its place
 //                in the list, and sorts its own by counting (bound by the
-//                caches that all of them read through: 65536 ids {KG} us);
+//                caches that all of them read through: 65536 ids 26 us);
 //   k_row_sums   every row of up to kPart tokens (zeros where it has none),
 //                and the parts of longer ones: kPart places of the list each;
 //   k_join_sums  the longer rows from their parts, in order.
@@ -24,7 +24,8 @@ using namespace px;
 constexpr int kPart = 16;      // places of the list that one part sums
 constexpr int kLocal = 4096;   // rows of a class at most (their counters are in LDS)
 constexpr int kGroupWaves = 16;
-constexpr int kFound = 256;    // tokens that a wave keeps in LDS
+constexpr int kFound = 512;    // tokens that a wave keeps in LDS, of a range of at most 2^kRange
+constexpr int kRange = 20;
 
 struct LookArgs {
   int64_t tokens, line;
@@ -73,24 +74,29 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
                                    __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
 }
 
-// Ids 64 apart, -1 from `end` on: enough of them on their way at once.
+// Ids 64 apart as 32 bits, enough of them on their way at once; from `end` on
+// and out of 32 bits they are all ones, which is no row.
 constexpr int kAhead = 16;
 template <typename I>
-__device__ __forceinline__ void load_ids(const LookArgs& a, int64_t t, int64_t end, I id[kAhead]) {
+__device__ __forceinline__ void load_ids(const LookArgs& a, int64_t t, int64_t end, uint32_t id[kAhead]) {
+  I v[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
     const int64_t at = t + 64 * i;
-    id[i] = static_cast<const I*>(a.ids)[at < end ? at : end - 1];
+    v[i] = static_cast<const I*>(a.ids)[at < end ? at : end - 1];
   }
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) id[i] = t + 64 * i < end ? id[i] : I{-1};
+  for (int i = 0; i < kAhead; ++i) {
+    const bool there = t + 64 * i < end && (sizeof(I) == 4 || static_cast<uint64_t>(v[i]) >> 32 == 0);
+    id[i] = there ? static_cast<uint32_t>(v[i]) : ~0u;
+  }
 }
 
 template <typename I>  // the ids' type
 __global__ __launch_bounds__(64 * kGroupWaves) void k_group(LookArgs a) {
   constexpr int NT = 64 * kGroupWaves;
   __shared__ int cursor[kLocal];
-  __shared__ int2 found[kGroupWaves][kFound];  // a wave's tokens of the class, in order, as many as fit
+  __shared__ uint32_t found[kGroupWaves][kFound];  // a wave's tokens of the class, in order: row, place in its range
   __shared__ int less[kGroupWaves], own[kGroupWaves], sums[kGroupWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = blockIdx.x;
   const int local = (a.rows + a.classes - 1) / a.classes;
@@ -100,30 +106,30 @@ __global__ __launch_bounds__(64 * kGroupWaves) void k_group(LookArgs a) {
   const int64_t end = begin + per < a.tokens ? begin + per : a.tokens;
   __syncthreads();
   int below = 0, hits = 0;
-  // The wave's tokens of the class, from place `at` of `out` on, the first
-  // `room` of them; below: those of lower classes.
-  auto search = [&](bool count, int2* out, int at, int room) {
+  // The wave's tokens of the class, in order: where(place, row, token).
+  auto search = [&](auto where) {
+    int at = 0;
     for (int64_t first = begin; first < end; first += 64 * kAhead) {
-      I id[kAhead];
-      load_ids(a, first + lane, end, id);
+      uint32_t id[kAhead];
+      load_ids<I>(a, first + lane, end, id);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const bool there = id[i] >= 0 && id[i] < a.rows;
-        const int c = static_cast<int>(id[i] & (a.classes - 1));
-        if (count) below += there && c < mine;
-        const bool hit = there && c == mine;
-        const uint64_t mask = __ballot(hit);
-        if (hit) {
-          const int row = static_cast<int>(id[i] >> a.shift), place = at + lanes_below(mask);
-          if (place < room) out[place] = make_int2(static_cast<int>(first + 64 * i) + lane, row);
-          if (count) atomicAdd(&cursor[row], 1);
+        const uint32_t c = id[i] < static_cast<uint32_t>(a.rows) ? id[i] & (a.classes - 1) : ~0u;
+        below += c < static_cast<uint32_t>(mine);
+        const uint64_t mask = __ballot(c == static_cast<uint32_t>(mine));
+        if (mask) {
+          if (c == static_cast<uint32_t>(mine))
+            where(at + lanes_below(mask), static_cast<int>(id[i] >> a.shift), static_cast<int>(first - begin) + 64 * i + lane);
+          at += __popcll(mask);
         }
-        at += __popcll(mask);
       }
     }
     return at;
   };
-  hits = search(true, found[wave], 0, kFound);
+  hits = search([&](int place, int row, int token) {
+    if (place < kFound) found[wave][place] = static_cast<uint32_t>(row) << kRange | token;
+    atomicAdd(&cursor[row], 1);
+  });
   below = wave_sum_int(below);
   if (lane == 0) less[wave] = below, own[wave] = hits;
   __syncthreads();
@@ -136,10 +142,14 @@ __global__ __launch_bounds__(64 * kGroupWaves) void k_group(LookArgs a) {
   }
   if (mine == a.classes - 1 && threadIdx.x == 0) *a.total = base + n;
   int2* stage = a.stage + base;
-  if (hits <= kFound) {
-    for (int i = lane; i < hits; i += 64) stage[at + i] = found[wave][i];
-  } else {
-    search(false, stage, at, n);  // (again: it has all the room)
+  const int token0 = static_cast<int>(begin);
+  if (hits <= kFound && per <= 1 << kRange) {
+    for (int i = lane; i < hits; i += 64) {
+      const uint32_t v = found[wave][i];
+      stage[at + i] = make_int2(token0 + static_cast<int>(v & ((1u << kRange) - 1)), static_cast<int>(v >> kRange));
+    }
+  } else {  // (once more: they did not fit)
+    search([&](int place, int row, int token) { stage[at + place] = make_int2(token0 + token, row); });
   }
   __syncthreads();
   // The rows' places: an exclusive scan of the counts, kLocal / NT a lane.
@@ -259,7 +269,7 @@ struct Columns {
 // Workgroups of the first `part_groups` sum parts, the others rows; blockIdx.y
 // is the slab of columns. A row's lanes read its place and count, then its
 // tokens, then their gradients: for kEach rows at once.
-constexpr int kEach = 4;
+constexpr int kEach = 2;
 template <typename T, int LX, int NC>
 __global__ __launch_bounds__(256) void k_row_sums(LookArgs a, int part_groups) {
   using Sum = Columns<LX, NC>;

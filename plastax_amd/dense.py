@@ -27,9 +27,10 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from plastax_amd import _lib
-from plastax_amd.lowbit import DTYPES, _call, _check, _launch, _on_gpu
+from plastax_amd.lowbit import DTYPES, _call, _launch, _on_gpu
 
 _IDS = {torch.int32: 0, torch.int64: 1}
 _KEEP = 64  # PLX_RECUR_KEEP
@@ -37,12 +38,27 @@ MAX_NAMED = 1024  # PLX_MAX_NAMED
 _MAX_TOKENS, _MAX_UNITS = 1 << 30, 1 << 24
 
 
+def _plain(who: str, t: torch.Tensor) -> torch.Tensor:
+    """``t`` without autograd, with the values that it stands for in its memory."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{who}: no autograd here; detach the argument and call the gradients")
+    # (the level is -1 outside of dual_level(), where no tensor has a tangent)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{who}: no forward-mode autograd here; unpack the argument and its tangent")
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def _batch(who: str, t: torch.Tensor) -> torch.Tensor:
     """``t`` checked, each token's units next to each other."""
-    t = _check(who, t)
-    if t.shape[0] > _MAX_TOKENS or t.shape[1] > _MAX_UNITS:
-        raise ValueError(f"{who}: at most 2^30 tokens and 2^24 units, got {tuple(t.shape)}")
-    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+    if t.dim() != 2:
+        raise ValueError(f"{who}: a batch [tokens, units] expected, got {t.dim()} dimensions")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{who}: float32, bfloat16 or float16 expected, got {t.dtype}")
+    tokens, units = t.shape
+    if tokens > _MAX_TOKENS or units > _MAX_UNITS:
+        raise ValueError(f"{who}: at most 2^30 tokens and 2^24 units, got {(tokens, units)}")
+    t = _plain(who, t)
+    return t if units <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
 def _ids(who: str, name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
@@ -50,21 +66,17 @@ def _ids(who: str, name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
         raise TypeError(f"{who}: {name} of int32 or int64 expected, got {t.dtype}")
     if t.dim() != dims:
         raise ValueError(f"{who}: {name} of {dims} dimensions expected, got {t.dim()}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _floats(who: str, name: str, t: torch.Tensor, shape: tuple[int, ...]) -> torch.Tensor:
     """A contiguous float32 argument beside a batch."""
     if t.dtype is not torch.float32:
         raise TypeError(f"{who}: {name} of float32 expected, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{who}: {name} of {shape} expected, got {tuple(t.shape)}")
-    return _plain(who, t).contiguous()
-
-
-def _plain(who: str, t: torch.Tensor) -> torch.Tensor:
-    """``t`` without autograd (:func:`plastax_amd.lowbit._check`'s rules, whatever its dimensions)."""
-    return _check(who, t if t.dim() == 2 else t.reshape(1, -1)).view(t.shape)
+    t = _plain(who, t)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _together(who: str, t: torch.Tensor, *others: torch.Tensor | None) -> None:
@@ -73,7 +85,7 @@ def _together(who: str, t: torch.Tensor, *others: torch.Tensor | None) -> None:
 
 def _space(device: torch.device, name: str, *args: object) -> tuple[torch.Tensor | None, int | None, int]:
     """The call's workspace: the tensor, its address and its bytes."""
-    need = _call(device, name, *args)
+    need = getattr(_lib.load(), name)(*args) if device.index == torch._C._cuda_getDevice() else _call(device, name, *args)
     if need < 0:
         raise ValueError(f"{name}: sizes out of range")
     if need == 0:
@@ -123,18 +135,13 @@ def look_up_grad(g: torch.Tensor, ids: torch.Tensor, rows: int, scale: float = 1
 # --------------------------------------------------------------------------
 # Layer norm
 # --------------------------------------------------------------------------
-def _params(who: str, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None) -> list[torch.Tensor | None]:
-    out: list[torch.Tensor | None] = []
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            out.append(None)
-            continue
-        if p.dtype not in (x.dtype, torch.float32) or p.dtype != weight.dtype:
-            raise TypeError(f"{who}: weight and bias both of {x.dtype} or of float32 expected, got {name} of {p.dtype}")
-        if tuple(p.shape) != (x.shape[1],):
-            raise ValueError(f"{who}: {name} of {x.shape[1]} units expected, got {tuple(p.shape)}")
-        out.append(_plain(who, p).contiguous())
-    return out
+def _param(who: str, name: str, x: torch.Tensor, p: torch.Tensor) -> torch.Tensor:
+    if p.dtype is not x.dtype and p.dtype is not torch.float32:
+        raise TypeError(f"{who}: weight and bias both of {x.dtype} or of float32 expected, got {name} of {p.dtype}")
+    if p.shape != x.shape[1:]:
+        raise ValueError(f"{who}: {name} of {x.shape[1]} units expected, got {tuple(p.shape)}")
+    p = _plain(who, p)
+    return p if p.is_contiguous() else p.contiguous()
 
 
 def normalise(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -149,7 +156,11 @@ def normalise(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     x = _batch("normalise", x)
     if not 0 <= eps < math.inf:
         raise ValueError(f"normalise: eps >= 0 expected, got {eps}")
-    weight, bias = _params("normalise", x, weight, bias)
+    weight = _param("normalise", "weight", x, weight)
+    if bias is not None:
+        if bias.dtype is not weight.dtype:
+            raise TypeError(f"normalise: weight and bias of one type expected, got {weight.dtype} and {bias.dtype}")
+        bias = _param("normalise", "bias", x, bias)
     _together("normalise", x, weight, bias)
     tokens, units = x.shape
     y = x.new_empty((tokens, units))
@@ -169,7 +180,7 @@ def normalise_grad(g: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         raise TypeError(f"normalise_grad: a gradient of x's type, {x.dtype}, expected, got {g.dtype}")
     if g.shape != x.shape:
         raise ValueError(f"normalise_grad: a gradient of {tuple(x.shape)} expected, got {tuple(g.shape)}")
-    weight, _ = _params("normalise_grad", x, weight, None)
+    weight = _param("normalise_grad", "weight", x, weight)
     tokens, units = x.shape
     kept = _floats("normalise_grad", "kept", kept, (tokens, 2))
     _together("normalise_grad", x, g, weight, kept)
@@ -240,7 +251,7 @@ def recur_grad(g: torch.Tensor, xz: torch.Tensor, kept: torch.Tensor, starts: to
     tokens = xz.shape[0]
     if g.dtype != xz.dtype:
         raise TypeError(f"recur_grad: a gradient of xz's type, {xz.dtype}, expected, got {g.dtype}")
-    if tuple(g.shape) != (tokens, units):
+    if g.shape != (tokens, units):
         raise ValueError(f"recur_grad: a gradient of {(tokens, units)} expected, got {tuple(g.shape)}")
     kept = _floats("recur_grad", "kept", kept, (-(-tokens // _KEEP), units))
     if g_last is not None:
@@ -267,9 +278,9 @@ def recur_step(xz: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
         raise ValueError(f"recur_step: x beside z, an even number of columns, expected, got {xz.shape[1]}")
     if state.dtype is not torch.float32:
         raise TypeError(f"recur_step: a state of float32 expected, got {state.dtype}")
-    if tuple(state.shape) != (sequences, units):
+    if state.shape != (sequences, units):
         raise ValueError(f"recur_step: a state of {(sequences, units)} expected, got {tuple(state.shape)}")
-    if _check("recur_step", state) is not state:
+    if _plain("recur_step", state) is not state:
         raise ValueError("recur_step: the state is updated in place: a negated view is not")
     if (units > 1 and state.stride(1) != 1) or (sequences > 1 and state.stride(0) < units):
         raise ValueError("recur_step: the state is updated in place: units next to each other and sequences apart "
@@ -290,9 +301,12 @@ def _named(who: str, logits: torch.Tensor, ids: torch.Tensor, top: torch.Tensor,
     if ids.shape[0] != logits.shape[0] or ids.shape[1] > MAX_NAMED:
         raise ValueError(f"{who}: ids of {logits.shape[0]} tokens and at most {MAX_NAMED} outputs each expected, "
                          f"got {tuple(ids.shape)}")
-    top = _check(who, top).contiguous()
+    if top.dtype not in DTYPES:
+        raise TypeError(f"{who}: top of float32, bfloat16 or float16 expected, got {top.dtype}")
     if top.shape != ids.shape:
         raise ValueError(f"{who}: top of {tuple(ids.shape)} expected, got {tuple(top.shape)}")
+    top = _plain(who, top)
+    top = top if top.is_contiguous() else top.contiguous()
     if not 0 < temperature < math.inf:
         raise ValueError(f"{who}: a temperature above 0 expected, got {temperature}")
     return logits, ids, top
