@@ -9,13 +9,15 @@
 #include "px_dense.h"
 
 using plx_detail::check_launch;
+using plx_detail::cu_count;
 using plx_detail::fail;
 
 namespace {
 
 using namespace px;
 
-constexpr int kNamed = PLX_MAX_NAMED;  // named outputs of a token at most: what they need is in LDS
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr double kLn2 = 0.693147180559945309;
 
 struct DistilArgs {
   int64_t tokens, outputs, line;
@@ -29,163 +31,249 @@ struct DistilArgs {
   float t;  // the temperature
 };
 
-// What a workgroup's waves share.
-template <int WAVES>
-struct DistilShared {
-  float top[WAVES], sum[WAVES];
-  float x[kNamed];
-  double p[kNamed], log_p[kNamed];
-  int id[kNamed];  // -1: names nothing
-  int any;
-};
-
 __device__ __forceinline__ float load_top(const DistilArgs& a, int64_t i) {
   if (a.top_type == PLX_LB_F32) return static_cast<const float*>(a.top)[i];
   if (a.top_type == PLX_LB_BF16) return to_f32(static_cast<const __bf16*>(a.top)[i]);
   return to_f32(static_cast<const _Float16*>(a.top)[i]);
 }
 
-// The waves' values joined, the same in every lane.
-template <int WAVES, typename F>
-__device__ __forceinline__ float over_waves(const float* part, F f) {
-  float v = part[threadIdx.x & (WAVES - 1)];
-#pragma unroll
-  for (int d = 1; d < WAVES; d *= 2) v = f(v, __shfl_xor(v, d, 64));
-  return v;
+// log2 of v > 0: its exponent, and the logarithm of a value from 0.5 to 1, so
+// that large sums lose nothing.
+__device__ __forceinline__ double log2_of(float v) {
+  if (!(v < INFINITY)) return v;  // (an infinity or a NaN)
+  return static_cast<double>(__builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(v))) +
+         static_cast<double>(__builtin_amdgcn_frexp_expf(v));
 }
 
-// The first wave's: the token's named outputs, their weights p, log p and
-// logits. In 64 bits, for the loss is a difference of logarithms (64 of 131072
-// outputs: nothing beside the row).
-template <int WAVES, typename T>
-__device__ __forceinline__ void name_outputs(const DistilArgs& a, int64_t token, const T* row,
-                                             DistilShared<WAVES>& sh) {
-  const int lane = threadIdx.x;
-  double m = -INFINITY;
+// A place of the teacher's: its weight p, the output (-1: none), its logit and
+// the teacher's.
+struct Named {
+  double p;
+  int id;
+  float x, top;
+};
+struct Teacher {
+  double largest, log_sum;  // of the teacher's logits; of exp((t - largest) / T)
+  bool any;
+};
+
+// One wave's: a token's places. In 64 bits, with log p kept apart, for the loss
+// is a difference of logarithms (64 of 131072 outputs: nothing beside the row).
+template <typename T>
+__device__ __forceinline__ Teacher name_outputs(const DistilArgs& a, int64_t token, const T* row, Named* named) {
+  const int lane = threadIdx.x & 63;
+  const double inv_t = 1.0 / a.t;
+  float m = -INFINITY;
   bool any = false;
   for (int i = lane; i < a.named; i += 64) {
     const int64_t id = load_id(a.ids, a.wide, token * a.named + i);
     const float t = load_top(a, token * a.named + i);
     const bool there = id >= 0 && id < a.outputs && t != -INFINITY;
-    sh.id[i] = there ? static_cast<int>(id) : -1;
-    sh.x[i] = there ? to_f32(row[id]) : 0.0f;
-    sh.log_p[i] = t;
+    named[i] = {0.0, there ? static_cast<int>(id) : -1, there ? to_f32(row[id]) : 0.0f, t};
     any |= there;
-    if (there) m = fmax(m, static_cast<double>(t));
+    if (there) m = fmaxf(m, t);
   }
-  any = __any(any);
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) m = fmax(m, __shfl_xor(m, d, 64));
+  m = wave_max(m);
   double sum = 0.0;
   for (int i = lane; i < a.named; i += 64) {
-    const double l = (sh.log_p[i] - m) / a.t, e = sh.id[i] >= 0 ? exp(l) : 0.0;
-    sh.log_p[i] = l;
-    sh.p[i] = e;
-    sum += e;
+    const double p = named[i].id >= 0 ? exp((static_cast<double>(named[i].top) - m) * inv_t) : 0.0;
+    named[i].p = p;
+    sum += p;
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
-  const double log_sum = log(sum);
-  for (int i = lane; i < a.named; i += 64) {
-    sh.p[i] /= sum;  // (only read where an output is named)
-    sh.log_p[i] -= log_sum;
-  }
-  if (lane == 0) sh.any = any;
+  const double inv = 1.0 / sum;
+  for (int i = lane; i < a.named; i += 64) named[i].p *= inv;  // (only read where an output is named)
+  return {m, log(sum), __any(any) != 0};
 }
 
-// The first wave's: the token's loss, from the row's largest logit and the sum
-// of exp((x - m) / T).
-template <int WAVES>
-__device__ __forceinline__ void write_loss(const DistilArgs& a, int64_t token, float m, float sum,
-                                           const DistilShared<WAVES>& sh) {
-  const int lane = threadIdx.x;
-  const double log_sum = log(static_cast<double>(sum));
+// What a row's values are taken from before the exponential: a logit's is
+// 2^(x c - shift), or 2^((x - m) c) where m is so large that m c is not finite
+// (a row of the type's lowest value alone).
+struct Shift {
+  float c, m, shift;
+  bool far;
+};
+__device__ __forceinline__ Shift shift_of(float m, float t) {
+  Shift s;
+  s.c = kLog2e / t, s.m = m, s.shift = m * s.c;
+  s.far = !(fabsf(s.shift) < 1e37f);
+  return s;
+}
+template <bool FAR>
+__device__ __forceinline__ float power(float x, const Shift& s) {
+  return __builtin_amdgcn_exp2f(FAR ? (x - s.m) * s.c : __builtin_fmaf(x, s.c, -s.shift));
+}
+
+// One wave's: the token's loss, from the sum of its outputs' powers (and what
+// the shift's rounding put into all of them).
+__device__ __forceinline__ void write_loss(const DistilArgs& a, int64_t token, const Shift& s, float sum,
+                                           const Teacher& t, const Named* named) {
+  const int lane = threadIdx.x & 63;
+  const double inv_t = 1.0 / a.t;
+  const double log_q = kLn2 * (log2_of(sum) - (s.far ? 0.0 : static_cast<double>(s.m) * s.c - s.shift));
   double loss = 0.0;
   for (int i = lane; i < a.named; i += 64) {
-    const double p = sh.p[i];
-    if (sh.id[i] >= 0 && !(p == 0.0))
-      loss += p * (sh.log_p[i] - (static_cast<double>(sh.x[i]) - m) / a.t + log_sum);
+    const Named v = named[i];
+    const double d = ((v.top - t.largest) - (static_cast<double>(v.x) - s.m)) * inv_t - t.log_sum + log_q;
+    if (v.id >= 0 && v.p != 0.0) loss += v.p * d;
   }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) loss += __shfl_xor(loss, d, 64);
-  if (lane == 0) a.loss[token] = sh.any ? static_cast<float>(loss * a.t * a.t) : 0.0f;
+  if (lane == 0) a.loss[token] = t.any ? static_cast<float>(loss * a.t * a.t) : 0.0f;
 }
 
 // The gradient at the named outputs, after the others' (the same output named
 // twice is written twice with the same value).
-template <int WAVES, typename T>
-__device__ __forceinline__ void write_named(const DistilArgs& a, T* out, float m, float c, float scale, float sum,
-                                            const DistilShared<WAVES>& sh) {
-  for (int i = threadIdx.x; i < a.named; i += WAVES * 64) {
-    const int id = sh.id[i];
-    if (id < 0) continue;
+template <int NT, typename T>
+__device__ __forceinline__ void write_named(const DistilArgs& a, T* out, const Shift& s, float scale, float r,
+                                            const Named* named) {
+  for (int i = threadIdx.x % NT; i < a.named; i += NT) {
+    const Named v = named[i];
+    if (v.id < 0) continue;
     double p = 0.0;
-    for (int j = 0; j < a.named; ++j) p += sh.id[j] == id ? sh.p[j] : 0.0;
-    const double q = static_cast<double>(__builtin_amdgcn_exp2f((sh.x[i] - m) * c)) / sum;
-    out[id] = from_f32<T>(static_cast<float>((q - p) * scale));
+    for (int j = 0; j < a.named; ++j) p += named[j].id == v.id ? named[j].p : 0.0;
+    const float q = s.far ? power<true>(v.x, s) : power<false>(v.x, s);
+    out[v.id] = from_f32<T>(static_cast<float>(static_cast<double>(q) * r - p * scale));
   }
 }
 
-// A workgroup per token. The row stays in registers, NC chunks of 16 bytes a
-// lane: it is read once and its gradient written once.
+// The waves' values joined, the same in every lane.
+template <int WAVES, typename F>
+__device__ __forceinline__ float over_waves(float v, float* part, F f) {
+  if (WAVES == 1) return v;
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = part[threadIdx.x & (WAVES - 1)];
+#pragma unroll
+  for (int d = 1; d < WAVES; d *= 2) v = f(v, __shfl_xor(v, d, 64));
+  return v;
+}
+
+// A row's chunks of 16 bytes without a branch in their loads: chunks past the
+// last whole one are read as the row's last 16 bytes, of which the values
+// behind the last whole chunk are its rest. (Rows of less than a chunk are
+// read value by value.)
+template <typename T, int NT, int NC>
+struct RowChunks {
+  static constexpr int W = kChunk<T>;
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  words v[NC];
+  __device__ __forceinline__ static int at(int k) { return (k * NT + static_cast<int>(threadIdx.x % NT)) * W; }
+  __device__ __forceinline__ void load(const T* row, int outputs) {
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      if (NC == 1 && NT == 64 && outputs < W)
+        v[k] = __builtin_bit_cast(words, load_pack<W>(row + at(k), outputs - at(k), -INFINITY));
+      else
+        v[k] = __builtin_bit_cast(
+            words, __builtin_nontemporal_load(reinterpret_cast<const typename Pack<T, W>::load*>(
+                       row + (at(k) + W <= outputs ? at(k) : outputs - W))));
+    }
+  }
+  __device__ __forceinline__ float get(int k, int i) const {
+    return to_f32(__builtin_bit_cast(typename Pack<T, W>::type, v[k])[i]);
+  }
+  // As new to the compiler, which would keep every value as float32 from one
+  // pass over them to the next.
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int k = 0; k < NC; ++k) asm volatile("" : "+v"(v[k]));
+  }
+  __device__ __forceinline__ float largest() const {
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+      for (int i = 0; i < W; ++i) m = fmaxf(m, get(k, i));
+    return m;
+  }
+  // f(k, first): values from `first` to W of the lane's chunk k are the row's.
+  template <typename F>
+  __device__ __forceinline__ void each(int outputs, F f) const {
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      if (at(k) + W <= outputs)
+        f(k, 0);
+      else if (at(k) < outputs)
+        f(k, outputs < W ? 0 : at(k) + W - outputs);
+    }
+  }
+  template <bool FAR>
+  __device__ __forceinline__ float sum(int outputs, const Shift& s) const {
+    float all = 0.0f;
+    each(outputs, [&](int k, int first) {
+      float part = 0.0f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float e = power<FAR>(get(k, i), s);
+        part += i < first || (NC == 1 && i >= outputs) ? 0.0f : e;
+      }
+      all += part;
+    });
+    return all;
+  }
+  template <bool FAR>
+  __device__ __forceinline__ void gradient(T* out, int outputs, const Shift& s, float r) const {
+    each(outputs, [&](int k, int first) {
+      float d[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) d[i] = power<FAR>(get(k, i), s) * r;
+      if (first == 0) {
+        store_pack<W, true>(out + at(k), outputs - at(k), d);
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+          if (i >= first) out[outputs - W + i] = from_f32<T>(d[i]);
+      }
+    });
+  }
+  __device__ __forceinline__ void zeros(T* out, int outputs) const {
+    const float d[W] = {};
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+      if (at(k) < outputs) store_pack<W, true>(out + at(k), outputs - at(k), d);
+  }
+};
+
+// A workgroup a token. The row stays in registers, NC
+// chunks a lane: it is read once and its gradient written once. The first wave
+// looks at the teacher's places before it loads the row (registers).
 template <typename T, int WAVES, int NC, bool GRAD>
 __global__ __launch_bounds__(WAVES * 64) void k_distil_row(DistilArgs a) {
-  constexpr int W = kChunk<T>, NT = WAVES * 64;
-  __shared__ DistilShared<WAVES> sh;
+  constexpr int NT = WAVES * 64;
+  extern __shared__ Named named[];
+  __shared__ float part[2][WAVES];
+  __shared__ int some;
   const int64_t token = blockIdx.x;
+  const int outputs = static_cast<int>(a.outputs);
+  const bool first = WAVES == 1 || threadIdx.x < 64;
   const T* row = static_cast<const T*>(a.x) + token * a.line;
-  typename Pack<T, W>::type v[NC];
-#pragma unroll
-  for (int k = 0; k < NC; ++k) {
-    const int64_t at = (static_cast<int64_t>(k) * NT + threadIdx.x) * W;
-    v[k] = load_pack<W, true>(row + at, a.outputs - at, -INFINITY);
+  Teacher teacher{};
+  if (first) teacher = name_outputs(a, token, row, named);
+  if (WAVES > 1 && threadIdx.x == 0) some = teacher.any;
+  RowChunks<T, NT, NC> chunks;
+  if (outputs > 0) chunks.load(row, outputs);
+  const float m = over_waves<WAVES>(wave_max(outputs > 0 ? chunks.largest() : -INFINITY), part[0],
+                                    [](float a, float b) { return fmaxf(a, b); });
+  const Shift s = shift_of(m, a.t);
+  chunks.again();
+  float sum = wave_sum(s.far ? chunks.template sum<true>(outputs, s) : chunks.template sum<false>(outputs, s));
+  sum = over_waves<WAVES>(sum, part[1], [](float a, float b) { return a + b; });
+  if (GRAD) {
+    T* out = static_cast<T*>(a.dx) + token * a.outputs;
+    const float scale = a.g[token] * a.t, r = scale / sum;
+    chunks.again();
+    if (!(WAVES > 1 ? some != 0 : teacher.any))
+      chunks.zeros(out, outputs);
+    else if (s.far)
+      chunks.template gradient<true>(out, outputs, s, r);
+    else
+      chunks.template gradient<false>(out, outputs, s, r);
+    if (WAVES > 1) __syncthreads();
+    write_named<NT>(a, out, s, scale, r, named);
   }
-  if (threadIdx.x < 64) name_outputs<WAVES>(a, token, row, sh);
-  const float c = 1.44269504088896341f / a.t;
-  float m = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < NC; ++k)
-#pragma unroll
-    for (int i = 0; i < W; ++i) m = fmaxf(m, to_f32(v[k][i]));
-  m = wave_max(m);
-  if ((threadIdx.x & 63) == 0) sh.top[threadIdx.x >> 6] = m;
-  __syncthreads();
-  m = over_waves<WAVES>(sh.top, [](float a, float b) { return fmaxf(a, b); });
-  // (x - m first: logits of the type's lowest value, and rows of nothing else,
-  // stay finite)
-  float sum = 0.0f;
-#pragma unroll
-  for (int k = 0; k < NC; ++k) {
-    if ((static_cast<int64_t>(k) * NT + threadIdx.x) * W >= a.outputs) break;
-    float part = 0.0f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const float x = to_f32(v[k][i]);
-      part += __builtin_amdgcn_exp2f((x - m) * c);
-    }
-    sum += part;
-  }
-  sum = wave_sum(sum);
-  if ((threadIdx.x & 63) == 0) sh.sum[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  sum = over_waves<WAVES>(sh.sum, [](float a, float b) { return a + b; });
-  if (threadIdx.x < 64) write_loss<WAVES>(a, token, m, sum, sh);
-  if (!GRAD) return;
-  T* out = static_cast<T*>(a.dx) + token * a.outputs;
-  const bool any = sh.any;
-  const float scale = a.g[token] * a.t, r = scale / sum;
-#pragma unroll
-  for (int k = 0; k < NC; ++k) {
-    const int64_t at = (static_cast<int64_t>(k) * NT + threadIdx.x) * W;
-    if (at >= a.outputs) break;
-    float d[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-      d[i] = any ? __builtin_amdgcn_exp2f((to_f32(v[k][i]) - m) * c) * r : 0.0f;
-    store_pack<W, true>(out + at, a.outputs - at, d);
-  }
-  __syncthreads();
-  write_named<WAVES>(a, out, m, c, scale, sum, sh);
+  if (first) write_loss(a, token, s, sum, teacher, named);
 }
 
 // Rows that no registers hold: a lane's largest logit and its sum go along the
@@ -193,72 +281,89 @@ __global__ __launch_bounds__(WAVES * 64) void k_distil_row(DistilArgs a) {
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(1024) void k_distil_stream(DistilArgs a) {
   constexpr int W = kChunk<T>, WAVES = 16, NT = 1024;
-  __shared__ DistilShared<WAVES> sh;
+  extern __shared__ Named named[];
+  __shared__ float part[2][WAVES];
+  __shared__ int some;
   const int64_t token = blockIdx.x;
   const T* row = static_cast<const T*>(a.x) + token * a.line;
-  if (threadIdx.x < 64) name_outputs<WAVES>(a, token, row, sh);
-  const float c = 1.44269504088896341f / a.t;
+  Teacher teacher{};
+  if (threadIdx.x < 64) teacher = name_outputs(a, token, row, named);
+  if (threadIdx.x == 0) some = teacher.any;
+  const float c = kLog2e / a.t;
   float m = -INFINITY, sum = 0.0f;
   for (int64_t at = static_cast<int64_t>(threadIdx.x) * W; at < a.outputs; at += NT * W) {
     const typename Pack<T, W>::type v = load_pack<W>(row + at, a.outputs - at, -INFINITY);
-    float top = m, part = 0.0f;
+    float top = m, more = 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) top = fmaxf(top, to_f32(v[i]));
     const float from = top == -INFINITY ? 0.0f : top;  // (a lane without a logit above -inf has the sum 0)
 #pragma unroll
-    for (int i = 0; i < W; ++i) part += __builtin_amdgcn_exp2f((to_f32(v[i]) - from) * c);
-    sum = sum * (m == top ? 1.0f : __builtin_amdgcn_exp2f((m - top) * c)) + part;
+    for (int i = 0; i < W; ++i) more += __builtin_amdgcn_exp2f((to_f32(v[i]) - from) * c);
+    sum = sum * (m == top ? 1.0f : __builtin_amdgcn_exp2f((m - top) * c)) + more;
     m = top;
   }
   const float own = m;
-  m = wave_max(m);
-  if ((threadIdx.x & 63) == 0) sh.top[threadIdx.x >> 6] = m;
-  __syncthreads();
-  m = over_waves<WAVES>(sh.top, [](float a, float b) { return fmaxf(a, b); });
+  m = over_waves<WAVES>(wave_max(m), part[0], [](float a, float b) { return fmaxf(a, b); });
   sum = wave_sum(sum * (own == m ? 1.0f : __builtin_amdgcn_exp2f((own - m) * c)));
-  if ((threadIdx.x & 63) == 0) sh.sum[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  sum = over_waves<WAVES>(sh.sum, [](float a, float b) { return a + b; });
-  if (threadIdx.x < 64) write_loss<WAVES>(a, token, m, sum, sh);
-  if (!GRAD) return;
-  T* out = static_cast<T*>(a.dx) + token * a.outputs;
-  const bool any = sh.any;
-  const float scale = a.g[token] * a.t, r = scale / sum;
-  for (int64_t at = static_cast<int64_t>(threadIdx.x) * W; at < a.outputs; at += NT * W) {
-    const typename Pack<T, W>::type v = load_pack<W, true>(row + at, a.outputs - at);
-    float d[W];
+  sum = over_waves<WAVES>(sum, part[1], [](float a, float b) { return a + b; });
+  Shift s = shift_of(m, a.t);
+  s.far = true;  // (as the sum was made)
+  if (GRAD) {
+    T* out = static_cast<T*>(a.dx) + token * a.outputs;
+    const float scale = a.g[token] * a.t, r = scale / sum;
+    const bool any = some != 0;
+    for (int64_t at = static_cast<int64_t>(threadIdx.x) * W; at < a.outputs; at += NT * W) {
+      const typename Pack<T, W>::type v = load_pack<W, true>(row + at, a.outputs - at);
+      float d[W];
 #pragma unroll
-    for (int i = 0; i < W; ++i) d[i] = any ? __builtin_amdgcn_exp2f((to_f32(v[i]) - m) * c) * r : 0.0f;
-    store_pack<W, true>(out + at, a.outputs - at, d);
+      for (int i = 0; i < W; ++i) d[i] = any ? power<true>(to_f32(v[i]), s) * r : 0.0f;
+      store_pack<W, true>(out + at, a.outputs - at, d);
+    }
+    __syncthreads();
+    write_named<NT>(a, out, s, scale, r, named);
   }
-  __syncthreads();
-  write_named<WAVES>(a, out, m, c, scale, sum, sh);
+  if (threadIdx.x < 64) write_loss(a, token, s, sum, teacher, named);
 }
 
+template <typename T, int WAVES, int NC, bool GRAD>
+void launch_row(const DistilArgs& a, hipStream_t s) {
+  k_distil_row<T, WAVES, NC, GRAD><<<static_cast<unsigned>(a.tokens), WAVES * 64, a.named * sizeof(Named), s>>>(a);
+}
+
+// Few waves with many chunks where there are tokens enough for every CU (a
+// token's places are looked at by one wave), else many with few.
 template <typename T, bool GRAD>
 void launch_distil(const DistilArgs& a, hipStream_t s) {
-  const unsigned rows = static_cast<unsigned>(a.tokens);
   const int64_t chunks = div_up(a.outputs, kChunk<T>);
+  const bool few = a.tokens < 2 * cu_count();
   if (chunks <= 64)
-    k_distil_row<T, 1, 1, GRAD><<<rows, 64, 0, s>>>(a);
+    launch_row<T, 1, 1, GRAD>(a, s);
+  else if (chunks <= 256 && few)
+    launch_row<T, 4, 1, GRAD>(a, s);
+  else if (chunks <= 128)
+    launch_row<T, 1, 2, GRAD>(a, s);
   else if (chunks <= 256)
-    k_distil_row<T, 4, 1, GRAD><<<rows, 256, 0, s>>>(a);
+    launch_row<T, 1, 4, GRAD>(a, s);
+  else if (chunks <= 1024 && few)
+    launch_row<T, 16, 1, GRAD>(a, s);
   else if (chunks <= 512)
-    k_distil_row<T, 4, 2, GRAD><<<rows, 256, 0, s>>>(a);
+    launch_row<T, 4, 2, GRAD>(a, s);
   else if (chunks <= 1024)
-    k_distil_row<T, 4, 4, GRAD><<<rows, 256, 0, s>>>(a);
+    launch_row<T, 4, 4, GRAD>(a, s);
   else if (chunks <= 2048)
-    k_distil_row<T, 8, 4, GRAD><<<rows, 512, 0, s>>>(a);
+    launch_row<T, 8, 4, GRAD>(a, s);
   else if (chunks <= 4096)
-    k_distil_row<T, 16, 4, GRAD><<<rows, 1024, 0, s>>>(a);
+    launch_row<T, 16, 4, GRAD>(a, s);
   else if (chunks <= 8192)
-    k_distil_row<T, 16, 8, GRAD><<<rows, 1024, 0, s>>>(a);
+    launch_row<T, 16, 8, GRAD>(a, s);
+  else if (chunks <= 16384)
+    launch_row<T, 16, 16, GRAD>(a, s);
   else
-    k_distil_stream<T, GRAD><<<rows, 1024, 0, s>>>(a);
+    k_distil_stream<T, GRAD><<<static_cast<unsigned>(a.tokens), 1024, a.named * sizeof(Named), s>>>(a);
 }
 
 int run_distil(const char* who, bool grad, const DistilArgs& all, int dtype, void* stream) {
-  if (!batch_fits(all.tokens, all.outputs) || all.named < 0 || all.named > kNamed || all.wide < 0 || all.wide > 1)
+  if (!batch_fits(all.tokens, all.outputs) || all.named < 0 || all.named > PLX_MAX_NAMED || all.wide < 0 || all.wide > 1)
     return fail(PLX_ERR_INVALID, who);
   if (!known_type(dtype) || !known_type(all.top_type)) return fail(PLX_ERR_UNSUPPORTED, who);
   if (!(all.t > 0.0f && all.t < INFINITY)) return fail(PLX_ERR_INVALID, who);

@@ -62,15 +62,34 @@ __device__ __forceinline__ int64_t load_id(const void* p, int wide, int64_t i) {
   return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
 }
 
+// Over a wave's lanes, the same in all of them: within rows of 16 lanes, then
+// over the rows, by the vector unit's own lane shifts (a shuffle goes through
+// LDS); always in the same order.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ float from_lane(float v, float other) {
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(__float_as_int(other), __float_as_int(v), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ float last_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d, 64);
-  return v;
+  v += from_lane<0x111>(v, 0.0f);  // from 1, 2, 4, 8 lanes below in the row
+  v += from_lane<0x112>(v, 0.0f);
+  v += from_lane<0x114>(v, 0.0f);
+  v += from_lane<0x118>(v, 0.0f);
+  v += from_lane<0x142, 0xA>(v, 0.0f);  // rows 0 and 2 to 1 and 3
+  v += from_lane<0x143, 0xC>(v, 0.0f);  // both to rows 2 and 3
+  return last_lane(v);
 }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v = fmaxf(v, __shfl_xor(v, d, 64));
-  return v;
+  v = fmaxf(v, from_lane<0x111>(v, v));
+  v = fmaxf(v, from_lane<0x112>(v, v));
+  v = fmaxf(v, from_lane<0x114>(v, v));
+  v = fmaxf(v, from_lane<0x118>(v, v));
+  v = fmaxf(v, from_lane<0x142, 0xA>(v, v));
+  v = fmaxf(v, from_lane<0x143, 0xC>(v, v));
+  return last_lane(v);
 }
 
 template <typename F>
