@@ -28,7 +28,9 @@ struct DistilArgs {
   float* loss;
   void* dx;
   int named, wide, top_type;
-  float t;  // the temperature
+  int whole;  // the gradient's rows begin on 64 bytes: its stores go past the caches (in rows that do not they
+              // would leave parts of lines: 2048 x 32003 bf16 60 us, past the caches 65)
+  float t;    // the temperature
 };
 
 __device__ __forceinline__ float load_top(const DistilArgs& a, int64_t i) {
@@ -159,24 +161,32 @@ struct RowChunks {
   static constexpr int W = kChunk<T>;
   typedef uint32_t words __attribute__((ext_vector_type(4)));
   words v[NC];
-  __device__ __forceinline__ static int at(int k) { return (k * NT + static_cast<int>(threadIdx.x % NT)) * W; }
+  int lane;
+  __device__ __forceinline__ int at(int k) const { return (k * NT + lane) * W; }
   __device__ __forceinline__ void load(const T* row, int outputs) {
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       if (NC == 1 && NT == 64 && outputs < W)
         v[k] = __builtin_bit_cast(words, load_pack<W>(row + at(k), outputs - at(k), -INFINITY));
       else
-        v[k] = __builtin_bit_cast(
-            words, __builtin_nontemporal_load(reinterpret_cast<const typename Pack<T, W>::load*>(
-                       row + (at(k) + W <= outputs ? at(k) : outputs - W))));
+        v[k] = __builtin_bit_cast(words, __builtin_nontemporal_load(chunk<const typename Pack<T, W>::load>(
+                                             row, at(k) + W <= outputs ? at(k) : outputs - W)));
     }
+  }
+  // The chunk at a value of a row (by the row's address, the same in all lanes,
+  // and a lane's 32 bits).
+  template <typename V, typename R>
+  __device__ __forceinline__ static V* chunk(R* row, int at) {
+    typedef typename std::conditional<std::is_const<V>::value, const char, char>::type byte;
+    return reinterpret_cast<V*>(reinterpret_cast<byte*>(row) + static_cast<unsigned>(at * static_cast<int>(sizeof(T))));
   }
   __device__ __forceinline__ float get(int k, int i) const {
     return to_f32(__builtin_bit_cast(typename Pack<T, W>::type, v[k])[i]);
   }
   // As new to the compiler, which would keep every value as float32 from one
-  // pass over them to the next.
+  // pass over them to the next, and every chunk's place.
   __device__ __forceinline__ void again() {
+    asm volatile("" : "+v"(lane));
 #pragma unroll
     for (int k = 0; k < NC; ++k) asm volatile("" : "+v"(v[k]));
   }
@@ -214,31 +224,47 @@ struct RowChunks {
     return all;
   }
   template <bool FAR>
-  __device__ __forceinline__ void gradient(T* out, int outputs, const Shift& s, float r) const {
-    each(outputs, [&](int k, int first) {
-      float d[W];
+  __device__ __forceinline__ void gradient(T* out, int outputs, int whole, const Shift& s, float r) const {
 #pragma unroll
-      for (int i = 0; i < W; ++i) d[i] = power<FAR>(get(k, i), s) * r;
-      if (first == 0) {
-        store_pack<W, true>(out + at(k), outputs - at(k), d);
+    for (int k = 0; k < NC; ++k)
+      if (at(k) < outputs) gradient<FAR>(out, outputs, whole, s, r, k);
+  }
+  template <bool FAR>
+  __device__ __forceinline__ void gradient(T* out, int outputs, int whole, const Shift& s, float r, int k) const {
+    float d[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) d[i] = power<FAR>(get(k, i), s) * r;
+    if (at(k) + W <= outputs) {
+      typename Pack<T, W>::load y;
+#pragma unroll
+      for (int i = 0; i < W; ++i) y[i] = from_f32<T>(d[i]);
+      typename Pack<T, W>::load* p = chunk<typename Pack<T, W>::load>(out, at(k));
+      if (whole) {
+        __builtin_nontemporal_store(y, p);
       } else {
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-          if (i >= first) out[outputs - W + i] = from_f32<T>(d[i]);
+        asm volatile("");  // (or the two become one store, through the caches)
+        *p = y;
+        asm volatile("");
       }
-    });
+    } else if (outputs < W) {
+      store_pack<W>(out, outputs, d);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (i >= at(k) + W - outputs) out[outputs - W + i] = from_f32<T>(d[i]);
+    }
   }
   __device__ __forceinline__ void zeros(T* out, int outputs) const {
     const float d[W] = {};
 #pragma unroll
     for (int k = 0; k < NC; ++k)
-      if (at(k) < outputs) store_pack<W, true>(out + at(k), outputs - at(k), d);
+      if (at(k) < outputs) store_pack<W>(out + at(k), outputs - at(k), d);
   }
 };
 
-// A workgroup a token. The row stays in registers, NC
-// chunks a lane: it is read once and its gradient written once. The first wave
-// looks at the teacher's places before it loads the row (registers).
+// A workgroup a token. The row stays in registers, NC chunks a lane: it is read
+// once and its gradient written once. The first wave looks at the teacher's
+// places before it loads the row (registers).
 template <typename T, int WAVES, int NC, bool GRAD>
 __global__ __launch_bounds__(WAVES * 64) void k_distil_row(DistilArgs a) {
   constexpr int NT = WAVES * 64;
@@ -253,6 +279,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_distil_row(DistilArgs a) {
   if (first) teacher = name_outputs(a, token, row, named);
   if (WAVES > 1 && threadIdx.x == 0) some = teacher.any;
   RowChunks<T, NT, NC> chunks;
+  chunks.lane = threadIdx.x;
   if (outputs > 0) chunks.load(row, outputs);
   const float m = over_waves<WAVES>(wave_max(outputs > 0 ? chunks.largest() : -INFINITY), part[0],
                                     [](float a, float b) { return fmaxf(a, b); });
@@ -267,9 +294,9 @@ __global__ __launch_bounds__(WAVES * 64) void k_distil_row(DistilArgs a) {
     if (!(WAVES > 1 ? some != 0 : teacher.any))
       chunks.zeros(out, outputs);
     else if (s.far)
-      chunks.template gradient<true>(out, outputs, s, r);
+      chunks.template gradient<true>(out, outputs, a.whole, s, r);
     else
-      chunks.template gradient<false>(out, outputs, s, r);
+      chunks.template gradient<false>(out, outputs, a.whole, s, r);
     if (WAVES > 1) __syncthreads();
     write_named<NT>(a, out, s, scale, r, named);
   }
@@ -327,7 +354,8 @@ __global__ __launch_bounds__(1024) void k_distil_stream(DistilArgs a) {
 
 template <typename T, int WAVES, int NC, bool GRAD>
 void launch_row(const DistilArgs& a, hipStream_t s) {
-  k_distil_row<T, WAVES, NC, GRAD><<<static_cast<unsigned>(a.tokens), WAVES * 64, a.named * sizeof(Named), s>>>(a);
+  k_distil_row<T, WAVES, NC, GRAD>
+      <<<static_cast<unsigned>(a.tokens), WAVES * 64, a.named * sizeof(Named), s>>>(a);
 }
 
 // Few waves with many chunks where there are tokens enough for every CU (a
@@ -347,13 +375,13 @@ void launch_distil(const DistilArgs& a, hipStream_t s) {
   else if (chunks <= 1024 && few)
     launch_row<T, 16, 1, GRAD>(a, s);
   else if (chunks <= 512)
-    launch_row<T, 4, 2, GRAD>(a, s);
+    launch_row<T, 2, 4, GRAD>(a, s);
   else if (chunks <= 1024)
-    launch_row<T, 4, 4, GRAD>(a, s);
+    launch_row<T, 2, 8, GRAD>(a, s);
   else if (chunks <= 2048)
-    launch_row<T, 8, 4, GRAD>(a, s);
+    launch_row<T, 4, 8, GRAD>(a, s);
   else if (chunks <= 4096)
-    launch_row<T, 16, 4, GRAD>(a, s);
+    launch_row<T, 8, 8, GRAD>(a, s);
   else if (chunks <= 8192)
     launch_row<T, 16, 8, GRAD>(a, s);
   else if (chunks <= 16384)
@@ -385,6 +413,7 @@ int run_distil(const char* who, bool grad, const DistilArgs& all, int dtype, voi
       if (grad) {
         a.g = all.g + first;
         a.dx = static_cast<T*>(all.dx) + first * all.outputs;
+        a.whole = ((reinterpret_cast<uintptr_t>(a.dx) | (a.outputs * sizeof(T))) & 63) == 0;
         launch_distil<T, true>(a, s);
       } else {
         launch_distil<T, false>(a, s);
