@@ -16,6 +16,8 @@ namespace {
 
 using namespace px;
 
+constexpr int kRows = 4;  // rows that a group of waves takes at a time, forwards
+
 struct NormArgs {
   int64_t tokens, x_line, g_line;
   int units;
@@ -29,69 +31,119 @@ struct NormArgs {
   float* part;   // [workgroups][2][units]
 };
 
-// Two sums over the WAVES waves that share a row. One barrier: the next sums
-// take another `part`.
-template <int WAVES>
-__device__ __forceinline__ float2 row_sum2(float a, float b, float2* part) {
-  a = wave_sum(a), b = wave_sum(b);
-  if (WAVES == 1) return make_float2(a, b);
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) part[wave] = make_float2(a, b);
-  __syncthreads();
-  float2 s = part[wave / WAVES * WAVES + (threadIdx.x & (WAVES - 1))];
+// N sums over the WAVES waves that share rows. One barrier: the next sums take
+// another `part`.
+template <int WAVES, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*part)[N]) {
 #pragma unroll
-  for (int d = 1; d < WAVES; d *= 2) s.x += __shfl_xor(s.x, d, 64), s.y += __shfl_xor(s.y, d, 64);
-  return s;
+  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  if (WAVES == 1) return;
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[wave][i] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = part[wave / WAVES * WAVES + (threadIdx.x & (WAVES - 1))][i];
+#pragma unroll
+    for (int d = 1; d < WAVES; d *= 2) v[i] += __shfl_xor(v[i], d, 64);
+  }
 }
 
-// ROWS rows a workgroup, each of WAVES waves, NC chunks of 16 bytes a lane.
-// The variance is the mean of the squares of x - mean, from registers.
-template <typename T, typename P, int ROWS, int WAVES, int NC>
+template <int WAVES>
+__device__ __forceinline__ float row_sum(float v, float (*part)[1]) {
+  float sums[1] = {v};
+  row_sums<WAVES>(sums, part);
+  return sums[0];
+}
+
+// R rows' chunks at `at`, one branch for all of them.
+template <int R, typename T>
+__device__ __forceinline__ void load_rows(const T* const (&row)[R], int at, int units,
+                                          typename Pack<T, kChunk<T>>::type (&v)[R]) {
+  constexpr int W = kChunk<T>;
+  if (at + W <= units) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = *reinterpret_cast<const typename Pack<T, W>::load*>(row[r] + at);
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = load_pack<W>(row[r] + at, units - at);
+  }
+}
+
+// ROWS groups of WAVES waves, NC chunks of 16 bytes a lane. A group takes R
+// rows at a time, for which it waits once, and goes on to gridDim.x * ROWS * R
+// rows further: a lane's weights stay in registers. The variance is the mean of
+// the squares of x - mean, from registers.
+template <typename T, typename P, int ROWS, int WAVES, int NC, int R>
 __global__ __launch_bounds__(ROWS* WAVES * 64) void k_normalise(NormArgs a) {
   constexpr int W = kChunk<T>, NT = WAVES * 64;
-  __shared__ float2 part[2][ROWS * WAVES];
+  __shared__ float part[2][ROWS * WAVES][R];
   const int lane = threadIdx.x % NT;
-  const int64_t token = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / NT;
-  const bool there = token < a.tokens;
-  const T* row = static_cast<const T*>(a.x) + (there ? token : 0) * a.x_line;
-  float v[NC][W];
-  float sum = 0.0f;
-#pragma unroll
-  for (int k = 0; k < NC; ++k) {
-    const int at = (k * NT + lane) * W;
-    const typename Pack<T, W>::type x = load_pack<W>(row + at, a.units - at);
-#pragma unroll
-    for (int i = 0; i < W; ++i) v[k][i] = to_f32(x[i]), sum += v[k][i];
-  }
   const float inv = 1.0f / static_cast<float>(a.units);
-  const float mean = row_sum2<WAVES>(sum, 0.0f, part[0]).x * inv;
-  float square = 0.0f;
-#pragma unroll
-  for (int k = 0; k < NC; ++k)
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      v[k][i] = (k * NT + lane) * W + i < a.units ? v[k][i] - mean : 0.0f;
-      square = __builtin_fmaf(v[k][i], v[k][i], square);
-    }
-  const float var = row_sum2<WAVES>(square, 0.0f, part[1]).x * inv;
-  const float r = 1.0f / sqrtf(var + a.eps);
-  if (!there) return;
-  if (lane == 0) reinterpret_cast<float2*>(a.kept)[token] = make_float2(mean, r);
-  T* out = static_cast<T*>(a.y) + token * a.units;
+  float w[NC][W], b[NC][W];
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
     const int at = (k * NT + lane) * W;
-    if (at >= a.units) break;
-    const typename Pack<P, W>::type w = load_pack<W>(static_cast<const P*>(a.weight) + at, a.units - at);
-    float y[W];
+    const typename Pack<P, W>::type p = load_pack<W>(static_cast<const P*>(a.weight) + at, a.units - at);
 #pragma unroll
-    for (int i = 0; i < W; ++i) y[i] = v[k][i] * r * to_f32(w[i]);
+    for (int i = 0; i < W; ++i) w[k][i] = to_f32(p[i]), b[k][i] = 0.0f;
     if (a.bias) {
-      const typename Pack<P, W>::type b = load_pack<W>(static_cast<const P*>(a.bias) + at, a.units - at);
+      const typename Pack<P, W>::type q = load_pack<W>(static_cast<const P*>(a.bias) + at, a.units - at);
 #pragma unroll
-      for (int i = 0; i < W; ++i) y[i] += to_f32(b[i]);
+      for (int i = 0; i < W; ++i) b[k][i] = to_f32(q[i]);
     }
-    store_pack<W>(out + at, a.units - at, y);
+  }
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS * R; first < a.tokens;
+       first += static_cast<int64_t>(gridDim.x) * ROWS * R) {
+    const int64_t token = first + threadIdx.x / NT * R;
+    const T* row[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      row[r] = static_cast<const T*>(a.x) + (token + r < a.tokens ? token + r : first) * a.x_line;
+    typename Pack<T, W>::type x[NC][R];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) load_rows<R>(row, (k * NT + lane) * W, a.units, x[k]);
+    float mean[R] = {}, r1[R] = {};
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < W; ++i) mean[r] += to_f32(x[k][r][i]);
+    row_sums<WAVES>(mean, part[0]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) mean[r] *= inv;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int left = a.units - (k * NT + lane) * W;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const float d = i < left ? to_f32(x[k][r][i]) - mean[r] : 0.0f;
+          r1[r] = __builtin_fmaf(d, d, r1[r]);
+        }
+    }
+    row_sums<WAVES>(r1, part[1]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      r1[r] = 1.0f / sqrtf(r1[r] * inv + a.eps);
+      if (token + r >= a.tokens) continue;
+      if (lane == 0) reinterpret_cast<float2*>(a.kept)[token + r] = make_float2(mean[r], r1[r]);
+      T* out = static_cast<T*>(a.y) + (token + r) * a.units;
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        const int at = (k * NT + lane) * W;
+        float y[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+          y[i] = __builtin_fmaf((to_f32(x[k][r][i]) - mean[r]) * r1[r], w[k][i], b[k][i]);
+        if (at < a.units) store_pack<W>(out + at, a.units - at, y);
+      }
+    }
   }
 }
 
@@ -99,7 +151,7 @@ __global__ __launch_bounds__(ROWS* WAVES * 64) void k_normalise(NormArgs a) {
 template <typename T, typename P>
 __global__ __launch_bounds__(1024) void k_normalise_stream(NormArgs a) {
   constexpr int W = kChunk<T>, WAVES = 16, STEP = 1024 * W;
-  __shared__ float2 part[2][WAVES];
+  __shared__ float part[2][WAVES][1];
   const int64_t token = blockIdx.x;
   const T* row = static_cast<const T*>(a.x) + token * a.x_line;
   float sum = 0.0f, square = 0.0f;
@@ -109,7 +161,7 @@ __global__ __launch_bounds__(1024) void k_normalise_stream(NormArgs a) {
     for (int i = 0; i < W; ++i) sum += to_f32(x[i]);
   }
   const float inv = 1.0f / static_cast<float>(a.units);
-  const float mean = row_sum2<WAVES>(sum, 0.0f, part[0]).x * inv;
+  const float mean = row_sum<WAVES>(sum, part[0]) * inv;
   for (int at = threadIdx.x * W; at < a.units; at += STEP) {
     const typename Pack<T, W>::type x = load_pack<W>(row + at, a.units - at);
 #pragma unroll
@@ -118,7 +170,7 @@ __global__ __launch_bounds__(1024) void k_normalise_stream(NormArgs a) {
       square = __builtin_fmaf(d, d, square);
     }
   }
-  const float var = row_sum2<WAVES>(square, 0.0f, part[1]).x * inv;
+  const float var = row_sum<WAVES>(square, part[1]) * inv;
   const float r = 1.0f / sqrtf(var + a.eps);
   if (threadIdx.x == 0) reinterpret_cast<float2*>(a.kept)[token] = make_float2(mean, r);
   T* out = static_cast<T*>(a.y) + token * a.units;
@@ -137,13 +189,14 @@ __global__ __launch_bounds__(1024) void k_normalise_stream(NormArgs a) {
   }
 }
 
-// The gradients: a workgroup takes every gridDim.x-th group of ROWS rows and
-// keeps its lanes' sums of g n and g in registers; they are joined over the
-// rows' groups in LDS and written as the workgroup's part.
+// The gradients, a row at a time: a lane keeps its sums of g n and g in
+// registers; they are joined over the groups in LDS and written as the
+// workgroup's part. (Two rows at a time, or the next one's loads ahead, gained
+// nothing: 16384 x 4096 bf16 94 us both, this 87.)
 template <typename T, typename P, int ROWS, int WAVES, int NC>
 __global__ __launch_bounds__(ROWS* WAVES * 64) void k_normalise_grad(NormArgs a) {
   constexpr int W = kChunk<T>, NT = WAVES * 64;
-  __shared__ float2 part[2][ROWS * WAVES];
+  __shared__ float part[2][ROWS * WAVES][2];
   __shared__ float joined[ROWS > 1 ? NT * W : 1];
   const int lane = threadIdx.x % NT, group = threadIdx.x / NT;
   const float inv = 1.0f / static_cast<float>(a.units);
@@ -158,47 +211,45 @@ __global__ __launch_bounds__(ROWS* WAVES * 64) void k_normalise_grad(NormArgs a)
   int slot = 0;
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * ROWS; first < a.tokens;
        first += static_cast<int64_t>(gridDim.x) * ROWS) {
-    const int64_t token = first + group;
+    const int64_t token = first + group, from = token < a.tokens ? token : first;
     const bool there = token < a.tokens;
-    const int64_t from = there ? token : 0;
-    const T* xr = static_cast<const T*>(a.x) + from * a.x_line;
-    const T* gr = static_cast<const T*>(a.g) + from * a.g_line;
+    const T* const xr[1] = {static_cast<const T*>(a.x) + from * a.x_line};
+    const T* const gr[1] = {static_cast<const T*>(a.g) + from * a.g_line};
     const float2 kept = reinterpret_cast<const float2*>(a.kept)[from];
-    typename Pack<T, W>::type x[NC], g[NC];
+    typename Pack<T, W>::type x[NC][1], g[NC][1];
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
-      const int at = (k * NT + lane) * W;
-      const int64_t left = there ? a.units - at : 0;
-      x[k] = load_pack<W>(xr + at, left), g[k] = load_pack<W>(gr + at, left);
+      load_rows<1>(xr, (k * NT + lane) * W, a.units, x[k]);
+      load_rows<1>(gr, (k * NT + lane) * W, a.units, g[k]);
     }
-    float s = 0.0f, sn = 0.0f;
+    float sums[2] = {0.0f, 0.0f};
+    if (there) {
 #pragma unroll
-    for (int k = 0; k < NC; ++k) {
+      for (int k = 0; k < NC; ++k)
 #pragma unroll
-      for (int i = 0; i < W; ++i) {  // (past the row's end g and w are zeros, and n is finite or the row's NaN)
-        const float d = to_f32(g[k][i]), n = (to_f32(x[k][i]) - kept.x) * kept.y, u = d * w[k][i];
-        dw[k][i] = __builtin_fmaf(d, n, dw[k][i]);
-        db[k][i] += d;
-        s += u;
-        sn = __builtin_fmaf(u, n, sn);
-      }
+        for (int i = 0; i < W; ++i) {  // (past the row's end g and w are zeros, and n is finite or the row's NaN)
+          const float d = to_f32(g[k][0][i]), n = (to_f32(x[k][0][i]) - kept.x) * kept.y, u = d * w[k][i];
+          dw[k][i] = __builtin_fmaf(d, n, dw[k][i]);
+          db[k][i] += d;
+          sums[0] += u;
+          sums[1] = __builtin_fmaf(u, n, sums[1]);
+        }
     }
-    const float2 sums = row_sum2<WAVES>(s, sn, part[slot]);
+    row_sums<WAVES>(sums, part[slot]);
     slot ^= 1;
     if (!there) continue;
-    const float mean = sums.x * inv, mean_n = sums.y * inv;
+    const float mean = sums[0] * inv, mean_n = sums[1] * inv;
     T* out = static_cast<T*>(a.y) + token * a.units;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int at = (k * NT + lane) * W;
-      if (at >= a.units) break;
       float d[W];
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        const float n = (to_f32(x[k][i]) - kept.x) * kept.y;
-        d[i] = kept.y * (to_f32(g[k][i]) * w[k][i] - mean - n * mean_n);
+        const float n = (to_f32(x[k][0][i]) - kept.x) * kept.y;
+        d[i] = kept.y * (to_f32(g[k][0][i]) * w[k][i] - mean - n * mean_n);
       }
-      store_pack<W>(out + at, a.units - at, d);
+      if (at < a.units) store_pack<W>(out + at, a.units - at, d);
     }
   }
   float* mine = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.units;
@@ -230,7 +281,7 @@ __global__ __launch_bounds__(ROWS* WAVES * 64) void k_normalise_grad(NormArgs a)
 template <typename T, typename P>
 __global__ __launch_bounds__(1024) void k_normalise_means(NormArgs a, float* means) {
   constexpr int W = kChunk<T>, WAVES = 16;
-  __shared__ float2 part[WAVES];
+  __shared__ float part[WAVES][2];
   const int64_t token = blockIdx.x;
   const T* xr = static_cast<const T*>(a.x) + token * a.x_line;
   const T* gr = static_cast<const T*>(a.g) + token * a.g_line;
@@ -246,9 +297,10 @@ __global__ __launch_bounds__(1024) void k_normalise_means(NormArgs a, float* mea
       sn += at + i < a.units ? u * ((to_f32(x[i]) - kept.x) * kept.y) : 0.0f;
     }
   }
-  const float2 sums = row_sum2<WAVES>(s, sn, part);
+  float sums[2] = {s, sn};
+  row_sums<WAVES>(sums, part);
   const float inv = 1.0f / static_cast<float>(a.units);
-  if (threadIdx.x == 0) reinterpret_cast<float2*>(means)[token] = make_float2(sums.x * inv, sums.y * inv);
+  if (threadIdx.x == 0) reinterpret_cast<float2*>(means)[token] = make_float2(sums[0] * inv, sums[1] * inv);
 }
 template <typename T, typename P>
 __global__ __launch_bounds__(256) void k_normalise_columns(NormArgs a, const float* means) {
@@ -271,24 +323,29 @@ __global__ __launch_bounds__(256) void k_normalise_columns(NormArgs a, const flo
 }
 
 // out [2][units] = the sums of the workgroups' parts: 64 columns a workgroup,
-// the parts over its 4 waves.
-__global__ __launch_bounds__(256) void k_normalise_join(int parts, int64_t n, const float* part, float* out) {
-  __shared__ float sums[4][64];
+// the parts over its 16 waves.
+__global__ __launch_bounds__(1024) void k_normalise_join(int parts, int64_t n, const float* part, float* out) {
+  __shared__ float sums[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 64 + lane;
   float s = 0.0f;
   if (at < n) {
-    const int per = (parts + 3) / 4, last = (wave + 1) * per < parts ? (wave + 1) * per : parts;
+    const int per = (parts + 15) / 16, last = (wave + 1) * per < parts ? (wave + 1) * per : parts;
 #pragma unroll 8
     for (int p = wave * per; p < last; ++p) s += part[p * n + at];
   }
   sums[wave][lane] = s;
   __syncthreads();
-  if (wave == 0 && at < n) out[at] = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
+  if (wave > 0 || at >= n) return;
+  for (int w = 1; w < 16; ++w) s += sums[w][lane];
+  out[at] = s;
 }
 
-// Workgroups of the gradients: enough for every CU, no more than there are
-// groups of rows.
+// How a level's rows are taken: as many waves as give each lane a chunk of 16
+// bytes (of wide levels more, up to 16 values); workgroups of 4 waves and more
+// forwards and of 16 backwards, those of the gradients two a CU where they hold
+// several rows (their barriers are for all of them), else one: every workgroup
+// has a part of dw and db to write.
 struct NormPlan {
   int waves, chunks, rows, groups;  // chunks 0: the forms that hold no rows
   int64_t bytes, means;
@@ -297,9 +354,9 @@ NormPlan norm_plan(int64_t tokens, int64_t units, int dtype) {
   const int64_t chunks = div_up(units, dtype == PLX_LB_F32 ? 4 : 8);
   NormPlan p{};
   p.waves = chunks <= 64 ? 1 : chunks <= 128 ? 2 : chunks <= 256 ? 4 : chunks <= 512 ? 8 : 16;
-  p.chunks = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : 0;
+  p.chunks = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : chunks <= 4096 && dtype == PLX_LB_F32 ? 4 : 0;
   p.rows = p.chunks ? 16 / p.waves : 1;
-  const int64_t groups = div_up(tokens, p.rows), most = cu_count();
+  const int64_t groups = div_up(tokens, p.rows), most = int64_t{cu_count()} * (p.rows > 1 ? 2 : 1);
   p.groups = static_cast<int>(groups < most ? groups : most);
   p.bytes = int64_t{8} * p.groups * units;
   p.means = p.bytes;
@@ -307,7 +364,7 @@ NormPlan norm_plan(int64_t tokens, int64_t units, int dtype) {
   return p;
 }
 
-template <typename F>
+template <typename T, typename F>
 void with_rows(const NormPlan& p, F f) {
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
@@ -324,12 +381,30 @@ void with_rows(const NormPlan& p, F f) {
     f(I8{}, I1{});
   else if (p.chunks == 1)
     f(I16{}, I1{});
-  else
+  else if (p.chunks == 2)
     f(I16{}, I2{});
+  else if constexpr (sizeof(T) == 4)
+    f(I16{}, I4{});
 }
 
 template <typename T, typename P>
 void launch_normalise(const NormArgs& all, const NormPlan& p, hipStream_t s) {
+  if (p.chunks) {
+    with_rows<T>(p, [&](auto waves, auto chunks) {
+      constexpr int WAVES = decltype(waves)::value, NC = decltype(chunks)::value, ROWS = WAVES < 4 ? 4 / WAVES : 1;
+      const int64_t most = int64_t{cu_count()} * (32 / (ROWS * WAVES));  // all waves that a CU holds
+      if (all.tokens > most * ROWS) {
+        constexpr int R = kRows / NC;
+        const int64_t groups = div_up(all.tokens, ROWS * R);
+        k_normalise<T, P, ROWS, WAVES, NC, R>
+            <<<static_cast<unsigned>(groups < most ? groups : most), ROWS * WAVES * 64, 0, s>>>(all);
+      } else {
+        k_normalise<T, P, ROWS, WAVES, NC, 1>
+            <<<static_cast<unsigned>(div_up(all.tokens, ROWS)), ROWS * WAVES * 64, 0, s>>>(all);
+      }
+    });
+    return;
+  }
   constexpr int64_t most = int64_t{1} << 20;  // workgroups of a launch: at most 2^30 lanes
   for (int64_t first = 0; first < all.tokens; first += most) {
     NormArgs a = all;
@@ -337,15 +412,7 @@ void launch_normalise(const NormArgs& all, const NormPlan& p, hipStream_t s) {
     a.x = static_cast<const T*>(all.x) + first * all.x_line;
     a.y = static_cast<T*>(all.y) + first * all.units;
     a.kept = all.kept + 2 * first;
-    if (!p.chunks) {
-      k_normalise_stream<T, P><<<static_cast<unsigned>(a.tokens), 1024, 0, s>>>(a);
-      continue;
-    }
-    with_rows(p, [&](auto waves, auto chunks) {
-      constexpr int WAVES = decltype(waves)::value, ROWS = WAVES < 4 ? 4 / WAVES : 1;
-      k_normalise<T, P, ROWS, WAVES, decltype(chunks)::value>
-          <<<static_cast<unsigned>(div_up(a.tokens, ROWS)), ROWS * WAVES * 64, 0, s>>>(a);
-    });
+    k_normalise_stream<T, P><<<static_cast<unsigned>(a.tokens), 1024, 0, s>>>(a);
   }
 }
 
@@ -366,7 +433,7 @@ void launch_grad(const NormArgs& a, const NormPlan& p, hipStream_t s) {
     k_normalise_columns<T, P><<<grid, 256, 0, s>>>(a, means);
     return;
   }
-  with_rows(p, [&](auto waves, auto chunks) {
+  with_rows<T>(p, [&](auto waves, auto chunks) {
     constexpr int WAVES = decltype(waves)::value, ROWS = 16 / WAVES;
     k_normalise_grad<T, P, ROWS, WAVES, decltype(chunks)::value>
         <<<static_cast<unsigned>(p.groups), ROWS * WAVES * 64, 0, s>>>(a);
@@ -427,7 +494,7 @@ int plx_normalise_grad(int64_t tokens, int64_t units, int32_t dtype, const void*
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t n = 2 * units;
   if (tokens == 0) {
-    k_normalise_join<<<static_cast<unsigned>(div_up(n, 64)), 256, 0, s>>>(0, n, nullptr, dparams);
+    k_normalise_join<<<static_cast<unsigned>(div_up(n, 64)), 1024, 0, s>>>(0, n, nullptr, dparams);
     return check_launch("plx_normalise_grad");
   }
   const NormPlan p = norm_plan(tokens, units, dtype);
@@ -439,7 +506,7 @@ int plx_normalise_grad(int64_t tokens, int64_t units, int32_t dtype, const void*
   a.x = x, a.g = g, a.weight = weight, a.y = dx, a.kept = const_cast<float*>(kept);
   a.part = static_cast<float*>(workspace);
   with_types(dtype, params, [&](auto* t, auto* q) { launch_grad<PLX_DENSE_TYPE(t), PLX_DENSE_TYPE(q)>(a, p, s); });
-  k_normalise_join<<<static_cast<unsigned>(div_up(n, 64)), 256, 0, s>>>(p.groups, n, a.part, dparams);
+  k_normalise_join<<<static_cast<unsigned>(div_up(n, 64)), 1024, 0, s>>>(p.groups, n, a.part, dparams);
   return check_launch("plx_normalise_grad");
 }
 

@@ -30,7 +30,7 @@ import torch
 from torch.autograd import forward_ad
 
 from plastax_amd import _lib
-from plastax_amd.lowbit import DTYPES, _call, _launch, _on_gpu
+from plastax_amd.lowbit import DTYPES, _call, _launch
 
 _IDS = {torch.int32: 0, torch.int64: 1}
 _KEEP = 64  # PLX_RECUR_KEEP
@@ -80,7 +80,12 @@ def _floats(who: str, name: str, t: torch.Tensor, shape: tuple[int, ...]) -> tor
 
 
 def _together(who: str, t: torch.Tensor, *others: torch.Tensor | None) -> None:
-    _on_gpu(who, t.device, *(o.device for o in others if o is not None))
+    device = t.device
+    if device.type != "cuda":
+        raise ValueError(f"{who}: arguments must be on the GPU, got {device}")
+    for o in others:
+        if o is not None and o.device != device:
+            raise ValueError(f"{who}: arguments are on different devices, {device} and {o.device}")
 
 
 def _space(device: torch.device, name: str, *args: object) -> tuple[torch.Tensor | None, int | None, int]:
@@ -190,7 +195,7 @@ def normalise_grad(g: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     _launch(x.device, "plx_normalise_grad", tokens, units, DTYPES[x.dtype], g.data_ptr(), g.stride(0), x.data_ptr(),
             x.stride(0), DTYPES[weight.dtype], weight.data_ptr(), kept.data_ptr(), dx.data_ptr(), dparams.data_ptr(),
             at, need)
-    return dx, dparams[0], dparams[1]
+    return dx, *dparams.unbind(0)
 
 
 # --------------------------------------------------------------------------

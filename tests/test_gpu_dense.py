@@ -129,7 +129,7 @@ def test_infinities_and_nan_stay_in_their_rows() -> None:
 # --------------------------------------------------------------------------
 # Layer norm
 # --------------------------------------------------------------------------
-UNITS = [1, 2, 7, 64, 255, 256, 257, 512, 513, 1003, 1024, 2048, 2050, 4096, 4100, 8192, 8200, 16384, 16390, 20001]
+UNITS = [1, 2, 7, 64, 255, 256, 257, 512, 513, 1003, 1024, 2048, 2050, 4096, 4100, 8192, 8200, 9000, 16384, 16390, 20001]
 
 
 def _levels(tokens, units, dtype, g) -> torch.Tensor:
