@@ -90,8 +90,11 @@ __device__ __forceinline__ Teacher name_outputs(const DistilArgs& a, int64_t tok
 }
 
 // What a row's values are taken from before the exponential: a logit's is
-// 2^(x c - shift), or 2^((x - m) c) where m is so large that m c is not finite
-// (a row of the type's lowest value alone).
+// 2^(x c - shift), one operation, with the rounding of shift = m c in all of a
+// row's exponents alike: half a unit at most while |m c| < 2^24, and taken out
+// of the loss again. From there on, where it would grow until the powers
+// overflow or vanish, a logit's is 2^((x - m) c), whose exponents are rounded
+// relative to themselves.
 struct Shift {
   float c, m, shift;
   bool far;
@@ -99,7 +102,7 @@ struct Shift {
 __device__ __forceinline__ Shift shift_of(float m, float t) {
   Shift s;
   s.c = kLog2e / t, s.m = m, s.shift = m * s.c;
-  s.far = !(fabsf(s.shift) < 1e37f);
+  s.far = !(fabsf(s.shift) < 16777216.0f);  // (a NaN is far)
   return s;
 }
 template <bool FAR>

@@ -361,6 +361,39 @@ def test_distil_and_its_gradient(outputs, dtype) -> None:
         assert torch.equal(dense.distil(x, ids, top, temperature), got[0])
 
 
+@pytest.mark.parametrize("dtype", plain.DTYPES, ids=str)
+@pytest.mark.parametrize("high", [20, 23, 26, 31, 34, 43, 90, 120])
+def test_distil_of_logits_far_from_nought(high, dtype) -> None:
+    """Rows around +-2^high, finite in the type, with temperatures that make steps of them whole units or small parts
+    of one: what is taken from every logit must not put its own rounding, 2^-24 of 2^high / T, into the exponents.
+    (Temperatures are powers of two, and the oracle's divisions exact.)
+
+    A power below float32's least normal number, 2^-126, may be 0. The sum of the powers is at least their largest,
+    2^(-1/2) with the shift's rounding of half a unit, so q is off by 2^-125 there at most and the gradient by T |g|
+    times that: for T = 2^71 more than the oracle's 1e-36, which holds for T near 1."""
+    if dtype == torch.float16:
+        high = min(high, 15) - 1
+    for n, (outputs, below) in enumerate(((40, 0), (3000, 19), (40000, 25), (300, 40))):
+        _say("far", high, dtype, outputs, below)
+        rng = torch.Generator(device=DEV).manual_seed(high * 8 + n)
+        temperature = 2.0 ** (max(high - below, -20) if below else 0)
+        step = 2.0**high * torch.finfo(dtype).eps
+        base = torch.tensor([2.0**high, -(2.0**high)] * 4, dtype=torch.float64, device=DEV)[:, None]
+        x = base + step * torch.randint(0, 9, (8, outputs), generator=rng, device=DEV)
+        x[4:] *= torch.rand((4, outputs), generator=rng, device=DEV).double()  # (and rows that spread down to nought)
+        x = x.to(dtype)
+        assert torch.isfinite(x).all()
+        ids = torch.randint(outputs, (8, 5), generator=rng, device=DEV)
+        top = temperature * torch.randn((8, 5), generator=rng, device=DEV)
+        weight = torch.randn((8,), generator=rng, device=DEV)
+        (loss, off), (d, d_off) = plain.distil(x, ids, top, temperature, weight)
+        got = dense.distil_grad(weight, x, ids, top, temperature)
+        plain.near(got[0], loss, off + plain.rounded(loss, torch.float32))
+        vanished = 2.0**-125 * temperature * weight.double().abs()[:, None]
+        plain.near(got[1], d, d_off + plain.rounded(d, dtype) + vanished)
+        assert torch.equal(dense.distil(x, ids, top, temperature), got[0])
+
+
 @pytest.mark.parametrize("dtype", plain.DTYPES)
 @pytest.mark.parametrize("outputs", [40, 1000, 33000, 70001])
 def test_masks_that_leave_a_row_nothing(outputs, dtype) -> None:
