@@ -1295,7 +1295,8 @@ PLX_EXPORT int plx_normalise_grad(int64_t tokens, int64_t units, int32_t dtype, 
  * [sequences][units] (float32; null: zeros), and last [sequences][units] is
  * its last h, or its state if it has no rows. Rows of no sequence have h = 0.
  * kept [ceil(tokens / 64)][units] (float32) is for plx_recur_grad. `ragged`:
- * whether starts is given. */
+ * whether starts is given. ceil(tokens / 64) ceil(units / 128) is at most
+ * 2^22. */
 #define PLX_RECUR_KEEP 64
 PLX_EXPORT int64_t plx_recur_workspace(int64_t tokens, int64_t units, int64_t sequences, int32_t ragged);
 PLX_EXPORT int plx_recur(int64_t tokens, int64_t units, int64_t sequences, int32_t dtype, const void* xz, int64_t line,
@@ -1320,7 +1321,8 @@ PLX_EXPORT int plx_recur_step(int64_t sequences, int64_t units, int32_t dtype, c
  * over the token's outputs, p = softmax(top / T) over the outputs that
  * ids [tokens][named] name; top [tokens][named] is of type `top_type`. A place
  * whose id is no output, or whose top is -inf, counts for nothing; a token
- * without any other has the loss 0. named is at most PLX_MAX_NAMED. */
+ * without any other has the loss 0. named is at most PLX_MAX_NAMED;
+ * T is from 2^-120 to 2^120. */
 #define PLX_MAX_NAMED 1024
 PLX_EXPORT int plx_distil(int64_t tokens, int64_t outputs, int32_t named, int32_t dtype, const void* logits,
                           int64_t line, const void* ids, int32_t wide, int32_t top_type, const void* top,

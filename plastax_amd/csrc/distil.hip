@@ -397,7 +397,7 @@ int run_distil(const char* who, bool grad, const DistilArgs& all, int dtype, voi
   if (!batch_fits(all.tokens, all.outputs) || all.named < 0 || all.named > PLX_MAX_NAMED || all.wide < 0 || all.wide > 1)
     return fail(PLX_ERR_INVALID, who);
   if (!known_type(dtype) || !known_type(all.top_type)) return fail(PLX_ERR_UNSUPPORTED, who);
-  if (!(all.t > 0.0f && all.t < INFINITY)) return fail(PLX_ERR_INVALID, who);
+  if (!(all.t >= 0x1p-120f && all.t <= 0x1p120f)) return fail(PLX_ERR_INVALID, who);  // (1 / T is normal too)
   if (all.tokens == 0) return PLX_OK;
   if (!all.loss || (all.outputs > 0 && !all.x) || (all.named > 0 && (!all.ids || !all.top)) ||
       (grad && (!all.g || (all.outputs > 0 && !all.dx))))

@@ -122,7 +122,8 @@ def look_up(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch
 def look_up_grad(g: torch.Tensor, ids: torch.Tensor, rows: int, scale: float = 1.0) -> torch.Tensor:
     """The table's gradient ``[rows, units]`` in float32: ``scale`` times the
     sums of the tokens' gradients g ``[tokens, units]`` by id, zeros for rows
-    that no token named. Ids outside of the rows count for nothing."""
+    that no token named. Ids outside of the rows count for nothing. At most 2^25
+    tokens."""
     g, ids = _batch("look_up_grad", g), _ids("look_up_grad", "ids", ids, 1)
     if not 0 <= rows <= _MAX_UNITS:
         raise ValueError(f"look_up_grad: 0 to 2^24 rows expected, got {rows}")
@@ -155,9 +156,9 @@ def normalise(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     variance over each token's units, and what the gradient needs (each token's
     mean and 1 / sqrt(var + eps), float32 ``[tokens, 2]``).
 
-    weight and bias ``[units]`` are both float32, or both of x's type. Squares
-    are float32: past its range (values above 2^63 or so) results are not what
-    the formula gives."""
+    weight and bias ``[units]`` are both float32, or both of x's type. The sum of
+    the squares of x - mean is float32: past its range (3.4e38 over the row)
+    results are not what the formula gives."""
     x = _batch("normalise", x)
     if not 0 <= eps < math.inf:
         raise ValueError(f"normalise: eps >= 0 expected, got {eps}")
@@ -228,7 +229,8 @@ def recur(xz: torch.Tensor, starts: torch.Tensor | None = None,
     all rows are one. It goes on from ``state[s]`` (float32 ``[sequences,
     units]``; zeros if None); last is its last h in float32, or its state if it
     has no rows. h ``[tokens, units]`` is 0 in rows of no sequence. kept is what
-    the gradient needs (float32, one row in 64). An infinity or a NaN stays in
+    the gradient needs (float32, one row in 64). At most 2^22 pieces of 64 rows
+    by 128 units. An infinity or a NaN stays in
     its sequence and unit, where what follows is not finite."""
     xz, units, starts, sequences, state = _sequences("recur", xz, starts, state)
     _together("recur", xz, starts, state)
@@ -312,8 +314,8 @@ def _named(who: str, logits: torch.Tensor, ids: torch.Tensor, top: torch.Tensor,
         raise ValueError(f"{who}: top of {tuple(ids.shape)} expected, got {tuple(top.shape)}")
     top = _plain(who, top)
     top = top if top.is_contiguous() else top.contiguous()
-    if not 0 < temperature < math.inf:
-        raise ValueError(f"{who}: a temperature above 0 expected, got {temperature}")
+    if not 2.0**-120 <= temperature <= 2.0**120:  # (its inverse is a normal number of float32 too)
+        raise ValueError(f"{who}: a temperature from 2^-120 to 2^120 expected, got {temperature}")
     return logits, ids, top
 
 

@@ -3,6 +3,9 @@ forms against differences (CPU only: no kernel is launched)."""
 
 from __future__ import annotations
 
+import contextlib
+import types
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -167,6 +170,48 @@ def test_teachers_are_checked() -> None:
         dense.distil_grad(torch.ones(5).half(), x, ids, top)
     with pytest.raises(ValueError, match="g of"):
         dense.distil_grad(torch.ones(5, 1), x, ids, top)
+
+
+@pytest.mark.parametrize("t", [1e-37, 2.0**-121, 2.0**121, 3e38])
+def test_temperatures_whose_inverse_float32_has_not_are_refused(lib, t) -> None:
+    x, ids, top = torch.zeros(5, 8), torch.zeros((5, 2), dtype=torch.int64), torch.zeros(5, 2)
+    with pytest.raises(ValueError, match="temperature"):
+        dense.distil(x, ids, top, t)
+    assert lib.plx_distil(5, 8, 2, 0, P, 8, P, 1, 0, P, t, P, None) == 1
+    assert lib.plx_distil_grad(5, 8, 2, P, 0, P, 8, P, 1, 0, P, t, P, P, None) == 1
+
+
+def test_plans_and_launches_run_with_the_arguments_device_current(monkeypatch) -> None:
+    """A plan counts the current device's CUs, as the launch does that its workspace is for."""
+    current, seen = [0], []
+
+    @contextlib.contextmanager
+    def device(index):
+        was, current[0] = current[0], index
+        yield
+        current[0] = was
+
+    names = ("plx_look_up_workspace", "plx_normalise_workspace", "plx_recur_workspace", "plx_recur")
+    entries = {n: (lambda *args, n=n: seen.append((n, current[0])) or 0) for n in names}
+    monkeypatch.setattr(_lib, "load", lambda: types.SimpleNamespace(**entries))
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    for index in (0, 1):
+        at = torch.device("cuda", index)
+        for name in names[:3]:
+            assert dense._space(at, name, 5, 8, 8) == (None, None, 0)
+        dense._launch(at, names[3])
+        assert seen == [(n, index) for n in names] and current == [0]
+        seen.clear()
+
+
+def test_sizes_out_of_range_have_no_workspace(lib) -> None:
+    assert lib.plx_look_up_workspace((1 << 25) + 1, 7, 8) == -1
+    assert lib.plx_look_up_workspace(1 << 25, 7, 8) > 0
+    assert lib.plx_recur_workspace(1 << 28, 128, 1, 0) > 0
+    assert lib.plx_recur_workspace((1 << 28) + 1, 128, 1, 0) == -1
+    assert lib.plx_recur_workspace(1 << 28, 129, 1, 0) == -1
 
 
 def test_entry_points_check_before_they_launch(lib) -> None:

@@ -486,6 +486,66 @@ def test_on_another_stream() -> None:
     assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("power", [-60, 50])
+def test_powers_of_two_go_through(power, dtype) -> None:
+    """Inputs times a power of two give results times it, to the last bit, in types of 8 exponent bits: nothing
+    overflows or vanishes on the way that the results hold. (normalise without eps: y the same.)"""
+    g, c = _gen(power + 99), 2.0**power
+    tokens, units = 700, 130
+    xz, d = _xz(tokens, units, dtype, g), _randn((tokens, units), g).to(dtype)
+    state, g_last = _randn((3, units), g), _randn((3, units), g)
+    starts = torch.tensor([0, 300, 300, 690], device=DEV)
+    more = xz.clone()
+    more[:, :units] *= c
+    (h, last, kept), (h2, last2, kept2) = dense.recur(xz, starts, state), dense.recur(more, starts, state * c)
+    assert torch.equal(h * c, h2) and torch.equal(last * c, last2) and torch.equal(kept * c, kept2)
+    dxz, ds = dense.recur_grad(d, xz, kept, starts, state, g_last)
+    dxz2, ds2 = dense.recur_grad(d * c, xz, kept, starts, state, g_last * c)
+    assert torch.equal(dxz * c, dxz2) and torch.equal(ds * c, ds2)
+    for units in (130, 3000, 20000):
+        x, d, w = (_randn((40, units), g).to(dtype) for _ in range(3))
+        w = w[0].contiguous()
+        (y, kept), (y2, kept2) = dense.normalise(x, w, None, 0.0), dense.normalise(x * c, w, None, 0.0)
+        assert torch.equal(y, y2)
+        got, got2 = dense.normalise_grad(d, x, w, kept), dense.normalise_grad(d * c, x * c, w, kept2)
+        assert torch.equal(got[0], got2[0]) and all(torch.equal(p * c, q) for p, q in zip(got[1:], got2[1:]))
+
+
+@pytest.mark.parametrize("dtype", plain.DTYPES, ids=str)
+def test_gates_that_are_all_or_nothing(dtype) -> None:
+    """z from where a sigmoid is 0 or 1 in the type to the largest values that it has."""
+    top = torch.finfo(dtype).max
+    z = torch.tensor([-top, -200.0, -100.0, -89.0, -30.0, 0.0, 30.0, 89.0, 100.0, 200.0, top], device=DEV)
+    tokens, units, g = 300, 11, _gen(5)
+    xz = _randn((tokens, 2 * units), g)
+    xz[:, units:] = z
+    xz[::7, units:] = z.flip(0)
+    state, g_last = _randn((2, units), g), _randn((2, units), g)
+    _check_recur(xz.to(dtype), [0, 130, tokens], state, _randn((tokens, units), g).to(dtype), g_last, torch.int32)
+
+
+def test_two_streams_at_once() -> None:
+    """Calls that run next to each other, each with its own workspace, give what they give alone."""
+    inputs = [_inputs(30 + k, BF16, 4000 + 777 * k, 900, 1024) for k in range(2)]
+    wants = []
+    for s in inputs:
+        wants.append(_together(s))
+        s["now"].zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(4):
+        gots = []
+        for s, stream in zip(inputs, streams):
+            with torch.cuda.stream(stream):
+                gots.append(_together(s))
+                s["now"].zero_()
+        torch.cuda.synchronize()
+        for got, want in zip(gots, wants):
+            assert all(torch.equal(p, q) for p, q in zip(got[:-1], want[:-1]))
+            assert torch.equal(got[-1], want[-1])
+
+
 def test_in_graphs() -> None:
     """Two captured graphs, replayed in turn on new inputs with eager calls between: every replay gives what the eager
     call gives."""
