@@ -5,6 +5,10 @@
 // With q = softmax(x / T) over a token's outputs and p = softmax(t / T) over
 // its named ones, loss = T^2 sum p (log p - log q) and
 // d loss / dx = T (q - p), p 0 where nothing is named.
+//
+// Bound by memory: a row is read once into registers, its largest logit, its
+// sum and its gradient are made from there, and the gradient is written once:
+// 8192 x 131072 bf16 858 us, 5.0 TB/s.
 
 #include "px_dense.h"
 
@@ -362,7 +366,11 @@ void launch_row(const DistilArgs& a, hipStream_t s) {
 }
 
 // Few waves with many chunks where there are tokens enough for every CU (a
-// token's places are looked at by one wave), else many with few.
+// token's places are looked at by one wave, for which the others wait: 2048 x
+// 3800 float32 15 us, with 16 waves 30), else many with few (200 x 3800 6.3 us,
+// with 2 waves 7.0; 1 x 3800 5.5 and 6.3). A row stays in registers as long as
+// it fits there (2048 x 60000 float32 184 us, as a stream 216; 32 x 60000 10.9
+// and 13.9).
 template <typename T, bool GRAD>
 void launch_distil(const DistilArgs& a, hipStream_t s) {
   const int64_t chunks = div_up(a.outputs, kChunk<T>);
