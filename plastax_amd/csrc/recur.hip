@@ -17,6 +17,13 @@
 // the tiles before it in its group of 8, for those of the groups before in the
 // row of 8 groups, and for what comes into the row: a long sequence is a chain
 // of rows of 64 tiles (a link takes some 3 us), and every sum has one order.
+//
+// 65536 x 1024 bf16: 116 us forwards for 403 MB, 3.5 TB/s, and 214 backwards for
+// 671 MB, 3.1: a workgroup's way through a tile (its turn, its loads, the
+// exchange in LDS, what it waits for, its stores) takes some 12 us, and the two
+// that a CU holds do not cover each other's all the time. Smaller tiles with
+// the next one's loads on their way took 185 and 368, four workgroups of half
+// the rows 136 forwards.
 
 #include "px_dense.h"
 
