@@ -13,7 +13,7 @@
 //   k_join_sums  the longer rows from their parts, in order.
 //
 // 65536 tokens, 131072 rows of 1024 units, bf16: looked up in 48 us (a row read
-// again is often in a cache); the gradient in 26, 131 and 17, of which the
+// again is often in a cache); the gradient in 26, 131 and 12, of which the
 // second writes 537 MB and reads 134, 5.1 TB/s. With few tokens a launch's
 // chain of loads is what it takes: 4 to 11 us each.
 
