@@ -304,7 +304,10 @@ __global__ __launch_bounds__(WAVES * 64) void k_distil_row(DistilArgs a) {
       chunks.template gradient<true>(out, outputs, a.whole, s, r);
     else
       chunks.template gradient<false>(out, outputs, a.whole, s, r);
-    if (WAVES > 1) __syncthreads();
+    if (WAVES > 1)
+      __syncthreads();
+    else  // (a wave's stores are made in their order, and its lanes see each other's: for the compiler)
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     write_named<NT>(a, out, s, scale, r, named);
   }
   if (first) write_loss(a, token, s, sum, teacher, named);

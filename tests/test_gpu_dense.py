@@ -525,6 +525,30 @@ def test_gates_that_are_all_or_nothing(dtype) -> None:
     _check_recur(xz.to(dtype), [0, 130, tokens], state, _randn((tokens, units), g).to(dtype), g_last, torch.int32)
 
 
+@pytest.mark.parametrize("units", [1, 8, 300])
+def test_gradients_of_broadcast_results(units) -> None:
+    """Gradients that stand for more values than they have (of a sum: all of them one), and inputs read again and again,
+    give what their copies give."""
+    g = _gen(units)
+    tokens = 90
+    x, xz, w = _randn((tokens, units), g), _xz(tokens, units, F32, g), _randn((units,), g)
+    ids, starts = torch.randint(7, (tokens,), generator=g, device=DEV), torch.tensor([0, 40, 90], device=DEV)
+    _, kept = dense.normalise(x, w)
+    _, _, walked = dense.recur(xz, starts)
+    for d in (_randn((1, 1), g).expand(tokens, units), _randn((1, units), g).expand(tokens, units),
+              _randn((tokens, 1), g).expand(tokens, units)):
+        c = d.contiguous()
+        assert torch.equal(dense.look_up_grad(d, ids, 7), dense.look_up_grad(c, ids, 7))
+        for call in (lambda v: dense.normalise_grad(v, x, w, kept), lambda v: dense.recur_grad(v, xz, walked, starts),
+                     lambda v: dense.normalise(v, w), lambda v: (dense.look_up(ids, v),)):
+            assert all(torch.equal(p, q) for p, q in zip(call(d), call(c)))
+    named, top, one = ids[:1, None].expand(tokens, 1) % units, _randn((1, 1), g).expand(tokens, 1), _randn((1,), g).expand(tokens)
+    flat = x[:1].expand(tokens, units)
+    got = dense.distil_grad(one, flat, named, top)
+    want = dense.distil_grad(one.contiguous(), flat.contiguous(), named.contiguous(), top.contiguous())
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_two_streams_at_once() -> None:
     """Calls that run next to each other, each with its own workspace, give what they give alone."""
     inputs = [_inputs(30 + k, BF16, 4000 + 777 * k, 900, 1024) for k in range(2)]
