@@ -11,12 +11,14 @@
 // in is known. A workgroup takes a tile, a few rows a wave of kSlab units, into
 // its registers, two units a lane; its waves' sums meet in LDS, the
 // tiles' in memory, and each wave walks its rows again from what comes in: xz
-// is read once. Tiles are taken in the order of a counter (a slab's), and wait for
-// earlier ones only, which are under way: every wait ends (and is bounded, for
-// a caller who has two calls share a workspace). A tile waits for the sums of
-// the tiles before it in its group of 8, for those of the groups before in the
-// row of 8 groups, and for what comes into the row: a long sequence is a chain
-// of rows of 64 tiles (a link takes some 3 us), and every sum has one order.
+// is read once. Tiles are taken in the order of a counter (a slab's), and wait
+// for earlier ones of their own slab only (lane_of's words), which are under
+// way: every wait ends, in whatever order the slabs' workgroups begin. (It is
+// bounded too, for a caller who has two calls share a workspace: NaN then.) A
+// tile waits for the sums of the tiles before it in its group of 8, for those of
+// the groups before in the row of 8 groups, and for what comes into the row: a
+// long sequence is a chain of rows of 64 tiles (a link takes some 3 us), and
+// every sum has one order.
 //
 // 65536 x 1024 bf16: 116 us forwards for 403 MB, 3.5 TB/s, and 214 backwards for
 // 671 MB, 3.1: a workgroup's way through a tile (its turn, its loads, the
@@ -26,6 +28,7 @@
 // the rows 136 forwards.
 
 #include "px_dense.h"
+#include "px_recur.h"
 
 using plx_detail::check_launch;
 using plx_detail::fail;
@@ -41,7 +44,6 @@ constexpr int kKeep = kWaves * kBack;     // rows of the gradients' tile: what c
 static_assert(kKeep == PLX_RECUR_KEEP && kKeep % kForth == 0, "a wave begins where its h is kept");
 constexpr int kTicket = 64;  // (a counter takes an atomic addition each 20 ns: one for all slabs took longer than the rows)
 constexpr int kGroup = 8;  // tiles of a group, groups of a row
-constexpr int kSlab = 128;                                     // units of a workgroup
 constexpr int64_t kMaxSequences = int64_t{1} << 30;
 
 struct RecurArgs {
@@ -120,24 +122,7 @@ __device__ __forceinline__ void gate(float z, float& a, float& b) {
 struct Pair {
   float v[2];
 };
-// A lane's two units of a row, without a branch: lanes past the row's end read
-// something of it. FORM kEven: a level's units are even in number; kOdd: the
-// last lane reads the pair before its single unit, and takes the second; kOne:
-// a level of one unit, read alone.
-enum { kEven, kOdd, kOne };
-struct Lane {
-  unsigned col, at, word, next;  // the first unit; where its pair, its word and the second's are read
-  int n;                         // of the two, how many are there
-};
-template <int FORM>
-__device__ __forceinline__ Lane lane_of(unsigned first, int units) {
-  Lane l;
-  l.col = first + (threadIdx.x & 63) * 2;
-  l.n = units - static_cast<int>(l.col);
-  l.word = l.n > 0 ? l.col : 0, l.next = l.n > 1 ? l.col + 1 : 0;
-  l.at = FORM == kOdd && l.n == 1 ? l.col - 1 : l.word;
-  return l;
-}
+// A lane's two units of a row.
 template <int FORM, typename T>
 __device__ __forceinline__ typename Pack<T, 2>::type load_two(const T* row, const Lane& l) {
   if (FORM == kOne) return typename Pack<T, 2>::type{row[0], row[0]};
@@ -390,7 +375,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur(RecurArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned slab = slab_of(a);
   const int64_t tile = take(a, slab, &sh.number), t = (tile * kWaves + wave) * kForth;
-  const Lane l = lane_of<FORM>(slab * kSlab, a.units);
+  const Lane l = lane_of<FORM>(slab * kSlab, lane, a.units);
   int of[kForth + 2];
   float A[kForth][2], H[kForth][2];
   if (a.tokens > 0) {
@@ -455,7 +440,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void k_recur_grad(RecurArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned slab = slab_of(a);
   const int64_t at = take(a, slab, &sh.number), tile = a.tiles > 0 ? a.tiles - 1 - at : 0, t = (tile * kWaves + wave) * kBack;
-  const Lane l = lane_of<FORM>(slab * kSlab, a.units);
+  const Lane l = lane_of<FORM>(slab * kSlab, lane, a.units);
   int of[kBack + 2];
   typename Pack<T, 2>::type x[kBack], g[kBack];
   float A[kBack][2], B[kBack][2];  // the gates
