@@ -65,6 +65,13 @@ __device__ __forceinline__ float row_sum(float v, float (*part)[1]) {
   return sums[0];
 }
 
+// sum / units, inv = 1 / units: a product with the rounding of inv taken out
+// again, so that a row of one value has it for its mean.
+__device__ __forceinline__ float mean_of(float sum, float units, float inv) {
+  const float m = sum * inv;
+  return __builtin_fmaf(__builtin_fmaf(-m, units, sum), inv, m);
+}
+
 // R rows' chunks at `at`, one branch for all of them.
 template <int R, typename T>
 __device__ __forceinline__ void load_rows(const T* const (&row)[R], int at, int units,
@@ -88,7 +95,7 @@ __global__ __launch_bounds__(ROWS* WAVES * 64) void k_normalise(NormArgs a) {
   constexpr int W = kChunk<T>, NT = WAVES * 64;
   __shared__ float part[2][ROWS * WAVES][R];
   const int lane = threadIdx.x % NT;
-  const float inv = 1.0f / static_cast<float>(a.units);
+  const float units = static_cast<float>(a.units), inv = 1.0f / units;
   float w[NC][W], b[NC][W];
 #pragma unroll
   for (int k = 0; k < NC; ++k) {
@@ -121,7 +128,7 @@ __global__ __launch_bounds__(ROWS* WAVES * 64) void k_normalise(NormArgs a) {
         for (int i = 0; i < W; ++i) mean[r] += to_f32(x[k][r][i]);
     row_sums<WAVES>(mean, part[0]);
 #pragma unroll
-    for (int r = 0; r < R; ++r) mean[r] *= inv;
+    for (int r = 0; r < R; ++r) mean[r] = mean_of(mean[r], units, inv);
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int left = a.units - (k * NT + lane) * W;
@@ -166,8 +173,8 @@ __global__ __launch_bounds__(1024) void k_normalise_stream(NormArgs a) {
 #pragma unroll
     for (int i = 0; i < W; ++i) sum += to_f32(x[i]);
   }
-  const float inv = 1.0f / static_cast<float>(a.units);
-  const float mean = row_sum<WAVES>(sum, part[0]) * inv;
+  const float units = static_cast<float>(a.units), inv = 1.0f / units;
+  const float mean = mean_of(row_sum<WAVES>(sum, part[0]), units, inv);
   for (int at = threadIdx.x * W; at < a.units; at += STEP) {
     const typename Pack<T, W>::type x = load_pack<W>(row + at, a.units - at);
 #pragma unroll

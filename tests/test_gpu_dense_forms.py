@@ -57,3 +57,21 @@ def test_rows_of_one_large_value(units, dtype) -> None:
     plain.near(got[0], dx, dx_off + plain.rounded(dx, dtype))
     assert not dw.any() and not got[1].any()
     plain.near(got[2], db, db_off)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("units", [3, 100, 1003, 1425, 3396, 9000, 20001])
+def test_the_mean_is_the_sum_over_the_units(units, dtype) -> None:
+    """A sum that is exact has a mean that is: a row of one value c (few bits, so that units * c is a float32 number)
+    has it for mean, and is normalised to the bias, also where one rounding of the mean, squared, would pass float32."""
+    base._say("mean", units, dtype)
+    g = base._gen(units, 4)
+    x = torch.tensor([2.0**110, -3 * 2.0**100, 5.0, 100.0, 0.0], device=DEV)[:, None].expand(5, units).to(dtype)
+    d, w, b = base._randn((5, units), g).to(dtype), base._randn((units,), g), base._randn((units,), g)
+    y, kept = dense.normalise(x, w, b, 2.0**-20)
+    assert torch.equal(kept[:, 0], x[:, 0].float()) and torch.equal(kept[:, 1], torch.full((5,), 2.0**10, device=DEV))
+    assert torch.equal(y, b.to(dtype).expand(5, units))
+    (_, _), (dx, dx_off), _, _ = plain.normalise(torch.zeros_like(x), w, b, 2.0**-20, d)
+    got = dense.normalise_grad(d, x, w, kept)
+    plain.near(got[0], dx, dx_off + plain.rounded(dx, dtype))
+    assert not got[1].any()
