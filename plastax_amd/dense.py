@@ -36,6 +36,7 @@ _IDS = {torch.int32: 0, torch.int64: 1}
 _KEEP = 64  # PLX_RECUR_KEEP
 MAX_NAMED = 1024  # PLX_MAX_NAMED
 _MAX_TOKENS, _MAX_UNITS = 1 << 30, 1 << 24
+_LEAST, _MOST = 2.0**-126, 2.0**128 - 2.0**104  # float32's normal numbers
 
 
 def _plain(who: str, t: torch.Tensor) -> torch.Tensor:
@@ -160,8 +161,8 @@ def normalise(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     the squares of x - mean is float32: past its range (3.4e38 over the row)
     results are not what the formula gives."""
     x = _batch("normalise", x)
-    if not 0 <= eps < math.inf:
-        raise ValueError(f"normalise: eps >= 0 expected, got {eps}")
+    if not (_LEAST <= eps <= _MOST or eps == 0):
+        raise ValueError(f"normalise: an eps that float32 has expected (0, or 2^-126 to 3.4e38), got {eps}")
     weight = _param("normalise", "weight", x, weight)
     if bias is not None:
         if bias.dtype is not weight.dtype:

@@ -306,3 +306,14 @@ def test_plain_gradients_are_the_differences() -> None:
     (loss, _), (d, _) = plain.distil(x, ids, top, 1.5, weight)
     assert float(loss[2]) == 0.0 and float(d[2].abs().max()) == 0.0 and float(loss.min()) >= 0.0
     _agree(_difference(lambda t: (plain.distil(t, ids, top, 1.5)[0][0] * weight).sum(), x, v), d, v)
+
+
+@pytest.mark.parametrize("eps", [1e-46, 1e-40, 2.0**-127, 1e39, 2.0**128])
+def test_eps_that_float32_has_not_is_refused(eps) -> None:
+    """1e-46 is 0 in float32: a row of one value would be NaN, where the formula gives the bias."""
+    x, w = torch.zeros(5, 8), torch.ones(8)
+    with pytest.raises(ValueError, match="eps"):
+        dense.normalise(x, w, eps=eps)
+    for fine in (0, 0.0, 2.0**-126, 2.0**127):
+        with pytest.raises(ValueError, match="GPU"):
+            dense.normalise(x, w, eps=fine)

@@ -1,5 +1,5 @@
 """plastax_amd.dense on the GPU at sizes that take the kernels' other forms: long runs of tiles, many tokens, frequent
-ids. Against the plain 64-bit forms, within the bounds that they count."""
+ids, the widest levels. Against the plain 64-bit forms, within the bounds that they count."""
 
 from __future__ import annotations
 
