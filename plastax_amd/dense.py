@@ -103,10 +103,17 @@ def _space(device: torch.device, name: str, *args: object) -> tuple[torch.Tensor
 # --------------------------------------------------------------------------
 # An input level by ids
 # --------------------------------------------------------------------------
+def _scale(who: str, scale: float) -> None:
+    if not (_LEAST <= abs(scale) <= _MOST or scale == 0 or not math.isfinite(scale)):
+        raise ValueError(f"{who}: a scale that float32 has expected (0, or 2^-126 to 3.4e38), got {scale}")
+
+
 def look_up(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """``scale * table[ids]`` ``[tokens, units]`` of a table ``[rows, units]``.
 
-    An id that the table has no row for (-1, padding) gives a row of zeros."""
+    scale is taken in float32. An id that the table has no row for (-1,
+    padding) gives a row of zeros."""
+    _scale("look_up", scale)
     table, ids = _batch("look_up", table), _ids("look_up", "ids", ids, 1)
     rows, units = table.shape
     if rows > _MAX_UNITS:
@@ -125,6 +132,7 @@ def look_up_grad(g: torch.Tensor, ids: torch.Tensor, rows: int, scale: float = 1
     sums of the tokens' gradients g ``[tokens, units]`` by id, zeros for rows
     that no token named. Ids outside of the rows count for nothing. At most 2^25
     tokens."""
+    _scale("look_up_grad", scale)
     g, ids = _batch("look_up_grad", g), _ids("look_up_grad", "ids", ids, 1)
     if not 0 <= rows <= _MAX_UNITS:
         raise ValueError(f"look_up_grad: 0 to 2^24 rows expected, got {rows}")

@@ -317,3 +317,18 @@ def test_eps_that_float32_has_not_is_refused(eps) -> None:
     for fine in (0, 0.0, 2.0**-126, 2.0**127):
         with pytest.raises(ValueError, match="GPU"):
             dense.normalise(x, w, eps=fine)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 2.0**128, 1e-40, -(2.0**-127), 1e-300])
+def test_scales_that_float32_has_not_are_refused(scale) -> None:
+    """1e39 is an infinity in float32, and 0 times it a NaN."""
+    table, ids = torch.zeros(7, 8), torch.zeros(5, dtype=torch.int64)
+    with pytest.raises(ValueError, match="scale"):
+        dense.look_up(ids, table, scale)
+    with pytest.raises(ValueError, match="scale"):
+        dense.look_up_grad(table[:5], ids, 7, scale)
+    for fine in (0, 1, -2.5, 2.0**-126, 2.0**127, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="GPU"):
+            dense.look_up(ids, table, fine)
+        with pytest.raises(ValueError, match="GPU"):
+            dense.look_up_grad(table[:5], ids, 7, fine)
