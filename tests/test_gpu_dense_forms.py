@@ -245,3 +245,16 @@ def test_recur_of_the_widest_levels() -> None:
     dxz2, ds2 = dense.recur_grad(d[:, :some], few, kept2)
     assert torch.equal(dxz[:, units - some : units], dxz2[:, :some]) and torch.equal(dxz[:, -some:], dxz2[:, some:])
     assert torch.equal(ds[:, -some:], ds2)
+
+
+def test_states_in_place_are_known_to_autograd() -> None:
+    """What a backward pass needs of a state is not what recur_step leaves there: the pass says so, as after torch's own
+    operations in place, in place of a wrong gradient."""
+    state, w = torch.ones((3, 8), device=DEV), torch.ones((3, 8), device=DEV, requires_grad=True)
+    seen = (state * w).sum()
+    with torch.no_grad():
+        dense.recur_step(torch.ones((3, 16), device=DEV), state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        seen.backward()
+    with torch.inference_mode():  # (such tensors have no versions)
+        dense.recur_step(torch.ones((3, 16), device=DEV), torch.zeros((3, 8), device=DEV))
