@@ -15,7 +15,12 @@
 // 65536 tokens, 131072 rows of 1024 units, bf16: looked up in 48 us (a row read
 // again is often in a cache); the gradient in 26, 131 and 12, of which the
 // second writes 537 MB and reads 134, 5.1 TB/s. With few tokens a launch's
-// chain of loads is what it takes: 4 to 11 us each.
+// chain of loads is what it takes: 4 to 11 us each. The sort reads tokens *
+// classes ids, whatever the units: 65536 tokens of 16 units are 28 us, nearly all
+// of it the sort's. One workgroup orders all tokens of a class, and one joins the
+// parts of 256 columns of a row: 65536 tokens of 131072 rows of 1024 units take
+// 145 us with ids that all differ, 160 where one in ten, 254 where half and 357
+// where all of them are one id (300 rows: 62, 75, 152 and 233).
 
 #include "px_dense.h"
 

@@ -10,7 +10,9 @@
 // and y (dx) written once. 16384 x 4096 bf16: 54 us forwards, 5.0 TB/s; the
 // gradients 79, 5.1 TB/s, and 4 for the join of dw and db. A row has as many
 // waves as hold it with a chunk of 16 bytes a lane, up to 16 waves, then up to
-// 4 chunks; several rows share a workgroup.
+// 4 chunks; several rows share a workgroup. Levels that fill 64 2^k lanes in part
+// leave the others idle: 47072 x 1425 bf16 (179 chunks, 256 lanes) 58 us and 108,
+// 4.6 and 3.7 TB/s.
 
 #include "px_dense.h"
 
@@ -204,8 +206,10 @@ __global__ __launch_bounds__(1024) void k_normalise_stream(NormArgs a) {
 
 // The gradients, a row at a time: a lane keeps its sums of g n and g in
 // registers; they are joined over the groups in LDS and written as the
-// workgroup's part. (Two rows at a time, or the next one's loads ahead, gained
-// nothing: 16384 x 4096 bf16 94 us both, this 87.)
+// workgroup's part. (16384 x 4096 bf16 79 us with two workgroups a CU, which fit
+// while a lane has at most 64 registers; 61 are used. With one a CU it was 87, and
+// 94 with two rows at a time or the next one's loads ahead, for which those
+// registers are not there.)
 template <typename T, typename P, int ROWS, int WAVES, int NC>
 __global__ __launch_bounds__(ROWS* WAVES * 64) void k_normalise_grad(NormArgs a) {
   constexpr int W = kChunk<T>, NT = WAVES * 64;

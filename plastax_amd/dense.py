@@ -165,9 +165,11 @@ def normalise(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
     variance over each token's units, and what the gradient needs (each token's
     mean and 1 / sqrt(var + eps), float32 ``[tokens, 2]``).
 
-    weight and bias ``[units]`` are both float32, or both of x's type. The sum of
-    the squares of x - mean is float32: past its range (3.4e38 over the row)
-    results are not what the formula gives."""
+    weight and bias ``[units]`` are both float32, or both of x's type. eps is
+    taken in float32, and a row's sums are float32, of x and of the squares of
+    x - mean (mean with the rounding of its sum): where they pass its range, 3.4e38,
+    or where the squares vanish, below 1e-38, beside an eps as small or 0, results
+    are not what the formula gives."""
     x = _batch("normalise", x)
     if not (_LEAST <= eps <= _MOST or eps == 0):
         raise ValueError(f"normalise: an eps that float32 has expected (0, or 2^-126 to 3.4e38), got {eps}")
@@ -286,8 +288,8 @@ def recur_grad(g: torch.Tensor, xz: torch.Tensor, kept: torch.Tensor, starts: to
 def recur_step(xz: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
     """One token of each sequence: xz ``[sequences, 2 units]``; the state
     (float32 ``[sequences, units]``, each sequence's units next to each other,
-    no two sequences in the same memory) is updated in place, and h is what it
-    became in xz's type."""
+    no two sequences in the same memory, nor in xz's) is updated in place, and h
+    is what it became in xz's type."""
     xz = _batch("recur_step", xz)
     sequences, units = xz.shape[0], xz.shape[1] // 2
     if xz.shape[1] % 2:
@@ -351,7 +353,8 @@ def distil_grad(g: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, top: t
                 temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """``(loss, dlogits)``: :func:`distil`'s losses, and the gradient of their
     sum weighted by g (float32 ``[tokens]``; 1 / tokens for a mean, 0 for a
-    token that is not learned from), in one pass over the logits."""
+    token that is not learned from), in one pass over the logits. g times the
+    temperature is float32."""
     logits, ids, top = _named("distil_grad", logits, ids, top, temperature)
     tokens, outputs = logits.shape
     g = _floats("distil_grad", "g", g, (tokens,))
