@@ -338,7 +338,8 @@ def distil(logits: torch.Tensor, ids: torch.Tensor, top: torch.Tensor, temperatu
     outputs that ids ``[tokens, named]`` name, top the teacher's logits for
     them. A place whose id is no output (-1), or whose top is -inf, counts for
     nothing; a token without any other place has the loss 0 (and the gradient
-    0). An output named twice counts twice."""
+    0). An output named twice counts twice. The temperature is taken in
+    float32."""
     logits, ids, top = _named("distil", logits, ids, top, temperature)
     _together("distil", logits, ids, top)
     tokens, outputs = logits.shape
